@@ -75,6 +75,28 @@ class StageDesc(ctypes.Structure):
     ]
 
 
+class CacheDesc(ctypes.Structure):
+    """Mirror of ``g2d_cache_desc``."""
+    _fields_ = [
+        ("half", _i32), ("head_dim", _i32), ("page_size", _i32), ("kv_heads", _i32),
+        ("pages", _i64), ("batch", _i64), ("table_width", _i64), ("table_stride", _i64), ("tokens", _i64),
+        ("k_codes", _vp), ("k_scale", _vp), ("v_codes", _vp), ("v_scale", _vp),
+        ("table", _vp), ("lengths", _vp), ("offsets", _vp),
+    ]
+
+
+class AttendDesc(ctypes.Structure):
+    """Mirror of ``g2d_attend_desc``."""
+    _fields_ = [
+        ("cache", CacheDesc),
+        ("heads", _i32), ("causal", _i32), ("scale", ctypes.c_float), ("softcap", ctypes.c_float),
+        ("q", _vp), ("q_token_stride", _i64), ("q_head_stride", _i64), ("out", _vp),
+        ("slopes", _vp), ("prefix", _vp),
+        ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
+        ("status", _vp),
+    ]
+
+
 _SIGNATURES = {
     "g2d_status_string": (ctypes.c_char_p, [ctypes.c_int]),
     "g2d_abi_version": (ctypes.c_int, []),
@@ -111,6 +133,13 @@ _SIGNATURES = {
     "g2d_ldl_of_inverse_pair": (ctypes.c_int, [ctypes.c_int, _i64, _vp, _i32, _vp, _vp, ctypes.c_size_t,
                                                _i64, _vp, _i32, _vp, _vp, ctypes.c_size_t, _vp, _vp]),
 }
+
+_SIGNATURES.update({
+    "g2d_cache_append": (ctypes.c_int, [ctypes.POINTER(CacheDesc), _vp, _i64, _i64, _vp, _i64, _i64, _vp]),
+    "g2d_cache_read": (ctypes.c_int, [ctypes.POINTER(CacheDesc), _vp, _vp, _vp]),
+    "g2d_attend_workspace_bytes": (ctypes.c_int, [ctypes.POINTER(AttendDesc), ctypes.POINTER(ctypes.c_size_t)]),
+    "g2d_cache_attend": (ctypes.c_int, [ctypes.POINTER(AttendDesc), _vp]),
+})
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
 _LIB = None

@@ -1,0 +1,149 @@
+"""Keys and values in packed 4-bit codes, and attention over them.
+
+Every row (the values of one token and one kv head) is rounded under its own abs-max scale, as ``int_abs_max_quantizer_*`` rounds a row of a
+super-entry to the codes -8..7 with an fp16 scale, and stored as ``packed_codes.pack_codes`` stores a row with ``qmin=-8, bits=4``: ``head_dim / 2``
+bytes of codes and 2 bytes of scale, 3.9 times less than 16-bit values at ``head_dim = 128``.
+
+The cache is paged.  A step's tokens belong to sequences: sequence ``b`` has the tokens ``offsets[b]:offsets[b + 1]`` of the step (without
+``offsets`` every sequence has the same number of them) and holds ``lengths[b]`` positions, this step's tokens being the last; position ``p`` lies in
+page ``page_table[b, p // page_size]``.  These three are read on the device, so a captured graph follows them.  What they say is never
+trusted with an address: positions beyond the table and page numbers outside the cache are absent (not written, read as zeros, seen by no query).
+Pages may be shared for reading; two tokens of a step that go to the same place leave the row of either, or a mixture.
+CUDA only, like the rest of the package; no gradients.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import NamedTuple
+
+import torch
+
+import _abi
+
+
+class PackedCache(NamedTuple):
+    """Codes ``uint8 [pages, kv_heads, page_size, head_dim / 2]`` and scales ``float16 [pages, kv_heads, page_size]`` of keys and of values."""
+
+    k_codes: torch.Tensor
+    k_scale: torch.Tensor
+    v_codes: torch.Tensor
+    v_scale: torch.Tensor
+
+
+def new_packed_cache(pages: int, page_size: int, kv_heads: int, head_dim: int, device) -> PackedCache:
+    """An empty cache (all codes and scales zero)."""
+    assert head_dim in (64, 128), "head_dim must be 64 or 128"
+    assert page_size >= 16 and page_size & (page_size - 1) == 0, "page_size must be a power of two, at least 16"
+    codes = lambda: torch.zeros(pages, kv_heads, page_size, head_dim // 2, dtype=torch.uint8, device=device)  # noqa: E731
+    scale = lambda: torch.zeros(pages, kv_heads, page_size, dtype=torch.float16, device=device)  # noqa: E731
+    return PackedCache(codes(), scale(), codes(), scale())
+
+
+def _fill(desc, cache: PackedCache, dtype, tokens: int, page_table, lengths, offsets):
+    """Checks the cache and what says where its tokens are, and writes them into the descriptor; returns the device."""
+    k_codes, k_scale, v_codes, v_scale = cache
+    device = k_codes.device
+    assert k_codes.is_cuda, "the packed cache requires CUDA tensors (there is no CPU path)"
+    pages, kv_heads, page_size, half_dim = k_codes.shape
+    assert k_codes.dtype == torch.uint8 and v_codes.dtype == torch.uint8 and v_codes.shape == k_codes.shape, "expected uint8 codes of keys and values of one shape"
+    assert k_scale.dtype == torch.float16 and v_scale.dtype == torch.float16, "expected float16 scales"
+    assert k_scale.shape == k_codes.shape[:3] and v_scale.shape == k_codes.shape[:3], "expected a scale per page, kv head and place"
+    assert all(t.is_contiguous() and t.device == device and t.data_ptr() % 16 == 0 for t in cache), "the cache's tensors must be contiguous, 16-byte aligned and on one device"
+    assert page_size >= 16 and page_size & (page_size - 1) == 0, "page_size must be a power of two, at least 16"
+    assert half_dim in (32, 64), "head_dim must be 64 or 128"
+    assert page_table.dim() == 2 and page_table.dtype == torch.int32 and page_table.device == device, "expected an int32 page table [batch, pages per sequence] on the cache's device"
+    batch = page_table.size(0)
+    assert page_table.stride(1) == 1 or page_table.size(1) <= 1, "the rows of the page table must be contiguous"
+    assert lengths.shape == (batch,) and lengths.dtype == torch.int32 and lengths.device == device and lengths.is_contiguous(), "expected contiguous int32 lengths [batch] on the cache's device"
+    if offsets is None:
+        assert tokens == 0 or (batch > 0 and tokens % batch == 0), "without offsets every sequence has the same number of tokens"
+    else:
+        assert offsets.shape == (batch + 1,) and offsets.dtype == torch.int32 and offsets.device == device and offsets.is_contiguous(), "expected contiguous int32 offsets [batch + 1] on the cache's device"
+    desc.half = _abi.half_code(dtype) if dtype in (torch.float16, torch.bfloat16) else -1
+    assert desc.half >= 0, "expected float16 or bfloat16 values"
+    desc.head_dim, desc.page_size, desc.kv_heads = 2 * half_dim, page_size, kv_heads
+    desc.pages, desc.batch, desc.table_width, desc.table_stride, desc.tokens = pages, batch, page_table.size(1), page_table.stride(0), tokens
+    desc.k_codes, desc.k_scale, desc.v_codes, desc.v_scale = k_codes.data_ptr(), k_scale.data_ptr(), v_codes.data_ptr(), v_scale.data_ptr()
+    desc.table, desc.lengths, desc.offsets = page_table.data_ptr(), lengths.data_ptr(), None if offsets is None else offsets.data_ptr()
+    return device
+
+
+def _rows(x: torch.Tensor, device, heads: int, dim: int, what: str) -> torch.Tensor:
+    """``x [tokens, heads, dim]`` as the kernels read it: any strides of tokens and heads that keep 16-byte vectors whole, else a copy."""
+    assert x.dim() == 3 and x.shape[1:] == (heads, dim), f"expected {what} [tokens, {heads}, {dim}]"
+    assert x.device == device, f"{what} must be on the cache's device"
+    if x.stride(2) != 1 or x.stride(0) % 8 or x.stride(1) % 8 or x.data_ptr() % 16:
+        x = x.contiguous()
+    return x if x.data_ptr() % 16 == 0 else x.clone()
+
+
+@torch.no_grad()
+def append_packed(cache: PackedCache, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, offsets: torch.Tensor | None = None) -> None:
+    """Round the step's keys and values ``[tokens, kv_heads, head_dim]`` (float16 or bfloat16; strided views, such as parts of a fused projection, are
+    read in place) and write them into the cache, in place.  ``lengths`` counts the step's tokens already.  A row with an infinity or a NaN reads back as NaN."""
+    assert k.dtype == v.dtype and k.dim() == 3 and k.shape == v.shape, "expected keys and values of one shape and type"
+    desc = _abi.CacheDesc()
+    device = _fill(desc, cache, k.dtype, k.size(0), page_table, lengths, offsets)
+    k, v = _rows(k, device, desc.kv_heads, desc.head_dim, "keys"), _rows(v, device, desc.kv_heads, desc.head_dim, "values")
+    with torch.cuda.device(device):
+        _abi.check(_abi.library().g2d_cache_append(ctypes.byref(desc), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), _abi.stream_of(k)), "g2d_cache_append")
+
+
+@torch.no_grad()
+def read_packed(cache: PackedCache, page_table: torch.Tensor, lengths: torch.Tensor, offsets: torch.Tensor | None = None, *, tokens: int,
+                dtype: torch.dtype) -> tuple[torch.Tensor, torch.Tensor]:
+    """The keys and values ``[tokens, kv_heads, head_dim]`` that the cache holds for the last tokens of every sequence, ``offsets`` saying how many (all of them, where
+    they add up to ``lengths``).  Rows of no sequence are zeros."""
+    desc = _abi.CacheDesc()
+    device = _fill(desc, cache, dtype, tokens, page_table, lengths, offsets)
+    new = torch.empty if offsets is None else torch.zeros
+    k, v = new(2, tokens, desc.kv_heads, desc.head_dim, dtype=dtype, device=device).unbind(0)
+    with torch.cuda.device(device):
+        _abi.check(_abi.library().g2d_cache_read(ctypes.byref(desc), k.data_ptr(), v.data_ptr(), _abi.stream_of(k)), "g2d_cache_read")
+    return k, v
+
+
+@torch.no_grad()
+def attend_packed(q: torch.Tensor, cache: PackedCache, page_table: torch.Tensor, lengths: torch.Tensor, offsets: torch.Tensor | None = None, *,
+                  scale: float | None = None, causal: bool = True, softcap: float = 0.0, slopes: torch.Tensor | None = None,
+                  prefix: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of the step's queries ``q [tokens, heads, head_dim]`` (float16 or bfloat16) over the cache: ``[tokens, heads, head_dim]`` in q's type.
+
+    ``heads`` is a multiple of the cache's kv heads; query head ``h`` reads kv head ``h // (heads // kv_heads)``.  The scores are ``scale * q . k`` (``1 /
+    sqrt(head_dim)`` by default), with ``softcap > 0`` then ``softcap * tanh(score / softcap)``, with ``slopes`` (float32 ``[heads]``) then
+    ``+ slopes[h] * (j - p)`` for a query at position p and a key at j.  A query sees its sequence's keys up to its own position, and those before
+    ``prefix[b]`` (int32 ``[batch]``) wherever it stands; with ``causal=False`` all of them.  A query that sees no key gets zeros.  Rows of ``out`` that belong
+    to no sequence are left as they are (zeros, without ``out``).  What a step appends has to be in the cache before: call ``append_packed`` first."""
+    assert q.dim() == 3, "expected queries [tokens, heads, head_dim]"
+    desc = _abi.AttendDesc()
+    c = desc.cache
+    device = _fill(c, cache, q.dtype, q.size(0), page_table, lengths, offsets)
+    heads = q.size(1)
+    assert heads > 0 and heads % c.kv_heads == 0, "the number of heads must be a multiple of the cache's kv heads"
+    q = _rows(q, device, heads, c.head_dim, "queries")
+    assert math.isfinite(softcap) and softcap >= 0, "softcap must be finite and not negative"
+    scale = 1 / math.sqrt(c.head_dim) if scale is None else float(scale)
+    assert math.isfinite(scale), "scale must be finite"
+    if slopes is not None:
+        assert slopes.shape == (heads,) and slopes.dtype == torch.float32 and slopes.device == device and slopes.is_contiguous(), "expected contiguous float32 slopes [heads] on the cache's device"
+        desc.slopes = slopes.data_ptr()
+    if prefix is not None:
+        assert prefix.shape == lengths.shape and prefix.dtype == torch.int32 and prefix.device == device and prefix.is_contiguous(), "expected a contiguous int32 prefix [batch] on the cache's device"
+        desc.prefix = prefix.data_ptr()
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=device) if offsets is None else torch.zeros(q.shape, dtype=q.dtype, device=device)
+    else:
+        assert out.shape == q.shape and out.dtype == q.dtype and out.device == device and out.is_contiguous() and out.data_ptr() % 16 == 0, "out must be a contiguous, 16-byte aligned tensor like q"
+    if q.numel() == 0:
+        return out
+    desc.heads, desc.causal, desc.scale, desc.softcap = heads, bool(causal), scale, softcap
+    desc.q, desc.q_token_stride, desc.q_head_stride, desc.out = q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr()
+    lib = _abi.library()
+    need = ctypes.c_size_t()
+    _abi.check(lib.g2d_attend_workspace_bytes(ctypes.byref(desc), ctypes.byref(need)), "g2d_attend_workspace_bytes")
+    workspace = torch.empty(need.value, dtype=torch.uint8, device=device)
+    desc.workspace, desc.workspace_bytes, desc.status = workspace.data_ptr(), need.value, _abi.status_word(device).data_ptr()
+    with torch.cuda.device(device):
+        _abi.check(lib.g2d_cache_attend(ctypes.byref(desc), _abi.stream_of(q)), "g2d_cache_attend")
+    return out

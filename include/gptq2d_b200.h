@@ -315,6 +315,54 @@ int g2d_unpack_codes(int dtype, int64_t m, int64_t n, const uint8_t *codes, int6
  * reference, whose inputs are device tensors. */
 int g2d_symmetric_from_packed(int dtype, int64_t n, const void *packed, void *out, void *stream);
 
+/* ---- answering from packed codes (no counterpart in the reference, which ends at dequantised matrices) ---- */
+
+/* Keys and values in 4-bit codes, in pages: codes [pages, kv_heads, page_size, head_dim / 2] and fp16 scales [pages, kv_heads, page_size], 16-byte
+ * aligned, page_size a power of two from 16 up, head_dim 64 or 128.  A row (the head_dim values of a token and a kv head) is rounded as
+ * g2d_absmax_quantize_super_entry rounds a row with qmin = -8, qmax = 7 and an fp16 scale, and stored as g2d_pack_codes stores it with qmin = -8.
+ * The tokens of a step belong to `batch` sequences: sequence b has the tokens offsets[b] .. offsets[b + 1] - 1 (offsets null: tokens / batch each) and holds
+ * lengths[b] positions, its tokens of the step being the last of them; position p lies in page table[b * table_stride + p / page_size].
+ * lengths, offsets and table are read on the device only.  Positions beyond the table and pages outside [0, pages) are absent: not written, read as
+ * zeros, seen by nobody.  Tokens outside offsets[0] .. offsets[batch] - 1 are left alone everywhere. */
+typedef struct g2d_cache_desc {
+    int32_t half;                /* g2d_half of keys, values, queries and results */
+    int32_t head_dim, page_size, kv_heads;
+    int64_t pages, batch, table_width, table_stride, tokens;
+    uint8_t *k_codes;
+    void *k_scale;
+    uint8_t *v_codes;
+    void *v_scale;
+    const int32_t *table;        /* [batch, table_width], rows table_stride apart */
+    const int32_t *lengths;      /* [batch] */
+    const int32_t *offsets;      /* [batch + 1] or NULL */
+} g2d_cache_desc;
+
+/* The step's keys and values (element strides of tokens and heads, multiples of 8; 16-byte aligned) into the cache.  Two tokens of a step that the
+ * table sends to the same place leave codes and scale of either there. */
+int g2d_cache_append(const g2d_cache_desc *desc, const void *k, int64_t k_token_stride, int64_t k_head_stride, const void *v,
+                     int64_t v_token_stride, int64_t v_head_stride, void *stream);
+/* What the cache holds for the step's tokens, as values: k and v [tokens, kv_heads, head_dim]. */
+int g2d_cache_read(const g2d_cache_desc *desc, void *k, void *v, void *stream);
+
+/* Attention of the step's tokens over the cache.  Token i of a sequence with n tokens in the step stands at p = length - n + i; query head h reads kv
+ * head h / (heads / kv_heads).  Scores u = scale q . k, then softcap tanh(u / softcap) if softcap > 0, then + slopes[h] (j - p) if slopes is given.
+ * Seen are the keys j < length; causal: those with j <= p or j < prefix[b] among them.  A row that sees none becomes zeros. */
+typedef struct g2d_attend_desc {
+    g2d_cache_desc cache;
+    int32_t heads, causal;
+    float scale, softcap;
+    const void *q;               /* element strides below, multiples of 8; 16-byte aligned */
+    int64_t q_token_stride, q_head_stride;
+    void *out;                   /* [tokens, heads, head_dim], 16-byte aligned */
+    const float *slopes;         /* [heads] or NULL */
+    const int32_t *prefix;       /* [batch] or NULL */
+    void *workspace;             /* g2d_attend_workspace_bytes() bytes, 256-byte aligned */
+    size_t workspace_bytes;
+    int32_t *status;             /* optional device int32: set to -1 when a bounded wait ran out; results are NaN then */
+} g2d_attend_desc;
+int g2d_attend_workspace_bytes(const g2d_attend_desc *desc, size_t *bytes);
+int g2d_cache_attend(const g2d_attend_desc *desc, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
