@@ -97,6 +97,24 @@ class AttendDesc(ctypes.Structure):
     ]
 
 
+class LinearDesc(ctypes.Structure):
+    """Mirror of ``g2d_linear_desc``."""
+    _fields_ = [
+        ("half", _i32), ("bits", _i32),
+        ("m", _i64), ("n", _i64), ("tokens", _i64),
+        ("x", _vp), ("x_stride", _i64),
+        ("codes", _vp), ("row_bytes", _i64), ("groups", _i64),
+        ("scale", _vp), ("scale_row_stride", _i64), ("scale_group_stride", _i64),
+        ("zero", _vp), ("zero_row_stride", _i64), ("zero_group_stride", _i64),
+        ("qmin", _dbl),
+        ("adapters", _i64), ("rank", _i32), ("reserved", _i32),
+        ("down", _vp), ("up", _vp), ("scaling", _vp), ("index", _vp),
+        ("out", _vp), ("out_stride", _i64),
+        ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
+        ("status", _vp),
+    ]
+
+
 _SIGNATURES = {
     "g2d_status_string": (ctypes.c_char_p, [ctypes.c_int]),
     "g2d_abi_version": (ctypes.c_int, []),
@@ -137,6 +155,8 @@ _SIGNATURES = {
 _SIGNATURES.update({
     "g2d_cache_append": (ctypes.c_int, [ctypes.POINTER(CacheDesc), _vp, _i64, _i64, _vp, _i64, _i64, _vp]),
     "g2d_cache_read": (ctypes.c_int, [ctypes.POINTER(CacheDesc), _vp, _vp, _vp]),
+    "g2d_linear_workspace_bytes": (ctypes.c_int, [ctypes.POINTER(LinearDesc), ctypes.POINTER(ctypes.c_size_t)]),
+    "g2d_packed_linear": (ctypes.c_int, [ctypes.POINTER(LinearDesc), _vp]),
     "g2d_attend_workspace_bytes": (ctypes.c_int, [ctypes.POINTER(AttendDesc), ctypes.POINTER(ctypes.c_size_t)]),
     "g2d_cache_attend": (ctypes.c_int, [ctypes.POINTER(AttendDesc), _vp]),
 })

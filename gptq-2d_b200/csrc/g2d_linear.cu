@@ -1,0 +1,317 @@
+// y = x W^T for a matrix W held as packed 4-bit codes, few tokens:  y[t, o] = sum_g s[o, g] sum_{k in g} (c[o, k] + qmin - z[o, g]) x[t, k]  (+ adapters).
+//
+// The rows of W are the rows of A of m16n8k16 products, the tokens its columns.  A code goes to the tensor cores as it lies in its word: the bits of c in the lowest
+// (or next) four bits of a 16-bit float are c (or 16 c) times the smallest subnormal, exactly, so eight codes cost a shift and four ANDs; the products
+// with the 16 c go to sums of their own.  fp16 activations are taken as they are; bf16 ones times 2^56, for codes of c 2^-133 (activations from 2^72 up overflow).
+// What the codes' origin and zero point add is (qmin - z) sum x, from sums of x over each group that the CTA forms while it brings x to shared memory.
+// A lane reads 16 bytes of codes (32 columns) of two rows, four times ahead; x lies in shared memory in the order in which such
+// words hold their columns, so a fragment of it is one 16-byte load.  With groups of an odd number of 64 columns a lane reads 8 bytes at a time.
+//
+// A CTA has 16 ROW_TILES rows; its eight warps split them and the columns; a cluster of CTAs splits the columns further, and sums meet through shared memory
+// in a fixed order.  Bound: HBM (half a byte per weight), for small matrices the latency of one chain of loads.
+#include "g2d_linear.cuh"
+#include "g2d_tc.cuh"
+
+namespace g2d {
+
+constexpr int ROWS_WARPS = 8, ROWS_THREADS = 32 * ROWS_WARPS;
+
+template <bool BF16>
+__device__ __forceinline__ void mma_codes(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    if (BF16)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// KB: columns of a block, 128 or 64; NT: tiles of eight tokens
+template <bool BF16, int NT, int KB, int ROW_TILES>
+__global__ void __launch_bounds__(ROWS_THREADS, 2) linear_rows_kernel(const LinearArgs a) {
+    constexpr int WORDS = KB / 32, K_GROUPS = ROWS_WARPS / ROW_TILES, ROWS = 16 * ROW_TILES, TOKENS = 8 * NT, CHUNKS = KB / 8, AHEAD = 4;
+    extern __shared__ __align__(16) unsigned char linear_smem_raw[];
+    const int splits = (int)gridDim.x, rank = (int)blockIdx.x;  // a cluster has all CTAs along x
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int64_t row0 = (int64_t)blockIdx.y * ROWS;
+    const int token0 = blockIdx.z * TOKENS;
+    const int64_t blocks = ceil_div(a.n, (int64_t)KB), b_first = rank * blocks / splits, b_last = (rank + 1) * blocks / splits;
+    const int mine = (int)(b_last - b_first), most = (int)ceil_div(blocks, (int64_t)splits);  // the same layout in every CTA of the cluster
+    uint4 *const xs = reinterpret_cast<uint4 *>(linear_smem_raw);            // [block][word][tile of tokens][lane]
+    float *const sums = reinterpret_cast<float *>(xs + (int64_t)most * WORDS * NT * 32);  // [block][token]
+    float *const part = sums + most * TOKENS;                                // [k group][token][row], then the results
+    const int tile = warp % ROW_TILES, kg = warp / ROW_TILES;
+    const int w0 = (int)((int64_t)kg * mine / K_GROUPS), w1 = (int)((int64_t)(kg + 1) * mine / K_GROUPS);
+
+    // the first codes are on their way while x is brought
+    uint32_t code[AHEAD][2][WORDS];
+    const int64_t row_lo = row0 + tile * 16 + g, row_hi = row_lo + 8;
+    const auto fetch = [&](int slot, int block) {
+        const int64_t k = (b_first + block) * KB + t * (KB / 4);
+        const bool inside = block < w1 && k < a.n;  // n is a multiple of 32: a lane's columns are all inside or, 64 of 128 (or 32 of 64), checked by word
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int64_t row = h ? row_hi : row_lo;
+            const uint8_t *const p = a.codes + row * a.row_bytes + (k >> 1);
+#pragma unroll
+            for (int w = 0; w < WORDS; ++w) code[slot][h][w] = 0u;
+            if (inside && row < a.m) {
+                if constexpr (WORDS == 4) {
+                    const uint4 v = __ldg(reinterpret_cast<const uint4 *>(p));
+                    code[slot][h][0] = v.x; code[slot][h][1] = v.y; code[slot][h][2] = v.z; code[slot][h][3] = v.w;
+                } else {
+                    const uint2 v = __ldg(reinterpret_cast<const uint2 *>(p));
+                    code[slot][h][0] = v.x; code[slot][h][1] = v.y;
+                }
+            }
+        }
+    };
+#pragma unroll
+    for (int s = 0; s < AHEAD; ++s) fetch(s, w0 + s);
+
+    // ---- x: a thread takes eight columns of a token; the CHUNKS threads of a block and token stand together and add up its sum ----
+    for (int e0 = 0; e0 < mine * TOKENS * CHUNKS; e0 += ROWS_THREADS) {
+        const int e = e0 + threadIdx.x, chunk = e % CHUNKS, token = e / CHUNKS % TOKENS, block = e / (CHUNKS * TOKENS);
+        const int64_t k = (b_first + block) * KB + 8 * chunk;
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (block < mine && k < a.n && token0 + token < a.tokens) v = __ldg(reinterpret_cast<const uint4 *>((const uint16_t *)a.x + (int64_t)(token0 + token) * a.x_stride + k));
+        float sum = 0.f;
+        uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            sum += bits_to_float(u[i] & 0xffffu, BF16) + bits_to_float(u[i] >> 16, BF16);
+            if (BF16) {
+                __nv_bfloat162 p = *reinterpret_cast<__nv_bfloat162 *>(&u[i]);
+                p = __hmul2(p, __float2bfloat162_rn(72057594037927936.f));  // 2^56
+                u[i] = *reinterpret_cast<uint32_t *>(&p);
+            }
+        }
+#pragma unroll
+        for (int o = 1; o < CHUNKS; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (block < mine) {
+            // columns (0, 4), (2, 6), (1, 5), (3, 7): two codes of a word that lie sixteen bits apart
+            const uint4 f = make_uint4(__byte_perm(u[0], u[2], 0x5410), __byte_perm(u[1], u[3], 0x5410), __byte_perm(u[0], u[2], 0x7632), __byte_perm(u[1], u[3], 0x7632));
+            const int w = chunk % WORDS, lane_of = (token & 7) * 4 + chunk / WORDS;
+            xs[((block * WORDS + w) * NT + (token >> 3)) * 32 + lane_of] = f;
+            if (chunk == 0) sums[block * TOKENS + token] = sum;
+        }
+    }
+    __syncthreads();
+
+    // ---- products ----
+    constexpr float BACK = BF16 ? 151115727451828646838272.f : 16777216.f;  // 2^(133 - 56) = 2^77, or 2^24
+    const int per_group = (int)(a.group / KB);  // blocks of a group (one scale per row: all)
+    float total[NT][4];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) total[j][0] = total[j][1] = total[j][2] = total[j][3] = 0.f;
+    const bool single = a.group >= a.n;
+    const float *const scale_lo = a.scale + min(row_lo, a.m - 1) * a.scale_row, *const scale_hi = a.scale + min(row_hi, a.m - 1) * a.scale_row;
+    const float *const zero_lo = a.zero + min(row_lo, a.m - 1) * a.zero_row, *const zero_hi = a.zero + min(row_hi, a.m - 1) * a.zero_row;
+    int block = w0;
+    while (block < w1) {
+        // a run of blocks under one scale
+        const int64_t group = single ? 0 : (b_first + block) / per_group;
+        const int end = single ? w1 : (int)min((int64_t)w1, (group + 1) * per_group - b_first);
+        const float s_lo = __ldg(scale_lo + group * a.scale_group), s_hi = __ldg(scale_hi + group * a.scale_group);
+        const float o_lo = a.qmin - __ldg(zero_lo + group * a.zero_group), o_hi = a.qmin - __ldg(zero_hi + group * a.zero_group);
+        float low[NT][4], high[NT][4], xsum[NT][2];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            low[j][0] = low[j][1] = low[j][2] = low[j][3] = high[j][0] = high[j][1] = high[j][2] = high[j][3] = xsum[j][0] = xsum[j][1] = 0.f;
+        }
+        while (block < end) {
+#pragma unroll
+            for (int s = 0; s < AHEAD; ++s) {
+                // the slots go round with the blocks of the whole share, not of the run
+                if (((block - w0) & (AHEAD - 1)) != s || block >= end) continue;
+                const uint4 *const xb = xs + (int64_t)block * WORDS * NT * 32 + lane;
+                uint32_t lo[WORDS], hi[WORDS];
+#pragma unroll
+                for (int w = 0; w < WORDS; ++w) lo[w] = code[s][0][w], hi[w] = code[s][1][w];
+                fetch(s, block + AHEAD);
+#pragma unroll
+                for (int w = 0; w < WORDS; ++w) {
+                    const uint32_t lo8 = lo[w] >> 8, hi8 = hi[w] >> 8;
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) {
+                        const uint4 f = xb[(w * NT + j) * 32];
+                        mma_codes<BF16>(low[j], lo[w] & 0x000f000fu, hi[w] & 0x000f000fu, lo8 & 0x000f000fu, hi8 & 0x000f000fu, f.x, f.y);
+                        mma_codes<BF16>(high[j], lo[w] & 0x00f000f0u, hi[w] & 0x00f000f0u, lo8 & 0x00f000f0u, hi8 & 0x00f000f0u, f.z, f.w);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    const float2 v = *reinterpret_cast<const float2 *>(sums + block * TOKENS + 8 * j + 2 * t);
+                    xsum[j][0] += v.x;
+                    xsum[j][1] += v.y;
+                }
+                ++block;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const float products = fmaf(high[j][x], 0.0625f, low[j][x]) * BACK;
+                total[j][x] = fmaf(x < 2 ? s_lo : s_hi, fmaf(x < 2 ? o_lo : o_hi, xsum[j][x & 1], products), total[j][x]);
+            }
+        }
+    }
+    // ---- sums of the warps, then of the cluster ----
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) part[(kg * TOKENS + 8 * j + 2 * t + (x & 1)) * ROWS + tile * 16 + 8 * (x >> 1) + g] = total[j][x];
+    __syncthreads();
+    if (K_GROUPS > 1) {
+        for (int e = threadIdx.x; e < TOKENS * ROWS; e += ROWS_THREADS) {
+            float sum = part[e];
+#pragma unroll
+            for (int k = 1; k < K_GROUPS; ++k) sum += part[k * TOKENS * ROWS + e];
+            part[e] = sum;
+        }
+        __syncthreads();
+    }
+    if (splits > 1) cluster_sync();
+    if (a.rank) after_the_launch_before();
+    // results: the cluster's CTAs share them, each a part of the rows and tokens; consecutive threads have consecutive rows
+    const int results = min(TOKENS, a.tokens - token0) * ROWS;
+    for (int e = rank * ROWS_THREADS + threadIdx.x; e < results; e += splits * ROWS_THREADS) {
+        const int token = token0 + e / ROWS;
+        const int64_t row = row0 + e % ROWS;
+        float sum = 0.f;
+        if (splits > 1) {
+            for (int k = 0; k < splits; ++k) sum += peer_float(part + e, k);
+        } else {
+            sum = part[e];
+        }
+        if (row >= a.m) continue;
+        const int id = adapter_of(a, token);
+        if (id >= 0) {
+            const uint4 *const up = reinterpret_cast<const uint4 *>((const uint16_t *)a.up + ((int64_t)id * a.m + row) * a.rank);
+            const uint16_t *const inner = a.inner + (int64_t)token * INNER_LD;
+            float more = 0.f;
+            for (int r = 0; r < a.rank; r += 8) {
+                const uint4 u = __ldg(up + r / 8), hi = *reinterpret_cast<const uint4 *>(inner + r), lo = *reinterpret_cast<const uint4 *>(inner + RANK_MAX + r);
+                const uint32_t uu[4] = {u.x, u.y, u.z, u.w}, hh[4] = {hi.x, hi.y, hi.z, hi.w}, ll[4] = {lo.x, lo.y, lo.z, lo.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    more = fmaf(bits_to_float(uu[i] & 0xffffu, BF16), bits_to_float(hh[i] & 0xffffu, BF16) + bits_to_float(ll[i] & 0xffffu, BF16), more);
+                    more = fmaf(bits_to_float(uu[i] >> 16, BF16), bits_to_float(hh[i] >> 16, BF16) + bits_to_float(ll[i] >> 16, BF16), more);
+                }
+            }
+            sum = fmaf(more, a.factor[token], sum);
+        }
+        ((uint16_t *)a.out)[token * a.out_stride + row] = (uint16_t)float_to_bits(sum, BF16);
+    }
+    if (splits > 1) {
+        __syncwarp();
+        cluster_sync();  // the others' shared memory is read until here
+    }
+}
+
+template <bool BF16, int NT, int KB, int ROW_TILES>
+static int launch_rows_kernel(const LinearArgs &a, cudaStream_t st) {
+    static PerDeviceOnce configured;
+    constexpr int K_GROUPS = ROWS_WARPS / ROW_TILES, ROWS = 16 * ROW_TILES, TOKENS = 8 * NT;
+    constexpr size_t MOST = 200 * 1024;
+    const int64_t blocks = ceil_div(a.n, (int64_t)KB), rows = ceil_div(a.m, (int64_t)ROWS), tiles = ceil_div((int64_t)a.tokens, (int64_t)TOKENS);
+    const auto bytes = [&](int64_t splits) {
+        const int64_t most = ceil_div(blocks, splits);
+        return (size_t)(most * (KB * TOKENS * 2 + TOKENS * 4) + K_GROUPS * TOKENS * ROWS * 4);
+    };
+    // as many parts of the columns as it takes for two CTAs per SM, of four blocks per warp at least; more where x would not fit
+    int splits = 1;
+    while (splits < 8 && ((rows * tiles * splits < 2 * 148 && blocks >= 2 * splits * K_GROUPS * 4) || bytes(splits) > 96 * 1024)) splits *= 2;
+    if (bytes(splits) > MOST) return G2D_ERR_TOO_LARGE;
+    if (rows > 65535 || tiles > 65535) return G2D_ERR_TOO_LARGE;
+    if (configured.run([&] { return cudaFuncSetAttribute(linear_rows_kernel<BF16, NT, KB, ROW_TILES>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)MOST) == cudaSuccess; }) != G2D_OK)
+        return G2D_ERR_CUDA;
+    return launch_dependent(linear_rows_kernel<BF16, NT, KB, ROW_TILES>, dim3((unsigned)splits, (unsigned)rows, (unsigned)tiles), ROWS_THREADS, bytes(splits), splits, a.rank > 0, st, a);
+}
+
+template <bool BF16, int NT>
+static int launch_rows_tokens(const LinearArgs &a, cudaStream_t st) {
+    const bool odd = a.group < a.n && a.group % 128 != 0;
+    const bool small = a.m * a.n < (int64_t)148 * 2 * 128 * 1024;
+    if (odd) return small ? launch_rows_kernel<BF16, NT, 64, 4>(a, st) : launch_rows_kernel<BF16, NT, 64, 8>(a, st);
+    return small ? launch_rows_kernel<BF16, NT, 128, 4>(a, st) : launch_rows_kernel<BF16, NT, 128, 8>(a, st);
+}
+
+int launch_linear_rows(const LinearArgs &a, cudaStream_t st) {
+    if (a.tokens <= 8) return a.bf16 ? launch_rows_tokens<true, 1>(a, st) : launch_rows_tokens<false, 1>(a, st);
+    return a.bf16 ? launch_rows_tokens<true, 2>(a, st) : launch_rows_tokens<false, 2>(a, st);
+}
+
+}  // namespace g2d
+
+using namespace g2d;
+
+static size_t linear_bytes(const g2d_linear_desc *d) {
+    return d->rank > 0 ? (((size_t)d->tokens * (INNER_LD * 2 + 4) + 255) & ~(size_t)255) : 0;
+}
+
+static int linear_check(const g2d_linear_desc *d) {
+    if (!d || (d->half != G2D_FP16 && d->half != G2D_BF16) || d->m < 0 || d->n < 0 || d->tokens < 0 || d->groups < 1 || d->rank < 0 || d->adapters < 0) return G2D_ERR_BAD_ARGUMENT;
+    if (d->bits != 4 || d->n % 32 != 0 || d->row_bytes % 16 != 0 || d->rank % 8 != 0 || d->rank > RANK_MAX) return G2D_ERR_UNSUPPORTED;
+    if (d->row_bytes < d->n / 2) return G2D_ERR_BAD_ARGUMENT;
+    if (d->groups > 1 && (d->n % d->groups != 0 || d->n / d->groups % 64 != 0)) return G2D_ERR_UNSUPPORTED;
+    if (d->m > 0x3fffffff || d->n > 0x3fffffff || d->tokens > 0x3fffffff || d->adapters > 0x7fffffff) return G2D_ERR_TOO_LARGE;
+    return G2D_OK;
+}
+
+extern "C" int g2d_linear_workspace_bytes(const g2d_linear_desc *desc, size_t *bytes) {
+    const int status = linear_check(desc);
+    if (status != G2D_OK) return status;
+    if (!bytes) return G2D_ERR_BAD_ARGUMENT;
+    *bytes = linear_bytes(desc);
+    return G2D_OK;
+}
+
+extern "C" int g2d_packed_linear(const g2d_linear_desc *d, void *stream) {
+    const int status = linear_check(d);
+    if (status != G2D_OK) return status;
+    if (d->m == 0 || d->tokens == 0) return G2D_OK;
+    if (!d->out || ((uintptr_t)d->out & 1) != 0 || d->out_stride < d->m) return G2D_ERR_BAD_ARGUMENT;
+    if (d->n == 0) return G2D_ERR_UNSUPPORTED;
+    if (!d->x || !d->codes || !d->scale || !d->zero || (((uintptr_t)d->x | (uintptr_t)d->codes) & 15) != 0 || d->x_stride % 8 != 0) return G2D_ERR_BAD_ARGUMENT;
+    if (d->rank > 0 && (!d->down || !d->up || !d->index || (((uintptr_t)d->down | (uintptr_t)d->up) & 15) != 0)) return G2D_ERR_BAD_ARGUMENT;
+    if (d->rank > 0 && (!d->workspace || d->workspace_bytes < linear_bytes(d) || ((uintptr_t)d->workspace & 255) != 0)) return G2D_ERR_WORKSPACE;
+    LinearArgs a;
+    a.x = d->x;
+    a.codes = d->codes;
+    a.scale = d->scale;
+    a.zero = d->zero;
+    a.out = d->out;
+    a.m = d->m;
+    a.n = d->n;
+    a.row_bytes = d->row_bytes;
+    a.x_stride = d->x_stride;
+    a.out_stride = d->out_stride;
+    a.scale_row = d->scale_row_stride;
+    a.scale_group = d->scale_group_stride;
+    a.zero_row = d->zero_row_stride;
+    a.zero_group = d->zero_group_stride;
+    a.group = d->n / d->groups;
+    a.tokens = (int)d->tokens;
+    a.bf16 = d->half == G2D_BF16;
+    a.qmin = (float)d->qmin;
+    a.down = d->down;
+    a.up = d->up;
+    a.scaling = d->scaling;
+    a.index = d->index;
+    a.adapters = d->adapters;
+    a.rank = d->adapters > 0 ? d->rank : 0;
+    a.inner = (uint16_t *)d->workspace;
+    a.factor = d->rank > 0 ? (float *)((char *)d->workspace + (size_t)d->tokens * INNER_LD * 2) : nullptr;
+    a.status = d->status;
+    a.wait_cycles = WAIT_CYCLES;
+    cudaStream_t st = (cudaStream_t)stream;
+    if (a.rank > 0) {
+        const int launched = launch_inner(a, st);
+        if (launched != G2D_OK) return launched;
+    }
+    return launch_linear_rows(a, st);
+}

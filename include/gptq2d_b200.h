@@ -363,6 +363,39 @@ typedef struct g2d_attend_desc {
 int g2d_attend_workspace_bytes(const g2d_attend_desc *desc, size_t *bytes);
 int g2d_cache_attend(const g2d_attend_desc *desc, void *stream);
 
+/* out[t, o] = sum_k (code[o, k] + qmin - zero[o, g(k)]) scale[o, g(k)] x[t, k]  +  scaling[i] sum_r up[i, o, r] sum_k down[i, r, k] x[t, k],  i = index[t]:
+ * activations times the transpose of a matrix in packed 4-bit codes (g2d_pack_codes; n a multiple of 32, row_bytes a multiple of 16), and beside it the low-rank
+ * adapter of each token's request.  Tokens whose index lies outside [0, adapters) have none.  `groups` equal groups of columns (1, or of a multiple of
+ * 64 columns each) have scales and zero points of their own, float, addressed by row and group strides in elements (0 = broadcast).  code + qmin - zero is
+ * rounded to x's type where there are many tokens: exact for integers up to 256 (bf16) or 2048 (fp16).  Sums are float32; out is rounded once.
+ * Few tokens: bf16 activations of 2^72 and more overflow. */
+typedef struct g2d_linear_desc {
+    int32_t half, bits;          /* g2d_half of x, down, up and out; 4 */
+    int64_t m, n, tokens;
+    const void *x;               /* [tokens, n], rows x_stride apart (a multiple of 8), 16-byte aligned */
+    int64_t x_stride;
+    const uint8_t *codes;        /* [m, row_bytes], 16-byte aligned */
+    int64_t row_bytes, groups;
+    const float *scale;
+    int64_t scale_row_stride, scale_group_stride;
+    const float *zero;
+    int64_t zero_row_stride, zero_group_stride;
+    double qmin;
+    int64_t adapters;
+    int32_t rank, reserved;      /* a multiple of 8 up to 64, 0 for no adapters; reserved must be 0 */
+    const void *down;            /* [adapters, rank, n], 16-byte aligned */
+    const void *up;              /* [adapters, m, rank], 16-byte aligned */
+    const float *scaling;        /* [adapters], or NULL for 1 */
+    const int32_t *index;        /* [tokens] */
+    void *out;                   /* [tokens, m], rows out_stride apart */
+    int64_t out_stride;
+    void *workspace;             /* g2d_linear_workspace_bytes() bytes, 256-byte aligned */
+    size_t workspace_bytes;
+    int32_t *status;             /* optional device int32: set to -1 when a bounded wait ran out; out is NaN then */
+} g2d_linear_desc;
+int g2d_linear_workspace_bytes(const g2d_linear_desc *desc, size_t *bytes);
+int g2d_packed_linear(const g2d_linear_desc *desc, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
