@@ -44,9 +44,31 @@ __device__ __forceinline__ float dot8(const uint4 &p, const uint4 &q, int bf16, 
     return sum;
 }
 
-__global__ void __launch_bounds__(INNER_THREADS) inner_rows_kernel(const LinearArgs a) {
+// All threads of a CTA: the adapters of the `tile` <= INNER_THREADS tokens from token0 on, in the order in which they appear
+__device__ void write_plan(const LinearArgs &a, int *plan, int tile, int token0) {
+    __shared__ int ids[INNER_THREADS], counts[INNER_THREADS / 32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int id = (int)threadIdx.x < tile ? adapter_of(a, token0 + threadIdx.x) : -1;
+    ids[threadIdx.x] = id;
+    __syncthreads();
+    bool first = id >= 0;
+    for (int k = 0; k < (int)threadIdx.x && first; ++k) first = ids[k] != id;
+    const unsigned found = __ballot_sync(0xffffffffu, first);
+    if (lane == 0) counts[warp] = __popc(found);
+    __syncthreads();
+    int before = 0, all = 0;
+    for (int w = 0; w < INNER_THREADS / 32; ++w) {
+        if (w < warp) before += counts[w];
+        all += counts[w];
+    }
+    if (first) plan[1 + before + __popc(found & ((1u << lane) - 1u))] = id;
+    if (threadIdx.x == 0) plan[0] = all;
+}
+
+__global__ void __launch_bounds__(INNER_THREADS) inner_rows_kernel(const LinearArgs a, int *plan, int tile) {
     __shared__ float part[RANK_MAX], tops[2];
     let_the_next_launch_start();
+    if (plan && blockIdx.x == INNER_SPLIT - 1) write_plan(a, plan, tile, 0);  // 64 tokens at most: one tile
     const int token = blockIdx.x / INNER_SPLIT, rank = (int)cluster_rank(), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int id = adapter_of(a, token);
     const int64_t chunks = a.n / 8, c0 = rank * chunks / INNER_SPLIT, c1 = (rank + 1) * chunks / INNER_SPLIT;  // eight columns each
@@ -88,7 +110,7 @@ __device__ __forceinline__ void mma_16(float (&d)[4], uint32_t a0, uint32_t a1, 
 }
 
 template <bool BF16>
-__global__ void __launch_bounds__(INNER_THREADS) inner_block_kernel(const LinearArgs a) {
+__global__ void __launch_bounds__(INNER_THREADS) inner_block_kernel(const LinearArgs a, int *plan, int tile) {
     constexpr int WARPS = INNER_THREADS / 32, TILES = RANK_MAX / 8;
     __shared__ float part[WARPS / 2][INNER_BLOCK][RANK_MAX + 2];  // two warps at a time
     __shared__ int ids[INNER_BLOCK];
@@ -96,6 +118,7 @@ __global__ void __launch_bounds__(INNER_THREADS) inner_block_kernel(const Linear
     let_the_next_launch_start();
     const int block = blockIdx.x / INNER_SPLIT, rank = (int)cluster_rank(), warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int token0 = block * INNER_BLOCK;
+    if (plan && rank == INNER_SPLIT - 1 && blockIdx.y == 0 && token0 % tile == 0) write_plan(a, plan + (int64_t)(token0 / tile) * (tile + 1), tile, token0);
     if (threadIdx.x < INNER_BLOCK) ids[threadIdx.x] = adapter_of(a, token0 + threadIdx.x);
     __syncthreads();
     const int64_t steps = ceil_div(a.n, (int64_t)32), s0 = rank * steps / INNER_SPLIT, s1 = (rank + 1) * steps / INNER_SPLIT;  // 32 columns each; n is a multiple of 32
@@ -166,12 +189,12 @@ __global__ void __launch_bounds__(INNER_THREADS) inner_block_kernel(const Linear
     }
 }
 
-int launch_inner(const LinearArgs &a, cudaStream_t st) {
+int launch_inner(const LinearArgs &a, int *plan, int tile, cudaStream_t st) {
     // Both sides of the line: see the figures above.
-    if (a.tokens <= 64) return launch_dependent(inner_rows_kernel, dim3((unsigned)a.tokens * INNER_SPLIT), INNER_THREADS, 0, INNER_SPLIT, false, st, a);
+    if (a.tokens <= 64) return launch_dependent(inner_rows_kernel, dim3((unsigned)a.tokens * INNER_SPLIT), INNER_THREADS, 0, INNER_SPLIT, false, st, a, plan, tile);
     const unsigned blocks = (unsigned)ceil_div((int64_t)a.tokens, (int64_t)INNER_BLOCK);
     const dim3 grid(blocks * INNER_SPLIT, (unsigned)(a.adapters < 4 ? a.adapters + 1 : 4));
-    return launch_dependent(a.bf16 ? inner_block_kernel<true> : inner_block_kernel<false>, grid, INNER_THREADS, 0, INNER_SPLIT, false, st, a);
+    return launch_dependent(a.bf16 ? inner_block_kernel<true> : inner_block_kernel<false>, grid, INNER_THREADS, 0, INNER_SPLIT, false, st, a, plan, tile);
 }
 
 }  // namespace g2d

@@ -249,8 +249,27 @@ int launch_linear_rows(const LinearArgs &a, cudaStream_t st) {
 
 using namespace g2d;
 
-static size_t linear_bytes(const g2d_linear_desc *d) {
-    return d->rank > 0 ? (((size_t)d->tokens * (INNER_LD * 2 + 4) + 255) & ~(size_t)255) : 0;
+// Up to here the tokens are columns of m16n8k16 products; both sides of the line: see the figures above.
+constexpr int64_t ROWS_TOKENS = 16;
+
+struct LinearSpace {
+    size_t factor, plan, partial, all;  // inner values first
+};
+static LinearSpace linear_space(const g2d_linear_desc *d) {
+    const auto whole = [](size_t bytes) { return (bytes + 255) & ~(size_t)255; };
+    LinearSpace s{};
+    size_t at = 0;
+    const bool many = d->tokens > ROWS_TOKENS;
+    const LinearTcPlan p = many ? linear_tc_plan(d->m, d->n, d->tokens) : LinearTcPlan{};
+    if (d->rank > 0) {
+        s.factor = at += whole((size_t)d->tokens * INNER_LD * 2);
+        s.plan = at += whole((size_t)d->tokens * sizeof(float));
+        if (many) at += whole((size_t)p.token_tiles * (p.tile + 1) * sizeof(int));
+    }
+    s.partial = at;
+    if (many && p.splits > 1) at += whole((size_t)p.splits * d->tokens * d->m * sizeof(float));
+    s.all = at;
+    return s;
 }
 
 static int linear_check(const g2d_linear_desc *d) {
@@ -266,7 +285,7 @@ extern "C" int g2d_linear_workspace_bytes(const g2d_linear_desc *desc, size_t *b
     const int status = linear_check(desc);
     if (status != G2D_OK) return status;
     if (!bytes) return G2D_ERR_BAD_ARGUMENT;
-    *bytes = linear_bytes(desc);
+    *bytes = linear_space(desc).all;
     return G2D_OK;
 }
 
@@ -278,7 +297,8 @@ extern "C" int g2d_packed_linear(const g2d_linear_desc *d, void *stream) {
     if (d->n == 0) return G2D_ERR_UNSUPPORTED;
     if (!d->x || !d->codes || !d->scale || !d->zero || (((uintptr_t)d->x | (uintptr_t)d->codes) & 15) != 0 || d->x_stride % 8 != 0) return G2D_ERR_BAD_ARGUMENT;
     if (d->rank > 0 && (!d->down || !d->up || !d->index || (((uintptr_t)d->down | (uintptr_t)d->up) & 15) != 0)) return G2D_ERR_BAD_ARGUMENT;
-    if (d->rank > 0 && (!d->workspace || d->workspace_bytes < linear_bytes(d) || ((uintptr_t)d->workspace & 255) != 0)) return G2D_ERR_WORKSPACE;
+    const LinearSpace space = linear_space(d);
+    if (space.all > 0 && (!d->workspace || d->workspace_bytes < space.all || ((uintptr_t)d->workspace & 255) != 0)) return G2D_ERR_WORKSPACE;
     LinearArgs a;
     a.x = d->x;
     a.codes = d->codes;
@@ -305,13 +325,16 @@ extern "C" int g2d_packed_linear(const g2d_linear_desc *d, void *stream) {
     a.adapters = d->adapters;
     a.rank = d->adapters > 0 ? d->rank : 0;
     a.inner = (uint16_t *)d->workspace;
-    a.factor = d->rank > 0 ? (float *)((char *)d->workspace + (size_t)d->tokens * INNER_LD * 2) : nullptr;
+    a.factor = d->rank > 0 ? (float *)((char *)d->workspace + space.factor) : nullptr;
     a.status = d->status;
     a.wait_cycles = WAIT_CYCLES;
     cudaStream_t st = (cudaStream_t)stream;
+    const bool many = a.tokens > ROWS_TOKENS;
+    const LinearTcPlan p = many ? linear_tc_plan(a.m, a.n, a.tokens) : LinearTcPlan{};
+    int *const plan = many && a.rank > 0 ? (int *)((char *)d->workspace + space.plan) : nullptr;
     if (a.rank > 0) {
-        const int launched = launch_inner(a, st);
+        const int launched = launch_inner(a, plan, p.tile, st);
         if (launched != G2D_OK) return launched;
     }
-    return launch_linear_rows(a, st);
+    return many ? launch_linear_tc(a, p, plan, (float *)((char *)d->workspace + space.partial), st) : launch_linear_rows(a, st);
 }

@@ -39,11 +39,19 @@ __device__ __forceinline__ int adapter_of(const LinearArgs &a, int token) {
 __device__ __forceinline__ float bits_to_float(uint32_t bits, int bf16) { return bf16 ? __uint_as_float(bits << 16) : __half2float(__ushort_as_half((unsigned short)bits)); }
 __device__ __forceinline__ uint32_t float_to_bits(float v, int bf16) { return bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v)); }
 
-int launch_inner(const LinearArgs &a, cudaStream_t st);        // inner values and factors of all tokens
-int launch_linear_rows(const LinearArgs &a, cudaStream_t st);  // few tokens
+// Many tokens: tiles of 128 rows x `tile` tokens, the columns in `splits` parts.
+struct LinearTcPlan {
+    int tile, row_tiles, token_tiles, splits;
+};
+LinearTcPlan linear_tc_plan(int64_t m, int64_t n, int64_t tokens);
 
-template <typename Kernel>
-inline int launch_dependent(Kernel kernel, dim3 grid, int threads, size_t smem, int cluster, bool dependent, cudaStream_t st, const LinearArgs &a) {
+// Inner values and factors of all tokens; where `plan` is given, also the adapters of each tile of `tile` tokens: plan[i * (tile + 1)] of them, their numbers behind it
+int launch_inner(const LinearArgs &a, int *plan, int tile, cudaStream_t st);
+int launch_linear_rows(const LinearArgs &a, cudaStream_t st);  // few tokens
+int launch_linear_tc(const LinearArgs &a, const LinearTcPlan &p, const int *plan, float *partial, cudaStream_t st);
+
+template <typename... Params, typename... Args>
+inline int launch_dependent(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, int cluster, bool dependent, cudaStream_t st, const Args &...args) {
     cudaLaunchConfig_t config{};
     config.gridDim = grid;
     config.blockDim = dim3((unsigned)threads);
@@ -64,7 +72,7 @@ inline int launch_dependent(Kernel kernel, dim3 grid, int threads, size_t smem, 
     }
     config.attrs = attributes;
     config.numAttrs = count;
-    return cudaLaunchKernelEx(&config, kernel, a) == cudaSuccess ? check_launch() : G2D_ERR_CUDA;
+    return cudaLaunchKernelEx(&config, kernel, Params(args)...) == cudaSuccess ? check_launch() : G2D_ERR_CUDA;
 }
 
 // shared memory of another CTA of the cluster
