@@ -109,9 +109,10 @@ __device__ __forceinline__ void mma_16(float (&d)[4], uint32_t a0, uint32_t a1, 
             : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-template <bool BF16>
-__global__ void __launch_bounds__(INNER_THREADS) inner_block_kernel(const LinearArgs a, int *plan, int tile) {
-    constexpr int WARPS = INNER_THREADS / 32, TILES = RANK_MAX / 8;
+// TILES: of eight inner values each
+template <bool BF16, int TILES>
+__global__ void __launch_bounds__(INNER_THREADS, TILES == 8 ? 1 : 2) inner_block_kernel(const LinearArgs a, int *plan, int tile) {
+    constexpr int WARPS = INNER_THREADS / 32;
     __shared__ float part[WARPS / 2][INNER_BLOCK][RANK_MAX + 2];  // two warps at a time
     __shared__ int ids[INNER_BLOCK];
     __shared__ float tops[4][2];
@@ -136,23 +137,35 @@ __global__ void __launch_bounds__(INNER_THREADS) inner_block_kernel(const Linear
             for (int j = 0; j < TILES; ++j) acc[i][j][0] = acc[i][j][1] = acc[i][j][2] = acc[i][j][3] = 0.f;
         if (id >= 0) {
             const uint16_t *const d = (const uint16_t *)a.down + (int64_t)id * a.rank * a.n;
-            for (int64_t s = s0 + warp; s < s1; s += WARPS) {
-                uint4 xr[4];
+            const uint16_t *const x = (const uint16_t *)a.x + 8 * t;
+            // a step's loads are under way while the one before is multiplied
+            uint4 xr[4], br[TILES];
+            const auto fetch = [&](int64_t s, uint4 (&xv)[4], uint4 (&bv)[TILES]) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int token = token0 + 8 * i + g;
-                    xr[i] = token < a.tokens ? *reinterpret_cast<const uint4 *>((const uint16_t *)a.x + token * a.x_stride + s * 32 + 8 * t) : make_uint4(0u, 0u, 0u, 0u);
+                    xv[i] = s < s1 && token < a.tokens ? __ldg(reinterpret_cast<const uint4 *>(x + token * a.x_stride + s * 32)) : make_uint4(0u, 0u, 0u, 0u);
                 }
+#pragma unroll
+                for (int j = 0; j < TILES; ++j)
+                    bv[j] = s < s1 && 8 * j < a.rank ? __ldg(reinterpret_cast<const uint4 *>(d + (int64_t)(8 * j + g) * a.n + s * 32 + 8 * t)) : make_uint4(0u, 0u, 0u, 0u);
+            };
+            fetch(s0 + warp, xr, br);
+            for (int64_t s = s0 + warp; s < s1; s += WARPS) {
+                uint4 xn[4], bn[TILES];
+                fetch(s + WARPS, xn, bn);
 #pragma unroll
                 for (int j = 0; j < TILES; ++j) {
-                    if (8 * j >= a.rank) break;
-                    const uint4 b = *reinterpret_cast<const uint4 *>(d + (int64_t)(8 * j + g) * a.n + s * 32 + 8 * t);
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        mma_16<BF16>(acc[i][j], xr[2 * i].x, xr[2 * i + 1].x, xr[2 * i].y, xr[2 * i + 1].y, b.x, b.y);
-                        mma_16<BF16>(acc[i][j], xr[2 * i].z, xr[2 * i + 1].z, xr[2 * i].w, xr[2 * i + 1].w, b.z, b.w);
+                        mma_16<BF16>(acc[i][j], xr[2 * i].x, xr[2 * i + 1].x, xr[2 * i].y, xr[2 * i + 1].y, br[j].x, br[j].y);
+                        mma_16<BF16>(acc[i][j], xr[2 * i].z, xr[2 * i + 1].z, xr[2 * i].w, xr[2 * i + 1].w, br[j].z, br[j].w);
                     }
                 }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) xr[i] = xn[i];
+#pragma unroll
+                for (int j = 0; j < TILES; ++j) br[j] = bn[j];
             }
         }
         // the warps' sums, in order: the upper four into shared memory, the lower four add theirs
@@ -171,6 +184,10 @@ __global__ void __launch_bounds__(INNER_THREADS) inner_block_kernel(const Linear
             __syncthreads();
         }
         for (int e = threadIdx.x; e < INNER_BLOCK * RANK_MAX; e += INNER_THREADS) {
+            if (e % RANK_MAX >= 8 * TILES) {
+                part[0][e / RANK_MAX][e % RANK_MAX] = 0.f;
+                continue;
+            }
             float sum = 0.f;
 #pragma unroll
             for (int w = 0; w < WARPS / 2; ++w) sum += part[w][e / RANK_MAX][e % RANK_MAX];
@@ -194,7 +211,10 @@ int launch_inner(const LinearArgs &a, int *plan, int tile, cudaStream_t st) {
     if (a.tokens <= 64) return launch_dependent(inner_rows_kernel, dim3((unsigned)a.tokens * INNER_SPLIT), INNER_THREADS, 0, INNER_SPLIT, false, st, a, plan, tile);
     const unsigned blocks = (unsigned)ceil_div((int64_t)a.tokens, (int64_t)INNER_BLOCK);
     const dim3 grid(blocks * INNER_SPLIT, (unsigned)(a.adapters < 4 ? a.adapters + 1 : 4));
-    return launch_dependent(a.bf16 ? inner_block_kernel<true> : inner_block_kernel<false>, grid, INNER_THREADS, 0, INNER_SPLIT, false, st, a, plan, tile);
+    const auto launch = [&](auto kernel) { return launch_dependent(kernel, grid, INNER_THREADS, 0, INNER_SPLIT, false, st, a, plan, tile); };
+    if (a.rank <= 16) return a.bf16 ? launch(inner_block_kernel<true, 2>) : launch(inner_block_kernel<false, 2>);
+    if (a.rank <= 32) return a.bf16 ? launch(inner_block_kernel<true, 4>) : launch(inner_block_kernel<false, 4>);
+    return a.bf16 ? launch(inner_block_kernel<true, 8>) : launch(inner_block_kernel<false, 8>);
 }
 
 }  // namespace g2d

@@ -39,9 +39,9 @@ __device__ __forceinline__ int adapter_of(const LinearArgs &a, int token) {
 __device__ __forceinline__ float bits_to_float(uint32_t bits, int bf16) { return bf16 ? __uint_as_float(bits << 16) : __half2float(__ushort_as_half((unsigned short)bits)); }
 __device__ __forceinline__ uint32_t float_to_bits(float v, int bf16) { return bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v)); }
 
-// Many tokens: tiles of 128 rows x `tile` tokens, the columns in `splits` parts.
+// Many tokens: tiles of 128 rows (duo: 256, by two CTAs) x `tile` tokens, the columns in `splits` parts.
 struct LinearTcPlan {
-    int tile, row_tiles, token_tiles, splits;
+    int tile, duo, row_tiles, token_tiles, splits;
 };
 LinearTcPlan linear_tc_plan(int64_t m, int64_t n, int64_t tokens);
 
