@@ -14,14 +14,19 @@
 
 namespace g2d {
 
-constexpr int LT_THREADS = 512, LT_CODE_BYTES = 128 * 128, LT_W_BYTES = 128 * 128, LT_SUB = 2, LT_CODE_CHUNKS = 4, LT_SLICE = 8;
+constexpr int LT_CODE_BYTES = 128 * 128, LT_W_BYTES = 128 * 128, LT_SUB = 2, LT_CODE_CHUNKS = 4, LT_SLICE = 8;
 
 // DUO: a pair of CTAs on 256 rows x NT tokens (cta_group::2), each with its rows of W and half of the tokens' rows of x
 template <int NT, bool DUO>
 struct LinearShape {
     static constexpr int X_ROWS = DUO ? NT / 2 : NT, X_BYTES = X_ROWS * KH * 2, STAGE = LT_SUB * (X_BYTES + LT_W_BYTES);  // two chunks of 64 columns
     static constexpr int CODE_STAGES = 2, STAGES = NT == 64 ? 4 : 3;
-    static constexpr int CODERS = NT >= 128 ? 4 : 8, READERS = NT >= 128 ? 8 : 4;  // warps
+    static constexpr int CODERS = 8, READERS = NT >= 128 ? 8 : 4;  // warps; the coders of a team take a stage together
+    static constexpr int TEAMS = NT == 64 ? 2 : 1;                  // that take the stages in turn
+    static constexpr int THREADS = 32 * (4 + TEAMS * CODERS + READERS);
+    // registers of a thread that loads or issues, codes, reads: by warpgroups no more than the launch gives (96 or, of 768 threads, 80 each)
+    static constexpr int ISSUE_REGISTERS = NT == 64 ? 40 : 48, CODE_REGISTERS = NT == 64 ? 72 : 64, READ_REGISTERS = 152;
+    static_assert(4 * ISSUE_REGISTERS + TEAMS * CODERS * CODE_REGISTERS + READERS * READ_REGISTERS <= THREADS / 32 * (NT == 64 ? 80 : 96), "setmaxnreg would wait forever");
     static constexpr int MINE = NT * 4 / READERS;                               // columns of a reading warp
     static constexpr int ACCUMULATORS = 512 / NT;
     static constexpr size_t SMEM = (size_t)STAGES * STAGE + CODE_STAGES * LT_CODE_BYTES + 1024;
@@ -77,18 +82,20 @@ __device__ __forceinline__ uint32_t add2(uint32_t u, uint32_t v) {
     const __half2 r = __hadd2(*reinterpret_cast<__half2 *>(&u), *reinterpret_cast<__half2 *>(&v));
     return *reinterpret_cast<const uint32_t *>(&r);
 }
-// The eight codes of a word, in order, as pairs of code - 8: the bits of a code under the exponent of 1024 (fp16) or 128 (bf16), and that minus 1032 or 136
+// The eight codes of a word, in order, as pairs: the bits of a code under the exponent of 1024 (fp16) or 128 (bf16), plus `add`: -1024 or -128, the origin of
+// the codes and the zero point
 template <bool BF16>
-__device__ __forceinline__ uint4 decoded(uint32_t w) {
-    constexpr uint32_t MAGIC = BF16 ? 0x43004300u : 0x64006400u, LESS = BF16 ? 0xc308c308u : 0xe408e408u;
+__device__ __forceinline__ uint4 decoded(uint32_t w, uint32_t add) {
+    constexpr uint32_t MAGIC = BF16 ? 0x43004300u : 0x64006400u;
     const uint32_t w4 = w >> 4;
     uint4 r;
-    r.x = add2<BF16>((__byte_perm(w, w4, 0x4400) & 0x000f000fu) | MAGIC, LESS);
-    r.y = add2<BF16>((__byte_perm(w, w4, 0x5511) & 0x000f000fu) | MAGIC, LESS);
-    r.z = add2<BF16>((__byte_perm(w, w4, 0x6622) & 0x000f000fu) | MAGIC, LESS);
-    r.w = add2<BF16>((__byte_perm(w, w4, 0x7733) & 0x000f000fu) | MAGIC, LESS);
+    r.x = add2<BF16>((__byte_perm(w, w4, 0x4400) & 0x000f000fu) | MAGIC, add);
+    r.y = add2<BF16>((__byte_perm(w, w4, 0x5511) & 0x000f000fu) | MAGIC, add);
+    r.z = add2<BF16>((__byte_perm(w, w4, 0x6622) & 0x000f000fu) | MAGIC, add);
+    r.w = add2<BF16>((__byte_perm(w, w4, 0x7733) & 0x000f000fu) | MAGIC, add);
     return r;
 }
+__device__ __forceinline__ uint32_t word_of(const uint4 &v, int w) { return (w & 3) == 0 ? v.x : (w & 3) == 1 ? v.y : (w & 3) == 2 ? v.z : v.w; }
 __device__ __forceinline__ void store_16(uint32_t at, const uint4 &v) { asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory"); }
 __device__ __forceinline__ uint4 load_16(uint32_t at) {
     uint4 v;
@@ -99,16 +106,15 @@ __device__ __forceinline__ uint4 load_16(uint32_t at) {
 template <int NT, bool DUO>
 struct LinearBarriers {
     using S = LinearShape<NT, DUO>;
-    uint64_t x_full[S::STAGES], w_full[S::STAGES], empty[S::STAGES], code_full[S::CODE_STAGES], code_empty[S::CODE_STAGES], acc_full[S::ACCUMULATORS], acc_empty[S::ACCUMULATORS], drained;
+    uint64_t x_full[S::STAGES], w_here[S::STAGES], w_full[S::STAGES], empty[S::STAGES], code_full[S::CODE_STAGES], code_empty[S::CODE_STAGES], acc_full[S::ACCUMULATORS], acc_empty[S::ACCUMULATORS], drained;
     uint32_t tmem;
     int failed;
 };
 
 template <bool BF16, int NT, bool DUO>
-__global__ void __launch_bounds__(LT_THREADS, 1) linear_tc_kernel(const __grid_constant__ LinearTcJob job) {
+__global__ void __launch_bounds__(LinearShape<NT, DUO>::THREADS, 1) linear_tc_kernel(const __grid_constant__ LinearTcJob job) {
     using S = LinearShape<NT, DUO>;
     constexpr int CTAS = DUO ? 2 : 1, ACC = S::ACCUMULATORS;
-    constexpr bool HEAVY = S::MINE > 64;  // the readers need more than 128 registers
     extern __shared__ unsigned char linear_tc_smem[];
     __shared__ __align__(8) LinearBarriers<NT, DUO> bar;
     const LinearArgs &a = job.a;
@@ -127,12 +133,13 @@ __global__ void __launch_bounds__(LT_THREADS, 1) linear_tc_kernel(const __grid_c
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::STAGES; ++s) {
             mbar_init(&bar.x_full[s], 1);
-            mbar_init(&bar.w_full[s], CTAS * S::CODERS);
+            mbar_init(&bar.w_here[s], S::CODERS);
+            mbar_init(&bar.w_full[s], CTAS);
             mbar_init(&bar.empty[s], 1);
         }
         for (int s = 0; s < S::CODE_STAGES; ++s) {
             mbar_init(&bar.code_full[s], 1);
-            mbar_init(&bar.code_empty[s], S::CODERS);
+            mbar_init(&bar.code_empty[s], S::TEAMS * S::CODERS);
         }
         for (int s = 0; s < ACC; ++s) {
             mbar_init(&bar.acc_full[s], 1);
@@ -159,10 +166,10 @@ __global__ void __launch_bounds__(LT_THREADS, 1) linear_tc_kernel(const __grid_c
     };
     const auto adapter_at = [&](const LinearItem &it, int j) { return job.plan[(int64_t)it.token_tile * (NT + 1) + 1 + j]; };
     const auto item = [&](int number, LinearItem &it) { return linear_item<NT, DUO>(job, rank, number, it); };
-    const int first_coder = 4, first_reader = 4 + S::CODERS;
+    const int first_coder = 4, first_reader = 4 + S::TEAMS * S::CODERS;
 
     if (warp < 4) {
-        if (HEAVY) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::ISSUE_REGISTERS));
         if (warp == 0 && lane == 0) {  // x
             LinearItem it;
             int c = 0;
@@ -219,46 +226,78 @@ __global__ void __launch_bounds__(LT_THREADS, 1) linear_tc_kernel(const __grid_c
                 }
             }
             for (int k = max(c - S::CODE_STAGES, 0); k < c; ++k) mbar_wait(&bar.code_full[k % S::CODE_STAGES], (k / S::CODE_STAGES) & 1);
-        } else if (warp == 1 && lane == 0 && rank == 0) {  // products
-            constexpr uint32_t DESC = idesc_16(NT, BF16 ? 1 : 0, DUO ? 2 * MT : MT);
+        } else if (DUO && warp == 3 && lane == 0) {
+            // A warp that arrives at another CTA's barrier waits until all it wrote has arrived too (900 cycles): the warps that write arrive here, and this one passes it on
             LinearItem it;
-            int c = 0, slice = 0;
+            int c = 0;
+            bool go = true;
+            for (int i = 0; go && item(i, it); ++i) {
+                const int stages = (it.c1 - it.c0 + LT_SUB - 1) / LT_SUB + adapters_in(it);
+                for (int k = 0; go && k < stages; ++k, ++c) {
+                    go = !bar.failed && wait(&bar.w_here[c % S::STAGES], (c / S::STAGES) & 1, 20);
+                    if (go) mbar_arrive_at(leaders(&bar.w_full[c % S::STAGES]));
+                }
+            }
+        } else if (warp == 1 && lane == 0 && rank == 0) {  // products
+            // One thread issues them all: what it does per product (128 cycles for a pair of CTAs, 32 for narrow tiles) is kept short
+            constexpr uint32_t DESC = idesc_16(NT, BF16 ? 1 : 0, DUO ? 2 * MT : MT);
+            const uint64_t ws = umma_desc(base + LT_SUB * S::X_BYTES), xs = umma_desc(base);
+            LinearItem it;
+            int stage = 0, slice = 0;
+            uint32_t parity = 0;
             const auto ready = [&] {
-                const int stage = c % S::STAGES, round = c / S::STAGES;
-                if (bar.failed || !wait(&bar.w_full[stage], round & 1, 20) || !wait(&bar.x_full[stage], round & 1, 20)) return false;
+                if (bar.failed || !wait(DUO ? &bar.w_full[stage] : &bar.w_here[stage], parity, 20) || !wait(&bar.x_full[stage], parity, 20)) return false;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 return true;
             };
-            const auto product = [&](int w, int x, bool opens, bool closes, int steps) {  // chunks w and x of the stage
-                const int buf = slice % ACC;
-                if (opens && slice >= ACC) {
-                    if (!wait(&bar.acc_empty[buf], (slice / ACC - 1) & 1, 20)) return false;
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                }
-                const uint32_t d = tmem + (uint32_t)(buf * NT), at = base + (c % S::STAGES) * S::STAGE, xs = at + x * S::X_BYTES, ws = at + LT_SUB * S::X_BYTES + w * LT_W_BYTES;
-                for (int ks = 0; ks < steps; ++ks) mma<DUO>(d, ws + ks * 32, xs + ks * 32, DESC, (opens && ks == 0) ? 0u : 1u);
-                if (closes) {
-                    commit<DUO>(&bar.acc_full[buf]);
-                    ++slice;
-                }
+            const auto open = [&] {
+                if (slice < ACC) return true;
+                if (!wait(&bar.acc_empty[slice % ACC], (slice / ACC - 1) & 1, 20)) return false;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 return true;
+            };
+            const auto issue = [&](uint64_t w, uint64_t x, uint32_t accumulate) {
+                const uint32_t d = tmem + (uint32_t)((slice % ACC) * NT);
+                if (DUO) umma_16_duo(d, w, x, DESC, accumulate);
+                else umma_16(d, w, x, DESC, accumulate);
+            };
+            const auto done = [&] {
+                commit<DUO>(&bar.empty[stage]);
+                if (++stage == S::STAGES) stage = 0, parity ^= 1;
             };
             bool go = true;
             for (int i = 0; go && item(i, it); ++i) {
                 bool opens = true;
+                int in_group = it.c0 % job.group_chunks;
                 for (int ch = it.c0; go && ch < it.c1; ch += LT_SUB) {
                     go = ready();
-                    for (int s = 0; go && s < LT_SUB; ++s) {
-                        const bool closes = slice_ends(job, ch + s, it.c1 - 1);
-                        go = product(s, s, opens, closes, KH / 16);
-                        opens = closes;
+                    const uint64_t w0 = ws + (uint64_t)((uint32_t)(stage * S::STAGE) >> 4), x0 = xs + (uint64_t)((uint32_t)(stage * S::STAGE) >> 4);
+#pragma unroll
+                    for (int s = 0; s < LT_SUB; ++s) {
+                        if (opens) go = go && open();
+                        if (!go) break;
+                        const uint64_t w = w0 + (uint64_t)(s * (LT_W_BYTES >> 4)), x = x0 + (uint64_t)(s * (S::X_BYTES >> 4));
+                        issue(w, x, opens ? 0u : 1u);
+#pragma unroll
+                        for (int ks = 1; ks < KH / 16; ++ks) issue(w + 2 * ks, x + 2 * ks, 1u);
+                        const bool group_ends = in_group == job.group_chunks - 1;
+                        opens = group_ends || (in_group & (LT_SLICE - 1)) == LT_SLICE - 1 || ch + s == it.c1 - 1;  // as slice_ends has it
+                        in_group = group_ends ? 0 : in_group + 1;
+                        if (opens) commit<DUO>(&bar.acc_full[slice++ % ACC]);
                     }
-                    commit<DUO>(&bar.empty[c++ % S::STAGES]);
+                    done();
                 }
                 const int extra = go ? adapters_in(it) : 0;
-                for (int e = 0; go && e < extra; ++e) {
-                    go = ready() && product(0, 0, true, false, (a.rank + 15) / 16) && product(0, 1, false, true, (a.rank + 15) / 16);
-                    commit<DUO>(&bar.empty[c++ % S::STAGES]);
+                for (int e = 0; go && e < extra; ++e) {  // the rows of `up` against both parts of the inner values
+                    go = ready() && open();
+                    if (!go) break;
+                    const uint64_t w0 = ws + (uint64_t)((uint32_t)(stage * S::STAGE) >> 4), x0 = xs + (uint64_t)((uint32_t)(stage * S::STAGE) >> 4);
+                    for (int ks = 0; 16 * ks < a.rank; ++ks) {
+                        issue(w0 + 2 * ks, x0 + 2 * ks, ks > 0);
+                        issue(w0 + 2 * ks, x0 + (S::X_BYTES >> 4) + 2 * ks, 1u);
+                    }
+                    commit<DUO>(&bar.acc_full[slice++ % ACC]);
+                    done();
                 }
             }
             if (bar.failed) {  // every product that was issued completes, or has its time to, before what it reads and writes is given back
@@ -270,70 +309,85 @@ __global__ void __launch_bounds__(LT_THREADS, 1) linear_tc_kernel(const __grid_c
         }
         __syncwarp();
     } else if (warp < first_reader) {
-        if (HEAVY) asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::CODE_REGISTERS));
         // ---- operands: a thread has a row and, with four warps, both chunks of a stage, else one ----
-        constexpr int EACH = LT_SUB * 4 / S::CODERS;  // chunks
-        const int id = threadIdx.x - 32 * first_coder, row = id & 127, first = (id >> 7) * EACH;
+        const int team = (warp - first_coder) / S::CODERS, id = threadIdx.x - 32 * (first_coder + team * S::CODERS), row = id & 127, first = id >> 7;  // one chunk of the stage
         LinearItem it;
-        int c = 0, cc = 0;
-        bool go = true;
+        int stage = 0, turn = 0, code_stage = 0;
+        uint32_t parity = 1, code_parity = 0;  // of the stage's last release (the first time round there is none to wait for)
+        bool go = true, again = false;
+        const auto advance = [&] {
+            if (++stage == S::STAGES) stage = 0, parity ^= 1, again = true;
+            if (++turn == S::TEAMS) turn = 0;
+        };
         const auto free_stage = [&] {
-            const int stage = c % S::STAGES, round = c / S::STAGES;
-            if (round > 0) go = go && wait(&bar.empty[stage], (round - 1) & 1, 20);
+            if (again) go = go && wait(&bar.empty[stage], parity, 20);
             go = __all_sync(0xffffffffu, go && !bar.failed);
             return go;
         };
+        constexpr float ORIGIN = BF16 ? 128.f : 1024.f;
         for (int i = 0; go && item(i, it); ++i) {
             const float *const zero = a.zero + min((int64_t)it.row0 + row, a.m - 1) * a.zero_row;
-            const auto shift_of = [&](int ch) { return 8.f + a.qmin - __ldg(zero + (int64_t)(min(ch, job.chunks - 1) / job.group_chunks) * a.zero_group); };
-            float next_shift = shift_of(it.c0 + first);
-            int group_end = -1;  // first chunk past the group whose shift is at hand
-            uint32_t shift = 0u;
-            bool shifted = false;
-            for (int ch = it.c0; ch < it.c1; ch += LT_SUB, ++c) {
-                const int code_stage = cc % S::CODE_STAGES;
-                if (ch % LT_CODE_CHUNKS == 0) go = wait(&bar.code_full[code_stage], (cc / S::CODE_STAGES) & 1, 20);
-                uint4 raw[EACH][2];
-                const uint32_t from = codes_base + code_stage * LT_CODE_BYTES + row * 128;
-#pragma unroll
-                for (int s = 0; s < EACH; ++s)
-#pragma unroll
-                    for (int w = 0; w < 2; ++w) raw[s][w] = load_16(from + ((((ch % LT_CODE_CHUNKS + first + s) * 2 + w) ^ (row & 7)) << 4));
-                if (!free_stage()) break;
-                const uint32_t to = base + (c % S::STAGES) * S::STAGE + LT_SUB * S::X_BYTES + row * 128;
-#pragma unroll
-                for (int s = 0; s < EACH; ++s) {
-                    if (ch + first + s >= group_end) {
-                        const uint32_t bits = float_to_bits(next_shift, BF16);
-                        shift = bits | (bits << 16);
-                        shifted = __any_sync(0xffffffffu, next_shift != 0.f);
-                        group_end = ((ch + first + s) / job.group_chunks + 1) * job.group_chunks;
-                        next_shift = shift_of(S::CODERS == 8 && job.group_chunks == 1 ? group_end + 1 : group_end);  // one of two chunks: every other group
+            const int groups = (job.chunks - 1) / job.group_chunks + 1;
+            // the zero point of the next group that this thread meets is on its way
+            int group = -1, group_end = -1;
+            const auto zero_of = [&](int g) { return __ldg(zero + (int64_t)min(g, groups - 1) * a.zero_group); };
+            float next_zero = 0.f;
+            int next_group = -2;
+            uint32_t once = 0u, shift = 0u;
+            bool exact = true;
+            for (int ch = it.c0; ch < it.c1; ch += LT_SUB) {
+                const int quarter = ch % LT_CODE_CHUNKS;
+                // by all teams, theirs or not: a wait that left out a phase could take the one before for it
+                if (quarter == 0 && !wait(&bar.code_full[code_stage], code_parity, 20)) go = false;
+                if (turn == team) {
+                    if (ch + first >= group_end) {  // another group
+                        group = (ch + first) / job.group_chunks;
+                        group_end = (group + 1) * job.group_chunks;
+                        const float by = a.qmin - (group == next_group ? next_zero : zero_of(group));
+                        next_group = (max(group_end, ch + first + LT_SUB * S::TEAMS)) / job.group_chunks;
+                        next_zero = zero_of(next_group);
+                        // one addition where -1024 + qmin - zero is a number of the type (integers up to 2048; bf16: -128, 256), else two, the first exact
+                        const uint32_t whole = float_to_bits(by - ORIGIN, BF16), apart = float_to_bits(by + 8.f, BF16);
+                        exact = __all_sync(0xffffffffu, bits_to_float(whole, BF16) == by - ORIGIN);
+                        once = exact ? whole | (whole << 16) : (BF16 ? 0xc308c308u : 0xe408e408u);
+                        shift = apart | (apart << 16);
                     }
+                    const uint32_t from = codes_base + code_stage * LT_CODE_BYTES + row * 128;
+                    const uint4 raw[2] = {load_16(from + ((((quarter + first) * 2) ^ (row & 7)) << 4)), load_16(from + ((((quarter + first) * 2 + 1) ^ (row & 7)) << 4))};
+                    if (!free_stage()) break;  // for the whole warp
+                    const uint32_t to = base + stage * S::STAGE + LT_SUB * S::X_BYTES + first * LT_W_BYTES + row * 128;
+                    if (exact) {
 #pragma unroll
-                    for (int w = 0; w < 8; ++w) {
-                        const uint4 &r = raw[s][w >> 2];
-                        uint4 v = decoded<BF16>((w & 3) == 0 ? r.x : (w & 3) == 1 ? r.y : (w & 3) == 2 ? r.z : r.w);
-                        if (shifted) v = make_uint4(add2<BF16>(v.x, shift), add2<BF16>(v.y, shift), add2<BF16>(v.z, shift), add2<BF16>(v.w, shift));
-                        store_16(to + (first + s) * LT_W_BYTES + ((w ^ (row & 7)) << 4), v);
+                        for (int w = 0; w < 8; ++w) store_16(to + ((w ^ (row & 7)) << 4), decoded<BF16>(word_of(raw[w >> 2], w), once));
+                    } else {
+#pragma unroll
+                        for (int w = 0; w < 8; ++w) {
+                            const uint4 v = decoded<BF16>(word_of(raw[w >> 2], w), once);
+                            store_16(to + ((w ^ (row & 7)) << 4), make_uint4(add2<BF16>(v.x, shift), add2<BF16>(v.y, shift), add2<BF16>(v.z, shift), add2<BF16>(v.w, shift)));
+                        }
                     }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&bar.w_here[stage]);
                 }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) arrive(&bar.w_full[c % S::STAGES]);
-                if (ch % LT_CODE_CHUNKS + LT_SUB >= LT_CODE_CHUNKS || ch + LT_SUB >= it.c1) {
+                advance();
+                if (quarter + LT_SUB >= LT_CODE_CHUNKS || ch + LT_SUB >= it.c1) {
                     if (lane == 0) mbar_arrive(&bar.code_empty[code_stage]);  // behind the warp's barrier: all lanes have read
-                    ++cc;
+                    if (++code_stage == S::CODE_STAGES) code_stage = 0, code_parity ^= 1;
                 }
             }
             const int extra = go ? adapters_in(it) : 0;
-            for (int e = 0; go && e < extra; ++e, ++c) {  // rows of `up`, which the TMA brings: the stage is free for them
-                if (!free_stage()) break;
-                if (lane == 0) arrive(&bar.w_full[c % S::STAGES]);
+            for (int e = 0; go && e < extra; ++e) {  // rows of `up`, which the TMA brings: the stage is free for them
+                if (turn == team) {
+                    if (!free_stage()) break;
+                    if (lane == 0) mbar_arrive(&bar.w_here[stage]);
+                }
+                advance();
             }
         }
     } else {
-        if (HEAVY) asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::READ_REGISTERS));
         // ---- results: a thread has a row and MINE tokens ----
         constexpr int MINE = S::MINE;
         const int q = warp & 3, t0 = ((warp - first_reader) >> 2) * MINE;
@@ -360,9 +414,10 @@ __global__ void __launch_bounds__(LT_THREADS, 1) linear_tc_kernel(const __grid_c
             };
             const uint32_t from = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)t0;
             const auto factor_of = [&](int ch) { return __ldg(scale + (int64_t)(min(ch, job.chunks - 1) / job.group_chunks) * a.scale_group); };
+            float factor = factor_of(it.c0);
             for (int ch = it.c0; go && ch < it.c1; ++ch) {
                 if (!slice_ends(job, ch, it.c1 - 1)) continue;
-                const float factor = factor_of(ch);
+                const float next_factor = factor_of(ch + 1);  // under way while the slice is awaited and read
                 if (!arrived()) break;
 #pragma unroll
                 for (int cb = 0; cb < MINE / 16; ++cb) {
@@ -372,6 +427,7 @@ __global__ void __launch_bounds__(LT_THREADS, 1) linear_tc_kernel(const __grid_c
                     for (int x = 0; x < 16; ++x) total[cb * 16 + x] = fmaf(__uint_as_float(v[x]), factor, total[cb * 16 + x]);
                 }
                 leave();
+                factor = next_factor;
             }
             const int extra = go ? adapters_in(it) : 0;
             for (int e = 0; go && e < extra; ++e) {
@@ -501,7 +557,7 @@ static int launch_tc(const LinearArgs &a, const LinearTcPlan &p, const int *plan
     if (a.rank == 0) job.inner = job.up = job.x;
     const int64_t items = (int64_t)p.row_tiles * p.token_tiles * p.splits;
     const unsigned grid = DUO ? 2 * (unsigned)(items < 74 ? items : 74) : (unsigned)(items < 148 ? items : 148);
-    const int launched = launch_dependent(linear_tc_kernel<BF16, NT, DUO>, dim3(grid), LT_THREADS, S::SMEM, DUO ? 2 : 1, a.rank > 0, st, job);
+    const int launched = launch_dependent(linear_tc_kernel<BF16, NT, DUO>, dim3(grid), S::THREADS, S::SMEM, DUO ? 2 : 1, a.rank > 0, st, job);
     if (launched != G2D_OK || p.splits == 1) return launched;
     const int64_t blocks = ceil_div((int64_t)a.tokens * a.m, (int64_t)256);
     linear_join_kernel<<<(unsigned)(blocks < 148 * 8 ? blocks : 148 * 8), 256, 0, st>>>(a, partial, p.splits);
