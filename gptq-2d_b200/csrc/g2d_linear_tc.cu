@@ -103,6 +103,18 @@ __device__ __forceinline__ uint4 load_16(uint32_t at) {
     return v;
 }
 
+// One thread of the warp, all of whose threads are here.  The compiler knows that a branch on this leaves one thread, and keeps what a product's instruction takes
+// from uniform registers there; behind a comparison of lane numbers it does not.
+__device__ __forceinline__ bool elected() {
+    uint32_t one;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(one));
+    return one != 0;
+}
+
 template <int NT, bool DUO>
 struct LinearBarriers {
     using S = LinearShape<NT, DUO>;
@@ -238,7 +250,7 @@ __global__ void __launch_bounds__(LinearShape<NT, DUO>::THREADS, 1) linear_tc_ke
                     if (go) mbar_arrive_at(leaders(&bar.w_full[c % S::STAGES]));
                 }
             }
-        } else if (warp == 1 && lane == 0 && rank == 0) {  // products
+        } else if (warp == 1 && rank == 0 && elected()) {  // products
             // One thread issues them all: what it does per product (128 cycles for a pair of CTAs, 32 for narrow tiles) is kept short
             constexpr uint32_t DESC = idesc_16(NT, BF16 ? 1 : 0, DUO ? 2 * MT : MT);
             const uint64_t ws = umma_desc(base + LT_SUB * S::X_BYTES), xs = umma_desc(base);
