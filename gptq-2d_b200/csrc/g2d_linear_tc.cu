@@ -21,8 +21,8 @@ template <int NT, bool DUO>
 struct LinearShape {
     static constexpr int X_ROWS = DUO ? NT / 2 : NT, X_BYTES = X_ROWS * KH * 2, STAGE = LT_SUB * (X_BYTES + LT_W_BYTES);  // two chunks of 64 columns
     static constexpr int CODE_STAGES = 2, STAGES = NT == 64 ? 4 : 3;
-    static constexpr int CODERS = 8, READERS = NT >= 128 ? 8 : 4;  // warps; the coders of a team take a stage together
-    static constexpr int TEAMS = NT == 64 ? 2 : 1;                  // that take the stages in turn
+    static constexpr int CODERS = 4, READERS = NT >= 128 ? 8 : 4;  // warps; the coders of a team take a stage together, a row per thread
+    static constexpr int TEAMS = NT == 64 ? 4 : 2;                  // that take the stages in turn: one waits and fences while another works
     static constexpr int THREADS = 32 * (4 + TEAMS * CODERS + READERS);
     // registers of a thread that loads or issues, codes, reads: by warpgroups no more than the launch gives (96 or, of 768 threads, 80 each)
     static constexpr int ISSUE_REGISTERS = NT == 64 ? 40 : 48, CODE_REGISTERS = NT == 64 ? 72 : 64, READ_REGISTERS = 152;
@@ -115,6 +115,8 @@ __device__ __forceinline__ bool elected() {
     return one != 0;
 }
 
+__device__ __forceinline__ void arrive_relaxed(uint32_t bar) { asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
+
 template <int NT, bool DUO>
 struct LinearBarriers {
     using S = LinearShape<NT, DUO>;
@@ -132,9 +134,8 @@ __global__ void __launch_bounds__(LinearShape<NT, DUO>::THREADS, 1) linear_tc_ke
     const LinearArgs &a = job.a;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = DUO ? (int)cluster_rank() : 0;
     const uint32_t base = (smem_u32(linear_tc_smem) + 1023u) & ~1023u, codes_base = base + S::STAGES * S::STAGE;
-    const auto await = [](uint64_t *b, uint32_t parity, unsigned nap, long long cycles) { return DUO ? mbar_wait_cluster(b, parity, nap, cycles) : mbar_wait(b, parity, nap, cycles); };
     const auto wait = [&](uint64_t *b, uint32_t parity, unsigned nap) {
-        if (await(b, parity, nap, a.wait_cycles)) return true;
+        if (mbar_wait(b, parity, nap, a.wait_cycles)) return true;
         bar.failed = 1;
         return false;
     };
@@ -221,7 +222,7 @@ __global__ void __launch_bounds__(LinearShape<NT, DUO>::THREADS, 1) linear_tc_ke
             }
             // landed, or had their time to, before the memory is given back
             if (rank == 0)
-                for (int k = max(c - S::STAGES, 0); k < c; ++k) await(&bar.x_full[k % S::STAGES], (k / S::STAGES) & 1, 32, WAIT_CYCLES);
+                for (int k = max(c - S::STAGES, 0); k < c; ++k) mbar_wait(&bar.x_full[k % S::STAGES], (k / S::STAGES) & 1);
             if (DUO && !bar.failed) {  // the leader's commits arrive here as well: none may be under way when this CTA ends
                 for (int k = max(c - S::STAGES, 0); k < c; ++k) wait(&bar.empty[k % S::STAGES], (k / S::STAGES) & 1, 32);
             }
@@ -239,7 +240,9 @@ __global__ void __launch_bounds__(LinearShape<NT, DUO>::THREADS, 1) linear_tc_ke
             }
             for (int k = max(c - S::CODE_STAGES, 0); k < c; ++k) mbar_wait(&bar.code_full[k % S::CODE_STAGES], (k / S::CODE_STAGES) & 1);
         } else if (DUO && warp == 3 && lane == 0) {
-            // A warp that arrives at another CTA's barrier waits until all it wrote has arrived too (900 cycles): the warps that write arrive here, and this one passes it on
+            // The coders arrive at this CTA's barrier; this thread passes it on to the leader's.  What they wrote stays in this CTA's shared memory and is read by this
+            // SM's tensor core alone: they have brought it there by their proxy fence before they arrive, so that the message itself need order nothing (with
+            // .release it takes a thousand cycles of this chain: 8192 x 28672, 2048 tokens, 940 and 885 us).
             LinearItem it;
             int c = 0;
             bool go = true;
@@ -247,7 +250,7 @@ __global__ void __launch_bounds__(LinearShape<NT, DUO>::THREADS, 1) linear_tc_ke
                 const int stages = (it.c1 - it.c0 + LT_SUB - 1) / LT_SUB + adapters_in(it);
                 for (int k = 0; go && k < stages; ++k, ++c) {
                     go = !bar.failed && wait(&bar.w_here[c % S::STAGES], (c / S::STAGES) & 1, 20);
-                    if (go) mbar_arrive_at(leaders(&bar.w_full[c % S::STAGES]));
+                    if (go) arrive_relaxed(leaders(&bar.w_full[c % S::STAGES]));
                 }
             }
         } else if (warp == 1 && rank == 0 && elected()) {  // products
@@ -314,35 +317,39 @@ __global__ void __launch_bounds__(LinearShape<NT, DUO>::THREADS, 1) linear_tc_ke
             }
             if (bar.failed) {  // every product that was issued completes, or has its time to, before what it reads and writes is given back
                 commit<DUO>(&bar.drained);
-                await(&bar.drained, 0, 32, WAIT_CYCLES);
+                mbar_wait(&bar.drained, 0);
             } else {
-                for (int k = max(slice - ACC, 0); k < slice; ++k) await(&bar.acc_full[k % ACC], (k / ACC) & 1, 32, WAIT_CYCLES);
+                for (int k = max(slice - ACC, 0); k < slice; ++k) mbar_wait(&bar.acc_full[k % ACC], (k / ACC) & 1);
             }
         }
         __syncwarp();
     } else if (warp < first_reader) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::CODE_REGISTERS));
         // ---- operands: a thread has a row and, with four warps, both chunks of a stage, else one ----
-        const int team = (warp - first_coder) / S::CODERS, id = threadIdx.x - 32 * (first_coder + team * S::CODERS), row = id & 127, first = id >> 7;  // one chunk of the stage
+        const int team = (warp - first_coder) / S::CODERS, id = threadIdx.x - 32 * (first_coder + team * S::CODERS), row = id;
         LinearItem it;
         int stage = 0, turn = 0, code_stage = 0;
         uint32_t parity = 1, code_parity = 0;  // of the stage's last release (the first time round there is none to wait for)
         bool go = true, again = false;
-        const auto advance = [&] {
-            if (++stage == S::STAGES) stage = 0, parity ^= 1, again = true;
-            if (++turn == S::TEAMS) turn = 0;
-        };
+        const auto released = [&] { return !again || wait(&bar.empty[stage], parity, 20); };
         const auto free_stage = [&] {
-            if (again) go = go && wait(&bar.empty[stage], parity, 20);
+            go = go && released();
             go = __all_sync(0xffffffffu, go && !bar.failed);
             return go;
+        };
+        const auto advance = [&](bool mine) {
+            // Where a team does not come back to the same stages, it awaits the other turns' releases too (they come before its own): a wait that left out a
+            // phase could take the one before for it.
+            if (!mine && S::STAGES % S::TEAMS != 0) go = go && released();
+            if (++stage == S::STAGES) stage = 0, parity ^= 1, again = true;
+            if (++turn == S::TEAMS) turn = 0;
         };
         constexpr float ORIGIN = BF16 ? 128.f : 1024.f;
         for (int i = 0; go && item(i, it); ++i) {
             const float *const zero = a.zero + min((int64_t)it.row0 + row, a.m - 1) * a.zero_row;
             const int groups = (job.chunks - 1) / job.group_chunks + 1;
             // the zero point of the next group that this thread meets is on its way
-            int group = -1, group_end = -1;
+            int group_end = -1;
             const auto zero_of = [&](int g) { return __ldg(zero + (int64_t)min(g, groups - 1) * a.zero_group); };
             float next_zero = 0.f;
             int next_group = -2;
@@ -350,40 +357,45 @@ __global__ void __launch_bounds__(LinearShape<NT, DUO>::THREADS, 1) linear_tc_ke
             bool exact = true;
             for (int ch = it.c0; ch < it.c1; ch += LT_SUB) {
                 const int quarter = ch % LT_CODE_CHUNKS;
-                // by all teams, theirs or not: a wait that left out a phase could take the one before for it
+                // by all teams, theirs or not, as for the releases
                 if (quarter == 0 && !wait(&bar.code_full[code_stage], code_parity, 20)) go = false;
                 if (turn == team) {
-                    if (ch + first >= group_end) {  // another group
-                        group = (ch + first) / job.group_chunks;
-                        group_end = (group + 1) * job.group_chunks;
-                        const float by = a.qmin - (group == next_group ? next_zero : zero_of(group));
-                        next_group = (max(group_end, ch + first + LT_SUB * S::TEAMS)) / job.group_chunks;
-                        next_zero = zero_of(next_group);
-                        // one addition where -1024 + qmin - zero is a number of the type (integers up to 2048; bf16: -128, 256), else two, the first exact
-                        const uint32_t whole = float_to_bits(by - ORIGIN, BF16), apart = float_to_bits(by + 8.f, BF16);
-                        exact = __all_sync(0xffffffffu, bits_to_float(whole, BF16) == by - ORIGIN);
-                        once = exact ? whole | (whole << 16) : (BF16 ? 0xc308c308u : 0xe408e408u);
-                        shift = apart | (apart << 16);
-                    }
                     const uint32_t from = codes_base + code_stage * LT_CODE_BYTES + row * 128;
-                    const uint4 raw[2] = {load_16(from + ((((quarter + first) * 2) ^ (row & 7)) << 4)), load_16(from + ((((quarter + first) * 2 + 1) ^ (row & 7)) << 4))};
+                    uint4 raw[2 * LT_SUB];
+#pragma unroll
+                    for (int w = 0; w < 2 * LT_SUB; ++w) raw[w] = load_16(from + (((quarter * 2 + w) ^ (row & 7)) << 4));
                     if (!free_stage()) break;  // for the whole warp
-                    const uint32_t to = base + stage * S::STAGE + LT_SUB * S::X_BYTES + first * LT_W_BYTES + row * 128;
-                    if (exact) {
 #pragma unroll
-                        for (int w = 0; w < 8; ++w) store_16(to + ((w ^ (row & 7)) << 4), decoded<BF16>(word_of(raw[w >> 2], w), once));
-                    } else {
+                    for (int s = 0; s < LT_SUB; ++s) {
+                        if (ch + s >= group_end) {  // another group
+                            const int group = (ch + s) / job.group_chunks;
+                            group_end = (group + 1) * job.group_chunks;
+                            const float by = a.qmin - (group == next_group ? next_zero : zero_of(group));
+                            next_group = (group_end > ch + LT_SUB - 1 ? max(group_end, ch + LT_SUB * S::TEAMS) : group_end) / job.group_chunks;
+                            next_zero = zero_of(next_group);
+                            // one addition where -1024 + qmin - zero is a number of the type (integers up to 2048; bf16: -128, 256), else two, the first exact
+                            const uint32_t whole = float_to_bits(by - ORIGIN, BF16), apart = float_to_bits(by + 8.f, BF16);
+                            exact = __all_sync(0xffffffffu, bits_to_float(whole, BF16) == by - ORIGIN);
+                            once = exact ? whole | (whole << 16) : (BF16 ? 0xc308c308u : 0xe408e408u);
+                            shift = apart | (apart << 16);
+                        }
+                        const uint32_t to = base + stage * S::STAGE + LT_SUB * S::X_BYTES + s * LT_W_BYTES + row * 128;
+                        if (exact) {
 #pragma unroll
-                        for (int w = 0; w < 8; ++w) {
-                            const uint4 v = decoded<BF16>(word_of(raw[w >> 2], w), once);
-                            store_16(to + ((w ^ (row & 7)) << 4), make_uint4(add2<BF16>(v.x, shift), add2<BF16>(v.y, shift), add2<BF16>(v.z, shift), add2<BF16>(v.w, shift)));
+                            for (int w = 0; w < 8; ++w) store_16(to + ((w ^ (row & 7)) << 4), decoded<BF16>(word_of(raw[2 * s + (w >> 2)], w), once));
+                        } else {
+#pragma unroll
+                            for (int w = 0; w < 8; ++w) {
+                                const uint4 v = decoded<BF16>(word_of(raw[2 * s + (w >> 2)], w), once);
+                                store_16(to + ((w ^ (row & 7)) << 4), make_uint4(add2<BF16>(v.x, shift), add2<BF16>(v.y, shift), add2<BF16>(v.z, shift), add2<BF16>(v.w, shift)));
+                            }
                         }
                     }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&bar.w_here[stage]);
                 }
-                advance();
+                advance(turn == team);
                 if (quarter + LT_SUB >= LT_CODE_CHUNKS || ch + LT_SUB >= it.c1) {
                     if (lane == 0) mbar_arrive(&bar.code_empty[code_stage]);  // behind the warp's barrier: all lanes have read
                     if (++code_stage == S::CODE_STAGES) code_stage = 0, code_parity ^= 1;
@@ -395,7 +407,7 @@ __global__ void __launch_bounds__(LinearShape<NT, DUO>::THREADS, 1) linear_tc_ke
                     if (!free_stage()) break;
                     if (lane == 0) mbar_arrive(&bar.w_here[stage]);
                 }
-                advance();
+                advance(turn == team);
             }
         }
     } else {
