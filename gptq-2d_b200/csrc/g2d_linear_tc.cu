@@ -14,28 +14,30 @@
 
 namespace g2d {
 
-constexpr int LT_CODE_BYTES = 128 * 128, LT_W_BYTES = 128 * 128, LT_SUB = 2, LT_CODE_CHUNKS = 4, LT_SLICE = 8;
+constexpr int LT_W_BYTES = 128 * 128, LT_CODE_BYTES = 128 * 32, LT_SLICE = 8;
 
-// DUO: a pair of CTAs on 256 rows x NT tokens (cta_group::2), each with its rows of W and half of the tokens' rows of x
+// DUO: a pair of CTAs on 256 rows x NT tokens (cta_group::2), each with its rows of W and half of the tokens' rows of x.
+// A slot holds one chunk of 64 columns: x, W as 16-bit values, and the codes of the chunk that its W will be next.
 template <int NT, bool DUO>
 struct LinearShape {
-    static constexpr int X_ROWS = DUO ? NT / 2 : NT, X_BYTES = X_ROWS * KH * 2, STAGE = LT_SUB * (X_BYTES + LT_W_BYTES);  // two chunks of 64 columns
-    static constexpr int CODE_STAGES = 2, STAGES = NT == 64 ? 4 : 3;
-    static constexpr int CODERS = 4, READERS = NT >= 128 ? 8 : 4;  // warps; the coders of a team take a stage together, a row per thread
-    static constexpr int TEAMS = NT == 64 ? 4 : 2;                  // that take the stages in turn: one waits and fences while another works
-    static constexpr int THREADS = 32 * (4 + TEAMS * CODERS + READERS);
-    // registers of a thread that loads or issues, codes, reads: by warpgroups no more than the launch gives (96 or, of 768 threads, 80 each)
-    static constexpr int ISSUE_REGISTERS = NT == 64 ? 40 : 48, CODE_REGISTERS = NT == 64 ? 72 : 64, READ_REGISTERS = 152;
-    static_assert(4 * ISSUE_REGISTERS + TEAMS * CODERS * CODE_REGISTERS + READERS * READ_REGISTERS <= THREADS / 32 * (NT == 64 ? 80 : 96), "setmaxnreg would wait forever");
-    static constexpr int MINE = NT * 4 / READERS;                               // columns of a reading warp
+    static constexpr int X_ROWS = DUO ? NT / 2 : NT, X_BYTES = X_ROWS * KH * 2, SLOT = X_BYTES + LT_W_BYTES;
+    static constexpr int SLOTS = NT == 64 ? 8 : 6;
+    // Two warps per slot turn codes into values, a thread two rows: everything that they wait for comes in the order of their own turns, and while those of one slot wait,
+    // load or fence, those of the others work.
+    static constexpr int TEAM = 2, CODERS = TEAM * SLOTS, READERS = NT >= 128 ? 8 : 4;  // warps
+    static constexpr int THREADS = 32 * (4 + CODERS + READERS);
+    static constexpr int MINE = NT * 4 / READERS;  // columns of a reading warp
     static constexpr int ACCUMULATORS = 512 / NT;
-    static constexpr size_t SMEM = (size_t)STAGES * STAGE + CODE_STAGES * LT_CODE_BYTES + 1024;
+    static constexpr size_t SMEM = (size_t)SLOTS * (SLOT + LT_CODE_BYTES) + 1024;
+    // registers of a thread that loads or issues, codes, reads: by warpgroups no more than the launch gives, 80 for each of 768 threads
+    static constexpr int ISSUE_REGISTERS = NT == 64 ? 64 : 56, CODE_REGISTERS = NT == 64 ? 64 : 40, READ_REGISTERS = 152;
+    static_assert(THREADS == 768 && 4 * ISSUE_REGISTERS + CODERS * CODE_REGISTERS + READERS * READ_REGISTERS <= 24 * 80, "setmaxnreg would wait forever");
 };
 
 struct LinearTcJob {
     CUtensorMap x, inner, codes, up;
     LinearArgs a;
-    int row_tiles, token_tiles, splits, chunks, group_chunks;  // chunks: an even number of them
+    int row_tiles, token_tiles, splits, chunks, group_chunks;
     const int *plan;  // per tile of tokens: how many adapters, and which
     float *partial;   // [splits][tokens][m], where splits > 1
 };
@@ -52,9 +54,8 @@ __device__ __forceinline__ bool linear_item(const LinearTcJob &job, int rank, in
     it.token_tile = (int)(tile / job.row_tiles);
     it.row0 = (int)(tile % job.row_tiles) * (DUO ? 256 : 128) + rank * 128;
     it.token0 = it.token_tile * NT;
-    const int quads = (job.chunks + LT_CODE_CHUNKS - 1) / LT_CODE_CHUNKS;  // splits begin where codes' stages do
-    it.c0 = (int)((int64_t)it.split * quads / job.splits) * LT_CODE_CHUNKS;
-    it.c1 = min((int)((int64_t)(it.split + 1) * quads / job.splits) * LT_CODE_CHUNKS, job.chunks);
+    it.c0 = (int)((int64_t)it.split * job.chunks / job.splits);
+    it.c1 = (int)((int64_t)(it.split + 1) * job.chunks / job.splits);
     return true;
 }
 // whether a slice ends with chunk ch
@@ -115,12 +116,16 @@ __device__ __forceinline__ bool elected() {
     return one != 0;
 }
 
+// A warp that arrives at another CTA's barrier with .release waits until all it wrote has arrived everywhere (a thousand cycles, in the middle of the pipeline's chain:
+// 8192 x 28672, 2048 tokens, 940 and 885 us).  What the coders write stays in their CTA's shared memory and is read by that SM's tensor core alone; they have brought it
+// there by their proxy fence before they arrive, so that the message itself need order nothing.
 __device__ __forceinline__ void arrive_relaxed(uint32_t bar) { asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
 
 template <int NT, bool DUO>
 struct LinearBarriers {
     using S = LinearShape<NT, DUO>;
-    uint64_t x_full[S::STAGES], w_here[S::STAGES], w_full[S::STAGES], empty[S::STAGES], code_full[S::CODE_STAGES], code_empty[S::CODE_STAGES], acc_full[S::ACCUMULATORS], acc_empty[S::ACCUMULATORS], drained;
+    // full: x has landed (or the rows of an adapter) and W is written, in both CTAs: the leader's; empty: the products have read the slot
+    uint64_t full[S::SLOTS], empty[S::SLOTS], code_full[S::SLOTS], code_empty[S::SLOTS], acc_full[S::ACCUMULATORS], acc_empty[S::ACCUMULATORS], drained;
     uint32_t tmem;
     int failed;
 };
@@ -128,31 +133,23 @@ struct LinearBarriers {
 template <bool BF16, int NT, bool DUO>
 __global__ void __launch_bounds__(LinearShape<NT, DUO>::THREADS, 1) linear_tc_kernel(const __grid_constant__ LinearTcJob job) {
     using S = LinearShape<NT, DUO>;
-    constexpr int CTAS = DUO ? 2 : 1, ACC = S::ACCUMULATORS;
+    constexpr int CTAS = DUO ? 2 : 1, ACC = S::ACCUMULATORS, SLOTS = S::SLOTS;
     extern __shared__ unsigned char linear_tc_smem[];
     __shared__ __align__(8) LinearBarriers<NT, DUO> bar;
     const LinearArgs &a = job.a;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = DUO ? (int)cluster_rank() : 0;
-    const uint32_t base = (smem_u32(linear_tc_smem) + 1023u) & ~1023u, codes_base = base + S::STAGES * S::STAGE;
+    const uint32_t base = (smem_u32(linear_tc_smem) + 1023u) & ~1023u, codes_base = base + SLOTS * S::SLOT;
     const auto wait = [&](uint64_t *b, uint32_t parity, unsigned nap) {
         if (mbar_wait(b, parity, nap, a.wait_cycles)) return true;
         bar.failed = 1;
         return false;
     };
-    const auto arrive = [&](uint64_t *b) {  // at the leader's barrier
-        if (DUO) mbar_arrive_at(leaders(b));
-        else mbar_arrive(b);
-    };
     if (threadIdx.x == 0) {
-        for (int s = 0; s < S::STAGES; ++s) {
-            mbar_init(&bar.x_full[s], 1);
-            mbar_init(&bar.w_here[s], S::CODERS);
-            mbar_init(&bar.w_full[s], CTAS);
+        for (int s = 0; s < SLOTS; ++s) {
+            mbar_init(&bar.full[s], 1 + CTAS * S::TEAM);
             mbar_init(&bar.empty[s], 1);
-        }
-        for (int s = 0; s < S::CODE_STAGES; ++s) {
             mbar_init(&bar.code_full[s], 1);
-            mbar_init(&bar.code_empty[s], S::TEAMS * S::CODERS);
+            mbar_init(&bar.code_empty[s], S::TEAM);
         }
         for (int s = 0; s < ACC; ++s) {
             mbar_init(&bar.acc_full[s], 1);
@@ -179,89 +176,84 @@ __global__ void __launch_bounds__(LinearShape<NT, DUO>::THREADS, 1) linear_tc_ke
     };
     const auto adapter_at = [&](const LinearItem &it, int j) { return job.plan[(int64_t)it.token_tile * (NT + 1) + 1 + j]; };
     const auto item = [&](int number, LinearItem &it) { return linear_item<NT, DUO>(job, rank, number, it); };
-    const int first_coder = 4, first_reader = 4 + S::TEAMS * S::CODERS;
+    const int first_coder = 4, first_reader = 4 + S::CODERS;
 
+    // Every role counts the turns of the slots over all items of the CTA: a chunk of columns is a turn, and an adapter two (its inner values' upper and lower parts).
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::ISSUE_REGISTERS));
         if (warp == 0 && lane == 0) {  // x
             LinearItem it;
-            int c = 0;
-            const auto begin = [&](uint32_t bytes) {  // the next stage is free and expects so many bytes in each CTA
-                const int stage = c % S::STAGES, round = c / S::STAGES;
-                if (bar.failed || (round > 0 && !wait(&bar.empty[stage], (round - 1) & 1, 32))) return false;
+            int slot = 0;
+            uint32_t parity = 1, turns = 0;
+            const auto begin = [&](uint32_t bytes) {  // the next slot is free and expects so many bytes in each CTA
+                if (bar.failed || (turns >= SLOTS && !wait(&bar.empty[slot], parity, 32))) return false;
                 // DUO: both CTAs' bytes count at the leader's barrier (they may do so before it expects them: the phase waits for its arrival)
-                if (rank == 0) mbar_expect_tx(&bar.x_full[stage], CTAS * bytes);
+                if (rank == 0) mbar_expect_tx(&bar.full[slot], CTAS * bytes);
                 return true;
             };
-            const auto bring = [&](uint32_t at, const CUtensorMap *map, int column, int row) {
-                uint64_t *const full = &bar.x_full[c % S::STAGES];
-                const uint32_t to = base + (c % S::STAGES) * S::STAGE + at;
-                if (DUO) tma_load_2d_duo(to, map, column, row, leaders(full));
-                else tma_load_2d(to, map, column, row, full);
+            const auto bring = [&](const CUtensorMap *map, int column, int row) {
+                if (DUO) tma_load_2d_duo(base + slot * S::SLOT, map, column, row, leaders(&bar.full[slot]));
+                else tma_load_2d(base + slot * S::SLOT, map, column, row, &bar.full[slot]);
+            };
+            const auto next = [&] {
+                ++turns;
+                if (++slot == SLOTS) slot = 0, parity ^= 1;
             };
             bool go = true;
             for (int i = 0; go && item(i, it); ++i) {
                 const int token = it.token0 + rank * S::X_ROWS;
-                for (int ch = it.c0; go && ch < it.c1; ch += LT_SUB) {
-                    go = begin(LT_SUB * S::X_BYTES);
+                for (int ch = it.c0; go && ch < it.c1; ++ch) {
+                    go = begin(S::X_BYTES);
                     if (!go) break;
-                    for (int s = 0; s < LT_SUB; ++s) bring(s * S::X_BYTES, &job.x, (ch + s) * KH, token);
-                    ++c;
+                    bring(&job.x, ch * KH, token);
+                    next();
                 }
-                const int extra = go ? adapters_in(it) : 0;
+                const int extra = go ? 2 * adapters_in(it) : 0;
                 for (int e = 0; go && e < extra; ++e) {
-                    go = begin(LT_SUB * S::X_BYTES + LT_W_BYTES);
+                    go = begin(S::X_BYTES + LT_W_BYTES);
                     if (!go) break;
-                    for (int s = 0; s < LT_SUB; ++s) bring(s * S::X_BYTES, &job.inner, s * RANK_MAX, token);
-                    uint64_t *const full = &bar.x_full[c % S::STAGES];
-                    const uint32_t to = base + (c % S::STAGES) * S::STAGE + LT_SUB * S::X_BYTES;
-                    if (DUO) tma_load_3d_duo(to, &job.up, 0, it.row0, adapter_at(it, e), leaders(full));
-                    else tma_load_3d(to, &job.up, 0, it.row0, adapter_at(it, e), full);
-                    ++c;
+                    bring(&job.inner, (e & 1) * RANK_MAX, token);
+                    const uint32_t to = base + slot * S::SLOT + S::X_BYTES;
+                    if (DUO) tma_load_3d_duo(to, &job.up, 0, it.row0, adapter_at(it, e >> 1), leaders(&bar.full[slot]));
+                    else tma_load_3d(to, &job.up, 0, it.row0, adapter_at(it, e >> 1), &bar.full[slot]);
+                    next();
                 }
             }
-            // landed, or had their time to, before the memory is given back
-            if (rank == 0)
-                for (int k = max(c - S::STAGES, 0); k < c; ++k) mbar_wait(&bar.x_full[k % S::STAGES], (k / S::STAGES) & 1);
-            if (DUO && !bar.failed) {  // the leader's commits arrive here as well: none may be under way when this CTA ends
-                for (int k = max(c - S::STAGES, 0); k < c; ++k) wait(&bar.empty[k % S::STAGES], (k / S::STAGES) & 1, 32);
+            // What was loaded has landed, and the leader's commits have arrived here, before this CTA ends: the last turn of every slot is awaited to its end.  After a
+            // time-out the loads have their time to land.
+            if (!bar.failed) {
+                for (uint32_t k = turns > SLOTS ? turns - SLOTS : 0; k < turns; ++k) wait(&bar.empty[k % SLOTS], (k / SLOTS) & 1, 32);
+            } else if (rank == 0) {
+                let_it_land();
             }
         } else if (warp == 2 && lane == 0) {  // codes
             LinearItem it;
-            int c = 0;
+            int slot = 0;
+            uint32_t used = 0, parity = 0;  // slots whose codes were loaded before; each slot's parity
             bool go = true;
             for (int i = 0; go && item(i, it); ++i) {
-                for (int ch = it.c0; ch < it.c1; ch += LT_CODE_CHUNKS, ++c) {
-                    const int stage = c % S::CODE_STAGES, round = c / S::CODE_STAGES;
-                    if (bar.failed || (round > 0 && !wait(&bar.code_empty[stage], (round - 1) & 1, 32))) { go = false; break; }
-                    mbar_expect_tx(&bar.code_full[stage], LT_CODE_BYTES);
-                    tma_load_2d(codes_base + stage * LT_CODE_BYTES, &job.codes, ch * (KH / 2), it.row0, &bar.code_full[stage]);
+                for (int ch = it.c0; ch < it.c1; ++ch) {
+                    const uint32_t bit = 1u << slot;
+                    if (bar.failed || ((used & bit) && !wait(&bar.code_empty[slot], (parity >> slot) & 1, 32))) { go = false; break; }
+                    if (used & bit) parity ^= bit;
+                    used |= bit;
+                    mbar_expect_tx(&bar.code_full[slot], LT_CODE_BYTES);
+                    tma_load_2d(codes_base + slot * LT_CODE_BYTES, &job.codes, ch * (KH / 2), it.row0, &bar.code_full[slot]);
+                    if (++slot == SLOTS) slot = 0;
                 }
+                if (go) slot = (slot + 2 * adapters_in(it)) % SLOTS;
             }
-            for (int k = max(c - S::CODE_STAGES, 0); k < c; ++k) mbar_wait(&bar.code_full[k % S::CODE_STAGES], (k / S::CODE_STAGES) & 1);
-        } else if (DUO && warp == 3 && lane == 0) {
-            // The coders arrive at this CTA's barrier; this thread passes it on to the leader's.  What they wrote stays in this CTA's shared memory and is read by this
-            // SM's tensor core alone: they have brought it there by their proxy fence before they arrive, so that the message itself need order nothing (with
-            // .release it takes a thousand cycles of this chain: 8192 x 28672, 2048 tokens, 940 and 885 us).
-            LinearItem it;
-            int c = 0;
-            bool go = true;
-            for (int i = 0; go && item(i, it); ++i) {
-                const int stages = (it.c1 - it.c0 + LT_SUB - 1) / LT_SUB + adapters_in(it);
-                for (int k = 0; go && k < stages; ++k, ++c) {
-                    go = !bar.failed && wait(&bar.w_here[c % S::STAGES], (c / S::STAGES) & 1, 20);
-                    if (go) arrive_relaxed(leaders(&bar.w_full[c % S::STAGES]));
-                }
-            }
+            // every load is awaited by the coders before they end; after a time-out they have their time to land
+            if (bar.failed) let_it_land();
         } else if (warp == 1 && rank == 0 && elected()) {  // products
             // One thread issues them all: what it does per product (128 cycles for a pair of CTAs, 32 for narrow tiles) is kept short
             constexpr uint32_t DESC = idesc_16(NT, BF16 ? 1 : 0, DUO ? 2 * MT : MT);
-            const uint64_t ws = umma_desc(base + LT_SUB * S::X_BYTES), xs = umma_desc(base);
+            const uint64_t ws = umma_desc(base + S::X_BYTES), xs = umma_desc(base);
             LinearItem it;
-            int stage = 0, slice = 0;
+            int slot = 0, slice = 0;
             uint32_t parity = 0;
             const auto ready = [&] {
-                if (bar.failed || !wait(DUO ? &bar.w_full[stage] : &bar.w_here[stage], parity, 20) || !wait(&bar.x_full[stage], parity, 20)) return false;
+                if (!wait(&bar.full[slot], parity, 20)) return false;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 return true;
             };
@@ -271,48 +263,38 @@ __global__ void __launch_bounds__(LinearShape<NT, DUO>::THREADS, 1) linear_tc_ke
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 return true;
             };
-            const auto issue = [&](uint64_t w, uint64_t x, uint32_t accumulate) {
+            const auto issue = [&](int ks, uint32_t accumulate) {
                 const uint32_t d = tmem + (uint32_t)((slice % ACC) * NT);
-                if (DUO) umma_16_duo(d, w, x, DESC, accumulate);
-                else umma_16(d, w, x, DESC, accumulate);
+                const uint64_t at = (uint64_t)((uint32_t)(slot * S::SLOT) >> 4) + 2 * ks;
+                if (DUO) umma_16_duo(d, ws + at, xs + at, DESC, accumulate);
+                else umma_16(d, ws + at, xs + at, DESC, accumulate);
             };
-            const auto done = [&] {
-                commit<DUO>(&bar.empty[stage]);
-                if (++stage == S::STAGES) stage = 0, parity ^= 1;
+            const auto done = [&](bool closes) {
+                commit<DUO>(&bar.empty[slot]);
+                if (closes) commit<DUO>(&bar.acc_full[slice++ % ACC]);
+                if (++slot == SLOTS) slot = 0, parity ^= 1;
             };
             bool go = true;
             for (int i = 0; go && item(i, it); ++i) {
                 bool opens = true;
                 int in_group = it.c0 % job.group_chunks;
-                for (int ch = it.c0; go && ch < it.c1; ch += LT_SUB) {
-                    go = ready();
-                    const uint64_t w0 = ws + (uint64_t)((uint32_t)(stage * S::STAGE) >> 4), x0 = xs + (uint64_t)((uint32_t)(stage * S::STAGE) >> 4);
-#pragma unroll
-                    for (int s = 0; s < LT_SUB; ++s) {
-                        if (opens) go = go && open();
-                        if (!go) break;
-                        const uint64_t w = w0 + (uint64_t)(s * (LT_W_BYTES >> 4)), x = x0 + (uint64_t)(s * (S::X_BYTES >> 4));
-                        issue(w, x, opens ? 0u : 1u);
-#pragma unroll
-                        for (int ks = 1; ks < KH / 16; ++ks) issue(w + 2 * ks, x + 2 * ks, 1u);
-                        const bool group_ends = in_group == job.group_chunks - 1;
-                        opens = group_ends || (in_group & (LT_SLICE - 1)) == LT_SLICE - 1 || ch + s == it.c1 - 1;  // as slice_ends has it
-                        in_group = group_ends ? 0 : in_group + 1;
-                        if (opens) commit<DUO>(&bar.acc_full[slice++ % ACC]);
-                    }
-                    done();
-                }
-                const int extra = go ? adapters_in(it) : 0;
-                for (int e = 0; go && e < extra; ++e) {  // the rows of `up` against both parts of the inner values
-                    go = ready() && open();
+                for (int ch = it.c0; ch < it.c1; ++ch) {
+                    go = !bar.failed && ready() && (!opens || open());
                     if (!go) break;
-                    const uint64_t w0 = ws + (uint64_t)((uint32_t)(stage * S::STAGE) >> 4), x0 = xs + (uint64_t)((uint32_t)(stage * S::STAGE) >> 4);
-                    for (int ks = 0; 16 * ks < a.rank; ++ks) {
-                        issue(w0 + 2 * ks, x0 + 2 * ks, ks > 0);
-                        issue(w0 + 2 * ks, x0 + (S::X_BYTES >> 4) + 2 * ks, 1u);
-                    }
-                    commit<DUO>(&bar.acc_full[slice++ % ACC]);
-                    done();
+                    issue(0, opens ? 0u : 1u);
+#pragma unroll
+                    for (int ks = 1; ks < KH / 16; ++ks) issue(ks, 1u);
+                    const bool group_ends = in_group == job.group_chunks - 1;
+                    opens = group_ends || (in_group & (LT_SLICE - 1)) == LT_SLICE - 1 || ch == it.c1 - 1;  // as slice_ends has it
+                    in_group = group_ends ? 0 : in_group + 1;
+                    done(opens);
+                }
+                const int extra = go ? 2 * adapters_in(it) : 0;
+                for (int e = 0; e < extra; ++e) {  // the rows of `up` against the upper, then the lower parts of the inner values
+                    go = !bar.failed && ready() && ((e & 1) || open());
+                    if (!go) break;
+                    for (int ks = 0; 16 * ks < a.rank; ++ks) issue(ks, (e & 1) || ks > 0 ? 1u : 0u);
+                    done(e & 1);
                 }
             }
             if (bar.failed) {  // every product that was issued completes, or has its time to, before what it reads and writes is given back
@@ -325,90 +307,86 @@ __global__ void __launch_bounds__(LinearShape<NT, DUO>::THREADS, 1) linear_tc_ke
         __syncwarp();
     } else if (warp < first_reader) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::CODE_REGISTERS));
-        // ---- operands: a thread has a row and, with four warps, both chunks of a stage, else one ----
-        const int team = (warp - first_coder) / S::CODERS, id = threadIdx.x - 32 * (first_coder + team * S::CODERS), row = id;
+        // ---- operands: the rows `row` and `row` + 64 of the turns of one slot ----
+        const int slot = (warp - first_coder) / S::TEAM, row = (warp - first_coder) % S::TEAM * 32 + lane;
+        const uint32_t to = base + slot * S::SLOT + S::X_BYTES + row * 128, from = codes_base + slot * LT_CODE_BYTES + row * 32;
+        constexpr float ORIGIN = BF16 ? 128.f : 1024.f;
         LinearItem it;
-        int stage = 0, turn = 0, code_stage = 0;
-        uint32_t parity = 1, code_parity = 0;  // of the stage's last release (the first time round there is none to wait for)
-        bool go = true, again = false;
-        const auto released = [&] { return !again || wait(&bar.empty[stage], parity, 20); };
-        const auto free_stage = [&] {
-            go = go && released();
+        int first = 0;  // the slot of the item's first turn
+        uint32_t turns = 0, coded = 0;
+        bool go = true;
+        const auto free_slot = [&] {
+            if (turns > 0) go = go && wait(&bar.empty[slot], (turns - 1) & 1, 20);
             go = __all_sync(0xffffffffu, go && !bar.failed);
+            ++turns;
             return go;
         };
-        const auto advance = [&](bool mine) {
-            // Where a team does not come back to the same stages, it awaits the other turns' releases too (they come before its own): a wait that left out a
-            // phase could take the one before for it.
-            if (!mine && S::STAGES % S::TEAMS != 0) go = go && released();
-            if (++stage == S::STAGES) stage = 0, parity ^= 1, again = true;
-            if (++turn == S::TEAMS) turn = 0;
+        const auto written = [&] {
+            if (lane == 0) {
+                if (DUO) arrive_relaxed(leaders(&bar.full[slot]));
+                else mbar_arrive(&bar.full[slot]);
+            }
         };
-        constexpr float ORIGIN = BF16 ? 128.f : 1024.f;
         for (int i = 0; go && item(i, it); ++i) {
-            const float *const zero = a.zero + min((int64_t)it.row0 + row, a.m - 1) * a.zero_row;
-            const int groups = (job.chunks - 1) / job.group_chunks + 1;
-            // the zero point of the next group that this thread meets is on its way
-            int group_end = -1;
-            const auto zero_of = [&](int g) { return __ldg(zero + (int64_t)min(g, groups - 1) * a.zero_group); };
-            float next_zero = 0.f;
-            int next_group = -2;
-            uint32_t once = 0u, shift = 0u;
+            const float *const zero0 = a.zero + min((int64_t)it.row0 + row, a.m - 1) * a.zero_row, *const zero1 = a.zero + min((int64_t)it.row0 + row + 64, a.m - 1) * a.zero_row;
+            int ch = it.c0 + (slot - first + SLOTS) % SLOTS, group_end = -1, next_group = -1;
+            float next0 = 0.f, next1 = 0.f;  // the zero points of the group that this thread meets next, on their way
+            uint32_t once0 = 0u, once1 = 0u, shift0 = 0u, shift1 = 0u;
             bool exact = true;
-            for (int ch = it.c0; ch < it.c1; ch += LT_SUB) {
-                const int quarter = ch % LT_CODE_CHUNKS;
-                // by all teams, theirs or not, as for the releases
-                if (quarter == 0 && !wait(&bar.code_full[code_stage], code_parity, 20)) go = false;
-                if (turn == team) {
-                    const uint32_t from = codes_base + code_stage * LT_CODE_BYTES + row * 128;
-                    uint4 raw[2 * LT_SUB];
+            for (; ch < it.c1; ch += SLOTS) {
+                if (ch >= group_end) {  // another group
+                    const int group = min(ch, job.chunks - 1) / job.group_chunks;
+                    group_end = (group + 1) * job.group_chunks;
+                    const float by0 = a.qmin - (group == next_group ? next0 : __ldg(zero0 + (int64_t)group * a.zero_group));
+                    const float by1 = a.qmin - (group == next_group ? next1 : __ldg(zero1 + (int64_t)group * a.zero_group));
+                    const int meets = (ch + (group_end - ch + SLOTS - 1) / SLOTS * SLOTS) / job.group_chunks;
+                    next_group = min(meets, (job.chunks - 1) / job.group_chunks);
+                    next0 = __ldg(zero0 + (int64_t)next_group * a.zero_group);
+                    next1 = __ldg(zero1 + (int64_t)next_group * a.zero_group);
+                    // one addition where -1024 + qmin - zero is a number of the type (integers up to 2048; bf16: -128, 256), else two, the first exact
+                    once0 = float_to_bits(by0 - ORIGIN, BF16);
+                    once1 = float_to_bits(by1 - ORIGIN, BF16);
+                    exact = __all_sync(0xffffffffu, bits_to_float(once0, BF16) == by0 - ORIGIN && bits_to_float(once1, BF16) == by1 - ORIGIN);
+                    once0 = exact ? once0 | (once0 << 16) : (BF16 ? 0xc308c308u : 0xe408e408u);
+                    once1 = exact ? once1 | (once1 << 16) : once0;
+                    shift0 = float_to_bits(by0 + 8.f, BF16) * 0x10001u;
+                    shift1 = float_to_bits(by1 + 8.f, BF16) * 0x10001u;
+                }
+                if (!wait(&bar.code_full[slot], coded++ & 1, 20)) go = false;
+                // rows of 32 bytes under the TMA's 32-byte swizzle: the two halves change places in every second group of four rows
+                const uint32_t flip = ((row >> 2) & 1) << 4;
+                if (!free_slot()) break;  // for the whole warp
 #pragma unroll
-                    for (int w = 0; w < 2 * LT_SUB; ++w) raw[w] = load_16(from + (((quarter * 2 + w) ^ (row & 7)) << 4));
-                    if (!free_stage()) break;  // for the whole warp
-#pragma unroll
-                    for (int s = 0; s < LT_SUB; ++s) {
-                        if (ch + s >= group_end) {  // another group
-                            const int group = (ch + s) / job.group_chunks;
-                            group_end = (group + 1) * job.group_chunks;
-                            const float by = a.qmin - (group == next_group ? next_zero : zero_of(group));
-                            next_group = (group_end > ch + LT_SUB - 1 ? max(group_end, ch + LT_SUB * S::TEAMS) : group_end) / job.group_chunks;
-                            next_zero = zero_of(next_group);
-                            // one addition where -1024 + qmin - zero is a number of the type (integers up to 2048; bf16: -128, 256), else two, the first exact
-                            const uint32_t whole = float_to_bits(by - ORIGIN, BF16), apart = float_to_bits(by + 8.f, BF16);
-                            exact = __all_sync(0xffffffffu, bits_to_float(whole, BF16) == by - ORIGIN);
-                            once = exact ? whole | (whole << 16) : (BF16 ? 0xc308c308u : 0xe408e408u);
-                            shift = apart | (apart << 16);
-                        }
-                        const uint32_t to = base + stage * S::STAGE + LT_SUB * S::X_BYTES + s * LT_W_BYTES + row * 128;
-                        if (exact) {
-#pragma unroll
-                            for (int w = 0; w < 8; ++w) store_16(to + ((w ^ (row & 7)) << 4), decoded<BF16>(word_of(raw[2 * s + (w >> 2)], w), once));
-                        } else {
-#pragma unroll
-                            for (int w = 0; w < 8; ++w) {
-                                const uint4 v = decoded<BF16>(word_of(raw[2 * s + (w >> 2)], w), once);
-                                store_16(to + ((w ^ (row & 7)) << 4), make_uint4(add2<BF16>(v.x, shift), add2<BF16>(v.y, shift), add2<BF16>(v.z, shift), add2<BF16>(v.w, shift)));
-                            }
-                        }
+                for (int part = 0; part < 4; ++part) {  // half a row at a time: few registers, and two other warps of the scheduler work meanwhile
+                    const int r = part >> 1, h = part & 1;
+                    const uint32_t at = to + r * (64 * 128), once = r ? once1 : once0, shift = r ? shift1 : shift0;
+                    const uint4 raw = load_16(from + r * (64 * 32) + ((h << 4) ^ flip));
+                    if (part == 3) {
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&bar.code_empty[slot]);
                     }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&bar.w_here[stage]);
+                    uint4 v[4];
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) v[w] = decoded<BF16>(word_of(raw, w), once);
+                    if (!exact) {
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) v[w] = make_uint4(add2<BF16>(v[w].x, shift), add2<BF16>(v[w].y, shift), add2<BF16>(v[w].z, shift), add2<BF16>(v[w].w, shift));
+                    }
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) store_16(at + (((4 * h + w) ^ (row & 7)) << 4), v[w]);
                 }
-                advance(turn == team);
-                if (quarter + LT_SUB >= LT_CODE_CHUNKS || ch + LT_SUB >= it.c1) {
-                    if (lane == 0) mbar_arrive(&bar.code_empty[code_stage]);  // behind the warp's barrier: all lanes have read
-                    if (++code_stage == S::CODE_STAGES) code_stage = 0, code_parity ^= 1;
-                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                written();
             }
-            const int extra = go ? adapters_in(it) : 0;
-            for (int e = 0; go && e < extra; ++e) {  // rows of `up`, which the TMA brings: the stage is free for them
-                if (turn == team) {
-                    if (!free_stage()) break;
-                    if (lane == 0) mbar_arrive(&bar.w_here[stage]);
-                }
-                advance(turn == team);
+            if (!go) break;
+            const int extra = 2 * adapters_in(it);
+            first = (first + it.c1 - it.c0) % SLOTS;
+            for (int e = (slot - first + SLOTS) % SLOTS; e < extra; e += SLOTS) {  // rows of `up`, which the TMA brings: the slot is free for them
+                if (!free_slot()) break;
+                written();
             }
+            first = (first + extra) % SLOTS;
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::READ_REGISTERS));
@@ -433,7 +411,10 @@ __global__ void __launch_bounds__(LinearShape<NT, DUO>::THREADS, 1) linear_tc_ke
             const auto leave = [&] {
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) arrive(&bar.acc_empty[slice % ACC]);
+                if (lane == 0) {
+                    if (DUO) mbar_arrive_at(leaders(&bar.acc_empty[slice % ACC]));
+                    else mbar_arrive(&bar.acc_empty[slice % ACC]);
+                }
                 ++slice;
             };
             const uint32_t from = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)t0;
@@ -522,9 +503,9 @@ static bool make_map_codes(CUtensorMap *map, const uint8_t *codes, int64_t rows,
     if (!fn) return false;
     const cuuint64_t dims[2] = {(cuuint64_t)bytes, (cuuint64_t)rows};
     const cuuint64_t strides[1] = {(cuuint64_t)pitch};
-    const cuuint32_t box[2] = {128, 128};
+    const cuuint32_t box[2] = {32, 128};
     const cuuint32_t elem[2] = {1, 1};
-    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t *>(codes), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t *>(codes), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_32B,
               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -555,9 +536,9 @@ LinearTcPlan linear_tc_plan(int64_t m, int64_t n, int64_t tokens) {
     }
     p.row_tiles = (int)rows;
     p.token_tiles = (int)columns;
-    const int64_t tiles = rows * columns, quads = ceil_div(n, (int64_t)(KH * LT_CODE_CHUNKS));
+    const int64_t tiles = rows * columns, chunks = ceil_div(n, (int64_t)KH);
     int64_t splits = (p.duo ? 74 : 148) / tiles;
-    if (splits > quads / 2) splits = quads / 2;
+    if (splits > chunks / 8) splits = chunks / 8;
     p.splits = splits < 1 ? 1 : (int)splits;
     return p;
 }
@@ -572,7 +553,7 @@ static int launch_tc(const LinearArgs &a, const LinearTcPlan &p, const int *plan
     job.row_tiles = p.row_tiles;
     job.token_tiles = p.token_tiles;
     job.splits = p.splits;
-    job.chunks = (int)ceil_div(a.n, (int64_t)(LT_SUB * KH)) * LT_SUB;
+    job.chunks = (int)ceil_div(a.n, (int64_t)KH);
     job.group_chunks = a.group >= a.n ? job.chunks : (int)(a.group / KH);
     job.plan = plan;
     job.partial = partial;
