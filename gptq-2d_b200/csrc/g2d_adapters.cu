@@ -115,21 +115,25 @@ __global__ void __launch_bounds__(INNER_THREADS, TILES == 8 ? 1 : 2) inner_block
     constexpr int WARPS = INNER_THREADS / 32;
     __shared__ float part[WARPS / 2][INNER_BLOCK][RANK_MAX + 2];  // two warps at a time
     __shared__ int ids[INNER_BLOCK];
+    __shared__ unsigned firsts;
     __shared__ float tops[4][2];
     let_the_next_launch_start();
     const int block = blockIdx.x / INNER_SPLIT, rank = (int)cluster_rank(), warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int token0 = block * INNER_BLOCK;
     if (plan && rank == INNER_SPLIT - 1 && blockIdx.y == 0 && token0 % tile == 0) write_plan(a, plan + (int64_t)(token0 / tile) * (tile + 1), tile, token0);
-    if (threadIdx.x < INNER_BLOCK) ids[threadIdx.x] = adapter_of(a, token0 + threadIdx.x);
+    if (warp == 0) {  // the block's adapters: each by its first token
+        const int id = adapter_of(a, token0 + lane);
+        ids[lane] = id;
+        const unsigned same = __match_any_sync(0xffffffffu, id);
+        const unsigned first = __ballot_sync(0xffffffffu, __ffs(same) - 1 == lane);
+        if (lane == 0) firsts = first;
+    }
     __syncthreads();
     const int64_t steps = ceil_div(a.n, (int64_t)32), s0 = rank * steps / INNER_SPLIT, s1 = (rank + 1) * steps / INNER_SPLIT;  // 32 columns each; n is a multiple of 32
     int number = 0;  // of the adapter among the block's
-    for (int first = 0; first < INNER_BLOCK; ++first) {
-        const int id = ids[first];
-        bool seen = false;
-        for (int k = 0; k < first; ++k) seen |= ids[k] == id;
-        if (seen) continue;
+    for (unsigned left = firsts; left; left &= left - 1) {
         if (number++ % gridDim.y != blockIdx.y) continue;  // the same for the whole cluster
+        const int id = ids[__ffs(left) - 1];
         float acc[2][TILES][4];
 #pragma unroll
         for (int i = 0; i < 2; ++i)
