@@ -435,25 +435,35 @@ __global__ void __launch_bounds__(LinearShape<NT, DUO>::THREADS, 1) linear_tc_ke
                 factor = next_factor;
             }
             const int extra = go ? adapters_in(it) : 0;
-            for (int e = 0; go && e < extra; ++e) {
-                const int id = adapter_at(it, e);
-                if (!arrived()) break;
+            if (extra > 0) {
+                // every 32 tokens' adapters and factors, a token per lane: loaded once per tile, whatever the number of adapters
+                int ids[MINE / 32];
+                float factors[MINE / 32];
 #pragma unroll
-                for (int cb = 0; cb < MINE / 16; ++cb) {
-                    const int token = it.token0 + t0 + cb * 16 + (lane & 15);
-                    const bool has = adapter_of(a, token) == id;
-                    const float f = has ? a.factor[token] : 0.f;
-                    const unsigned takes = __ballot_sync(0xffffffffu, has);
-                    if (takes == 0u) continue;
-                    uint32_t v[16];
-                    tmem_load_16(from + (uint32_t)((slice % ACC) * NT + cb * 16), v);
-#pragma unroll
-                    for (int x = 0; x < 16; ++x) {
-                        const float fx = __shfl_sync(0xffffffffu, f, x);
-                        if ((takes >> x) & 1u) total[cb * 16 + x] = fmaf(__uint_as_float(v[x]), fx, total[cb * 16 + x]);
-                    }
+                for (int cb = 0; cb < MINE / 32; ++cb) {
+                    const int token = it.token0 + t0 + cb * 32 + lane;
+                    ids[cb] = adapter_of(a, token);
+                    factors[cb] = ids[cb] >= 0 ? a.factor[token] : 0.f;
                 }
-                leave();
+                int id = adapter_at(it, 0);
+                for (int e = 0; go && e < extra; ++e) {
+                    const int next_id = e + 1 < extra ? adapter_at(it, e + 1) : 0;
+                    if (!arrived()) break;
+#pragma unroll
+                    for (int cb = 0; cb < MINE / 16; ++cb) {
+                        const unsigned takes = __ballot_sync(0xffffffffu, ids[cb / 2] == id) >> (cb % 2 * 16) & 0xffffu;
+                        if (takes == 0u) continue;
+                        uint32_t v[16];
+                        tmem_load_16(from + (uint32_t)((slice % ACC) * NT + cb * 16), v);
+#pragma unroll
+                        for (int x = 0; x < 16; ++x) {  // a token of another adapter keeps its sum, whatever this one's rows hold
+                            const float f = __shfl_sync(0xffffffffu, factors[cb / 2], cb % 2 * 16 + x);
+                            if ((takes >> x) & 1u) total[cb * 16 + x] = fmaf(__uint_as_float(v[x]), f, total[cb * 16 + x]);
+                        }
+                    }
+                    leave();
+                    id = next_id;
+                }
             }
             if (!go) {
 #pragma unroll
