@@ -356,8 +356,8 @@ __global__ void __launch_bounds__(LinearShape<NT, DUO>::THREADS, 1) linear_tc_ke
                 // rows of 32 bytes under the TMA's 32-byte swizzle: the two halves change places in every second group of four rows
                 const uint32_t flip = ((row >> 2) & 1) << 4;
                 if (!free_slot()) break;  // for the whole warp
-#pragma unroll
-                for (int part = 0; part < 4; ++part) {  // half a row at a time: few registers, and two other warps of the scheduler work meanwhile
+#pragma unroll 1
+                for (int part = 0; part < 4; ++part) {  // half a row at a time, in a loop: few registers, and few instructions for so many roles to share the caches with
                     const int r = part >> 1, h = part & 1;
                     const uint32_t at = to + r * (64 * 128), once = r ? once1 : once0, shift = r ? shift1 : shift0;
                     const uint4 raw = load_16(from + r * (64 * 32) + ((h << 4) ^ flip));
