@@ -18,15 +18,11 @@
 // over a long sequence the part -8 sum would leave its truncation behind.
 //
 // Bound: HBM (head_dim + 4 bytes per key and head), behind it the instructions per key.
-#include "g2d_cache.cuh"
-#include "g2d_tc.cuh"
+#include "g2d_attend.cuh"
 
 namespace g2d {
 
-int cache_view(const g2d_cache_desc *d, CacheView *c);
-
 constexpr int ATTEND_WARPS = 8, ATTEND_THREADS = 32 * ATTEND_WARPS, ATTEND_STAGES = 3, ATTEND_GRID = 148;
-constexpr float LOG2E = 1.4426950408889634f;
 
 template <int D>
 struct AttendStage {
@@ -39,14 +35,6 @@ struct AttendShared {
     uint64_t full[ATTEND_WARPS][ATTEND_STAGES];
     long long totals[ATTEND_WARPS];
 };
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-// cap tanh(u / cap) through one exponential: exact to 1e-7 of the cap, which is what a score's exponential sees
-__device__ __forceinline__ float capped(float u, float cap, float two_log2e_over_cap) { return cap - __fdividef(2.f * cap, 1.f + ex2(u * two_log2e_over_cap)); }
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -72,11 +60,6 @@ __device__ __forceinline__ int64_t attend_units(const AttendArgs &a, const Atten
 __device__ __forceinline__ int64_t attend_units(const AttendArgs &a, int b, int rows_per_item) {
     int blocks, items;
     return b < a.c.batch ? attend_units(a, attend_sequence(a, b), rows_per_item, blocks, items) : 0;
-}
-__device__ __forceinline__ int64_t warp_sum(int64_t v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
 }
 // All threads of a CTA of WARPS warps: the units of all sequences
 template <int WARPS>
@@ -610,7 +593,18 @@ static int launch_rows_for(const AttendArgs &a, cudaStream_t st) {
     return a.softcap > 0.f || a.slopes ? launch_rows<D, NT, true>(a, st) : launch_rows<D, NT, false>(a, st);
 }
 
-static size_t attend_bytes(int head_dim) { return (size_t)ATTEND_GRID * ATTEND_WARPS * 2 * 16 * (head_dim + 2) * sizeof(float); }
+// From here on a sequence's rows go by tiles; both sides of the line: see the figures in g2d_attend_tc.cu.
+constexpr int TILE_ROWS_FROM = 33;
+
+struct AttendSpace {
+    size_t tiles, all;  // the warps' partial results first
+};
+static AttendSpace attend_space(int head_dim) {
+    AttendSpace s;
+    s.tiles = ((size_t)ATTEND_GRID * ATTEND_WARPS * 2 * 16 * (head_dim + 2) * sizeof(float) + 255) & ~(size_t)255;
+    s.all = s.tiles + attend_tiles_bytes(head_dim);
+    return s;
+}
 
 }  // namespace g2d
 
@@ -621,7 +615,7 @@ extern "C" int g2d_attend_workspace_bytes(const g2d_attend_desc *desc, size_t *b
     if (!desc || !bytes) return G2D_ERR_BAD_ARGUMENT;
     const int status = cache_view(&desc->cache, &c);
     if (status != G2D_OK) return status;
-    *bytes = attend_bytes(c.head_dim);
+    *bytes = attend_space(c.head_dim).all;
     return G2D_OK;
 }
 
@@ -634,7 +628,7 @@ extern "C" int g2d_cache_attend(const g2d_attend_desc *d, void *stream) {
     if (a.c.tokens == 0 || a.c.batch == 0) return G2D_OK;
     if ((int64_t)a.c.tokens * d->heads > 0x7fffffff) return G2D_ERR_TOO_LARGE;
     if (!d->q || !d->out || (((uintptr_t)d->q | (uintptr_t)d->out) & 15) != 0 || ((d->q_token_stride | d->q_head_stride) & 7) != 0) return G2D_ERR_BAD_ARGUMENT;
-    if (!d->workspace || d->workspace_bytes < attend_bytes(a.c.head_dim) || ((uintptr_t)d->workspace & 255) != 0) return G2D_ERR_WORKSPACE;
+    if (!d->workspace || d->workspace_bytes < attend_space(a.c.head_dim).all || ((uintptr_t)d->workspace & 255) != 0) return G2D_ERR_WORKSPACE;
     a.q = d->q;
     a.out = d->out;
     a.q_token_stride = d->q_token_stride;
@@ -646,13 +640,22 @@ extern "C" int g2d_cache_attend(const g2d_attend_desc *d, void *stream) {
     a.softcap = d->softcap;
     a.slopes = d->slopes;
     a.prefix = d->prefix;
-    a.rows_from = 1;
-    a.rows_to = 0x7fffffff;
-    a.partial = (float *)d->workspace;
     a.status = d->status;
     a.wait_cycles = WAIT_CYCLES;
     cudaStream_t st = (cudaStream_t)stream;
-    const bool narrow = a.group <= 8 && (a.c.offsets || (int64_t)(a.c.tokens / a.c.batch) * a.group <= 8);
+    // How many rows a sequence has is known here only where all have the same; else the kernels share the sequences out between them.
+    const int64_t rows = a.c.offsets ? -1 : (int64_t)(a.c.tokens / a.c.batch) * a.group;
+    if (rows < 0 || rows >= TILE_ROWS_FROM) {
+        a.rows_from = TILE_ROWS_FROM;
+        a.rows_to = 0x7fffffff;
+        a.partial = (float *)((char *)d->workspace + attend_space(a.c.head_dim).tiles);
+        const int launched = launch_attend_tiles(a, st);
+        if (launched != G2D_OK || rows >= TILE_ROWS_FROM) return launched;
+    }
+    a.rows_from = 1;
+    a.rows_to = TILE_ROWS_FROM;
+    a.partial = (float *)d->workspace;
+    const bool narrow = a.group <= 8 && (rows < 0 || rows <= 8);
     if (a.c.head_dim == 128) return narrow ? launch_rows_for<128, 1>(a, st) : launch_rows_for<128, 2>(a, st);
     return narrow ? launch_rows_for<64, 1>(a, st) : launch_rows_for<64, 2>(a, st);
 }

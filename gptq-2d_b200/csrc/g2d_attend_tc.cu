@@ -1,0 +1,745 @@
+// Attention of many query rows per sequence over the packed cache, on tcgen05: prompts, and what is added to them.  The formulas are those of g2d_attend.cu.
+//
+// An item is 256 rows (token, head of the group) of one kv head: two tiles of 128 rows that share every block of 128 keys.  A unit is one block of one item; the units
+// of all items, one after the other, are dealt out evenly to the CTAs, whatever the lengths; an item that lies in one CTA's share is written at once, the others
+// leave partial results (two per CTA at most) that attend_tiles_join_kernel adds up in the order of the keys.
+//
+// A CTA: four warps turn codes into operands: K as code - 8 in the type of the queries, exactly, keys as rows; V as code - 8 in fp16, channels as rows (two keys' words interleaved
+// by a byte permutation).  One thread issues the products S = Q K^T and O += P V, S in tensor memory (128 columns a tile), P as fp16 over S, O beside them.  Eight warps, a row per
+// thread, read S, multiply it by the keys' scales, take maximum and exponentials, and write P = exponential times the value's scale, rounded once to fp16 under the power of two of the largest
+// scale so far.  While one tile's rows are at their exponentials the other's products run.
+//
+// The maximum that the exponentials refer to moves only when a row's scores exceed it by 2^8 (or the scales' power of two grows): then O is read and scaled in tensor memory.
+//
+// Bound: the exponentials (16 per cycle and SM: 2048 cycles for the 256 x 128 of a block, as long as its four products) and the instructions around them.
+#include "g2d_attend.cuh"
+
+namespace g2d {
+
+constexpr int TA_THREADS = 512, TA_ROWS = 256, TA_KEYS = 128, TA_GRID = 148, TA_SCALES = 4;
+constexpr int TA_PANEL = 128 * 128;  // bytes of 128 rows of 64 16-bit values
+constexpr float TA_SLACK = 8.f;      // how far scores may exceed the maximum that the exponentials refer to, as a power of two
+constexpr int TA_UNIT = 6;           // the largest scale is brought to 2^6 .. 2^7: times 2^8, still a number of fp16
+
+template <int D>
+struct TileShared {
+    static constexpr int Q = 0, Q_TILE = 128 * D * 2, K = 2 * Q_TILE, K_STAGE = 128 * D * 2, V = K + 2 * K_STAGE, V_STAGE = 128 * D * 2, SCALES = V + 2 * V_STAGE;
+    static constexpr int SCALE_STAGE = 2 * TA_KEYS * 4;  // ks, vs as floats
+    static constexpr size_t BYTES = SCALES + TA_SCALES * SCALE_STAGE + 1024;
+};
+// Blocks of an item in a CTA's share: written by one warp, read by the others' roles
+constexpr int TA_RUNS = 4;
+struct TileRun {
+    AttendSequence s;
+    int b, pair, head, first, n, blocks;  // n 0: there are no more
+};
+struct TileBarriers {
+    uint64_t run_full[TA_RUNS], run_empty[TA_RUNS], q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], scale_full[TA_SCALES], s_full[2], p_full[2], o_full[2], drained;
+    unsigned present[TA_SCALES][4];  // which keys of a block there are
+    int unit[TA_SCALES];             // exponent bits of the largest scale so far
+    int tops[4];
+    TileRun runs[TA_RUNS];
+    long long totals[TA_THREADS / 32];
+    uint32_t tmem;
+    int failed;
+};
+
+__device__ __forceinline__ void mma_from_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_store_32(uint32_t at, const uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, "
+        "%29, %30, %31, %32};" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]),
+        "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
+        "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void store_16s(uint32_t at, uint32_t x, uint32_t y, uint32_t z, uint32_t w) { asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x), "r"(y), "r"(z), "r"(w) : "memory"); }
+__device__ __forceinline__ void tmem_store_16(uint32_t at, const uint32_t (&v)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+                 "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+                 : "memory");
+}
+// pairs of floats: one instruction each
+__device__ __forceinline__ ulonglong2 load_4p(uint32_t at) {
+    ulonglong2 v;
+    asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(v.x), "=l"(v.y) : "r"(at));
+    return v;
+}
+__device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+    return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float &lo, float &hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2f(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint32_t halves_add(uint32_t u, uint32_t v, bool bf16) {
+    uint32_t r;
+    if (bf16) asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(u), "r"(v));
+    else asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(u), "r"(v));
+    return r;
+}
+
+// ---- units: for each sequence, each tile pair of rows (later rows see more keys), each kv head, the blocks of keys that the last of its rows sees ----
+__device__ __forceinline__ int tile_pairs(const AttendArgs &a, const AttendSequence &s) {
+    const int64_t rows = (int64_t)s.count * a.group;
+    return rows >= a.rows_from && rows < a.rows_to ? (int)((rows + TA_ROWS - 1) / TA_ROWS) : 0;
+}
+__device__ __forceinline__ int tile_blocks(const AttendArgs &a, const AttendSequence &s, int pair) {
+    const int64_t last = min((int64_t)s.count * a.group, (int64_t)(pair + 1) * TA_ROWS) - 1;
+    return max((visible_keys(a, s, (int)(last / a.group)) + TA_KEYS - 1) / TA_KEYS, 1);
+}
+__device__ __forceinline__ int64_t tile_units(const AttendArgs &a, int b) {
+    if (b >= a.c.batch) return 0;
+    const AttendSequence s = attend_sequence(a, b);
+    int64_t sum = 0;
+    for (int p = 0, n = tile_pairs(a, s); p < n; ++p) sum += tile_blocks(a, s, p);
+    return sum * a.c.kv_heads;
+}
+struct TileCursor {
+    int64_t u, end;
+    int b, pair, pairs, head, block, blocks;
+    AttendSequence s;
+    __device__ __forceinline__ void open(const AttendArgs &a) {  // sequence b, or the next one that has units
+        for (;; ++b) {
+            if (b >= a.c.batch) {  // not reached while u < end
+                end = u;
+                return;
+            }
+            s = attend_sequence(a, b);
+            pairs = tile_pairs(a, s);
+            if (pairs > 0) break;
+        }
+        pair = head = block = 0;
+        blocks = tile_blocks(a, s, 0);
+    }
+    // A warp: unit `at` of the list
+    __device__ __forceinline__ void find(const AttendArgs &a, int64_t at) {
+        const int lane = threadIdx.x & 31;
+        int64_t base = 0;
+        u = at;
+        b = a.c.batch;
+        for (int b0 = 0; b0 < a.c.batch; b0 += 32) {
+            int64_t sum = tile_units(a, b0 + lane);
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int64_t up = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= o) sum += up;
+            }
+            const unsigned past = __ballot_sync(0xffffffffu, base + sum > at);
+            if (past) {
+                const int k = __ffs(past) - 1;
+                const int64_t upto = __shfl_sync(0xffffffffu, sum, k > 0 ? k - 1 : 0);
+                if (k > 0) base += upto;
+                b = b0 + k;
+                break;
+            }
+            base += __shfl_sync(0xffffffffu, sum, 31);
+        }
+        open(a);
+        int64_t rest = at - base;
+        while (pair + 1 < pairs && rest >= (int64_t)blocks * a.c.kv_heads) {
+            rest -= (int64_t)blocks * a.c.kv_heads;
+            blocks = tile_blocks(a, s, ++pair);
+        }
+        head = (int)(rest / blocks);
+        block = (int)(rest % blocks);
+    }
+    __device__ __forceinline__ int run() const { return (int)min((int64_t)(blocks - block), end - u); }  // blocks of the item in this share
+    __device__ __forceinline__ void next(const AttendArgs &a) {                                           // the item behind this run
+        u += run();
+        if (u >= end) return;
+        block = 0;
+        if (++head < a.c.kv_heads) return;
+        head = 0;
+        if (++pair < pairs) {
+            blocks = tile_blocks(a, s, pair);
+            return;
+        }
+        ++b;
+        open(a);
+    }
+};
+// Partial results: for each of a slot's 256 rows, head_dim sums, the maximum and the sum of the exponentials
+template <int D>
+__device__ __forceinline__ float *tile_slot(const AttendArgs &a, int64_t slot) {
+    return a.partial + slot * (TA_ROWS * (D + 2));
+}
+
+template <int D, bool BF16, bool MODS>
+__global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const AttendArgs a) {
+    using M = TileShared<D>;
+    extern __shared__ unsigned char tiles_smem[];
+    __shared__ __align__(8) TileBarriers bar;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t base = (smem_u32(tiles_smem) + 1023u) & ~1023u;
+    const CacheView &c = a.c;
+    const auto wait = [&](uint64_t *b, uint32_t parity, unsigned nap) {
+        if (mbar_wait(b, parity, nap, a.wait_cycles)) return true;
+        bar.failed = 1;
+        return false;
+    };
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < TA_RUNS; ++s) {
+            mbar_init(&bar.run_full[s], 1);
+            mbar_init(&bar.run_empty[s], 1 + 4 + 8);  // the issuing thread, the coders' and the rows' warps
+        }
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(&bar.q_full[s], 4);
+            mbar_init(&bar.k_full[s], 4);
+            mbar_init(&bar.k_empty[s], 1);
+            mbar_init(&bar.v_full[s], 4);
+            mbar_init(&bar.v_empty[s], 1);
+            mbar_init(&bar.s_full[s], 1);
+            mbar_init(&bar.p_full[s], 4);
+            mbar_init(&bar.o_full[s], 1);
+        }
+        for (int s = 0; s < TA_SCALES; ++s) mbar_init(&bar.scale_full[s], 4);
+        mbar_init(&bar.drained, 1);
+        bar.failed = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) tmem_alloc<false>(&bar.tmem, 512);
+    int64_t units = 0;
+    for (int b = threadIdx.x; b < c.batch; b += TA_THREADS) units += tile_units(a, b);
+    units = warp_sum(units);
+    if (lane == 0) bar.totals[warp] = units;
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    let_the_next_launch_start();
+    units = 0;
+    for (int w = 0; w < TA_THREADS / 32; ++w) units += bar.totals[w];
+    const uint32_t tmem = bar.tmem;
+    const int64_t shares = min(units, (int64_t)gridDim.x), share = blockIdx.x;
+    // the run of that number, for every thread of a role; its entry stays until all roles have let it go
+    const auto run_of = [&](uint32_t number, bool &go) -> const TileRun & {
+        if (go) go = wait(&bar.run_full[number % TA_RUNS], (number / TA_RUNS) & 1, 20);
+        return bar.runs[number % TA_RUNS];
+    };
+    const auto let_go = [&](uint32_t number) { mbar_arrive(&bar.run_empty[number % TA_RUNS]); };
+    const auto second = [&](const TileRun &r) { return (int64_t)r.s.count * a.group - (int64_t)r.pair * TA_ROWS > 128; };  // whether the item has a second tile
+
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        if (warp == 0) {
+            // ---- the share's runs ----
+            TileCursor cur;
+            cur.u = cur.end = 0;
+            if (share < shares) {
+                cur.find(a, share * units / shares);
+                cur.end = (share + 1) * units / shares;
+            }
+            if (lane == 0) {
+                for (uint32_t number = 0;; ++number) {
+                    if (number >= TA_RUNS && (bar.failed || !wait(&bar.run_empty[number % TA_RUNS], (number / TA_RUNS - 1) & 1, 32))) break;
+                    TileRun &r = bar.runs[number % TA_RUNS];
+                    r.n = cur.u < cur.end ? cur.run() : 0;
+                    r.s = cur.s;
+                    r.b = cur.b;
+                    r.pair = cur.pair;
+                    r.head = cur.head;
+                    r.first = cur.block;
+                    r.blocks = cur.blocks;
+                    mbar_arrive(&bar.run_full[number % TA_RUNS]);
+                    if (cur.u >= cur.end) break;
+                    cur.next(a);
+                }
+            }
+        } else if (warp == 1 && elected()) {
+            // ---- products ----
+            constexpr uint32_t S_DESC = idesc_16(TA_KEYS, BF16 ? 1 : 0), O_DESC = idesc_16(D, 0);
+            const uint64_t q0 = umma_desc(base + M::Q), k0 = umma_desc(base + M::K), v0 = umma_desc(base + M::V);
+            uint32_t items = 0, pairs = 0, kc = 0, vc = 0, pc0 = 0, pc1 = 0;
+            const auto scores = [&](int tile, int stage) {
+#pragma unroll
+                for (int ks = 0; ks < D / 16; ++ks) {
+                    const uint64_t at = (uint64_t)((ks >> 2) * (TA_PANEL >> 4) + (ks & 3) * 2);
+                    umma_16(tmem + tile * TA_KEYS, q0 + (uint64_t)(tile * (M::Q_TILE >> 4)) + at, k0 + (uint64_t)(stage * (M::K_STAGE >> 4)) + at, S_DESC, ks > 0);
+                }
+                umma_commit(&bar.s_full[tile]);
+            };
+            const auto results = [&](int tile, int stage, bool more) {
+#pragma unroll
+                for (int ks = 0; ks < TA_KEYS / 16; ++ks)
+                    mma_from_tmem(tmem + 2 * TA_KEYS + tile * D, tmem + tile * TA_KEYS + ks * 8, v0 + (uint64_t)(stage * (M::V_STAGE >> 4) + (ks >> 2) * (D * 128 >> 4) + (ks & 3) * 2), O_DESC, more || ks > 0);
+            };
+            const auto after = [] { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); };
+            bool go = true;
+            for (;; ++items) {
+                const TileRun &run = run_of(items, go);
+                if (!go || run.n == 0) break;
+                const int n = run.n;
+                const bool two = second(run);
+                let_go(items);
+                go = wait(&bar.q_full[0], items & 1, 20) && (!two || wait(&bar.q_full[1], pairs++ & 1, 20)) && wait(&bar.k_full[kc & 1], (kc >> 1) & 1, 20);
+                if (!go) break;
+                after();
+                scores(0, kc & 1);
+                if (two) scores(1, kc & 1);
+                umma_commit(&bar.k_empty[kc++ & 1]);
+                for (int j = 0; j < n; ++j, ++vc) {
+                    const int vs = vc & 1, ks = kc & 1;
+                    go = !bar.failed && wait(&bar.v_full[vs], (vc >> 1) & 1, 20) && wait(&bar.p_full[0], pc0++ & 1, 20);
+                    if (!go) break;
+                    after();
+                    results(0, vs, j > 0);
+                    if (j + 1 < n) {
+                        go = wait(&bar.k_full[ks], (kc >> 1) & 1, 20);
+                        if (!go) break;
+                        after();
+                        scores(0, ks);  // over the P that the products before have read: they are carried out in order
+                    } else {
+                        umma_commit(&bar.o_full[0]);
+                    }
+                    if (two) {
+                        go = wait(&bar.p_full[1], pc1++ & 1, 20);
+                        if (!go) break;
+                        after();
+                        results(1, vs, j > 0);
+                    }
+                    umma_commit(&bar.v_empty[vs]);
+                    if (j + 1 < n) {
+                        if (two) scores(1, ks);
+                        umma_commit(&bar.k_empty[ks]);
+                        ++kc;
+                    } else if (two) {
+                        umma_commit(&bar.o_full[1]);
+                    }
+                }
+            }
+            if (bar.failed) {  // what was issued completes, or has its time to, before what it reads and writes is given back
+                umma_commit(&bar.drained);
+                mbar_wait(&bar.drained, 0);
+            } else if (vc > 0) {
+                mbar_wait(&bar.v_empty[(vc - 1) & 1], ((vc - 1) >> 1) & 1);
+                mbar_wait(&bar.k_empty[(kc - 1) & 1], ((kc - 1) >> 1) & 1);
+            }
+        }
+        __syncwarp();
+    } else if (warp < 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 120;");
+        // ---- operands ----
+        constexpr int WORDS = D / 8, VW = D / 64;  // words of a key; of a thread's keys in V
+        constexpr uint32_t MAGIC = BF16 ? 0x43004300u : 0x64006400u, LESS = BF16 ? 0xc308c308u : 0xe408e408u;
+        const int key = threadIdx.x - 128;                                             // of K and the scales
+        const int octet = (lane & 7) + 8 * ((warp - 4) & 1), word = ((lane >> 3) + 4 * ((warp - 4) >> 1)) * VW;  // of V: eight keys, VW words
+        int unit = 0;
+        uint32_t blocks_done = 0;
+        bool go = true;
+        uint4 kr[WORDS / 4];
+        uint32_t vr[8][VW];
+        float ks = 0.f, vs = 0.f;
+        bool here = false;
+        // the block that is on its way: number ahead_j of the run of number ahead
+        uint32_t ahead = 0, number = 0;
+        int ahead_n = 0, ahead_j = 0, ahead_keys = 0, ahead_first = 0, ahead_b = 0, ahead_head = 0;
+        const auto open_ahead = [&] {
+            const TileRun &r = run_of(ahead, go);
+            ahead_n = go ? r.n : 0;
+            ahead_keys = r.s.keys;
+            ahead_first = r.first;
+            ahead_b = r.b;
+            ahead_head = r.head;
+            ahead_j = 0;
+        };
+        const auto row_of = [&](int at) {  // row of the cache of a key of the block on its way, or -1
+            const int position = (ahead_first + ahead_j) * TA_KEYS + at;
+            return position < ahead_keys ? cache_row(c, ahead_b, position, ahead_head) : -1;
+        };
+        const auto fetch_k = [&] {
+            const int64_t row = ahead_n > 0 ? row_of(key) : -1;
+            here = row >= 0;
+#pragma unroll
+            for (int w = 0; w < WORDS / 4; ++w) kr[w] = here ? __ldg(reinterpret_cast<const uint4 *>(c.k_codes + row * (D / 2)) + w) : make_uint4(0u, 0u, 0u, 0u);
+            ks = here ? __half2float(c.k_scale[row]) : 0.f;
+            vs = here ? __half2float(c.v_scale[row]) : 0.f;
+        };
+        const auto fetch_v = [&] {
+            const int64_t row = ahead_n > 0 ? row_of(octet * 8) : -1;  // eight keys of one page: those past the last key lie in it, too, and count for nothing
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                if constexpr (VW == 2) {
+                    const uint2 v = row >= 0 ? __ldg(reinterpret_cast<const uint2 *>(c.v_codes + (row + k) * (D / 2) + word * 4)) : make_uint2(0u, 0u);
+                    vr[k][0] = v.x;
+                    vr[k][1] = v.y;
+                } else {
+                    vr[k][0] = row >= 0 ? __ldg(reinterpret_cast<const uint32_t *>(c.v_codes + (row + k) * (D / 2) + word * 4)) : 0u;
+                }
+            }
+        };
+        const auto step_ahead = [&] {
+            if (ahead_n == 0 || ++ahead_j < ahead_n) return;
+            ++ahead;
+            open_ahead();
+        };
+        open_ahead();
+        fetch_k();
+        fetch_v();
+        for (;; ++number) {
+            const int n = run_of(number, go).n;
+            if (!__all_sync(0xffffffffu, go) || n == 0) break;
+            unit = 0;
+            for (int j = 0; j < n; ++j, ++blocks_done) {
+                const int stage = blocks_done & 1, slot = blocks_done % TA_SCALES;
+                // ---- K, and the scales of the block ----
+                if (blocks_done >= 2) go = wait(&bar.k_empty[stage], ((blocks_done >> 1) - 1) & 1, 20);
+                go = __all_sync(0xffffffffu, go && !bar.failed);
+                if (!go) break;
+                const uint32_t kt = base + M::K + stage * M::K_STAGE + key * 128;
+#pragma unroll
+                for (int w = 0; w < WORDS; ++w) {
+                    const uint4 &r = kr[w >> 2];
+                    const uint32_t x = (w & 3) == 0 ? r.x : (w & 3) == 1 ? r.y : (w & 3) == 2 ? r.z : r.w, x4 = x >> 4;
+                    store_16s(kt + (w >> 3) * TA_PANEL + (((w & 7) ^ (key & 7)) << 4), halves_add((__byte_perm(x, x4, 0x4400) & 0x000f000fu) | MAGIC, LESS, BF16),
+                              halves_add((__byte_perm(x, x4, 0x5511) & 0x000f000fu) | MAGIC, LESS, BF16), halves_add((__byte_perm(x, x4, 0x6622) & 0x000f000fu) | MAGIC, LESS, BF16),
+                              halves_add((__byte_perm(x, x4, 0x7733) & 0x000f000fu) | MAGIC, LESS, BF16));
+                }
+                // the largest scale so far (one that is not finite sets no unit), and the values' scales in its power of two
+                const unsigned size = __float_as_uint(vs) & 0x7fffffffu;
+                const unsigned top = __reduce_max_sync(0xffffffffu, size < 0x7f800000u ? size : 0u), got = __ballot_sync(0xffffffffu, here);
+                if (lane == 0) bar.tops[warp - 4] = (int)(top >> 23);
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+                unit = max(max(unit, max(bar.tops[0], bar.tops[1])), max(bar.tops[2], bar.tops[3]));
+                const uint32_t sc = base + M::SCALES + slot * M::SCALE_STAGE + key * 4;
+                asm volatile("st.shared.f32 [%0], %1;" ::"r"(sc), "f"(ks * (MODS ? a.scale : a.scale * LOG2E)) : "memory");
+                asm volatile("st.shared.f32 [%0], %1;" ::"r"(sc + TA_KEYS * 4), "f"(vs * power_of_two(min(TA_UNIT - (unit - 127), 127))) : "memory");
+                if (lane == 0) bar.present[slot][warp - 4] = got;
+                if (threadIdx.x == 128) bar.unit[slot] = unit;
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                asm volatile("bar.sync 1, 128;" ::: "memory");  // the tops are read before the next block's are written
+                if (lane == 0) {
+                    mbar_arrive(&bar.scale_full[slot]);
+                    mbar_arrive(&bar.k_full[stage]);
+                }
+                step_ahead();
+                fetch_k();
+                // ---- V, transposed ----
+                if (blocks_done >= 2) go = wait(&bar.v_empty[stage], ((blocks_done >> 1) - 1) & 1, 20);
+                go = __all_sync(0xffffffffu, go && !bar.failed);
+                if (!go) break;
+                const uint32_t vt = base + M::V + stage * M::V_STAGE + (octet >> 3) * (D * 128);
+#pragma unroll
+                for (int w = 0; w < VW; ++w) {
+                    uint32_t lo[4], hi[4];  // of two keys each: the lower and the upper four codes
+#pragma unroll
+                    for (int p = 0; p < 4; ++p) {
+                        lo[p] = __byte_perm(vr[2 * p][w], vr[2 * p + 1][w], 0x5410);
+                        hi[p] = __byte_perm(vr[2 * p][w], vr[2 * p + 1][w], 0x7632);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const int d = (word + w) * 8 + e;
+                        uint32_t v[4];
+#pragma unroll
+                        for (int p = 0; p < 4; ++p) v[p] = halves_add((((e < 4 ? lo[p] : hi[p]) >> (4 * (e & 3))) & 0x000f000fu) | 0x64006400u, 0xe408e408u, false);
+                        store_16s(vt + d * 128 + (((octet & 7) ^ (d & 7)) << 4), v[0], v[1], v[2], v[3]);
+                    }
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bar.v_full[stage]);
+                fetch_v();
+            }
+            // the run's entry is needed no more: the block on its way belongs to the next one
+            if (!go) break;
+            __syncwarp();
+            if (lane == 0) let_go(number);
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
+        // ---- rows ----
+        const int tile = (warp - 8) >> 2, q = warp & 3, local = tile * 128 + q * 32 + lane;
+        const uint32_t s_at = tmem + ((uint32_t)(q * 32) << 16) + tile * TA_KEYS, o_at = tmem + ((uint32_t)(q * 32) << 16) + 2 * TA_KEYS + tile * D;
+        uint32_t sc = 0, tc = 0, oc = 0;  // blocks of the CTA, blocks and items of this tile
+        bool go = true;
+        for (uint32_t number = 0;; ++number) {
+            const TileRun &run = run_of(number, go);
+            if (!__all_sync(0xffffffffu, go) || run.n == 0) break;
+            const AttendSequence seq = run.s;
+            const int n = run.n, first = run.first;
+            const bool mine = tile == 0 || second(run), whole = first == 0 && n == run.blocks;
+            const int64_t r = (int64_t)run.pair * TA_ROWS + local, rows = (int64_t)seq.count * a.group;
+            const bool real = r < rows;
+            const int token = real ? (int)(r / a.group) : 0, h = run.head * a.group + (real ? (int)(r % a.group) : 0);
+            __syncwarp();
+            if (lane == 0) let_go(number);
+            if (!mine) {  // blocks that the other tile has alone
+                sc += n;
+                continue;
+            }
+            {
+                const uint4 *const from = reinterpret_cast<const uint4 *>((const uint16_t *)a.q + (int64_t)(seq.first + token) * a.q_token_stride + (int64_t)h * a.q_head_stride);
+                const uint32_t to = base + M::Q + tile * M::Q_TILE + (q * 32 + lane) * 128;
+#pragma unroll
+                for (int w = 0; w < D / 8; ++w) {
+                    const uint4 v = real ? __ldg(from + w) : make_uint4(0u, 0u, 0u, 0u);
+                    store_16s(to + (w >> 3) * TA_PANEL + (((w & 7) ^ (lane & 7)) << 4), v.x, v.y, v.z, v.w);
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bar.q_full[tile]);
+            }
+            const int limit = real ? visible_keys(a, seq, token) : 0x7fffffff;
+            const int least = __reduce_min_sync(0xffffffffu, limit);
+            const float slope = MODS && a.slopes ? a.slopes[h] : 0.f;
+            const int place = seq.length - seq.count + token;
+            float m = -INFINITY, l = 0.f;
+            int unit = 0;
+            for (int j = 0; j < n; ++j, ++sc, ++tc) {
+                const int slot = sc % TA_SCALES, key0 = (first + j) * TA_KEYS;
+                // The scores first: they come behind the scales, and a tile that left out blocks must not meet an earlier phase of the scales' barrier.
+                go = go && !bar.failed && wait(&bar.s_full[tile], tc & 1, 20) && wait(&bar.scale_full[slot], (sc / TA_SCALES) & 1, 20);
+                go = __all_sync(0xffffffffu, go);
+                if (!go) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t scales = base + M::SCALES + slot * M::SCALE_STAGE;
+                const bool masked = key0 + TA_KEYS > least || (bar.present[slot][0] & bar.present[slot][1] & bar.present[slot][2] & bar.present[slot][3]) != 0xffffffffu;
+                // Two passes over S in tensor memory, so that a thread need not hold a row: the maximum, then the exponentials.  Where scores are masked, capped or biased the
+                // first pass writes them back.
+                const bool stored = MODS || masked;
+                float top = -INFINITY;
+#pragma unroll 1
+                for (int cb = 0; cb < 4; ++cb) {
+                    uint32_t v[32];
+                    tmem_load_32(s_at + cb * 32, v);
+                    float u[32];
+#pragma unroll
+                    for (int x = 0; x < 32; x += 4) {
+                        const ulonglong2 k4 = load_4p(scales + (cb * 32 + x) * 4);
+                        unpack2(mul2(pack2(v[x], v[x + 1]), k4.x), u[x], u[x + 1]);
+                        unpack2(mul2(pack2(v[x + 2], v[x + 3]), k4.y), u[x + 2], u[x + 3]);
+                    }
+                    if (MODS) {
+#pragma unroll
+                        for (int x = 0; x < 32; ++x) {
+                            float w = u[x];
+                            if (a.softcap > 0.f) w = capped(w, a.softcap, 2.f * LOG2E / a.softcap);
+                            u[x] = fmaf(slope, (float)(key0 + cb * 32 + x - place), w) * LOG2E;
+                        }
+                    }
+                    if (stored) {
+                        if (masked) {
+                            const unsigned there = bar.present[slot][cb];
+#pragma unroll
+                            for (int x = 0; x < 32; ++x)
+                                if (key0 + cb * 32 + x >= limit || !((there >> x) & 1u)) u[x] = -INFINITY;
+                        }
+#pragma unroll
+                        for (int x = 0; x < 32; ++x) v[x] = __float_as_uint(u[x]);
+                        tmem_store_32(s_at + cb * 32, v);
+                    }
+#pragma unroll
+                    for (int x = 0; x < 32; x += 2) top = fmaxf(fmaxf(top, u[x]), u[x + 1]);
+                }
+                if (stored) tmem_stored();
+                // the maximum that the exponentials refer to, and the unit of the scales
+                const int new_unit = bar.unit[slot];
+                const bool first_seen = m == -INFINITY, moves = top > m + TA_SLACK || (first_seen && top > -INFINITY) || new_unit != unit;
+                if (__any_sync(0xffffffffu, moves)) {
+                    const float now = moves && top > m ? top : m;
+                    const float keep = first_seen ? 1.f : ex2(m - now);
+                    const float f = unit == 0 ? keep : keep * power_of_two(max(unit - new_unit, -126));
+                    l *= keep;
+                    m = now;
+                    unit = new_unit;
+                    if (j > 0) {
+#pragma unroll 1
+                        for (int cb = 0; cb < D / 32; ++cb) {
+                            uint32_t v[32];
+                            tmem_load_32(o_at + cb * 32, v);
+#pragma unroll
+                            for (int x = 0; x < 32; ++x) v[x] = __float_as_uint(__uint_as_float(v[x]) * f);
+                            tmem_store_32(o_at + cb * 32, v);
+                        }
+                    }
+                }
+                const float refer = m == -INFINITY ? 0.f : m;
+                const uint64_t less = pack2(__float_as_uint(-refer), __float_as_uint(-refer));
+                uint64_t sum = 0ull;
+#pragma unroll 1
+                for (int cb = 0; cb < 4; ++cb) {
+                    uint32_t v[32], p[16];
+                    tmem_load_32(s_at + cb * 32, v);
+#pragma unroll
+                    for (int x = 0; x < 32; x += 4) {
+                        const ulonglong2 k4 = load_4p(scales + (cb * 32 + x) * 4), v4 = load_4p(scales + (TA_KEYS + cb * 32 + x) * 4);
+#pragma unroll
+                        for (int y = 0; y < 2; ++y) {
+                            const uint64_t score = pack2(v[x + 2 * y], v[x + 2 * y + 1]);
+                            float e0, e1, w0, w1;
+                            unpack2(stored ? add2f(score, less) : fma2(score, y ? k4.y : k4.x, less), e0, e1);
+                            const uint64_t e = pack2(__float_as_uint(ex2(e0)), __float_as_uint(ex2(e1)));
+                            sum = add2f(sum, e);
+                            unpack2(mul2(e, y ? v4.y : v4.x), w0, w1);
+                            if (masked) {  // a masked key counts for nothing, whatever its scale
+                                if (v[x + 2 * y] == 0xff800000u) w0 = 0.f;
+                                if (v[x + 2 * y + 1] == 0xff800000u) w1 = 0.f;
+                            }
+                            p[x / 2 + y] = pack_halves(w0, w1, 0);
+                        }
+                    }
+                    tmem_store_16(s_at + cb * 16, p);  // over scores that this thread has read
+                }
+                float sum0, sum1;
+                unpack2(sum, sum0, sum1);
+                l += sum0 + sum1;
+                tmem_stored();
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bar.p_full[tile]);
+            }
+            // ---- this CTA's part of the item ----
+            if (go) go = wait(&bar.o_full[tile], oc & 1, 20);
+            ++oc;
+            go = __all_sync(0xffffffffu, go);
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            float f = power_of_two(max((unit - 127) - TA_UNIT, -126));
+            if (whole) f = l == 0.f ? 0.f : __fdividef(f, l);
+            if (!go) f = NAN;
+            const bool none = whole && l == 0.f && go;
+            float *const slot = tile_slot<D>(a, 2 * share + (first == 0 ? 1 : 0));
+#pragma unroll 1
+            for (int cb = 0; cb < D / 32; ++cb) {
+                uint32_t v[32];
+                if (go) {
+                    tmem_load_32(o_at + cb * 32, v);
+                } else {
+#pragma unroll
+                    for (int x = 0; x < 32; ++x) v[x] = 0u;
+                }
+                if (!real) continue;
+                float o[32];
+#pragma unroll
+                for (int x = 0; x < 32; ++x) o[x] = none ? 0.f : __uint_as_float(v[x]) * f;
+                if (whole) {
+                    uint4 *const to = reinterpret_cast<uint4 *>((uint16_t *)a.out + ((int64_t)(seq.first + token) * a.heads + h) * D + cb * 32);
+#pragma unroll
+                    for (int x = 0; x < 4; ++x)
+                        to[x] = make_uint4(pack_halves(o[8 * x], o[8 * x + 1], BF16), pack_halves(o[8 * x + 2], o[8 * x + 3], BF16), pack_halves(o[8 * x + 4], o[8 * x + 5], BF16),
+                                           pack_halves(o[8 * x + 6], o[8 * x + 7], BF16));
+                } else {
+                    float4 *const to = reinterpret_cast<float4 *>(slot + local * D + cb * 32);
+#pragma unroll
+                    for (int x = 0; x < 8; ++x) to[x] = make_float4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
+                }
+            }
+            if (real && !whole) {
+                slot[TA_ROWS * D + local] = m;
+                slot[TA_ROWS * D + TA_ROWS + local] = l;
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == 1) tmem_free<false>(tmem, 512);
+    if (threadIdx.x == 0 && bar.failed && a.status) atomicExch(a.status, -1);
+}
+
+// A CTA per share and 32 rows: where an item begins in the share and does not end there, adds up the parts that it has in this share and the ones behind, in the order of the keys.
+constexpr int TJ_THREADS = 256;
+template <int D>
+__global__ void __launch_bounds__(TJ_THREADS) attend_tiles_join_kernel(const AttendArgs a, int64_t most) {
+    constexpr int PER = D / 32;
+    __shared__ long long totals[TJ_THREADS / 32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int64_t units = 0;
+    for (int b = threadIdx.x; b < a.c.batch; b += TJ_THREADS) units += tile_units(a, b);
+    units = warp_sum(units);
+    if (lane == 0) totals[warp] = units;
+    __syncthreads();
+    units = 0;
+    for (int w = 0; w < TJ_THREADS / 32; ++w) units += totals[w];
+    const int64_t shares = min(units, most), share = blockIdx.x;
+    const int64_t end = share < shares ? (share + 1) * units / shares : 0;
+    TileCursor cur;
+    int64_t u0 = 0, u1 = 0;
+    if (share + 1 < shares) {
+        cur.find(a, end - 1);
+        u0 = end - 1 - cur.block;
+        u1 = u0 + cur.blocks;
+    }
+    after_the_launch_before();  // by every CTA: what follows on the stream must not start before the results are there
+    if (share + 1 >= shares || u1 <= end || u0 < share * units / shares) return;
+    const int64_t last = (u1 * shares - 1) / units;  // the share of unit u1 - 1: the last one that begins at or before it
+#pragma unroll 1
+    for (int i = warp; i < 32; i += TJ_THREADS / 32) {
+        const int local = blockIdx.y * 32 + i;
+        const int64_t r = (int64_t)cur.pair * TA_ROWS + local;
+        if (r >= (int64_t)cur.s.count * a.group) continue;
+        float acc[PER], top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int x = 0; x < PER; ++x) acc[x] = 0.f;
+        for (int64_t w = share; w <= last; ++w) {
+            const float *const slot = tile_slot<D>(a, 2 * w + (w == share ? 1 : 0));
+            const float m = __ldcg(slot + TA_ROWS * D + local), l = __ldcg(slot + TA_ROWS * D + TA_ROWS + local);
+            const float now = fmaxf(top, m), base = now == -INFINITY ? 0.f : now, mine = ex2(m - base), old = ex2(top - base);
+#pragma unroll
+            for (int x = 0; x < PER; ++x) acc[x] = acc[x] * old + __ldcg(slot + local * D + x * 32 + lane) * mine;
+            sum = sum * old + l * mine;
+            top = now;
+        }
+        const int token = (int)(r / a.group), h = cur.head * a.group + (int)(r % a.group);
+        uint16_t *const to = (uint16_t *)a.out + ((int64_t)(cur.s.first + token) * a.heads + h) * D;
+#pragma unroll
+        for (int x = 0; x < PER; ++x) {
+            const float o = sum == 0.f ? (acc[x] == acc[x] ? 0.f : acc[x]) : __fdividef(acc[x], sum);
+            to[x * 32 + lane] = (uint16_t)float_to_half_bits(o, a.c.bf16);
+        }
+    }
+}
+
+size_t attend_tiles_bytes(int head_dim) { return (size_t)TA_GRID * 2 * TA_ROWS * (head_dim + 2) * sizeof(float); }
+
+template <int D, bool BF16, bool MODS>
+static int launch_tiles(const AttendArgs &a, cudaStream_t st) {
+    static PerDeviceOnce configured;
+    constexpr size_t smem = TileShared<D>::BYTES;
+    if (configured.run([&] { return cudaFuncSetAttribute(attend_tiles_kernel<D, BF16, MODS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) == cudaSuccess; }) != G2D_OK) return G2D_ERR_CUDA;
+    attend_tiles_kernel<D, BF16, MODS><<<TA_GRID, TA_THREADS, smem, st>>>(a);
+    if (check_launch() != G2D_OK) return G2D_ERR_CUDA;
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(TA_GRID, TA_ROWS / 32);
+    config.blockDim = dim3(TJ_THREADS);
+    config.stream = st;
+    cudaLaunchAttribute attribute{};
+    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &attribute;
+    config.numAttrs = 1;
+    if (cudaLaunchKernelEx(&config, attend_tiles_join_kernel<D>, a, (int64_t)TA_GRID) != cudaSuccess) return G2D_ERR_CUDA;
+    return check_launch();
+}
+
+int launch_attend_tiles(const AttendArgs &a, cudaStream_t st) {
+    const bool mods = a.softcap > 0.f || a.slopes;
+    if (a.c.head_dim == 128) {
+        if (a.c.bf16) return mods ? launch_tiles<128, true, true>(a, st) : launch_tiles<128, true, false>(a, st);
+        return mods ? launch_tiles<128, false, true>(a, st) : launch_tiles<128, false, false>(a, st);
+    }
+    if (a.c.bf16) return mods ? launch_tiles<64, true, true>(a, st) : launch_tiles<64, true, false>(a, st);
+    return mods ? launch_tiles<64, false, true>(a, st) : launch_tiles<64, false, false>(a, st);
+}
+
+}  // namespace g2d

@@ -75,39 +75,4 @@ __device__ __forceinline__ uint32_t pack_halves(float lo, float hi, int bf16) {
     return r;
 }
 
-// ---- attention: what its kernels share (see g2d_attend.cu) ----
-struct AttendArgs {
-    CacheView c;
-    const void *q;
-    void *out;  // [tokens, heads, head_dim]
-    int64_t q_token_stride, q_head_stride;
-    int heads, group;
-    int causal;
-    float scale;             // of the scores
-    float softcap;           // 0: none
-    const float *slopes;     // per head, or null
-    const int32_t *prefix;   // per sequence, or null
-    int rows_from, rows_to;  // the kernel's sequences: those with rows_from <= queries x group < rows_to
-    float *partial;
-    int *status;
-    long long wait_cycles;
-};
-struct AttendSequence {
-    int first, count, length, keys, prefix;
-};
-__device__ __forceinline__ AttendSequence attend_sequence(const AttendArgs &a, int b) {
-    AttendSequence s;
-    tokens_of(a.c, b, s.first, s.count);
-    s.length = a.c.lengths[b];
-    s.keys = keys_of(a.c, s.length);
-    s.prefix = a.prefix ? a.prefix[b] : 0;
-    return s;
-}
-// how many keys, from the first on, token i of the sequence sees
-__device__ __forceinline__ int visible_keys(const AttendArgs &a, const AttendSequence &s, int i) {
-    if (!a.causal) return s.keys;
-    const int64_t p = (int64_t)s.length - s.count + i;
-    return (int)min((int64_t)s.keys, max(p + 1, max((int64_t)s.prefix, (int64_t)0)));
-}
-
 }  // namespace g2d

@@ -104,18 +104,6 @@ __device__ __forceinline__ uint4 load_16(uint32_t at) {
     return v;
 }
 
-// One thread of the warp, all of whose threads are here.  The compiler knows that a branch on this leaves one thread, and keeps what a product's instruction takes
-// from uniform registers there; behind a comparison of lane numbers it does not.
-__device__ __forceinline__ bool elected() {
-    uint32_t one;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "elect.sync _|p, 0xffffffff;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(one));
-    return one != 0;
-}
-
 // A warp that arrives at another CTA's barrier with .release waits until all it wrote has arrived everywhere (a thousand cycles, in the middle of the pipeline's chain:
 // 8192 x 28672, 2048 tokens, 940 and 885 us).  What the coders write stays in their CTA's shared memory and is read by that SM's tensor core alone; they have brought it
 // there by their proxy fence before they arrive, so that the message itself need order nothing.

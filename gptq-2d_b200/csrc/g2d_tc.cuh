@@ -105,6 +105,18 @@ __device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
+// One thread of the warp, all of whose threads are here.  The compiler knows that a branch on this leaves one thread, and keeps what a product's instruction takes
+// from uniform registers there; behind a comparison of lane numbers it does not.
+__device__ __forceinline__ bool elected() {
+    uint32_t one;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(one));
+    return one != 0;
+}
+
 // ---- shared state of a CTA of TC_THREADS threads: warp 0 loads, warp 1 issues the MMAs, warps 2-5 read the accumulators ----
 struct TcRing {
     uint64_t full[STAGES], empty[STAGES], accum;
