@@ -5,9 +5,10 @@
 // with k_j = s_j (c_j - 8), v_j likewise, codes c in 0 .. 15, and zeros where no j is left.  The rows of one kv head are all (token, head of its group).
 //
 // Work.  A unit is a block of 64 keys of one item (sequence, kv head, eight or sixteen rows).  The units of all items, one after the other, are dealt
-// out evenly to the warps of the grid, however long each sequence is: lengths are known on the device only.  A warp goes through its units with a running
-// maximum and sum per row and keeps its results in registers; an item that lies within one warp's share is written at once, the others leave
-// partial results (at most two per warp) that attend_join_kernel adds up in the order of the keys.
+// out evenly to the CTAs, and a CTA's to its warps, however long each sequence is: lengths are known on the device only.  A warp goes through its units with a
+// running maximum and sum per row and keeps its results in registers; an item that lies within one warp's share is written at once, the others leave
+// partial results (at most two per warp), which the CTA adds up in the order of the keys; what of an item lies in several CTAs (at most two parts
+// per CTA) attend_join_kernel adds up.
 //
 // Mathematics.  Codes go to the tensor cores as they are: the bits of c in the lowest (or next) four bits of an fp16 number are c 2^-24 (or c 2^-20), exactly,
 // so four codes cost two ANDs and a shift.  The scores are S^T = K Q^T with keys as the rows of A (m16n8k16), the channels of k in the order in which a word of
@@ -29,11 +30,17 @@ struct AttendStage {
     uint8_t k[CACHE_BLOCK * D / 2], v[CACHE_BLOCK * D / 2];
     __half ks[CACHE_BLOCK], vs[CACHE_BLOCK];
 };
+// A warp's part of an item that it has not the whole of
+struct AttendPart {
+    int b, item, first, last, blocks;  // blocks first .. last - 1 of `blocks`; last 0: no part
+    AttendSequence s;
+};
 template <int D>
 struct AttendShared {
     AttendStage<D> stage[ATTEND_WARPS][ATTEND_STAGES];
     uint64_t full[ATTEND_WARPS][ATTEND_STAGES];
     long long totals[ATTEND_WARPS];
+    AttendPart parts[2 * ATTEND_WARPS];
 };
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -124,11 +131,12 @@ struct AttendCursor {
     }
 };
 
-// Partial results: for each of a slot's rows, head_dim sums, the maximum and the sum of the exponentials
+// Partial results: for each of a slot's rows, head_dim sums, the maximum and the sum of the exponentials.  Two slots per CTA, behind them two per warp.
 template <int D, int ROWS>
 __device__ __forceinline__ float *attend_slot(const AttendArgs &a, int64_t slot) {
     return a.partial + slot * (ROWS * (D + 2));
 }
+constexpr int WARP_SLOTS = 2 * ATTEND_GRID;
 
 template <int D, int NT, bool MODS>
 __global__ void __launch_bounds__(ATTEND_THREADS, 1) attend_rows_kernel(const AttendArgs a) {
@@ -142,18 +150,23 @@ __global__ void __launch_bounds__(ATTEND_THREADS, 1) attend_rows_kernel(const At
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     let_the_next_launch_start();
+    if (lane < 2) sh.parts[2 * warp + lane].last = 0;
     const int64_t units = all_units<ATTEND_WARPS>(a, ROWS, sh.totals);  // its barrier is that of the initialisation as well
-    const int64_t shares = min(units, (int64_t)gridDim.x * ATTEND_WARPS);
-    const int64_t share = (int64_t)warp * gridDim.x + blockIdx.x;  // neighbours in the list on different SMs: few units still fill the GPU
-    if (share >= shares) return;
+    const int64_t shares = min(units, (int64_t)gridDim.x), share = blockIdx.x;
     AttendCursor cur;
-    cur.u = share * units / shares;
-    cur.end = (share + 1) * units / shares;
-    int64_t before;
-    cur.b = sequence_of_unit(a, ROWS, cur.u, before);
-    cur.open(a, ROWS);
-    cur.item = (int)((cur.u - before) / cur.blocks);
-    cur.block = (int)((cur.u - before) % cur.blocks);
+    cur.u = cur.end = 0;
+    if (share < shares) {
+        const int64_t u0 = share * units / shares, n = (share + 1) * units / shares - u0;
+        cur.u = u0 + warp * n / ATTEND_WARPS;
+        cur.end = u0 + (warp + 1) * n / ATTEND_WARPS;
+    }
+    if (cur.u < cur.end) {
+        int64_t before;
+        cur.b = sequence_of_unit(a, ROWS, cur.u, before);
+        cur.open(a, ROWS);
+        cur.item = (int)((cur.u - before) / cur.blocks);
+        cur.block = (int)((cur.u - before) % cur.blocks);
+    }
 
     // ---- loads: a block's keys lie in one page or in several; lane x brings piece x / 4 of codes or scales, of keys or values ----
     const int piece_shift = min(c.page_shift, 6), piece_keys = 1 << piece_shift, pieces = CACHE_BLOCK >> piece_shift;
@@ -454,7 +467,9 @@ __global__ void __launch_bounds__(ATTEND_THREADS, 1) attend_rows_kernel(const At
         }
         // ---- this warp's part of the item ----
         const bool whole = first_block == 0 && last_block == cur.blocks;
-        float *const slot = attend_slot<D, ROWS>(a, 2 * share + (first_block == 0 ? 1 : 0));
+        const int part = 2 * warp + (first_block == 0 ? 1 : 0);
+        float *const slot = attend_slot<D, ROWS>(a, WARP_SLOTS + 2 * ATTEND_WARPS * share + part);
+        if (!whole && lane == 0) sh.parts[part] = AttendPart{cur.b, cur.item, first_block, last_block, cur.blocks, seq};
         const float back = power_of_two(max(24 - 13 + (unit - 127), -126));
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
@@ -505,92 +520,149 @@ __global__ void __launch_bounds__(ATTEND_THREADS, 1) attend_rows_kernel(const At
         let_it_land();  // loads under way must not outlive the shared memory
         if (a.status) atomicExch(a.status, -1);
     }
-}
-
-// One CTA per output row: adds up the parts that an item has in several shares, in the order of the keys.
-constexpr int JOIN_WARPS = 4;
-template <int D, int NT>
-__global__ void __launch_bounds__(32 * JOIN_WARPS) attend_join_kernel(const AttendArgs a, int64_t warps) {
-    constexpr int ROWS = 8 * NT, PER = D / 32;
-    __shared__ long long totals[JOIN_WARPS];
-    __shared__ float sums[JOIN_WARPS][D], tops[JOIN_WARPS], parts[JOIN_WARPS];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int token = blockIdx.x / a.heads, h = blockIdx.x % a.heads;
-    int first, count, blocks, items;
-    const int b = sequence_of(a.c, token, first, count);
-    const int64_t units = all_units<JOIN_WARPS>(a, ROWS, totals);
-    int64_t before = 0;
-    for (int x = lane; x < b; x += 32) before += attend_units(a, x, ROWS);
-    before = warp_sum(before);
-    after_the_launch_before();  // by every CTA: what follows on the stream must not start before the results are there
-    if (b < 0) return;
-    const AttendSequence s = attend_sequence(a, b);
-    if (attend_units(a, s, ROWS, blocks, items) == 0) return;
-    const int row = (token - first) * a.group + h % a.group, item = row / ROWS * a.c.kv_heads + h / a.group, i = row % ROWS;
-    const int64_t shares = min(units, warps), u0 = before + (int64_t)item * blocks, u1 = u0 + blocks;
-    // share w has the units from w units / shares on: the last w with w units / shares <= u
-    const auto owner = [&](int64_t u) { return ((u + 1) * shares - 1) / units; };
-    const int64_t w0 = owner(u0), w1 = owner(u1 - 1);
-    if (w0 == w1) return;  // written already
-    float acc[PER], top = -INFINITY, sum = 0.f;
-#pragma unroll
-    for (int x = 0; x < PER; ++x) acc[x] = 0.f;
-    for (int64_t w = w0 + warp; w <= w1; w += JOIN_WARPS) {
-        const int64_t begins = w * units / shares;
-        const float *const slot = attend_slot<D, ROWS>(a, 2 * w + (begins <= u0 ? 1 : 0));
-        const float m = __ldcg(slot + ROWS * D + i), l = __ldcg(slot + ROWS * D + ROWS + i);
-        float v[PER];
-#pragma unroll
-        for (int x = 0; x < PER; ++x) v[x] = __ldcg(slot + i * D + x * 32 + lane);
-        const float now = fmaxf(top, m), base = now == -INFINITY ? 0.f : now, mine = ex2(m - base), old = ex2(top - base);
-#pragma unroll
-        for (int x = 0; x < PER; ++x) acc[x] = acc[x] * old + v[x] * mine;
-        sum = sum * old + l * mine;
-        top = now;
-    }
-#pragma unroll
-    for (int x = 0; x < PER; ++x) sums[warp][x * 32 + lane] = acc[x];
-    if (lane == 0) tops[warp] = top, parts[warp] = sum;
+    // ---- the warps' parts of an item, in the order of the keys: parts that stand together in the list ----
     __syncthreads();
-    if (threadIdx.x >= D) return;
-    float now = -INFINITY, all = 0.f, o = 0.f;
+    const auto next_part = [&](int p) {
+        while (p < 2 * ATTEND_WARPS && sh.parts[p].last == 0) ++p;
+        return p;
+    };
+    for (int p0 = next_part(0); p0 < 2 * ATTEND_WARPS;) {
+        const AttendPart &begin = sh.parts[p0];
+        unsigned mask = 1u << p0;
+        int p1 = p0, behind = next_part(p0 + 1);
+        while (behind < 2 * ATTEND_WARPS && sh.parts[behind].b == begin.b && sh.parts[behind].item == begin.item) {
+            p1 = behind;
+            mask |= 1u << behind;
+            behind = next_part(behind + 1);
+        }
+        const int count = __popc(mask), first = begin.first, last = sh.parts[p1].last;
+        const bool whole = first == 0 && last == begin.blocks;
+        const int head = begin.item % c.kv_heads, row0 = begin.item / c.kv_heads * ROWS, rows = begin.s.count * a.group;
+        const auto slot_of = [&](int i) {  // the i-th bit of the mask: parts stand close together, so that this is short
+            unsigned left = mask;
+            for (int k = 0; k < i; ++k) left &= left - 1;
+            return attend_slot<D, ROWS>(a, WARP_SLOTS + 2 * ATTEND_WARPS * share + __ffs(left) - 1);
+        };
+        for (int i = warp; i < ROWS && row0 + i < rows; i += ATTEND_WARPS) {
+            float acc[D / 32], m, l;
+            merge_parts<D>(count, [&](int k) { return slot_of(k) + i * D; }, [&](int k) { return slot_of(k) + ROWS * D + i; }, [&](int k) { return slot_of(k) + ROWS * D + ROWS + i; }, acc, m, l);
+            if (whole) {
+                const int token = (row0 + i) / a.group, h = head * a.group + (row0 + i) % a.group;
+                write_row<D>((uint16_t *)a.out + ((int64_t)(begin.s.first + token) * a.heads + h) * D, acc, l, c.bf16);
+            } else {
+                float *const slot = attend_slot<D, ROWS>(a, 2 * share + (first == 0 ? 1 : 0));
 #pragma unroll
-    for (int w = 0; w < JOIN_WARPS; ++w) now = fmaxf(now, tops[w]);
-    const float base = now == -INFINITY ? 0.f : now;
-#pragma unroll
-    for (int w = 0; w < JOIN_WARPS; ++w) {
-        const float f = ex2(tops[w] - base);
-        all += parts[w] * f;
-        o += sums[w][threadIdx.x] * f;
+                for (int x = 0; x < D / 32; ++x) slot[i * D + x * 32 + lane] = acc[x];
+                if (lane == 0) {
+                    slot[ROWS * D + i] = m;
+                    slot[ROWS * D + ROWS + i] = l;
+                }
+            }
+        }
+        p0 = behind;
     }
-    o = all == 0.f ? (o == o ? 0.f : o) : __fdividef(o, all);
-    ((uint16_t *)a.out)[((int64_t)token * a.heads + h) * D + threadIdx.x] = (uint16_t)float_to_half_bits(o, a.c.bf16);
+    after_the_launch_before();  // of the tiles' kernel: what follows waits for this one alone
 }
 
-template <int D, int NT, bool MODS>
-static int launch_rows(const AttendArgs &a, cudaStream_t st) {
-    static PerDeviceOnce configured;
-    constexpr size_t smem = sizeof(AttendShared<D>);
-    if (configured.run([&] { return cudaFuncSetAttribute(attend_rows_kernel<D, NT, MODS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) == cudaSuccess; }) != G2D_OK)
-        return G2D_ERR_CUDA;
-    attend_rows_kernel<D, NT, MODS><<<ATTEND_GRID, ATTEND_THREADS, smem, st>>>(a);
-    if (check_launch() != G2D_OK) return G2D_ERR_CUDA;
+// Adds up what items that lie in several CTAs' shares left, in the order of the keys.  A CTA per share and (tiles) 32 rows or (rows) all rows of an item: the one whose
+// share an item begins in and does not end in.
+constexpr int JOIN_THREADS = 256, TILE_JOINS = TA_ROWS / 32;
+struct JoinArgs {
+    AttendArgs tiles, rows;
+    int tile_ctas;  // the first so many are the tiles'
+};
+template <int D, int NT>
+__global__ void __launch_bounds__(JOIN_THREADS) attend_join_kernel(const JoinArgs j) {
+    constexpr int ROWS = 8 * NT, WARPS = JOIN_THREADS / 32;
+    __shared__ long long totals[WARPS];
+    const int warp = threadIdx.x >> 5;
+    if ((int)blockIdx.x < j.tile_ctas) {
+        const AttendArgs &a = j.tiles;
+        const int64_t units = all_tile_units<WARPS>(a, totals), shares = min(units, (int64_t)TA_GRID), share = blockIdx.x / TILE_JOINS;
+        TileCursor cur;
+        int64_t u0 = 0, u1 = 0, end = 0;
+        if (share + 1 < shares) {
+            end = (share + 1) * units / shares;
+            cur.find(a, end - 1);
+            u0 = end - 1 - cur.block;
+            u1 = u0 + cur.blocks;
+        }
+        after_the_launch_before();  // by every CTA: what follows on the stream must not start before the results are there
+        if (u1 <= end || u0 < share * units / shares) return;
+        const int count = (int)((u1 * shares - 1) / units - share) + 1;  // the share of unit u1 - 1 is the last one that begins at or before it
+        const auto slot_of = [&](int k) { return tile_slot<D>(a, 2 * (share + k) + (k == 0 ? 1 : 0)); };
+        for (int i = blockIdx.x % TILE_JOINS * 32 + warp, n = 0; n < 32 / WARPS; ++n, i += WARPS) {
+            const int r = cur.pair * TA_ROWS + i;
+            if (r >= cur.s.count * a.group) break;
+            float acc[D / 32], m, l;
+            merge_parts<D>(count, [&](int k) { return slot_of(k) + i * D; }, [&](int k) { return slot_of(k) + TA_ROWS * D + i; }, [&](int k) { return slot_of(k) + TA_ROWS * D + TA_ROWS + i; }, acc, m, l);
+            write_row<D>((uint16_t *)a.out + ((int64_t)(cur.s.first + r / a.group) * a.heads + cur.head * a.group + r % a.group) * D, acc, l, a.c.bf16);
+        }
+    } else {
+        const AttendArgs &a = j.rows;
+        const int64_t units = all_units<WARPS>(a, ROWS, totals), shares = min(units, (int64_t)ATTEND_GRID), share = blockIdx.x - j.tile_ctas;
+        AttendCursor cur;
+        int64_t u0 = 0, u1 = 0, end = 0;
+        if (share + 1 < shares) {
+            int64_t before;
+            end = (share + 1) * units / shares;
+            cur.u = end - 1;
+            cur.end = end;
+            cur.b = sequence_of_unit(a, ROWS, end - 1, before);
+            cur.open(a, ROWS);
+            cur.item = (int)((end - 1 - before) / cur.blocks);
+            u0 = before + (int64_t)cur.item * cur.blocks;
+            u1 = u0 + cur.blocks;
+        }
+        after_the_launch_before();
+        if (u1 <= end || u0 < share * units / shares) return;
+        const int count = (int)((u1 * shares - 1) / units - share) + 1;
+        const auto slot_of = [&](int k) { return attend_slot<D, ROWS>(a, 2 * (share + k) + (k == 0 ? 1 : 0)); };
+        for (int i = warp; i < ROWS; i += WARPS) {
+            const int r = cur.item / a.c.kv_heads * ROWS + i;
+            if (r >= cur.s.count * a.group) break;
+            float acc[D / 32], m, l;
+            merge_parts<D>(count, [&](int k) { return slot_of(k) + i * D; }, [&](int k) { return slot_of(k) + ROWS * D + i; }, [&](int k) { return slot_of(k) + ROWS * D + ROWS + i; }, acc, m, l);
+            write_row<D>((uint16_t *)a.out + ((int64_t)(cur.s.first + r / a.group) * a.heads + cur.item % a.c.kv_heads * a.group + r % a.group) * D, acc, l, a.c.bf16);
+        }
+    }
+}
+
+// A launch on the stream behind the one before, as a programmatic dependent launch
+template <typename Args>
+static int launch_behind(void (*kernel)(Args), unsigned grid, int threads, size_t smem, const Args &args, cudaStream_t st) {
     cudaLaunchConfig_t config{};
-    config.gridDim = dim3((unsigned)(a.c.tokens * a.heads));
-    config.blockDim = dim3(32 * JOIN_WARPS);
+    config.gridDim = dim3(grid);
+    config.blockDim = dim3((unsigned)threads);
+    config.dynamicSmemBytes = smem;
     config.stream = st;
     cudaLaunchAttribute attribute{};
     attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attribute.val.programmaticStreamSerializationAllowed = 1;
     config.attrs = &attribute;
     config.numAttrs = 1;
-    if (cudaLaunchKernelEx(&config, attend_join_kernel<D, NT>, a, (int64_t)ATTEND_GRID * ATTEND_WARPS) != cudaSuccess) return G2D_ERR_CUDA;
-    return check_launch();
+    return cudaLaunchKernelEx(&config, kernel, args) == cudaSuccess ? check_launch() : G2D_ERR_CUDA;
 }
 
+// rows and tiles: either or both; both launches share the sequences out between them
+template <int D, int NT, bool MODS>
+static int launch_rows(const AttendArgs &a, bool behind_tiles, cudaStream_t st) {
+    static PerDeviceOnce configured;
+    constexpr size_t smem = sizeof(AttendShared<D>);
+    if (configured.run([&] { return cudaFuncSetAttribute(attend_rows_kernel<D, NT, MODS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) == cudaSuccess; }) != G2D_OK)
+        return G2D_ERR_CUDA;
+    if (behind_tiles) return launch_behind(attend_rows_kernel<D, NT, MODS>, ATTEND_GRID, ATTEND_THREADS, smem, a, st);
+    attend_rows_kernel<D, NT, MODS><<<ATTEND_GRID, ATTEND_THREADS, smem, st>>>(a);
+    return check_launch();
+}
 template <int D, int NT>
-static int launch_rows_for(const AttendArgs &a, cudaStream_t st) {
-    return a.softcap > 0.f || a.slopes ? launch_rows<D, NT, true>(a, st) : launch_rows<D, NT, false>(a, st);
+static int launch_attend(const AttendArgs &rows, const AttendArgs &tiles, bool few, bool many, cudaStream_t st) {
+    int launched = G2D_OK;
+    if (many) launched = launch_attend_tiles(tiles, st);
+    if (launched == G2D_OK && few) launched = rows.softcap > 0.f || rows.slopes ? launch_rows<D, NT, true>(rows, many, st) : launch_rows<D, NT, false>(rows, many, st);
+    if (launched != G2D_OK) return launched;
+    const JoinArgs j{tiles, rows, many ? TA_GRID * TILE_JOINS : 0};
+    return launch_behind(attend_join_kernel<D, NT>, (unsigned)(j.tile_ctas + (few ? ATTEND_GRID : 0)), JOIN_THREADS, 0, j, st);
 }
 
 // From here on a sequence's rows go by tiles; both sides of the line: see the figures in g2d_attend_tc.cu.
@@ -601,7 +673,7 @@ struct AttendSpace {
 };
 static AttendSpace attend_space(int head_dim) {
     AttendSpace s;
-    s.tiles = ((size_t)ATTEND_GRID * ATTEND_WARPS * 2 * 16 * (head_dim + 2) * sizeof(float) + 255) & ~(size_t)255;
+    s.tiles = ((size_t)ATTEND_GRID * (ATTEND_WARPS + 1) * 2 * 16 * (head_dim + 2) * sizeof(float) + 255) & ~(size_t)255;
     s.all = s.tiles + attend_tiles_bytes(head_dim);
     return s;
 }
@@ -645,17 +717,15 @@ extern "C" int g2d_cache_attend(const g2d_attend_desc *d, void *stream) {
     cudaStream_t st = (cudaStream_t)stream;
     // How many rows a sequence has is known here only where all have the same; else the kernels share the sequences out between them.
     const int64_t rows = a.c.offsets ? -1 : (int64_t)(a.c.tokens / a.c.batch) * a.group;
-    if (rows < 0 || rows >= TILE_ROWS_FROM) {
-        a.rows_from = TILE_ROWS_FROM;
-        a.rows_to = 0x7fffffff;
-        a.partial = (float *)((char *)d->workspace + attend_space(a.c.head_dim).tiles);
-        const int launched = launch_attend_tiles(a, st);
-        if (launched != G2D_OK || rows >= TILE_ROWS_FROM) return launched;
-    }
+    const bool many = rows < 0 ? (int64_t)a.c.tokens * a.group >= TILE_ROWS_FROM : rows >= TILE_ROWS_FROM, few = rows < TILE_ROWS_FROM;
+    AttendArgs t = a;
+    t.rows_from = TILE_ROWS_FROM;
+    t.rows_to = 0x7fffffff;
+    t.partial = (float *)((char *)d->workspace + attend_space(a.c.head_dim).tiles);
     a.rows_from = 1;
     a.rows_to = TILE_ROWS_FROM;
     a.partial = (float *)d->workspace;
     const bool narrow = a.group <= 8 && (rows < 0 || rows <= 8);
-    if (a.c.head_dim == 128) return narrow ? launch_rows_for<128, 1>(a, st) : launch_rows_for<128, 2>(a, st);
-    return narrow ? launch_rows_for<64, 1>(a, st) : launch_rows_for<64, 2>(a, st);
+    if (a.c.head_dim == 128) return narrow ? launch_attend<128, 1>(a, t, few, many, st) : launch_attend<128, 2>(a, t, few, many, st);
+    return narrow ? launch_attend<64, 1>(a, t, few, many, st) : launch_attend<64, 2>(a, t, few, many, st);
 }

@@ -16,7 +16,7 @@
 
 namespace g2d {
 
-constexpr int TA_THREADS = 512, TA_ROWS = 256, TA_KEYS = 128, TA_GRID = 148, TA_SCALES = 4;
+constexpr int TA_THREADS = 512, TA_SCALES = 4;
 constexpr int TA_PANEL = 128 * 128;  // bytes of 128 rows of 64 16-bit values
 constexpr float TA_SLACK = 8.f;      // how far scores may exceed the maximum that the exponentials refer to, as a power of two
 constexpr int TA_UNIT = 6;           // the largest scale is brought to 2^6 .. 2^7: times 2^8, still a number of fp16
@@ -100,92 +100,6 @@ __device__ __forceinline__ uint32_t halves_add(uint32_t u, uint32_t v, bool bf16
     return r;
 }
 
-// ---- units: for each sequence, each tile pair of rows (later rows see more keys), each kv head, the blocks of keys that the last of its rows sees ----
-__device__ __forceinline__ int tile_pairs(const AttendArgs &a, const AttendSequence &s) {
-    const int64_t rows = (int64_t)s.count * a.group;
-    return rows >= a.rows_from && rows < a.rows_to ? (int)((rows + TA_ROWS - 1) / TA_ROWS) : 0;
-}
-__device__ __forceinline__ int tile_blocks(const AttendArgs &a, const AttendSequence &s, int pair) {
-    const int64_t last = min((int64_t)s.count * a.group, (int64_t)(pair + 1) * TA_ROWS) - 1;
-    return max((visible_keys(a, s, (int)(last / a.group)) + TA_KEYS - 1) / TA_KEYS, 1);
-}
-__device__ __forceinline__ int64_t tile_units(const AttendArgs &a, int b) {
-    if (b >= a.c.batch) return 0;
-    const AttendSequence s = attend_sequence(a, b);
-    int64_t sum = 0;
-    for (int p = 0, n = tile_pairs(a, s); p < n; ++p) sum += tile_blocks(a, s, p);
-    return sum * a.c.kv_heads;
-}
-struct TileCursor {
-    int64_t u, end;
-    int b, pair, pairs, head, block, blocks;
-    AttendSequence s;
-    __device__ __forceinline__ void open(const AttendArgs &a) {  // sequence b, or the next one that has units
-        for (;; ++b) {
-            if (b >= a.c.batch) {  // not reached while u < end
-                end = u;
-                return;
-            }
-            s = attend_sequence(a, b);
-            pairs = tile_pairs(a, s);
-            if (pairs > 0) break;
-        }
-        pair = head = block = 0;
-        blocks = tile_blocks(a, s, 0);
-    }
-    // A warp: unit `at` of the list
-    __device__ __forceinline__ void find(const AttendArgs &a, int64_t at) {
-        const int lane = threadIdx.x & 31;
-        int64_t base = 0;
-        u = at;
-        b = a.c.batch;
-        for (int b0 = 0; b0 < a.c.batch; b0 += 32) {
-            int64_t sum = tile_units(a, b0 + lane);
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int64_t up = __shfl_up_sync(0xffffffffu, sum, o);
-                if (lane >= o) sum += up;
-            }
-            const unsigned past = __ballot_sync(0xffffffffu, base + sum > at);
-            if (past) {
-                const int k = __ffs(past) - 1;
-                const int64_t upto = __shfl_sync(0xffffffffu, sum, k > 0 ? k - 1 : 0);
-                if (k > 0) base += upto;
-                b = b0 + k;
-                break;
-            }
-            base += __shfl_sync(0xffffffffu, sum, 31);
-        }
-        open(a);
-        int64_t rest = at - base;
-        while (pair + 1 < pairs && rest >= (int64_t)blocks * a.c.kv_heads) {
-            rest -= (int64_t)blocks * a.c.kv_heads;
-            blocks = tile_blocks(a, s, ++pair);
-        }
-        head = (int)(rest / blocks);
-        block = (int)(rest % blocks);
-    }
-    __device__ __forceinline__ int run() const { return (int)min((int64_t)(blocks - block), end - u); }  // blocks of the item in this share
-    __device__ __forceinline__ void next(const AttendArgs &a) {                                           // the item behind this run
-        u += run();
-        if (u >= end) return;
-        block = 0;
-        if (++head < a.c.kv_heads) return;
-        head = 0;
-        if (++pair < pairs) {
-            blocks = tile_blocks(a, s, pair);
-            return;
-        }
-        ++b;
-        open(a);
-    }
-};
-// Partial results: for each of a slot's 256 rows, head_dim sums, the maximum and the sum of the exponentials
-template <int D>
-__device__ __forceinline__ float *tile_slot(const AttendArgs &a, int64_t slot) {
-    return a.partial + slot * (TA_ROWS * (D + 2));
-}
-
 template <int D, bool BF16, bool MODS>
 __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const AttendArgs a) {
     using M = TileShared<D>;
@@ -219,17 +133,13 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const Atten
         bar.failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    let_the_next_launch_start();
+    const int64_t units = all_tile_units<TA_THREADS / 32>(a, bar.totals);  // its barrier is that of the initialisation as well
+    if (units == 0) return;                                                // sequences of few rows only
     if (warp == 1) tmem_alloc<false>(&bar.tmem, 512);
-    int64_t units = 0;
-    for (int b = threadIdx.x; b < c.batch; b += TA_THREADS) units += tile_units(a, b);
-    units = warp_sum(units);
-    if (lane == 0) bar.totals[warp] = units;
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    let_the_next_launch_start();
-    units = 0;
-    for (int w = 0; w < TA_THREADS / 32; ++w) units += bar.totals[w];
     const uint32_t tmem = bar.tmem;
     const int64_t shares = min(units, (int64_t)gridDim.x), share = blockIdx.x;
     // the run of that number, for every thread of a role; its entry stays until all roles have let it go
@@ -657,59 +567,6 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const Atten
     if (threadIdx.x == 0 && bar.failed && a.status) atomicExch(a.status, -1);
 }
 
-// A CTA per share and 32 rows: where an item begins in the share and does not end there, adds up the parts that it has in this share and the ones behind, in the order of the keys.
-constexpr int TJ_THREADS = 256;
-template <int D>
-__global__ void __launch_bounds__(TJ_THREADS) attend_tiles_join_kernel(const AttendArgs a, int64_t most) {
-    constexpr int PER = D / 32;
-    __shared__ long long totals[TJ_THREADS / 32];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    int64_t units = 0;
-    for (int b = threadIdx.x; b < a.c.batch; b += TJ_THREADS) units += tile_units(a, b);
-    units = warp_sum(units);
-    if (lane == 0) totals[warp] = units;
-    __syncthreads();
-    units = 0;
-    for (int w = 0; w < TJ_THREADS / 32; ++w) units += totals[w];
-    const int64_t shares = min(units, most), share = blockIdx.x;
-    const int64_t end = share < shares ? (share + 1) * units / shares : 0;
-    TileCursor cur;
-    int64_t u0 = 0, u1 = 0;
-    if (share + 1 < shares) {
-        cur.find(a, end - 1);
-        u0 = end - 1 - cur.block;
-        u1 = u0 + cur.blocks;
-    }
-    after_the_launch_before();  // by every CTA: what follows on the stream must not start before the results are there
-    if (share + 1 >= shares || u1 <= end || u0 < share * units / shares) return;
-    const int64_t last = (u1 * shares - 1) / units;  // the share of unit u1 - 1: the last one that begins at or before it
-#pragma unroll 1
-    for (int i = warp; i < 32; i += TJ_THREADS / 32) {
-        const int local = blockIdx.y * 32 + i;
-        const int64_t r = (int64_t)cur.pair * TA_ROWS + local;
-        if (r >= (int64_t)cur.s.count * a.group) continue;
-        float acc[PER], top = -INFINITY, sum = 0.f;
-#pragma unroll
-        for (int x = 0; x < PER; ++x) acc[x] = 0.f;
-        for (int64_t w = share; w <= last; ++w) {
-            const float *const slot = tile_slot<D>(a, 2 * w + (w == share ? 1 : 0));
-            const float m = __ldcg(slot + TA_ROWS * D + local), l = __ldcg(slot + TA_ROWS * D + TA_ROWS + local);
-            const float now = fmaxf(top, m), base = now == -INFINITY ? 0.f : now, mine = ex2(m - base), old = ex2(top - base);
-#pragma unroll
-            for (int x = 0; x < PER; ++x) acc[x] = acc[x] * old + __ldcg(slot + local * D + x * 32 + lane) * mine;
-            sum = sum * old + l * mine;
-            top = now;
-        }
-        const int token = (int)(r / a.group), h = cur.head * a.group + (int)(r % a.group);
-        uint16_t *const to = (uint16_t *)a.out + ((int64_t)(cur.s.first + token) * a.heads + h) * D;
-#pragma unroll
-        for (int x = 0; x < PER; ++x) {
-            const float o = sum == 0.f ? (acc[x] == acc[x] ? 0.f : acc[x]) : __fdividef(acc[x], sum);
-            to[x * 32 + lane] = (uint16_t)float_to_half_bits(o, a.c.bf16);
-        }
-    }
-}
-
 size_t attend_tiles_bytes(int head_dim) { return (size_t)TA_GRID * 2 * TA_ROWS * (head_dim + 2) * sizeof(float); }
 
 template <int D, bool BF16, bool MODS>
@@ -718,17 +575,6 @@ static int launch_tiles(const AttendArgs &a, cudaStream_t st) {
     constexpr size_t smem = TileShared<D>::BYTES;
     if (configured.run([&] { return cudaFuncSetAttribute(attend_tiles_kernel<D, BF16, MODS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) == cudaSuccess; }) != G2D_OK) return G2D_ERR_CUDA;
     attend_tiles_kernel<D, BF16, MODS><<<TA_GRID, TA_THREADS, smem, st>>>(a);
-    if (check_launch() != G2D_OK) return G2D_ERR_CUDA;
-    cudaLaunchConfig_t config{};
-    config.gridDim = dim3(TA_GRID, TA_ROWS / 32);
-    config.blockDim = dim3(TJ_THREADS);
-    config.stream = st;
-    cudaLaunchAttribute attribute{};
-    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attribute.val.programmaticStreamSerializationAllowed = 1;
-    config.attrs = &attribute;
-    config.numAttrs = 1;
-    if (cudaLaunchKernelEx(&config, attend_tiles_join_kernel<D>, a, (int64_t)TA_GRID) != cudaSuccess) return G2D_ERR_CUDA;
     return check_launch();
 }
 
