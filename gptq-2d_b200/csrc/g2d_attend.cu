@@ -23,7 +23,13 @@
 
 namespace g2d {
 
-constexpr int ATTEND_WARPS = 8, ATTEND_THREADS = 32 * ATTEND_WARPS, ATTEND_STAGES = 3, ATTEND_GRID = 148;
+constexpr int ATTEND_GRID = 148;
+// Warps per CTA (a CTA per SM) and stages per warp.  The work of a block is a chain of dependent steps, so warps count for more than stages.
+template <int D, int NT>
+struct AttendShape {
+    static constexpr int WARPS = NT == 1 ? 12 : 8, THREADS = 32 * WARPS, STAGES = NT == 1 ? (D == 128 ? 2 : 4) : 3;
+};
+constexpr int ATTEND_MOST_WARPS = 12;
 
 template <int D>
 struct AttendStage {
@@ -35,12 +41,13 @@ struct AttendPart {
     int b, item, first, last, blocks;  // blocks first .. last - 1 of `blocks`; last 0: no part
     AttendSequence s;
 };
-template <int D>
+template <int D, int NT>
 struct AttendShared {
-    AttendStage<D> stage[ATTEND_WARPS][ATTEND_STAGES];
-    uint64_t full[ATTEND_WARPS][ATTEND_STAGES];
-    long long totals[ATTEND_WARPS];
-    AttendPart parts[2 * ATTEND_WARPS];
+    using S = AttendShape<D, NT>;
+    AttendStage<D> stage[S::WARPS][S::STAGES];
+    uint64_t full[S::WARPS][S::STAGES];
+    long long totals[S::WARPS];
+    AttendPart parts[2 * S::WARPS];
 };
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -139,10 +146,11 @@ __device__ __forceinline__ float *attend_slot(const AttendArgs &a, int64_t slot)
 constexpr int WARP_SLOTS = 2 * ATTEND_GRID;
 
 template <int D, int NT, bool MODS>
-__global__ void __launch_bounds__(ATTEND_THREADS, 1) attend_rows_kernel(const AttendArgs a) {
+__global__ void __launch_bounds__(AttendShape<D, NT>::THREADS, 1) attend_rows_kernel(const AttendArgs a) {
+    constexpr int ATTEND_WARPS = AttendShape<D, NT>::WARPS, ATTEND_STAGES = AttendShape<D, NT>::STAGES;
     constexpr int ROWS = 8 * NT, KSTEPS = D / 16, MTILES = D / 16, WORDS = D / 32, CODE_BYTES = D / 2;
     extern __shared__ __align__(128) unsigned char attend_smem_raw[];
-    AttendShared<D> &sh = *reinterpret_cast<AttendShared<D> *>(attend_smem_raw);
+    AttendShared<D, NT> &sh = *reinterpret_cast<AttendShared<D, NT> *>(attend_smem_raw);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const CacheView &c = a.c;
     if (lane == 0) {
@@ -294,33 +302,38 @@ __global__ void __launch_bounds__(ATTEND_THREADS, 1) attend_rows_kernel(const At
             const bool masked = key0 + CACHE_BLOCK > least || (here & 0x11111111u) != (0x11111111u >> (32 - 4 * pieces));
             // ---- scores ----
             float s[4][NT][4];
+            uint32_t lo[4][WORDS], hi[4][WORDS];
 #pragma unroll
             for (int mt = 0; mt < 4; ++mt) {
-                uint32_t lo[WORDS], hi[WORDS];
                 const uint8_t *const at = st.k + (mt * 16 + pi_g) * CODE_BYTES + t * (D / 8);
                 if constexpr (WORDS == 4) {
                     const uint4 x = *reinterpret_cast<const uint4 *>(at), y = *reinterpret_cast<const uint4 *>(at + 8 * CODE_BYTES);
-                    lo[0] = x.x; lo[1] = x.y; lo[2] = x.z; lo[3] = x.w;
-                    hi[0] = y.x; hi[1] = y.y; hi[2] = y.z; hi[3] = y.w;
+                    lo[mt][0] = x.x; lo[mt][1] = x.y; lo[mt][2] = x.z; lo[mt][3] = x.w;
+                    hi[mt][0] = y.x; hi[mt][1] = y.y; hi[mt][2] = y.z; hi[mt][3] = y.w;
                 } else {
                     const uint2 x = *reinterpret_cast<const uint2 *>(at), y = *reinterpret_cast<const uint2 *>(at + 8 * CODE_BYTES);
-                    lo[0] = x.x; lo[1] = x.y;
-                    hi[0] = y.x; hi[1] = y.y;
+                    lo[mt][0] = x.x; lo[mt][1] = x.y;
+                    hi[mt][0] = y.x; hi[mt][1] = y.y;
                 }
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
                     s[mt][j][0] = s[mt][j][2] = start[j][0];
                     s[mt][j][1] = s[mt][j][3] = start[j][1];
                 }
+            }
 #pragma unroll
-                for (int w = 0; w < WORDS; ++w) {
-                    const uint32_t lo8 = lo[w] >> 8, hi8 = hi[w] >> 8;
+            for (int w = 0; w < WORDS; ++w) {  // four chains of products side by side
 #pragma unroll
-                    for (int j = 0; j < NT; ++j) {
-                        mma_f16(s[mt][j], lo[w] & 0x000f000fu, hi[w] & 0x000f000fu, lo8 & 0x000f000fu, hi8 & 0x000f000fu, qf[j][2 * w][0], qf[j][2 * w][1]);
-                        mma_f16(s[mt][j], lo[w] & 0x00f000f0u, hi[w] & 0x00f000f0u, lo8 & 0x00f000f0u, hi8 & 0x00f000f0u, qf[j][2 * w + 1][0], qf[j][2 * w + 1][1]);
-                    }
-                }
+                for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j)
+                        mma_f16(s[mt][j], lo[mt][w] & 0x000f000fu, hi[mt][w] & 0x000f000fu, (lo[mt][w] >> 8) & 0x000f000fu, (hi[mt][w] >> 8) & 0x000f000fu, qf[j][2 * w][0], qf[j][2 * w][1]);
+#pragma unroll
+                for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j)
+                        mma_f16(s[mt][j], lo[mt][w] & 0x00f000f0u, hi[mt][w] & 0x00f000f0u, (lo[mt][w] >> 8) & 0x00f000f0u, (hi[mt][w] >> 8) & 0x00f000f0u, qf[j][2 * w + 1][0],
+                                qf[j][2 * w + 1][1]);
             }
             // ---- scales, masks, maximum ----
             float vs[8], top[NT][2];
@@ -648,11 +661,11 @@ static int launch_behind(void (*kernel)(Args), unsigned grid, int threads, size_
 template <int D, int NT, bool MODS>
 static int launch_rows(const AttendArgs &a, bool behind_tiles, cudaStream_t st) {
     static PerDeviceOnce configured;
-    constexpr size_t smem = sizeof(AttendShared<D>);
+    constexpr size_t smem = sizeof(AttendShared<D, NT>);
     if (configured.run([&] { return cudaFuncSetAttribute(attend_rows_kernel<D, NT, MODS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) == cudaSuccess; }) != G2D_OK)
         return G2D_ERR_CUDA;
-    if (behind_tiles) return launch_behind(attend_rows_kernel<D, NT, MODS>, ATTEND_GRID, ATTEND_THREADS, smem, a, st);
-    attend_rows_kernel<D, NT, MODS><<<ATTEND_GRID, ATTEND_THREADS, smem, st>>>(a);
+    if (behind_tiles) return launch_behind(attend_rows_kernel<D, NT, MODS>, ATTEND_GRID, AttendShape<D, NT>::THREADS, smem, a, st);
+    attend_rows_kernel<D, NT, MODS><<<ATTEND_GRID, AttendShape<D, NT>::THREADS, smem, st>>>(a);
     return check_launch();
 }
 template <int D, int NT>
@@ -673,7 +686,7 @@ struct AttendSpace {
 };
 static AttendSpace attend_space(int head_dim) {
     AttendSpace s;
-    s.tiles = ((size_t)ATTEND_GRID * (ATTEND_WARPS + 1) * 2 * 16 * (head_dim + 2) * sizeof(float) + 255) & ~(size_t)255;
+    s.tiles = ((size_t)ATTEND_GRID * (ATTEND_MOST_WARPS + 1) * 2 * 16 * (head_dim + 2) * sizeof(float) + 255) & ~(size_t)255;
     s.all = s.tiles + attend_tiles_bytes(head_dim);
     return s;
 }

@@ -6,7 +6,7 @@
 // scale that is not finite, so that it reads back as NaN: absmax is taken over the bits of |v|, where both are larger than any number.
 //
 // Bound: HBM, 2 bytes read per value and half a byte written (the other way round for reading).  A lane takes eight values (16 bytes), so a row is that
-// of 16 or 8 neighbouring lanes and its absmax 3 or 4 shuffles.  Offsets are searched once per row, from the L1.
+// of 16 or 8 neighbouring lanes and its absmax 3 or 4 shuffles.
 #include "g2d_cache.cuh"
 
 namespace g2d {
@@ -19,79 +19,117 @@ __device__ __forceinline__ unsigned lanes_max(unsigned v) {
     for (int o = LANES / 2; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
     return v;
 }
+// A warp takes tokens that stand together, a token at a time: where it goes is found once for all of its rows, and its sequence once for as long as it lasts.
+struct CachePlace {
+    int b = -1, first = 0, count = 0, length = 0;
+    // row of the cache of kv head 0 of the token's position (heads lie page_size rows apart), -1 where there is none
+    __device__ __forceinline__ int64_t of(const CacheView &c, int token) {
+        if (b < 0 || token < first || token >= first + count) {
+            b = sequence_of(c, token, first, count);
+            if (b >= 0) length = max(c.lengths[b], -0x40000000);
+        }
+        return b < 0 ? -1 : cache_row(c, b, length - count + (token - first), 0);
+    }
+};
+__device__ __forceinline__ void tokens_of_warp(const CacheView &c, int &t0, int &t1) {
+    const int64_t warps = (int64_t)gridDim.x * (CACHE_THREADS / 32), w = (int64_t)blockIdx.x * (CACHE_THREADS / 32) + (threadIdx.x >> 5);
+    t0 = (int)(w * c.tokens / warps);
+    t1 = (int)((w + 1) * c.tokens / warps);
+}
 
-// rows: (token, head, key or value), the last fastest
+// x / scale rounded to the nearest of -8 .. 7.  `rc` is 1 / scale, rounded; one correction leaves the quotient within its last bit.  That is enough: a quotient q of an x of 11 bits at most
+// and a scale of 11 bits is either a half-integer exactly, and then both steps are exact as well, or more than 2^-16 of itself away from one.
+__device__ __forceinline__ uint32_t code_of(float x, float scale, float rc) {
+    const float q0 = x * rc, q = fmaf(fmaf(-q0, scale, x), rc, q0);
+    return (uint32_t)(__float2int_rn(fminf(fmaxf(q, -8.f), 7.f)) + 8);
+}
+
+// rows of a token: (head, key or value), the latter fastest; LANES lanes each
 template <int LANES>
 __global__ void __launch_bounds__(CACHE_THREADS) cache_append_kernel(const CacheView c, const uint16_t *__restrict__ k, const uint16_t *__restrict__ v, int64_t k_token, int64_t k_head,
                                                                      int64_t v_token, int64_t v_head) {
-    constexpr int PER_CTA = CACHE_THREADS / LANES;
-    const int64_t rows = (int64_t)c.tokens * c.kv_heads * 2;
-    const int part = threadIdx.x % LANES;
-    for (int64_t r0 = (int64_t)blockIdx.x * PER_CTA; r0 < rows; r0 += (int64_t)gridDim.x * PER_CTA) {  // the same trips for all lanes of a warp
-        const int64_t r = r0 + threadIdx.x / LANES;
-        uint4 raw = make_uint4(0u, 0u, 0u, 0u);
-        int64_t at = -1;
-        const bool value = r & 1;
-        if (r < rows) {
-            const int token = (int)((r >> 1) / c.kv_heads), head = (int)((r >> 1) % c.kv_heads);
-            raw = *reinterpret_cast<const uint4 *>((value ? v + token * v_token + head * v_head : k + token * k_token + head * k_head) + part * 8);
-            int first, count;
-            const int b = sequence_of(c, token, first, count);
-            if (b >= 0) {
-                const int64_t p = (int64_t)c.lengths[b] - count + (token - first);
-                at = cache_row(c, b, (int)max(min(p, (int64_t)0x7fffffff), (int64_t)-1), head);
+    constexpr int ROWS = 32 / LANES, BATCH = 4;  // rows of a warp at once, and so many times
+    const int lane = threadIdx.x & 31, part = lane % LANES, sub = lane / LANES, rows = 2 * c.kv_heads;
+    int t0, t1;
+    tokens_of_warp(c, t0, t1);
+    CachePlace place;
+    for (int token = t0; token < t1; ++token) {
+        const int64_t at = place.of(c, token);
+        if (at < 0) continue;
+        for (int r0 = 0; r0 < rows; r0 += ROWS * BATCH) {
+            uint4 raw[BATCH];
+#pragma unroll
+            for (int n = 0; n < BATCH; ++n) {
+                const int r = r0 + n * ROWS + sub, head = r >> 1;
+                raw[n] = r < rows ? __ldg(reinterpret_cast<const uint4 *>((r & 1 ? v + token * v_token + head * v_head : k + token * k_token + head * k_head) + part * 8)) : make_uint4(0u, 0u, 0u, 0u);
             }
-        }
-        float x[8];
-        const uint32_t word[4] = {raw.x, raw.y, raw.z, raw.w};
-        unsigned largest = 0u;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            x[e] = half_bits_to_float((word[e >> 1] >> (16 * (e & 1))) & 0xffffu, c.bf16);
-            largest = max(largest, __float_as_uint(x[e]) & 0x7fffffffu);
-        }
-        const float scale = absmax_scale_value(__uint_as_float(lanes_max<LANES>(largest)), 7.5f, G2D_FP16);
-        const bool finite = scale <= 65504.f;
-        uint32_t codes = 0u;
+            for (int n = 0; n < BATCH; ++n) {
+                const int r = r0 + n * ROWS + sub, head = r >> 1;
+                if (r0 + n * ROWS >= rows) break;  // for the whole warp
+                float x[8];
+                const uint32_t word[4] = {raw[n].x, raw[n].y, raw[n].z, raw[n].w};
+                unsigned largest = 0u;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float t = fminf(fmaxf(rintf(div_rn(x[e], scale)), -8.f), 7.f);
-            codes |= (finite ? (uint32_t)(__float2int_rn(t) + 8) : 8u) << (4 * e);  // a row that is not finite: zeros under a scale that is not
-        }
-        if (at >= 0) {
-            uint8_t *const to = (value ? c.v_codes : c.k_codes) + at * (LANES * 4);
-            reinterpret_cast<uint32_t *>(to)[part] = codes;
-            if (part == 0) (value ? c.v_scale : c.k_scale)[at] = __float2half_rn(scale);
+                for (int e = 0; e < 8; ++e) {
+                    x[e] = half_bits_to_float((word[e >> 1] >> (16 * (e & 1))) & 0xffffu, c.bf16);
+                    largest = max(largest, __float_as_uint(x[e]) & 0x7fffffffu);
+                }
+                const float scale = absmax_scale_value(__uint_as_float(lanes_max<LANES>(largest)), 7.5f, G2D_FP16);
+                const float rc = __frcp_rn(scale);
+                uint32_t codes = 0x88888888u;  // a row that is not finite: zeros under a scale that is not
+                if (scale <= 65504.f) {
+                    codes = 0u;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) codes |= code_of(x[e], scale, rc) << (4 * e);
+                }
+                if (r < rows) {
+                    const int64_t row = at + ((int64_t)head << c.page_shift);
+                    reinterpret_cast<uint32_t *>((r & 1 ? c.v_codes : c.k_codes) + row * (LANES * 4))[part] = codes;
+                    if (part == 0) (r & 1 ? c.v_scale : c.k_scale)[row] = __float2half_rn(scale);
+                }
+            }
         }
     }
 }
 
 template <int LANES>
 __global__ void __launch_bounds__(CACHE_THREADS) cache_read_kernel(const CacheView c, uint16_t *__restrict__ k, uint16_t *__restrict__ v) {
-    constexpr int PER_CTA = CACHE_THREADS / LANES;
-    const int64_t rows = (int64_t)c.tokens * c.kv_heads * 2;
-    const int part = threadIdx.x % LANES;
-    for (int64_t r = (int64_t)blockIdx.x * PER_CTA + threadIdx.x / LANES; r < rows; r += (int64_t)gridDim.x * PER_CTA) {
-        const bool value = r & 1;
-        const int token = (int)((r >> 1) / c.kv_heads), head = (int)((r >> 1) % c.kv_heads);
-        int first, count;
-        const int b = sequence_of(c, token, first, count);
-        if (b < 0) continue;  // a row of no sequence stays as it is
-        const int64_t p = (int64_t)c.lengths[b] - count + (token - first);
-        const int64_t at = cache_row(c, b, (int)max(min(p, (int64_t)0x7fffffff), (int64_t)-1), head);
-        uint32_t codes = 0x88888888u;  // a position that the cache does not hold reads as zeros
-        float scale = 0.f;
-        if (at >= 0) {
-            codes = reinterpret_cast<const uint32_t *>((value ? c.v_codes : c.k_codes) + at * (LANES * 4))[part];
-            scale = __half2float((value ? c.v_scale : c.k_scale)[at]);
-        }
-        uint32_t word[4];
+    constexpr int ROWS = 32 / LANES, BATCH = 4;
+    const int lane = threadIdx.x & 31, part = lane % LANES, sub = lane / LANES, rows = 2 * c.kv_heads;
+    int t0, t1;
+    tokens_of_warp(c, t0, t1);
+    CachePlace place;
+    for (int token = t0; token < t1; ++token) {
+        const int64_t at = place.of(c, token);
+        if (place.b < 0) continue;  // a row of no sequence stays as it is
+        for (int r0 = 0; r0 < rows; r0 += ROWS * BATCH) {
+            uint32_t codes[BATCH];
+            float scale[BATCH];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float lo = (float)((int)((codes >> (8 * e)) & 15u) - 8) * scale, hi = (float)((int)((codes >> (8 * e + 4)) & 15u) - 8) * scale;
-            word[e] = pack_halves(lo, hi, c.bf16);
+            for (int n = 0; n < BATCH; ++n) {
+                const int r = r0 + n * ROWS + sub;
+                const int64_t row = at + ((int64_t)(r >> 1) << c.page_shift);
+                codes[n] = 0x88888888u;  // a position that the cache does not hold reads as zeros
+                scale[n] = 0.f;
+                if (at >= 0 && r < rows) {
+                    codes[n] = reinterpret_cast<const uint32_t *>((r & 1 ? c.v_codes : c.k_codes) + row * (LANES * 4))[part];
+                    scale[n] = __half2float((r & 1 ? c.v_scale : c.k_scale)[row]);
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < BATCH; ++n) {
+                const int r = r0 + n * ROWS + sub;
+                if (r >= rows) continue;
+                uint32_t word[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float lo = (float)((int)((codes[n] >> (8 * e)) & 15u) - 8) * scale[n], hi = (float)((int)((codes[n] >> (8 * e + 4)) & 15u) - 8) * scale[n];
+                    word[e] = pack_halves(lo, hi, c.bf16);
+                }
+                reinterpret_cast<uint4 *>((r & 1 ? v : k) + ((int64_t)token * c.kv_heads + (r >> 1)) * (LANES * 8))[part] = make_uint4(word[0], word[1], word[2], word[3]);
+            }
         }
-        reinterpret_cast<uint4 *>((value ? v : k) + ((int64_t)token * c.kv_heads + head) * (LANES * 8))[part] = make_uint4(word[0], word[1], word[2], word[3]);
     }
 }
 
@@ -127,9 +165,9 @@ int cache_view(const g2d_cache_desc *d, CacheView *c) {
     return G2D_OK;
 }
 
-static unsigned cache_grid(const CacheView &c) {
-    const int64_t blocks = ceil_div((int64_t)c.tokens * c.kv_heads * 2 * (c.head_dim / 8), (int64_t)CACHE_THREADS);
-    return (unsigned)(blocks < 148 * 32 ? blocks : 148 * 32);
+static unsigned cache_grid(const CacheView &c) {  // a token per warp and up to eight CTAs per SM
+    const int64_t blocks = ceil_div((int64_t)c.tokens, (int64_t)(CACHE_THREADS / 32));
+    return (unsigned)(blocks < 148 * 8 ? blocks : 148 * 8);
 }
 
 }  // namespace g2d

@@ -222,9 +222,9 @@ static int launch_rows_kernel(const LinearArgs &a, cudaStream_t st) {
         const int64_t most = ceil_div(blocks, splits);
         return (size_t)(most * (KB * TOKENS * 2 + TOKENS * 4) + K_GROUPS * TOKENS * ROWS * 4);
     };
-    // as many parts of the columns as it takes for two CTAs per SM, of four blocks per warp at least; more where x would not fit
+    // as many parts of the columns as two CTAs per SM take at once, of four blocks per warp at least; more where x would not fit
     int splits = 1;
-    while (splits < 8 && ((rows * tiles * splits < 2 * 148 && blocks >= 2 * splits * K_GROUPS * 4) || bytes(splits) > 96 * 1024)) splits *= 2;
+    while (splits < 8 && ((rows * tiles * splits * 2 <= 2 * 148 && blocks >= 2 * splits * K_GROUPS * 4) || bytes(splits) > 96 * 1024)) splits *= 2;
     if (bytes(splits) > MOST) return G2D_ERR_TOO_LARGE;
     if (rows > 65535 || tiles > 65535) return G2D_ERR_TOO_LARGE;
     if (configured.run([&] { return cudaFuncSetAttribute(linear_rows_kernel<BF16, NT, KB, ROW_TILES>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)MOST) == cudaSuccess; }) != G2D_OK)
