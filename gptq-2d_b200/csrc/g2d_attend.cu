@@ -14,9 +14,10 @@
 // so four codes cost two ANDs and a shift.  The scores are S^T = K Q^T with keys as the rows of A (m16n8k16), the channels of k in the order in which a word of
 // codes holds them; Q in fp16 under a power of two per row (bf16 queries lose nothing: 8 bits, and what lies 2^-38 below the row's largest), and the
 // products start from -8 sum(q).  The results are O^T = V^T P^T, two keys' words interleaved by a byte permutation, P^T from S^T by
-// a transposing matrix move, P s_j in fp16 under a power of two of the block's largest scale: rounded once, to 11 bits, and -8 sum(P s) is formed by
-// the same products from the rounded values.  Every block's product starts anew and is added to the results in registers in fp32: the tensor cores truncate, and
-// over a long sequence the part -8 sum would leave its truncation behind.
+// a transposing matrix move, P s_j in fp16 under a power of two of the run's largest scale so far (it goes into the exponent, and into the sum of the exponentials alike):
+// rounded once, to 11 bits, and -8 sum(P s) is formed by the same products from the rounded values.  Every block's product starts anew and is added to the results in
+// registers in fp32: the tensor cores truncate, and over a long sequence the part -8 sum would leave its truncation behind.
+// Row g of the tiles of S^T stands for the keys 8 g .. 8 g + 7 of the block, one per tile and half: a lane's scales are one load then.
 //
 // Bound: HBM (head_dim + 4 bytes per key and head), behind it the instructions per key.
 #include "g2d_attend.cuh"
@@ -54,6 +55,11 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, const float (&c)[4]) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
 __device__ __forceinline__ uint32_t transposed(uint32_t a) {
     uint32_t d;
@@ -114,7 +120,7 @@ __device__ __forceinline__ int sequence_of_unit(const AttendArgs &a, int rows_pe
 
 // A place in the list of units
 struct AttendCursor {
-    int64_t u, end;
+    int u, end;  // units of the warp's share
     int b, item, block, blocks, items;
     AttendSequence s;
     __device__ __forceinline__ void open(const AttendArgs &a, int rows_per_item) {  // sequence b, or the next one that has units
@@ -164,23 +170,26 @@ __global__ void __launch_bounds__(AttendShape<D, NT>::THREADS, 1) attend_rows_ke
     AttendCursor cur;
     cur.u = cur.end = 0;
     if (share < shares) {
-        const int64_t u0 = share * units / shares, n = (share + 1) * units / shares - u0;
-        cur.u = u0 + warp * n / ATTEND_WARPS;
-        cur.end = u0 + (warp + 1) * n / ATTEND_WARPS;
-    }
-    if (cur.u < cur.end) {
-        int64_t before;
-        cur.b = sequence_of_unit(a, ROWS, cur.u, before);
-        cur.open(a, ROWS);
-        cur.item = (int)((cur.u - before) / cur.blocks);
-        cur.block = (int)((cur.u - before) % cur.blocks);
+        const int64_t u0 = share * units / shares, n = (share + 1) * units / shares - u0, mine = u0 + warp * n / ATTEND_WARPS;
+        cur.end = (int)(u0 + (warp + 1) * n / ATTEND_WARPS - mine);
+        if (cur.end > 0) {
+            int64_t before;
+            cur.b = sequence_of_unit(a, ROWS, mine, before);
+            cur.open(a, ROWS);
+            cur.item = (int)((mine - before) / cur.blocks);
+            cur.block = (int)((mine - before) % cur.blocks);
+        }
     }
 
     // ---- loads: a block's keys lie in one page or in several; lane x brings piece x / 4 of codes or scales, of keys or values ----
     const int piece_shift = min(c.page_shift, 6), piece_keys = 1 << piece_shift, pieces = CACHE_BLOCK >> piece_shift;
     AttendCursor ahead = cur;
+    const int what = lane & 3, to = (lane >> 2) * piece_keys;  // this lane's copies: codes of keys, of values, scales of keys, of values, of the keys from `to` on
+    const uint32_t key_bytes = what < 2 ? CODE_BYTES : 2;
+    const uint8_t *const source = what == 0 ? c.k_codes : what == 1 ? c.v_codes : what == 2 ? (const uint8_t *)c.k_scale : (const uint8_t *)c.v_scale;
+    const uint32_t target = (uint32_t)(what == 0 ? offsetof(AttendStage<D>, k) : what == 1 ? offsetof(AttendStage<D>, v) : what == 2 ? offsetof(AttendStage<D>, ks) : offsetof(AttendStage<D>, vs)) + to * key_bytes;
     auto page_of = [&](const AttendCursor &at) {  // the page of this lane's piece, or -1
-        const int key = at.block * CACHE_BLOCK + (lane >> 2) * piece_keys;
+        const int key = at.block * CACHE_BLOCK + to;
         if (at.u >= at.end || lane >= 4 * pieces || key >= at.s.keys) return -1;
         const int page = c.table[at.b * c.table_stride + (key >> c.page_shift)];
         return page < c.pages ? page : -1;
@@ -190,20 +199,13 @@ __global__ void __launch_bounds__(AttendShape<D, NT>::THREADS, 1) attend_rows_ke
 #pragma unroll
     for (int s = 0; s < ATTEND_STAGES; ++s) present[s] = 0u;
     auto issue = [&](int stage, unsigned &here) {
-        AttendStage<D> &st = sh.stage[warp][stage];
-        uint64_t *bar = &sh.full[warp][stage];
+        uint64_t *const bar = &sh.full[warp][stage];
         here = __ballot_sync(0xffffffffu, next_page >= 0);
-        const int whole = __popc(here & 0x11111111u);
-        if (lane == 0) mbar_expect_tx(bar, (uint32_t)(whole * piece_keys * (2 * CODE_BYTES + 4)));
+        if (lane == 0) mbar_expect_tx(bar, (uint32_t)(__popc(here & 0x11111111u) * piece_keys * (2 * CODE_BYTES + 4)));
         __syncwarp();
         if (next_page >= 0) {
-            const int place = (ahead.block * CACHE_BLOCK + (lane >> 2) * piece_keys) & (c.page_size - 1), head = ahead.item % c.kv_heads, to = (lane >> 2) * piece_keys;
-            const int64_t row = (((int64_t)next_page * c.kv_heads + head) << c.page_shift) + place;
-            const int what = lane & 3;
-            if (what == 0) bulk_load(st.k + to * CODE_BYTES, c.k_codes + row * CODE_BYTES, piece_keys * CODE_BYTES, bar);
-            else if (what == 1) bulk_load(st.v + to * CODE_BYTES, c.v_codes + row * CODE_BYTES, piece_keys * CODE_BYTES, bar);
-            else if (what == 2) bulk_load(st.ks + to, c.k_scale + row, piece_keys * 2, bar);
-            else bulk_load(st.vs + to, c.v_scale + row, piece_keys * 2, bar);
+            const int64_t row = (((int64_t)next_page * c.kv_heads + ahead.item % c.kv_heads) << c.page_shift) + ((ahead.block * CACHE_BLOCK + to) & (c.page_size - 1));
+            bulk_load(reinterpret_cast<unsigned char *>(&sh.stage[warp][stage]) + target, source + row * key_bytes, piece_keys * key_bytes, bar);
         }
         ahead.step(a, ROWS);
         next_page = page_of(ahead);
@@ -212,16 +214,16 @@ __global__ void __launch_bounds__(AttendShape<D, NT>::THREADS, 1) attend_rows_ke
     for (int s = 0; s < ATTEND_STAGES; ++s)
         if (ahead.u < ahead.end) issue(s, present[s]);
 
-    const int pi_g = (g & 4) | ((g & 1) << 1) | ((g >> 1) & 1);  // row g of S^T is key pi_g: lanes with neighbouring t then read V from both halves of the banks
     int stage = 0, phase = 0;
     bool sound = true;
     while (cur.u < cur.end) {
         // ---- a run of blocks of one item ----
         const int head = cur.item % c.kv_heads, row0 = cur.item / c.kv_heads * ROWS, rows = cur.s.count * a.group;
-        const int first_block = cur.block, last_block = (int)min((int64_t)cur.blocks, (int64_t)cur.block + (cur.end - cur.u));
+        const int first_block = cur.block, last_block = min(cur.blocks, cur.block + (cur.end - cur.u));
         const AttendSequence seq = cur.s;
         uint32_t qf[NT][KSTEPS][2];
-        float factor[NT][2], start[NT][2], slope[NT][2];
+        uint64_t factor[NT];
+        float start[NT][2], slope[NT][2];
         int limit[NT][2], place[NT][2], least = 0x7fffffff;
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
@@ -246,7 +248,7 @@ __global__ void __launch_bounds__(AttendShape<D, NT>::THREADS, 1) attend_rows_ke
             largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
             largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
             const int e2 = range_exponent(__uint_as_float(largest));
-            const float down = power_of_two(-e2);
+            const float down = power_of_two(-e2) * (a.scale < 0.f ? -1.f : 1.f);  // the scale's sign goes into the queries: the order of a row's products is that of its scores
             float sum = 0.f;
 #pragma unroll
             for (int w = 0; w < WORDS; ++w) {
@@ -263,14 +265,16 @@ __global__ void __launch_bounds__(AttendShape<D, NT>::THREADS, 1) attend_rows_ke
             }
             sum += __shfl_xor_sync(0xffffffffu, sum, 1);
             sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            const float my_factor = 16777216.f * a.scale * (MODS ? 1.f : LOG2E) * power_of_two(e2), my_start = -8.f / 16777216.f * sum;
+            const float my_factor = fmaxf(16777216.f * fabsf(a.scale) * (MODS ? 1.f : LOG2E) * power_of_two(e2), 1e-38f),  // above zero: minus infinity stays what it is
+                        my_start = -8.f / 16777216.f * sum;
             const int my_limit = real ? visible_keys(a, seq, token) : seq.keys;
             const float my_slope = MODS && a.slopes ? a.slopes[h] : 0.f;
             const int my_place = seq.length - seq.count + token;
+            float two_factors[2];
 #pragma unroll
             for (int x2 = 0; x2 < 2; ++x2) {
                 const int from = (2 * t + x2) * 4;
-                factor[j][x2] = __shfl_sync(0xffffffffu, my_factor, from);
+                two_factors[x2] = __shfl_sync(0xffffffffu, my_factor, from);
                 start[j][x2] = __shfl_sync(0xffffffffu, my_start, from);
                 limit[j][x2] = __shfl_sync(0xffffffffu, my_limit, from);
                 if (MODS) {
@@ -279,136 +283,160 @@ __global__ void __launch_bounds__(AttendShape<D, NT>::THREADS, 1) attend_rows_ke
                 }
                 least = min(least, limit[j][x2]);
             }
+            factor[j] = pack2(two_factors[0], two_factors[1]);
         }
         least = __reduce_min_sync(0xffffffffu, least);
-        float m[NT][2], l[NT][2], o[MTILES][NT][4];
-        int unit = 0;  // the scales' power of two, as the exponent bits of a float
+        // per row: the largest score so far in units of its factor, the reference of the exponentials (as a power of two), their sum; `unit`: the scales' power of two, as exponent bits
+        float m[NT][2], refer[NT][2];
+        uint64_t l[NT], o[MTILES][NT][2];
+        int unit = 0, lift = 0;
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
             m[j][0] = m[j][1] = -INFINITY;
-            l[j][0] = l[j][1] = 0.f;
+            refer[j][0] = refer[j][1] = -INFINITY;
+            l[j] = 0ull;
 #pragma unroll
-            for (int e = 0; e < MTILES; ++e) o[e][j][0] = o[e][j][1] = o[e][j][2] = o[e][j][3] = 0.f;
+            for (int e = 0; e < MTILES; ++e) o[e][j][0] = o[e][j][1] = 0ull;
         }
-        for (int block = first_block; block < last_block; ++block) {
-            const AttendStage<D> &st = sh.stage[warp][stage];
-            unsigned here = 0u;
-#pragma unroll
-            for (int s = 0; s < ATTEND_STAGES; ++s)
-                if (s == stage) here = present[s];
-            if (sound && !mbar_wait(&sh.full[warp][stage], phase, 20, a.wait_cycles)) sound = false;
-            sound = __all_sync(0xffffffffu, sound);
-            const int key0 = block * CACHE_BLOCK;
-            const bool masked = key0 + CACHE_BLOCK > least || (here & 0x11111111u) != (0x11111111u >> (32 - 4 * pieces));
+        // MASKED: some row does not see all 64 keys of the block, or some are not there
+        const auto take = [&](auto masked, const AttendStage<D> &st, int key0, unsigned here) {
+            constexpr bool MASKED = decltype(masked)::value;
             // ---- scores ----
             float s[4][NT][4];
-            uint32_t lo[4][WORDS], hi[4][WORDS];
+            {
+                uint32_t lo[4][WORDS], hi[4][WORDS];
+#pragma unroll
+                for (int mt = 0; mt < 4; ++mt) {
+                    const uint8_t *const at = st.k + (8 * g + 2 * mt) * CODE_BYTES + t * (D / 8);
+                    if constexpr (WORDS == 4) {
+                        const uint4 x = *reinterpret_cast<const uint4 *>(at), y = *reinterpret_cast<const uint4 *>(at + CODE_BYTES);
+                        lo[mt][0] = x.x; lo[mt][1] = x.y; lo[mt][2] = x.z; lo[mt][3] = x.w;
+                        hi[mt][0] = y.x; hi[mt][1] = y.y; hi[mt][2] = y.z; hi[mt][3] = y.w;
+                    } else {
+                        const uint2 x = *reinterpret_cast<const uint2 *>(at), y = *reinterpret_cast<const uint2 *>(at + CODE_BYTES);
+                        lo[mt][0] = x.x; lo[mt][1] = x.y;
+                        hi[mt][0] = y.x; hi[mt][1] = y.y;
+                    }
+                }
+#pragma unroll
+                for (int w = 0; w < WORDS; ++w) {  // four chains of products side by side
+#pragma unroll
+                    for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+                        for (int j = 0; j < NT; ++j) {
+                            const uint32_t a0 = lo[mt][w] & 0x000f000fu, a1 = hi[mt][w] & 0x000f000fu, a2 = (lo[mt][w] >> 8) & 0x000f000fu, a3 = (hi[mt][w] >> 8) & 0x000f000fu;
+                            if (w == 0) mma_f16(s[mt][j], a0, a1, a2, a3, qf[j][0][0], qf[j][0][1], {start[j][0], start[j][1], start[j][0], start[j][1]});
+                            else mma_f16(s[mt][j], a0, a1, a2, a3, qf[j][2 * w][0], qf[j][2 * w][1]);
+                        }
+#pragma unroll
+                    for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+                        for (int j = 0; j < NT; ++j)
+                            mma_f16(s[mt][j], lo[mt][w] & 0x00f000f0u, hi[mt][w] & 0x00f000f0u, (lo[mt][w] >> 8) & 0x00f000f0u, (hi[mt][w] >> 8) & 0x00f000f0u, qf[j][2 * w + 1][0],
+                                    qf[j][2 * w + 1][1]);
+                }
+            }
+            // ---- scales: of the keys 8 g .. 8 g + 7, key 2 mt + half for the rows of tile mt ----
+            const uint4 kraw = *reinterpret_cast<const uint4 *>(st.ks + 8 * g), vraw = *reinterpret_cast<const uint4 *>(st.vs + 8 * g);
+            const uint32_t kw[4] = {kraw.x, kraw.y, kraw.z, kraw.w};
+            uint32_t vw[4] = {vraw.x, vraw.y, vraw.z, vraw.w};
+            unsigned gone = 0u;  // MASKED: keys that are not there
+            if constexpr (MASKED) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    if (key0 + 8 * g + k >= seq.keys || !((here >> (4 * ((8 * g + k) >> piece_shift))) & 1u)) gone |= 1u << k;
+#pragma unroll
+                for (int mt = 0; mt < 4; ++mt) {  // what lies there may be anything
+                    if ((gone >> (2 * mt)) & 1u) vw[mt] &= 0xffff0000u;
+                    if ((gone >> (2 * mt + 1)) & 1u) vw[mt] &= 0x0000ffffu;
+                }
+            }
+            unsigned largest = 0u;  // of the values' scales, as the bits of a half; one that is not finite may be masked for some rows: it sets no unit
 #pragma unroll
             for (int mt = 0; mt < 4; ++mt) {
-                const uint8_t *const at = st.k + (mt * 16 + pi_g) * CODE_BYTES + t * (D / 8);
-                if constexpr (WORDS == 4) {
-                    const uint4 x = *reinterpret_cast<const uint4 *>(at), y = *reinterpret_cast<const uint4 *>(at + 8 * CODE_BYTES);
-                    lo[mt][0] = x.x; lo[mt][1] = x.y; lo[mt][2] = x.z; lo[mt][3] = x.w;
-                    hi[mt][0] = y.x; hi[mt][1] = y.y; hi[mt][2] = y.z; hi[mt][3] = y.w;
-                } else {
-                    const uint2 x = *reinterpret_cast<const uint2 *>(at), y = *reinterpret_cast<const uint2 *>(at + 8 * CODE_BYTES);
-                    lo[mt][0] = x.x; lo[mt][1] = x.y;
-                    hi[mt][0] = y.x; hi[mt][1] = y.y;
-                }
-#pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    s[mt][j][0] = s[mt][j][2] = start[j][0];
-                    s[mt][j][1] = s[mt][j][3] = start[j][1];
-                }
+                const unsigned x = vw[mt] & 0x7fffu, y = (vw[mt] >> 16) & 0x7fffu;
+                largest = max(largest, max(x < 0x7c00u ? x : 0u, y < 0x7c00u ? y : 0u));
             }
-#pragma unroll
-            for (int w = 0; w < WORDS; ++w) {  // four chains of products side by side
-#pragma unroll
-                for (int mt = 0; mt < 4; ++mt)
-#pragma unroll
-                    for (int j = 0; j < NT; ++j)
-                        mma_f16(s[mt][j], lo[mt][w] & 0x000f000fu, hi[mt][w] & 0x000f000fu, (lo[mt][w] >> 8) & 0x000f000fu, (hi[mt][w] >> 8) & 0x000f000fu, qf[j][2 * w][0], qf[j][2 * w][1]);
-#pragma unroll
-                for (int mt = 0; mt < 4; ++mt)
-#pragma unroll
-                    for (int j = 0; j < NT; ++j)
-                        mma_f16(s[mt][j], lo[mt][w] & 0x00f000f0u, hi[mt][w] & 0x00f000f0u, (lo[mt][w] >> 8) & 0x00f000f0u, (hi[mt][w] >> 8) & 0x00f000f0u, qf[j][2 * w + 1][0],
-                                qf[j][2 * w + 1][1]);
-            }
-            // ---- scales, masks, maximum ----
-            float vs[8], top[NT][2];
-            unsigned largest = 0u;
+            largest = __reduce_max_sync(0xffffffffu, largest);
+            const int new_unit = max(unit, (int)(__float_as_uint(__half2float(__ushort_as_half((unsigned short)largest))) >> 23));
+            const int new_lift = new_unit == 0 ? 0 : 13 - (new_unit - 127);  // brings the largest scale to 2^13 .. 2^14; of halves: from -2 to 37
+            const float grown = power_of_two(new_lift - lift);
+            unit = new_unit;
+            lift = new_lift;
+            // ---- scores in units of the factors, and their maximum ----
+            float top[NT][2];
 #pragma unroll
             for (int j = 0; j < NT; ++j) top[j][0] = top[j][1] = -INFINITY;
-            unsigned hidden[NT][2];  // bit 2 mt + half: masked keys
-#pragma unroll
-            for (int j = 0; j < NT; ++j) hidden[j][0] = hidden[j][1] = 0u;
+            unsigned hidden[NT][2];
 #pragma unroll
             for (int mt = 0; mt < 4; ++mt) {
+                const float2 ks = __half22float2(*reinterpret_cast<const __half2 *>(&kw[mt]));
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
-                    const int key = mt * 16 + half * 8 + pi_g;
-                    const float ks = __half2float(st.ks[key]);
-                    float sv = __half2float(st.vs[key]);
-                    const bool gone = masked && (key0 + key >= seq.keys || !((here >> (4 * (key >> piece_shift))) & 1u));
-                    if (gone) sv = 0.f;  // what lies there may be anything
-                    vs[2 * mt + half] = sv;
-                    const unsigned size = __float_as_uint(sv) & 0x7fffffffu;
-                    largest = max(largest, size < 0x7f800000u ? size : 0u);  // one that is not finite may be masked for some rows: it sets no unit
+                    const uint64_t k2 = half ? pack2(ks.y, ks.y) : pack2(ks.x, ks.x);
 #pragma unroll
                     for (int j = 0; j < NT; ++j) {
-#pragma unroll
-                        for (int x2 = 0; x2 < 2; ++x2) {
-                            float u = s[mt][j][2 * half + x2] * factor[j][x2] * ks;
-                            if (MODS) {
-                                if (a.softcap > 0.f) u = capped(u, a.softcap, 2.f * LOG2E / a.softcap);
-                                u = fmaf(slope[j][x2], (float)(key0 + key - place[j][x2]), u) * LOG2E;
-                            }
-                            if (gone || (masked && key0 + key >= limit[j][x2])) {
-                                u = -INFINITY;
-                                hidden[j][x2] |= 1u << (2 * mt + half);
-                            }
-                            s[mt][j][2 * half + x2] = u;
-                            top[j][x2] = fmaxf(top[j][x2], u);
+                        float &u0 = s[mt][j][2 * half], &u1 = s[mt][j][2 * half + 1];
+                        unpack2(mul2(pack2(u0, u1), k2), u0, u1);
+                        if constexpr (MODS) {
+                            float f0, f1;
+                            unpack2(factor[j], f0, f1);
+                            u0 *= f0;
+                            u1 *= f1;
+                            if (a.softcap > 0.f) u0 = capped(u0, a.softcap, 2.f * LOG2E / a.softcap), u1 = capped(u1, a.softcap, 2.f * LOG2E / a.softcap);
+                            const int key = key0 + 8 * g + 2 * mt + half;
+                            u0 = fmaf(slope[j][0], (float)(key - place[j][0]), u0) * LOG2E;
+                            u1 = fmaf(slope[j][1], (float)(key - place[j][1]), u1) * LOG2E;
                         }
+                        if constexpr (MASKED) {
+                            const int key = key0 + 8 * g + 2 * mt + half;
+                            const bool not_there = (gone >> (2 * mt + half)) & 1u;
+                            if (mt == 0 && half == 0) hidden[j][0] = hidden[j][1] = 0u;
+                            if (not_there || key >= limit[j][0]) u0 = -INFINITY, hidden[j][0] |= 1u << (2 * mt + half);
+                            if (not_there || key >= limit[j][1]) u1 = -INFINITY, hidden[j][1] |= 1u << (2 * mt + half);
+                        }
+                        top[j][0] = fmaxf(top[j][0], u0);
+                        top[j][1] = fmaxf(top[j][1], u1);
                     }
                 }
             }
-            largest = __reduce_max_sync(0xffffffffu, largest);
-            const int new_unit = max(unit, (int)(largest >> 23));
-            const float grown = unit == 0 ? 1.f : power_of_two(max(unit - new_unit, -126));  // nothing to scale yet
-            unit = new_unit;
-            const float vnorm = power_of_two(min(13 - (unit - 127), 127));
-            float keep[NT][2];
+            uint64_t keep[NT], less[NT];
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
+                float f[2] = {1.f, 1.f}, k[2], r[2];
+                if constexpr (!MODS) unpack2(factor[j], f[0], f[1]);
 #pragma unroll
                 for (int x2 = 0; x2 < 2; ++x2) {
 #pragma unroll
                     for (int off = 4; off < 32; off <<= 1) top[j][x2] = fmaxf(top[j][x2], __shfl_xor_sync(0xffffffffu, top[j][x2], off));
-                    const float now = fmaxf(m[j][x2], top[j][x2]);
-                    const float base = now == -INFINITY ? 0.f : now;
-                    keep[j][x2] = ex2(m[j][x2] - base);
-                    m[j][x2] = now;
-                    l[j][x2] *= keep[j][x2];
-                    top[j][x2] = base;
-                    keep[j][x2] *= grown;
+                    const float old = m[j][x2];
+                    m[j][x2] = fmaxf(old, top[j][x2]);
+                    const float now = m[j][x2] == -INFINITY ? 0.f : m[j][x2] * f[x2];
+                    k[x2] = old == -INFINITY ? grown : ex2(old * f[x2] - now) * grown;
+                    r[x2] = now - (float)lift;
+                    refer[j][x2] = m[j][x2] == -INFINITY ? -INFINITY : r[x2];
                 }
+                keep[j] = pack2(k[0], k[1]);
+                less[j] = pack2(-r[0], -r[1]);
+                l[j] = mul2(l[j], keep[j]);
             }
             // ---- exponentials and their products with the scales, transposed ----
             uint32_t pf[4][NT][2];
 #pragma unroll
             for (int mt = 0; mt < 4; ++mt) {
+                const float2 vs = __half22float2(*reinterpret_cast<const __half2 *>(&vw[mt]));
 #pragma unroll
-                for (int j = 0; j < NT; ++j) {
+                for (int half = 0; half < 2; ++half) {
+                    const uint64_t v2 = half ? pack2(vs.y, vs.y) : pack2(vs.x, vs.x);
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        const float p0 = ex2(s[mt][j][2 * half] - top[j][0]), p1 = ex2(s[mt][j][2 * half + 1] - top[j][1]);
-                        l[j][0] += p0;
-                        l[j][1] += p1;
-                        const float w = vs[2 * mt + half] * vnorm;
-                        float w0 = p0 * w, w1 = p1 * w;
-                        if (masked) {  // a masked key counts for nothing, whatever its scale
+                    for (int j = 0; j < NT; ++j) {
+                        const uint64_t u = pack2(s[mt][j][2 * half], s[mt][j][2 * half + 1]);
+                        float e0, e1, w0, w1;
+                        unpack2(MODS ? add2(u, less[j]) : fma2(u, factor[j], less[j]), e0, e1);
+                        const uint64_t p = pack2(ex2(e0), ex2(e1));
+                        l[j] = add2(l[j], p);
+                        unpack2(mul2(p, v2), w0, w1);
+                        if constexpr (MASKED) {  // a masked key counts for nothing, whatever its scale
                             if ((hidden[j][0] >> (2 * mt + half)) & 1u) w0 = 0.f;
                             if ((hidden[j][1] >> (2 * mt + half)) & 1u) w1 = 0.f;
                         }
@@ -416,35 +444,32 @@ __global__ void __launch_bounds__(AttendShape<D, NT>::THREADS, 1) attend_rows_ke
                     }
                 }
             }
-            // ---- results: sixteen keys at a time ----
-            float acc[MTILES][NT][4];
+            // ---- results: sixteen keys at a time, from -8 2^-24 times the sum of the products (sixteen times as much at odd places of a word) ----
+            float base[NT][2][4];
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
-                float less[4] = {0.f, 0.f, 0.f, 0.f};  // -8 2^-24 sum of the products, in every row
+                float b[4];
+                mma_f16(b, 0x80088008u, 0x80088008u, 0x80088008u, 0x80088008u, pf[0][j][0], pf[0][j][1], {0.f, 0.f, 0.f, 0.f});
 #pragma unroll
-                for (int mt = 0; mt < 4; ++mt) mma_f16(less, 0x80088008u, 0x80088008u, 0x80088008u, 0x80088008u, pf[mt][j][0], pf[mt][j][1]);
+                for (int mt = 1; mt < 4; ++mt) mma_f16(b, 0x80088008u, 0x80088008u, 0x80088008u, 0x80088008u, pf[mt][j][0], pf[mt][j][1]);
 #pragma unroll
-                for (int e = 0; e < MTILES; ++e) {
-                    const float f = e & 1 ? 16.f : 1.f;  // odd places of a word are sixteen times as large
-                    acc[e][j][0] = acc[e][j][2] = f * less[0];
-                    acc[e][j][1] = acc[e][j][3] = f * less[1];
-                }
+                for (int x = 0; x < 4; ++x) base[j][0][x] = b[x & 1], base[j][1][x] = 16.f * b[x & 1];
             }
+            float acc[MTILES][NT][4];
 #pragma unroll
             for (int mt = 0; mt < 4; ++mt) {
-                // rows 2t, 2t + 1 (and 8 more) of S^T are the keys t' and t' + 2, t' = 2 (t / 2) ... in the order of pi
-                const int k0 = mt * 16 + ((2 * t) & 4) + (t & 1), k1 = k0 + 2;
-                uint32_t lo[2][2], hi[2][2];  // [pair of keys][word]: nibbles 0..3 and 4..7 of both keys
+                const int k0 = 16 * t + 2 * mt;  // rows 2 t and 2 t + 1 of tile mt: the keys k0 and k0 + 8, and the ones behind them
+                uint32_t lo[2][2], hi[2][2];     // [pair of keys][word]: nibbles 0..3 and 4..7 of both keys
 #pragma unroll
                 for (int pair = 0; pair < 2; ++pair) {
                     if constexpr (D == 128) {
-                        const uint2 x = *reinterpret_cast<const uint2 *>(st.v + (k0 + 8 * pair) * CODE_BYTES + g * 8), y = *reinterpret_cast<const uint2 *>(st.v + (k1 + 8 * pair) * CODE_BYTES + g * 8);
+                        const uint2 x = *reinterpret_cast<const uint2 *>(st.v + (k0 + pair) * CODE_BYTES + g * 8), y = *reinterpret_cast<const uint2 *>(st.v + (k0 + pair + 8) * CODE_BYTES + g * 8);
                         lo[pair][0] = __byte_perm(x.x, y.x, 0x5410);
                         hi[pair][0] = __byte_perm(x.x, y.x, 0x7632);
                         lo[pair][1] = __byte_perm(x.y, y.y, 0x5410);
                         hi[pair][1] = __byte_perm(x.y, y.y, 0x7632);
                     } else {
-                        const uint32_t x = *reinterpret_cast<const uint32_t *>(st.v + (k0 + 8 * pair) * CODE_BYTES + g * 4), y = *reinterpret_cast<const uint32_t *>(st.v + (k1 + 8 * pair) * CODE_BYTES + g * 4);
+                        const uint32_t x = *reinterpret_cast<const uint32_t *>(st.v + (k0 + pair) * CODE_BYTES + g * 4), y = *reinterpret_cast<const uint32_t *>(st.v + (k0 + pair + 8) * CODE_BYTES + g * 4);
                         lo[pair][0] = __byte_perm(x, y, 0x5410);
                         lo[pair][1] = __byte_perm(x, y, 0x7632);
                     }
@@ -459,7 +484,10 @@ __global__ void __launch_bounds__(AttendShape<D, NT>::THREADS, 1) attend_rows_ke
                         f[x] = (nibble & 2 ? word >> 8 : word) & (nibble & 1 ? 0x00f000f0u : 0x000f000fu);
                     }
 #pragma unroll
-                    for (int j = 0; j < NT; ++j) mma_f16(acc[e][j], f[0], f[1], f[2], f[3], pf[mt][j][0], pf[mt][j][1]);
+                    for (int j = 0; j < NT; ++j) {
+                        if (mt == 0) mma_f16(acc[e][j], f[0], f[1], f[2], f[3], pf[mt][j][0], pf[mt][j][1], base[j][e & 1]);
+                        else mma_f16(acc[e][j], f[0], f[1], f[2], f[3], pf[mt][j][0], pf[mt][j][1]);
+                    }
                 }
             }
 #pragma unroll
@@ -467,7 +495,19 @@ __global__ void __launch_bounds__(AttendShape<D, NT>::THREADS, 1) attend_rows_ke
 #pragma unroll
                 for (int j = 0; j < NT; ++j)
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) o[e][j][x] = fmaf(o[e][j][x], keep[j][x & 1], acc[e][j][x]);
+                    for (int x = 0; x < 2; ++x) o[e][j][x] = fma2(o[e][j][x], keep[j], pack2(acc[e][j][2 * x], acc[e][j][2 * x + 1]));
+        };
+        for (int block = first_block; block < last_block; ++block) {
+            unsigned here = 0u;
+#pragma unroll
+            for (int s = 0; s < ATTEND_STAGES; ++s)
+                if (s == stage) here = present[s];
+            if (sound && !mbar_wait(&sh.full[warp][stage], phase, 20, a.wait_cycles)) sound = false;
+            sound = __all_sync(0xffffffffu, sound);
+            const int key0 = block * CACHE_BLOCK;
+            const bool masked = key0 + CACHE_BLOCK > least || (here & 0x11111111u) != (0x11111111u >> (32 - 4 * pieces));
+            if (masked) take(std::true_type(), sh.stage[warp][stage], key0, here);
+            else take(std::false_type(), sh.stage[warp][stage], key0, here);
             __syncwarp();  // all lanes have read the stage
             if (sound && ahead.u < ahead.end) {
                 unsigned loaded;
@@ -483,25 +523,28 @@ __global__ void __launch_bounds__(AttendShape<D, NT>::THREADS, 1) attend_rows_ke
         const int part = 2 * warp + (first_block == 0 ? 1 : 0);
         float *const slot = attend_slot<D, ROWS>(a, WARP_SLOTS + 2 * ATTEND_WARPS * share + part);
         if (!whole && lane == 0) sh.parts[part] = AttendPart{cur.b, cur.item, first_block, last_block, cur.blocks, seq};
-        const float back = power_of_two(max(24 - 13 + (unit - 127), -126));
+        constexpr float BACK = 16777216.f;
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
+            float sums[2];
+            unpack2(l[j], sums[0], sums[1]);
 #pragma unroll
             for (int x2 = 0; x2 < 2; ++x2) {
                 const int r = row0 + 8 * j + 2 * t + x2;
-                float sum = l[j][x2];
+                float sum = sums[x2];
 #pragma unroll
                 for (int off = 4; off < 32; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
                 if (r >= rows) continue;
-                float f = back;
-                if (whole) f = sum == 0.f ? 0.f : __fdividef(f, sum);
+                float f = BACK;
+                if (whole) f = sum == 0.f ? 0.f : __fdividef(BACK, sum);
                 if (!sound) f = NAN;
                 float value[D / 8];  // D / 8 neighbouring channels, from g * D / 8 on
 #pragma unroll
                 for (int e = 0; e < D / 8; ++e) {
                     constexpr int HALF = D / 16;
-                    const float x = e < HALF ? o[e][j][x2] : o[e - HALF][j][2 + x2];
-                    value[e] = x * (e & 1 ? 0.0625f * f : f);
+                    float x0, x1;
+                    unpack2(e < HALF ? o[e < HALF ? e : 0][j][0] : o[e < HALF ? 0 : e - HALF][j][1], x0, x1);
+                    value[e] = (x2 ? x1 : x0) * (e & 1 ? 0.0625f * f : f);
                 }
                 if (whole && sum == 0.f && sound) {
 #pragma unroll
@@ -520,14 +563,16 @@ __global__ void __launch_bounds__(AttendShape<D, NT>::THREADS, 1) attend_rows_ke
 #pragma unroll
                     for (int w = 0; w < D / 32; ++w) to[w] = make_float4(value[4 * w], value[4 * w + 1], value[4 * w + 2], value[4 * w + 3]);
                     if (g == 0) {
-                        slot[ROWS * D + i] = m[j][x2];
+                        slot[ROWS * D + i] = refer[j][x2];
                         slot[ROWS * D + ROWS + i] = sum;
                     }
                 }
             }
         }
         // on to the next run
-        for (int k = last_block - first_block; k > 0; --k) cur.step(a, ROWS);
+        cur.u += last_block - first_block - 1;
+        cur.block = last_block - 1;
+        cur.step(a, ROWS);
     }
     if (!sound && lane == 0) {
         let_it_land();  // loads under way must not outlive the shared memory
@@ -619,8 +664,8 @@ __global__ void __launch_bounds__(JOIN_THREADS) attend_join_kernel(const JoinArg
         if (share + 1 < shares) {
             int64_t before;
             end = (share + 1) * units / shares;
-            cur.u = end - 1;
-            cur.end = end;
+            cur.u = 0;
+            cur.end = 1;
             cur.b = sequence_of_unit(a, ROWS, end - 1, before);
             cur.open(a, ROWS);
             cur.item = (int)((end - 1 - before) / cur.blocks);

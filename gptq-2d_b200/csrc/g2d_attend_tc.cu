@@ -66,32 +66,10 @@ __device__ __forceinline__ void tmem_store_16(uint32_t at, const uint32_t (&v)[1
                  "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
                  : "memory");
 }
-// pairs of floats: one instruction each
 __device__ __forceinline__ ulonglong2 load_4p(uint32_t at) {
     ulonglong2 v;
     asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(v.x), "=l"(v.y) : "r"(at));
     return v;
-}
-__device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
-    return r;
-}
-__device__ __forceinline__ void unpack2(uint64_t v, float &lo, float &hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t add2f(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
 }
 __device__ __forceinline__ uint32_t halves_add(uint32_t u, uint32_t v, bool bf16) {
     uint32_t r;
@@ -498,9 +476,9 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const Atten
                         for (int y = 0; y < 2; ++y) {
                             const uint64_t score = pack2(v[x + 2 * y], v[x + 2 * y + 1]);
                             float e0, e1, w0, w1;
-                            unpack2(stored ? add2f(score, less) : fma2(score, y ? k4.y : k4.x, less), e0, e1);
+                            unpack2(stored ? add2(score, less) : fma2(score, y ? k4.y : k4.x, less), e0, e1);
                             const uint64_t e = pack2(__float_as_uint(ex2(e0)), __float_as_uint(ex2(e1)));
-                            sum = add2f(sum, e);
+                            sum = add2(sum, e);
                             unpack2(mul2(e, y ? v4.y : v4.x), w0, w1);
                             if (masked) {  // a masked key counts for nothing, whatever its scale
                                 if (v[x + 2 * y] == 0xff800000u) w0 = 0.f;

@@ -48,15 +48,15 @@ __device__ __forceinline__ uint32_t code_of(float x, float scale, float rc) {
 template <int LANES>
 __global__ void __launch_bounds__(CACHE_THREADS) cache_append_kernel(const CacheView c, const uint16_t *__restrict__ k, const uint16_t *__restrict__ v, int64_t k_token, int64_t k_head,
                                                                      int64_t v_token, int64_t v_head) {
-    constexpr int ROWS = 32 / LANES, BATCH = 4;  // rows of a warp at once, and so many times
-    const int lane = threadIdx.x & 31, part = lane % LANES, sub = lane / LANES, rows = 2 * c.kv_heads;
+    constexpr int ROWS = 32 / LANES, BATCH = 4;  // rows of a warp at once, and so many times; a CTA along y takes so many of each token's
+    const int lane = threadIdx.x & 31, part = lane % LANES, sub = lane / LANES, rows = 2 * c.kv_heads, r0 = blockIdx.y * (ROWS * BATCH);
     int t0, t1;
     tokens_of_warp(c, t0, t1);
     CachePlace place;
     for (int token = t0; token < t1; ++token) {
         const int64_t at = place.of(c, token);
         if (at < 0) continue;
-        for (int r0 = 0; r0 < rows; r0 += ROWS * BATCH) {
+        {
             uint4 raw[BATCH];
 #pragma unroll
             for (int n = 0; n < BATCH; ++n) {
@@ -96,14 +96,14 @@ __global__ void __launch_bounds__(CACHE_THREADS) cache_append_kernel(const Cache
 template <int LANES>
 __global__ void __launch_bounds__(CACHE_THREADS) cache_read_kernel(const CacheView c, uint16_t *__restrict__ k, uint16_t *__restrict__ v) {
     constexpr int ROWS = 32 / LANES, BATCH = 4;
-    const int lane = threadIdx.x & 31, part = lane % LANES, sub = lane / LANES, rows = 2 * c.kv_heads;
+    const int lane = threadIdx.x & 31, part = lane % LANES, sub = lane / LANES, rows = 2 * c.kv_heads, r0 = blockIdx.y * (ROWS * BATCH);
     int t0, t1;
     tokens_of_warp(c, t0, t1);
     CachePlace place;
     for (int token = t0; token < t1; ++token) {
         const int64_t at = place.of(c, token);
         if (place.b < 0) continue;  // a row of no sequence stays as it is
-        for (int r0 = 0; r0 < rows; r0 += ROWS * BATCH) {
+        {
             uint32_t codes[BATCH];
             float scale[BATCH];
 #pragma unroll
@@ -165,9 +165,10 @@ int cache_view(const g2d_cache_desc *d, CacheView *c) {
     return G2D_OK;
 }
 
-static unsigned cache_grid(const CacheView &c) {  // a token per warp and up to eight CTAs per SM
-    const int64_t blocks = ceil_div((int64_t)c.tokens, (int64_t)(CACHE_THREADS / 32));
-    return (unsigned)(blocks < 148 * 8 ? blocks : 148 * 8);
+static dim3 cache_grid(const CacheView &c) {  // a token and four times a warp's rows per warp, up to eight CTAs per SM
+    const int64_t blocks = ceil_div((int64_t)c.tokens, (int64_t)(CACHE_THREADS / 32)), groups = ceil_div((int64_t)2 * c.kv_heads * (c.head_dim / 8), (int64_t)(32 * 4));
+    const int64_t most = groups < 148 * 8 ? 148 * 8 / groups : 1;
+    return dim3((unsigned)(blocks < most ? blocks : most), (unsigned)groups);
 }
 
 }  // namespace g2d
