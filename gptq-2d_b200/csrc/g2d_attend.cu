@@ -47,7 +47,7 @@ struct AttendShared {
     using S = AttendShape<D, NT>;
     AttendStage<D> stage[S::WARPS][S::STAGES];
     uint64_t full[S::WARPS][S::STAGES];
-    long long totals[S::WARPS];
+    unsigned totals[S::WARPS];
     AttendPart parts[2 * S::WARPS];
 };
 
@@ -71,51 +71,17 @@ __device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t b
 }
 
 // Units of sequence b: of each kv head and each `rows_per_item` rows, its blocks of keys (one at least: rows without keys get their zeros)
-__device__ __forceinline__ int64_t attend_units(const AttendArgs &a, const AttendSequence &s, int rows_per_item, int &blocks, int &items) {
-    const int64_t rows = (int64_t)s.count * a.group;
-    blocks = max((s.keys + CACHE_BLOCK - 1) / CACHE_BLOCK, 1);
-    items = rows >= a.rows_from && rows < a.rows_to ? a.c.kv_heads * (int)((rows + rows_per_item - 1) / rows_per_item) : 0;
-    return (int64_t)items * blocks;
+template <int ROWS>
+__device__ __forceinline__ unsigned attend_units(const AttendArgs &a, const AttendSequence &s, int &blocks, int &items) {
+    const unsigned rows = (unsigned)(s.count * a.group);  // of no more than tokens x heads
+    blocks = max((int)(((unsigned)s.keys + CACHE_BLOCK - 1) / CACHE_BLOCK), 1);
+    items = rows >= (unsigned)a.rows_from && rows < (unsigned)a.rows_to ? a.c.kv_heads * (int)((rows + ROWS - 1) / ROWS) : 0;
+    return (unsigned)items * blocks;
 }
-__device__ __forceinline__ int64_t attend_units(const AttendArgs &a, int b, int rows_per_item) {
+template <int ROWS>
+__device__ __forceinline__ unsigned attend_units(const AttendArgs &a, int b) {
     int blocks, items;
-    return b < a.c.batch ? attend_units(a, attend_sequence(a, b), rows_per_item, blocks, items) : 0;
-}
-// All threads of a CTA of WARPS warps: the units of all sequences
-template <int WARPS>
-__device__ __forceinline__ int64_t all_units(const AttendArgs &a, int rows_per_item, long long (&totals)[WARPS]) {
-    int64_t mine = 0;
-    for (int b = threadIdx.x; b < a.c.batch; b += 32 * WARPS) mine += attend_units(a, b, rows_per_item);
-    mine = warp_sum(mine);
-    if ((threadIdx.x & 31) == 0) totals[threadIdx.x >> 5] = mine;
-    __syncthreads();
-    int64_t all = 0;
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) all += totals[w];
-    return all;
-}
-// A warp: the sequence that unit u belongs to, and the units before it
-__device__ __forceinline__ int sequence_of_unit(const AttendArgs &a, int rows_per_item, int64_t u, int64_t &before) {
-    const int lane = threadIdx.x & 31;
-    int64_t base = 0;
-    for (int b0 = 0; b0 < a.c.batch; b0 += 32) {
-        int64_t sum = attend_units(a, b0 + lane, rows_per_item);
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int64_t up = __shfl_up_sync(0xffffffffu, sum, o);
-            if (lane >= o) sum += up;
-        }
-        const unsigned past = __ballot_sync(0xffffffffu, base + sum > u);
-        if (past) {
-            const int at = __ffs(past) - 1;
-            const int64_t upto = __shfl_sync(0xffffffffu, sum, at > 0 ? at - 1 : 0);
-            before = base + (at > 0 ? upto : 0);
-            return b0 + at;
-        }
-        base += __shfl_sync(0xffffffffu, sum, 31);
-    }
-    before = base;
-    return a.c.batch;
+    return b < a.c.batch ? attend_units<ROWS>(a, attend_sequence(a, b), blocks, items) : 0u;
 }
 
 // A place in the list of units
@@ -123,24 +89,26 @@ struct AttendCursor {
     int u, end;  // units of the warp's share
     int b, item, block, blocks, items;
     AttendSequence s;
-    __device__ __forceinline__ void open(const AttendArgs &a, int rows_per_item) {  // sequence b, or the next one that has units
+    template <int ROWS>
+    __device__ __forceinline__ void open(const AttendArgs &a) {  // sequence b, or the next one that has units
         for (;; ++b) {
             if (b >= a.c.batch) {  // not reached while u < end
                 end = u;
                 return;
             }
             s = attend_sequence(a, b);
-            if (attend_units(a, s, rows_per_item, blocks, items) > 0) return;
+            if (attend_units<ROWS>(a, s, blocks, items) > 0) return;
         }
     }
-    __device__ __forceinline__ void step(const AttendArgs &a, int rows_per_item) {
+    template <int ROWS>
+    __device__ __forceinline__ void step(const AttendArgs &a) {
         if (++u >= end) return;
         if (++block < blocks) return;
         block = 0;
         if (++item < items) return;
         item = 0;
         ++b;
-        open(a, rows_per_item);
+        open<ROWS>(a);
     }
 };
 
@@ -165,17 +133,21 @@ __global__ void __launch_bounds__(AttendShape<D, NT>::THREADS, 1) attend_rows_ke
     }
     let_the_next_launch_start();
     if (lane < 2) sh.parts[2 * warp + lane].last = 0;
-    const int64_t units = all_units<ATTEND_WARPS>(a, ROWS, sh.totals);  // its barrier is that of the initialisation as well
-    const int64_t shares = min(units, (int64_t)gridDim.x), share = blockIdx.x;
+    const auto units_of = [&](int b) { return attend_units<ROWS>(a, b); };
+    unsigned mine_units;
+    const AttendShares shares(count_units<ATTEND_WARPS>(c.batch, units_of, sh.totals, mine_units), gridDim.x);
+    const unsigned share = blockIdx.x;
     AttendCursor cur;
     cur.u = cur.end = 0;
-    if (share < shares) {
-        const int64_t u0 = share * units / shares, n = (share + 1) * units / shares - u0, mine = u0 + warp * n / ATTEND_WARPS;
-        cur.end = (int)(u0 + (warp + 1) * n / ATTEND_WARPS - mine);
-        if (cur.end > 0) {
-            int64_t before;
-            cur.b = sequence_of_unit(a, ROWS, mine, before);
-            cur.open(a, ROWS);
+    if (share < shares.count) {
+        // of n units the first warps have one each, where there are not enough for all: a warp between two others of an item has a part of it
+        const unsigned u0 = shares.begin(share), n = shares.begin(share + 1) - u0, active = min(n, (unsigned)ATTEND_WARPS);
+        if ((unsigned)warp < active) {
+            const unsigned mine = u0 + warp * n / active;
+            cur.end = (int)(u0 + (warp + 1) * n / active - mine);
+            unsigned before;
+            cur.b = sequence_of_unit(c.batch, units_of, mine_units, mine, before);
+            cur.template open<ROWS>(a);
             cur.item = (int)((mine - before) / cur.blocks);
             cur.block = (int)((mine - before) % cur.blocks);
         }
@@ -207,7 +179,7 @@ __global__ void __launch_bounds__(AttendShape<D, NT>::THREADS, 1) attend_rows_ke
             const int64_t row = (((int64_t)next_page * c.kv_heads + ahead.item % c.kv_heads) << c.page_shift) + ((ahead.block * CACHE_BLOCK + to) & (c.page_size - 1));
             bulk_load(reinterpret_cast<unsigned char *>(&sh.stage[warp][stage]) + target, source + row * key_bytes, piece_keys * key_bytes, bar);
         }
-        ahead.step(a, ROWS);
+        ahead.template step<ROWS>(a);
         next_page = page_of(ahead);
     };
 #pragma unroll
@@ -572,7 +544,7 @@ __global__ void __launch_bounds__(AttendShape<D, NT>::THREADS, 1) attend_rows_ke
         // on to the next run
         cur.u += last_block - first_block - 1;
         cur.block = last_block - 1;
-        cur.step(a, ROWS);
+        cur.template step<ROWS>(a);
     }
     if (!sound && lane == 0) {
         let_it_land();  // loads under way must not outlive the shared memory
@@ -586,24 +558,21 @@ __global__ void __launch_bounds__(AttendShape<D, NT>::THREADS, 1) attend_rows_ke
     };
     for (int p0 = next_part(0); p0 < 2 * ATTEND_WARPS;) {
         const AttendPart &begin = sh.parts[p0];
-        unsigned mask = 1u << p0;
-        int p1 = p0, behind = next_part(p0 + 1);
+        int p1 = p0, count = 1, behind = next_part(p0 + 1);
         while (behind < 2 * ATTEND_WARPS && sh.parts[behind].b == begin.b && sh.parts[behind].item == begin.item) {
             p1 = behind;
-            mask |= 1u << behind;
+            ++count;
             behind = next_part(behind + 1);
         }
-        const int count = __popc(mask), first = begin.first, last = sh.parts[p1].last;
+        const int first = begin.first, last = sh.parts[p1].last;
         const bool whole = first == 0 && last == begin.blocks;
         const int head = begin.item % c.kv_heads, row0 = begin.item / c.kv_heads * ROWS, rows = begin.s.count * a.group;
-        const auto slot_of = [&](int i) {  // the i-th bit of the mask: parts stand close together, so that this is short
-            unsigned left = mask;
-            for (int k = 0; k < i; ++k) left &= left - 1;
-            return attend_slot<D, ROWS>(a, WARP_SLOTS + 2 * ATTEND_WARPS * share + __ffs(left) - 1);
-        };
+        // the parts of an item but its first are the first ones of the warps that follow
+        const float *const from = attend_slot<D, ROWS>(a, WARP_SLOTS + 2 * ATTEND_WARPS * (int64_t)share + p0), *const next = attend_slot<D, ROWS>(a, WARP_SLOTS + 2 * ATTEND_WARPS * (int64_t)share + (p0 & ~1));
         for (int i = warp; i < ROWS && row0 + i < rows; i += ATTEND_WARPS) {
             float acc[D / 32], m, l;
-            merge_parts<D>(count, [&](int k) { return slot_of(k) + i * D; }, [&](int k) { return slot_of(k) + ROWS * D + i; }, [&](int k) { return slot_of(k) + ROWS * D + ROWS + i; }, acc, m, l);
+            const auto row = [&](int k) { return (k == 0 ? from : next + k * (2 * ROWS * (D + 2))) + i * D; };
+            merge_parts<D>(count, row, ROWS * D + i - i * D, ROWS * D + ROWS + i - i * D, acc, m, l);
             if (whole) {
                 const int token = (row0 + i) / a.group, h = head * a.group + (row0 + i) % a.group;
                 write_row<D>((uint16_t *)a.out + ((int64_t)(begin.s.first + token) * a.heads + h) * D, acc, l, c.bf16);
@@ -632,55 +601,61 @@ struct JoinArgs {
 template <int D, int NT>
 __global__ void __launch_bounds__(JOIN_THREADS) attend_join_kernel(const JoinArgs j) {
     constexpr int ROWS = 8 * NT, WARPS = JOIN_THREADS / 32;
-    __shared__ long long totals[WARPS];
+    __shared__ unsigned totals[WARPS];
     const int warp = threadIdx.x >> 5;
+    unsigned mine, u0 = 0, u1 = 0, end = 0;
     if ((int)blockIdx.x < j.tile_ctas) {
         const AttendArgs &a = j.tiles;
-        const int64_t units = all_tile_units<WARPS>(a, totals), shares = min(units, (int64_t)TA_GRID), share = blockIdx.x / TILE_JOINS;
+        const AttendShares shares(count_tile_units<WARPS>(a, totals, mine), TA_GRID);
+        const unsigned share = blockIdx.x / TILE_JOINS;
         TileCursor cur;
-        int64_t u0 = 0, u1 = 0, end = 0;
-        if (share + 1 < shares) {
-            end = (share + 1) * units / shares;
-            cur.find(a, end - 1);
+        if (share + 1 < shares.count) {
+            end = shares.begin(share + 1);
+            cur.find(a, mine, end - 1);
             u0 = end - 1 - cur.block;
             u1 = u0 + cur.blocks;
         }
         after_the_launch_before();  // by every CTA: what follows on the stream must not start before the results are there
-        if (u1 <= end || u0 < share * units / shares) return;
-        const int count = (int)((u1 * shares - 1) / units - share) + 1;  // the share of unit u1 - 1 is the last one that begins at or before it
-        const auto slot_of = [&](int k) { return tile_slot<D>(a, 2 * (share + k) + (k == 0 ? 1 : 0)); };
+        if (u1 <= end || u0 < shares.begin(share)) return;
+        const int count = (int)(shares.of(u1 - 1) - share) + 1;
+        constexpr int SLOT = TA_ROWS * (D + 2);
+        const float *const from = tile_slot<D>(a, 2 * share + 1), *const next = tile_slot<D>(a, 2 * share);
         for (int i = blockIdx.x % TILE_JOINS * 32 + warp, n = 0; n < 32 / WARPS; ++n, i += WARPS) {
             const int r = cur.pair * TA_ROWS + i;
             if (r >= cur.s.count * a.group) break;
             float acc[D / 32], m, l;
-            merge_parts<D>(count, [&](int k) { return slot_of(k) + i * D; }, [&](int k) { return slot_of(k) + TA_ROWS * D + i; }, [&](int k) { return slot_of(k) + TA_ROWS * D + TA_ROWS + i; }, acc, m, l);
+            const auto row = [&](int k) { return (k == 0 ? from : next + (int64_t)k * (2 * SLOT)) + i * D; };
+            merge_parts<D>(count, row, TA_ROWS * D + i - i * D, TA_ROWS * D + TA_ROWS + i - i * D, acc, m, l);
             write_row<D>((uint16_t *)a.out + ((int64_t)(cur.s.first + r / a.group) * a.heads + cur.head * a.group + r % a.group) * D, acc, l, a.c.bf16);
         }
     } else {
         const AttendArgs &a = j.rows;
-        const int64_t units = all_units<WARPS>(a, ROWS, totals), shares = min(units, (int64_t)ATTEND_GRID), share = blockIdx.x - j.tile_ctas;
+        const auto units_of = [&](int b) { return attend_units<ROWS>(a, b); };
+        const AttendShares shares(count_units<WARPS>(a.c.batch, units_of, totals, mine), ATTEND_GRID);
+        const unsigned share = blockIdx.x - j.tile_ctas;
         AttendCursor cur;
-        int64_t u0 = 0, u1 = 0, end = 0;
-        if (share + 1 < shares) {
-            int64_t before;
-            end = (share + 1) * units / shares;
+        if (share + 1 < shares.count) {
+            unsigned before;
+            end = shares.begin(share + 1);
             cur.u = 0;
             cur.end = 1;
-            cur.b = sequence_of_unit(a, ROWS, end - 1, before);
-            cur.open(a, ROWS);
+            cur.b = sequence_of_unit(a.c.batch, units_of, mine, end - 1, before);
+            cur.template open<ROWS>(a);
             cur.item = (int)((end - 1 - before) / cur.blocks);
-            u0 = before + (int64_t)cur.item * cur.blocks;
+            u0 = before + (unsigned)cur.item * cur.blocks;
             u1 = u0 + cur.blocks;
         }
         after_the_launch_before();
-        if (u1 <= end || u0 < share * units / shares) return;
-        const int count = (int)((u1 * shares - 1) / units - share) + 1;
-        const auto slot_of = [&](int k) { return attend_slot<D, ROWS>(a, 2 * (share + k) + (k == 0 ? 1 : 0)); };
+        if (u1 <= end || u0 < shares.begin(share)) return;
+        const int count = (int)(shares.of(u1 - 1) - share) + 1;
+        constexpr int SLOT = ROWS * (D + 2);
+        const float *const from = attend_slot<D, ROWS>(a, 2 * share + 1), *const next = attend_slot<D, ROWS>(a, 2 * share);
         for (int i = warp; i < ROWS; i += WARPS) {
             const int r = cur.item / a.c.kv_heads * ROWS + i;
             if (r >= cur.s.count * a.group) break;
             float acc[D / 32], m, l;
-            merge_parts<D>(count, [&](int k) { return slot_of(k) + i * D; }, [&](int k) { return slot_of(k) + ROWS * D + i; }, [&](int k) { return slot_of(k) + ROWS * D + ROWS + i; }, acc, m, l);
+            const auto row = [&](int k) { return (k == 0 ? from : next + (int64_t)k * (2 * SLOT)) + i * D; };
+            merge_parts<D>(count, row, ROWS * D + i - i * D, ROWS * D + ROWS + i - i * D, acc, m, l);
             write_row<D>((uint16_t *)a.out + ((int64_t)(cur.s.first + r / a.group) * a.heads + cur.item % a.c.kv_heads * a.group + r % a.group) * D, acc, l, a.c.bf16);
         }
     }
@@ -757,6 +732,10 @@ extern "C" int g2d_cache_attend(const g2d_attend_desc *d, void *stream) {
     if (d->heads < 1 || d->heads % a.c.kv_heads != 0 || !(d->softcap >= 0.f)) return G2D_ERR_BAD_ARGUMENT;
     if (a.c.tokens == 0 || a.c.batch == 0) return G2D_OK;
     if ((int64_t)a.c.tokens * d->heads > 0x7fffffff) return G2D_ERR_TOO_LARGE;
+    {  // units of 64 keys and eight rows: counted in 32 bits
+        const int64_t capacity = (int64_t)a.c.table_width << a.c.page_shift, blocks = ceil_div(capacity < 0x7fffffff ? capacity : 0x7fffffff, (int64_t)CACHE_BLOCK) + 1;
+        if (blocks * ((int64_t)a.c.tokens * d->heads / 8 + 2 * (int64_t)a.c.kv_heads * a.c.batch) > 0x7fffffff) return G2D_ERR_TOO_LARGE;
+    }
     if (!d->q || !d->out || (((uintptr_t)d->q | (uintptr_t)d->out) & 15) != 0 || ((d->q_token_stride | d->q_head_stride) & 7) != 0) return G2D_ERR_BAD_ARGUMENT;
     if (!d->workspace || d->workspace_bytes < attend_space(a.c.head_dim).all || ((uintptr_t)d->workspace & 255) != 0) return G2D_ERR_WORKSPACE;
     a.q = d->q;

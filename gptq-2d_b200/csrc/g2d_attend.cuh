@@ -73,20 +73,69 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
     return r;
 }
-__device__ __forceinline__ int64_t warp_sum(int64_t v) {
+// ---- the list of units, and its shares ----
+// Units are counted in 32 bits (the entry point refuses what could have more).  Share i of `count` has the units from begin(i) on.
+struct AttendShares {
+    unsigned count, each, more;  // the first `more` shares have each + 1
+    __device__ __forceinline__ AttendShares(unsigned units, unsigned most) : count(min(units, most)), each(count ? units / count : 0u), more(count ? units - each * count : 0u) {}
+    __device__ __forceinline__ unsigned begin(unsigned i) const { return i * each + min(i, more); }
+    __device__ __forceinline__ unsigned of(unsigned u) const { return u < more * (each + 1) ? u / (each + 1) : more + (u - more * (each + 1)) / each; }
+};
+__device__ __forceinline__ unsigned warp_add(unsigned v) { return __reduce_add_sync(0xffffffffu, v); }
+// All threads of a CTA of WARPS warps: the units of all sequences, units(b) of one, and this lane's first one (of sequence `lane`).  Few sequences: every warp by itself.
+template <int WARPS, typename Units>
+__device__ __forceinline__ unsigned count_units(int batch, Units units, unsigned (&totals)[WARPS], unsigned &mine) {
+    const int lane = threadIdx.x & 31;
+    mine = units(lane);
+    if (batch <= 32) return warp_add(mine);
+    unsigned sum = 0u;
+    for (int b = threadIdx.x; b < batch; b += 32 * WARPS) sum += units(b);
+    sum = warp_add(sum);
+    if (lane == 0) totals[threadIdx.x >> 5] = sum;
+    __syncthreads();
+    unsigned all = 0u;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
+    for (int w = 0; w < WARPS; ++w) all += totals[w];
+    return all;
+}
+// A warp: which of its lanes' counts the unit `at` falls into, the first of them beginning at `base` (32: none); `base` becomes where that count begins, or the end
+__device__ __forceinline__ int lane_of_unit(unsigned count, unsigned at, unsigned &base) {
+    const int lane = threadIdx.x & 31;
+    unsigned sum = count;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const unsigned up = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += up;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, base + sum > at);
+    const int found = past ? __ffs(past) - 1 : 32;
+    if (found > 0) base += __shfl_sync(0xffffffffu, sum, found - 1);
+    return found;
+}
+// A warp: the sequence that unit `at` belongs to, and where its units begin; `mine` as count_units has left it
+template <typename Units>
+__device__ __forceinline__ int sequence_of_unit(int batch, Units units, unsigned mine, unsigned at, unsigned &base) {
+    base = 0u;
+    for (int b0 = 0; b0 < batch; b0 += 32) {
+        const int k = lane_of_unit(b0 == 0 ? mine : units(b0 + (int)(threadIdx.x & 31)), at, base);
+        if (k < 32) return b0 + k;
+    }
+    return batch;
 }
 
-
-// Parts of a row's result, in the order of the keys: D sums, the maximum that their exponentials refer to (of the scores as powers of two) and the sum of these.
-// A warp: adds up `count` parts, part i's sums at sums(i), its maximum and sum at maximum(i) and total(i); lane x returns the sums of the channels x, x + 32, ..
-template <int D, typename Sums, typename Maximum, typename Total>
-__device__ __forceinline__ void merge_parts(int count, Sums sums, Maximum maximum, Total total, float (&acc)[D / 32], float &m, float &l) {
+// Parts of a row's result, in the order of the keys: D sums, the reference of their exponentials (a power of two) and the sum of these.
+// A warp: adds up `count` parts; the row's sums of part i are at row(i), its reference and its sum of exponentials `reference` and `total` floats behind.  Lane x gets the
+// sums of the channels x, x + 32, ..
+template <int D, typename Row>
+__device__ __forceinline__ void merge_parts(int count, Row row, int reference, int total, float (&acc)[D / 32], float &m, float &l) {
     const int lane = threadIdx.x & 31;
-    m = -INFINITY;
-    for (int i = lane; i < count; i += 32) m = fmaxf(m, __ldcg(maximum(i)));
+    float mine = -INFINITY, t = 0.f;
+    if (lane < count) {
+        mine = __ldcg(row(lane) + reference);
+        t = __ldcg(row(lane) + total);
+    }
+    m = mine;
+    for (int i = lane + 32; i < count; i += 32) m = fmaxf(m, __ldcg(row(i) + reference));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     const float base = m == -INFINITY ? 0.f : m;
@@ -94,19 +143,32 @@ __device__ __forceinline__ void merge_parts(int count, Sums sums, Maximum maximu
 #pragma unroll
     for (int x = 0; x < D / 32; ++x) acc[x] = 0.f;
     for (int i0 = 0; i0 < count; i0 += 32) {
-        float w = 0.f, t = 0.f;
-        if (i0 + lane < count) {
-            w = ex2(__ldcg(maximum(i0 + lane)) - base);
-            t = __ldcg(total(i0 + lane));
+        if (i0 > 0) {
+            mine = -INFINITY;
+            t = 0.f;
+            if (i0 + lane < count) {
+                mine = __ldcg(row(i0 + lane) + reference);
+                t = __ldcg(row(i0 + lane) + total);
+            }
         }
+        const float w = ex2(mine - base);
         const int here = min(32, count - i0);
-#pragma unroll 4
-        for (int i = 0; i < here; ++i) {
-            const float f = __shfl_sync(0xffffffffu, w, i);
-            l = fmaf(__shfl_sync(0xffffffffu, t, i), f, l);
-            const float *const from = sums(i0 + i) + lane;
+#pragma unroll 1
+        for (int i = 0; i < here; i += 4) {  // four parts' loads travel together
+            float v[4][D / 32];
 #pragma unroll
-            for (int x = 0; x < D / 32; ++x) acc[x] = fmaf(__ldcg(from + x * 32), f, acc[x]);
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int x = 0; x < D / 32; ++x) v[k][x] = i + k < here ? __ldcg(row(i0 + i + k) + x * 32 + lane) : 0.f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float f = __shfl_sync(0xffffffffu, w, (i + k) & 31), tk = __shfl_sync(0xffffffffu, t, (i + k) & 31);
+                if (i + k < here) {
+                    l = fmaf(tk, f, l);
+#pragma unroll
+                    for (int x = 0; x < D / 32; ++x) acc[x] = fmaf(v[k][x], f, acc[x]);
+                }
+            }
         }
     }
 }
@@ -128,52 +190,36 @@ __device__ __forceinline__ int tile_blocks(const AttendArgs &a, const AttendSequ
     const unsigned last = min((unsigned)(s.count * a.group), (unsigned)(pair + 1) * TA_ROWS) - 1u;
     return max((int)(((unsigned)visible_keys(a, s, (int)(last / (unsigned)a.group)) + TA_KEYS - 1) / TA_KEYS), 1);
 }
-constexpr int FEW_SEQUENCES = 32;  // up to here the lanes of a warp share a sequence's pairs, beyond each has sequences of its own
-__device__ __forceinline__ int64_t tile_units(const AttendArgs &a, int b) {  // a thread
-    if (b >= a.c.batch) return 0;
+__device__ __forceinline__ unsigned tile_units(const AttendArgs &a, int b) {  // a thread
+    if (b >= a.c.batch) return 0u;
     const AttendSequence s = attend_sequence(a, b);
-    int64_t sum = 0;
+    unsigned sum = 0u;
     for (int p = 0, n = tile_pairs(a, s); p < n; ++p) sum += tile_blocks(a, s, p);
     return sum * a.c.kv_heads;
 }
-__device__ __forceinline__ int64_t warp_tile_units(const AttendArgs &a, const AttendSequence &s) {  // a warp
-    int64_t sum = 0;
-    for (int p = threadIdx.x & 31, n = tile_pairs(a, s); p < n; p += 32) sum += tile_blocks(a, s, p);
-    return warp_sum(sum) * a.c.kv_heads;
-}
-// All threads of a CTA of WARPS warps: the units of all sequences
-template <int WARPS>
-__device__ __forceinline__ int64_t all_tile_units(const AttendArgs &a, long long (&totals)[WARPS]) {
-    int64_t mine = 0;
-    if (a.c.batch < FEW_SEQUENCES) {
-        for (int b = threadIdx.x >> 5; b < a.c.batch; b += WARPS) mine += warp_tile_units(a, attend_sequence(a, b));
-    } else {
-        for (int b = threadIdx.x; b < a.c.batch; b += 32 * WARPS) mine += tile_units(a, b);
-        mine = warp_sum(mine);
-    }
-    if ((threadIdx.x & 31) == 0) totals[threadIdx.x >> 5] = mine;
-    __syncthreads();
-    int64_t all = 0;
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) all += totals[w];
-    return all;
-}
-// A warp: which of the 32 counts of its lanes the unit `at` of the list that begins at `base` falls into (32: none); `base` becomes where that count begins, or the end
-__device__ __forceinline__ int lane_of_unit(int64_t count, int64_t at, int64_t &base) {
+// The units of sequence `lane`, or of sequence b, by a whole warp: up to 32 sequences, whose pairs of tiles the lanes share
+__device__ __forceinline__ unsigned tile_units_of_few(const AttendArgs &a) {
     const int lane = threadIdx.x & 31;
-    int64_t sum = count;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int64_t up = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += up;
+    unsigned mine = 0u;
+    for (int b = 0; b < a.c.batch; ++b) {
+        const AttendSequence s = attend_sequence(a, b);
+        unsigned sum = 0u;
+        for (int p = lane, n = tile_pairs(a, s); p < n; p += 32) sum += tile_blocks(a, s, p);
+        sum = warp_add(sum) * a.c.kv_heads;
+        if (b == lane) mine = sum;
     }
-    const unsigned past = __ballot_sync(0xffffffffu, base + sum > at);
-    const int found = past ? __ffs(past) - 1 : 32;
-    if (found > 0) base += __shfl_sync(0xffffffffu, sum, found - 1);
-    return found;
+    return mine;
+}
+template <int WARPS>
+__device__ __forceinline__ unsigned count_tile_units(const AttendArgs &a, unsigned (&totals)[WARPS], unsigned &mine) {
+    if (a.c.batch <= 8) {
+        mine = tile_units_of_few(a);
+        return warp_add(mine);
+    }
+    return count_units<WARPS>(a.c.batch, [&](int b) { return tile_units(a, b); }, totals, mine);
 }
 struct TileCursor {
-    int64_t u, end;
+    unsigned u, end;
     int b, pair, pairs, head, block, blocks;
     AttendSequence s;
     __device__ __forceinline__ void open(const AttendArgs &a) {  // sequence b, or the next one that has units
@@ -190,29 +236,14 @@ struct TileCursor {
         blocks = tile_blocks(a, s, 0);
     }
     // A warp: unit `at` of the list, which has more
-    __device__ __forceinline__ void find(const AttendArgs &a, int64_t at) {
+    __device__ __forceinline__ void find(const AttendArgs &a, unsigned mine, unsigned at) {
         const int lane = threadIdx.x & 31;
-        int64_t base = 0;
+        unsigned base;
         u = at;
-        b = 0;
-        if (a.c.batch < FEW_SEQUENCES) {
-            for (; b < a.c.batch; ++b) {
-                const int64_t here = warp_tile_units(a, attend_sequence(a, b));
-                if (base + here > at) break;
-                base += here;
-            }
-        } else {
-            for (; b < a.c.batch; b += 32) {
-                const int k = lane_of_unit(tile_units(a, b + lane), at, base);
-                if (k < 32) {
-                    b += k;
-                    break;
-                }
-            }
-        }
+        b = sequence_of_unit(a.c.batch, [&](int i) { return tile_units(a, i); }, mine, at, base);
         open(a);
         for (int p0 = 0; p0 < pairs; p0 += 32) {
-            const int k = lane_of_unit(p0 + lane < pairs ? (int64_t)tile_blocks(a, s, p0 + lane) * a.c.kv_heads : 0, at, base);
+            const int k = lane_of_unit(p0 + lane < pairs ? (unsigned)tile_blocks(a, s, p0 + lane) * a.c.kv_heads : 0u, at, base);
             if (k < 32) {
                 pair = p0 + k;
                 break;
@@ -222,7 +253,7 @@ struct TileCursor {
         head = (int)((at - base) / blocks);
         block = (int)((at - base) % blocks);
     }
-    __device__ __forceinline__ int run() const { return (int)min((int64_t)(blocks - block), end - u); }  // blocks of the item in this share
+    __device__ __forceinline__ int run() const { return (int)min((unsigned)(blocks - block), end - u); }  // blocks of the item in this share
     __device__ __forceinline__ void next(const AttendArgs &a) {                                           // the item behind this run
         u += run();
         if (u >= end) return;

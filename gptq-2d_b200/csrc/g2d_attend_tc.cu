@@ -39,7 +39,7 @@ struct TileBarriers {
     int unit[TA_SCALES];             // exponent bits of the largest scale so far
     int tops[4];
     TileRun runs[TA_RUNS];
-    long long totals[TA_THREADS / 32];
+    unsigned totals[TA_THREADS / 32];
     uint32_t tmem;
     int failed;
 };
@@ -112,14 +112,16 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const Atten
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     let_the_next_launch_start();
-    const int64_t units = all_tile_units<TA_THREADS / 32>(a, bar.totals);  // its barrier is that of the initialisation as well
+    unsigned mine_units;
+    const unsigned units = count_tile_units<TA_THREADS / 32>(a, bar.totals, mine_units);
     if (units == 0) return;                                                // sequences of few rows only
     if (warp == 1) tmem_alloc<false>(&bar.tmem, 512);
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = bar.tmem;
-    const int64_t shares = min(units, (int64_t)gridDim.x), share = blockIdx.x;
+    const AttendShares shares(units, gridDim.x);
+    const unsigned share = blockIdx.x;
     // the run of that number, for every thread of a role; its entry stays until all roles have let it go
     const auto run_of = [&](uint32_t number, bool &go) -> const TileRun & {
         if (go) go = wait(&bar.run_full[number % TA_RUNS], (number / TA_RUNS) & 1, 20);
@@ -134,9 +136,9 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const Atten
             // ---- the share's runs ----
             TileCursor cur;
             cur.u = cur.end = 0;
-            if (share < shares) {
-                cur.find(a, share * units / shares);
-                cur.end = (share + 1) * units / shares;
+            if (share < shares.count) {
+                cur.find(a, mine_units, shares.begin(share));
+                cur.end = shares.begin(share + 1);
             }
             if (lane == 0) {
                 for (uint32_t number = 0;; ++number) {
