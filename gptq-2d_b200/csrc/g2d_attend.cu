@@ -66,8 +66,15 @@ __device__ __forceinline__ uint32_t transposed(uint32_t a) {
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
     return d;
 }
-__device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+// Codes are read once per step: they leave the L2 before what every step reads again (lengths, tables, the kernels' own instructions)
+__device__ __forceinline__ uint64_t read_once() {
+    uint64_t policy;
+    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+    return policy;
+}
+__device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *bar, uint64_t policy) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)), "l"(policy)
+                 : "memory");
 }
 
 // Units of sequence b: of each kv head and each `rows_per_item` rows, its blocks of keys (one at least: rows without keys get their zeros)
@@ -166,6 +173,7 @@ __global__ void __launch_bounds__(AttendShape<D, NT>::THREADS, 1) attend_rows_ke
         const int page = c.table[at.b * c.table_stride + (key >> c.page_shift)];
         return page < c.pages ? page : -1;
     };
+    const uint64_t policy = read_once();
     int next_page = page_of(ahead);
     unsigned present[ATTEND_STAGES];  // which pieces of a stage were loaded: four bits each
 #pragma unroll
@@ -177,7 +185,7 @@ __global__ void __launch_bounds__(AttendShape<D, NT>::THREADS, 1) attend_rows_ke
         __syncwarp();
         if (next_page >= 0) {
             const int64_t row = (((int64_t)next_page * c.kv_heads + ahead.item % c.kv_heads) << c.page_shift) + ((ahead.block * CACHE_BLOCK + to) & (c.page_size - 1));
-            bulk_load(reinterpret_cast<unsigned char *>(&sh.stage[warp][stage]) + target, source + row * key_bytes, piece_keys * key_bytes, bar);
+            bulk_load(reinterpret_cast<unsigned char *>(&sh.stage[warp][stage]) + target, source + row * key_bytes, piece_keys * key_bytes, bar, policy);
         }
         ahead.template step<ROWS>(a);
         next_page = page_of(ahead);
