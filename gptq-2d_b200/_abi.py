@@ -7,8 +7,10 @@ CUDA graph.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
+import struct
 
 import torch
 
@@ -97,22 +99,11 @@ class AttendDesc(ctypes.Structure):
     ]
 
 
-class LinearDesc(ctypes.Structure):
-    """Mirror of ``g2d_linear_desc``."""
-    _fields_ = [
-        ("half", _i32), ("bits", _i32),
-        ("m", _i64), ("n", _i64), ("tokens", _i64),
-        ("x", _vp), ("x_stride", _i64),
-        ("codes", _vp), ("row_bytes", _i64), ("groups", _i64),
-        ("scale", _vp), ("scale_row_stride", _i64), ("scale_group_stride", _i64),
-        ("zero", _vp), ("zero_row_stride", _i64), ("zero_group_stride", _i64),
-        ("qmin", _dbl),
-        ("adapters", _i64), ("rank", _i32), ("reserved", _i32),
-        ("down", _vp), ("up", _vp), ("scaling", _vp), ("index", _vp),
-        ("out", _vp), ("out_stride", _i64),
-        ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
-        ("status", _vp),
-    ]
+# Descriptors of the calls of a serving step, which are as short as the host code around them: packed in one go instead of field by field (2 us less
+# for thirty fields).  Native alignment, so the formats follow the header's fields in order.
+CACHE_DESC = struct.Struct("@4i5q7P")  # g2d_cache_desc
+ATTEND_DESC = struct.Struct("@4i5q7P" "2i2fP2q3PPNP")  # g2d_attend_desc
+LINEAR_DESC = struct.Struct("@2i3qPqP2qP2qP2qdq2i4PPqPNP")  # g2d_linear_desc
 
 
 _SIGNATURES = {
@@ -153,12 +144,12 @@ _SIGNATURES = {
 }
 
 _SIGNATURES.update({
-    "g2d_cache_append": (ctypes.c_int, [ctypes.POINTER(CacheDesc), _vp, _i64, _i64, _vp, _i64, _i64, _vp]),
-    "g2d_cache_read": (ctypes.c_int, [ctypes.POINTER(CacheDesc), _vp, _vp, _vp]),
-    "g2d_linear_workspace_bytes": (ctypes.c_int, [ctypes.POINTER(LinearDesc), ctypes.POINTER(ctypes.c_size_t)]),
-    "g2d_packed_linear": (ctypes.c_int, [ctypes.POINTER(LinearDesc), _vp]),
-    "g2d_attend_workspace_bytes": (ctypes.c_int, [ctypes.POINTER(AttendDesc), ctypes.POINTER(ctypes.c_size_t)]),
-    "g2d_cache_attend": (ctypes.c_int, [ctypes.POINTER(AttendDesc), _vp]),
+    "g2d_cache_append": (ctypes.c_int, [ctypes.c_char_p, _vp, _i64, _i64, _vp, _i64, _i64, _vp]),
+    "g2d_cache_read": (ctypes.c_int, [ctypes.c_char_p, _vp, _vp, _vp]),
+    "g2d_linear_workspace_bytes": (ctypes.c_int, [ctypes.c_char_p, ctypes.POINTER(ctypes.c_size_t)]),
+    "g2d_packed_linear": (ctypes.c_int, [ctypes.c_char_p, _vp]),
+    "g2d_attend_workspace_bytes": (ctypes.c_int, [ctypes.c_char_p, ctypes.POINTER(ctypes.c_size_t)]),
+    "g2d_cache_attend": (ctypes.c_int, [ctypes.c_char_p, _vp]),
 })
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
@@ -211,6 +202,19 @@ def ptr(t: torch.Tensor | None):
 
 def stream_of(t: torch.Tensor):
     return torch.cuda.current_stream(t.device).cuda_stream
+
+
+_NO_CONTEXT = contextlib.nullcontext()
+
+
+def on_device(index: int):
+    """``torch.cuda.device(index)`` where another device is the current one."""
+    return _NO_CONTEXT if torch.cuda.current_device() == index else torch.cuda.device(index)
+
+
+def raw_stream(index: int) -> int:
+    """The handle of torch's current stream of the device."""
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 _STATUS_WORDS: dict[int, torch.Tensor] = {}
