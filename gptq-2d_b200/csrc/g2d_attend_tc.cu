@@ -4,10 +4,11 @@
 // of all items, one after the other, are dealt out evenly to the CTAs, whatever the lengths; an item that lies in one CTA's share is written at once, the others
 // leave partial results (two per CTA at most) that attend_tiles_join_kernel adds up in the order of the keys.
 //
-// A CTA: four warps turn codes into operands: K as code - 8 in the type of the queries, exactly, keys as rows; V as code - 8 in fp16, channels as rows (two keys' words interleaved
-// by a byte permutation).  One thread issues the products S = Q K^T and O += P V, S in tensor memory (128 columns a tile), P as fp16 over S, O beside them.  Eight warps, a row per
-// thread, read S, multiply it by the keys' scales, take maximum and exponentials, and write P = exponential times the value's scale, rounded once to fp16 under the power of two of the largest
-// scale so far.  While one tile's rows are at their exponentials the other's products run.
+// A CTA: four warps turn codes of keys into an operand, code - 8 in the type of the queries, exactly, keys as rows; four others codes of values, code - 8 in fp16, channels as
+// rows (two keys' words interleaved by a byte permutation).  One thread issues the products S = Q K^T and O += P V, S in tensor memory (128 columns a tile), P as fp16 over
+// S, O beside them.  Sixteen warps, two threads per row with 64 keys each, read S, multiply it by the keys' scales, take maximum and exponentials, and write P = exponential
+// times the value's scale, rounded once to fp16 under the power of two of the largest scale so far.  Four such warps per scheduler keep the exponentials' unit busy (with eight warps, a
+// thread per row, a block took 7200 cycles, half of them waits).
 //
 // The maximum that the exponentials refer to moves only when a row's scores exceed it by 2^8 (or the scales' power of two grows): then O is read and scaled in tensor memory.
 //
@@ -16,7 +17,7 @@
 
 namespace g2d {
 
-constexpr int TA_THREADS = 512, TA_SCALES = 4;
+constexpr int TA_THREADS = 896, TA_SCALES = 4, TA_ROW_WARPS = 16;
 constexpr int TA_PANEL = 128 * 128;  // bytes of 128 rows of 64 16-bit values
 constexpr float TA_SLACK = 8.f;      // how far scores may exceed the maximum that the exponentials refer to, as a power of two
 constexpr int TA_UNIT = 6;           // the largest scale is brought to 2^6 .. 2^7: times 2^8, still a number of fp16
@@ -34,11 +35,12 @@ struct TileRun {
     int b, pair, head, first, n, blocks;  // n 0: there are no more
 };
 struct TileBarriers {
-    uint64_t run_full[TA_RUNS], run_empty[TA_RUNS], q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], scale_full[TA_SCALES], s_full[2], p_full[2], o_full[2], drained;
+    uint64_t run_full[TA_RUNS], run_empty[TA_RUNS], q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], scale_full[TA_SCALES], s_full[2], p_full[2], o_full[2], tops_full, halves[2], drained;
     unsigned present[TA_SCALES][4];  // which keys of a block there are
     int unit[TA_SCALES];             // exponent bits of the largest scale so far
-    int tops[4];
+    int tops[2][4];                  // [block's parity][warp]
     TileRun runs[TA_RUNS];
+    float tops2[2][2][2][128];       // [block's parity][tile][half of the keys][row]: the halves' maxima, and at the end their sums
     unsigned totals[TA_THREADS / 32];
     uint32_t tmem;
     int failed;
@@ -66,11 +68,6 @@ __device__ __forceinline__ void tmem_store_16(uint32_t at, const uint32_t (&v)[1
                  "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
                  : "memory");
 }
-__device__ __forceinline__ ulonglong2 load_4p(uint32_t at) {
-    ulonglong2 v;
-    asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(v.x), "=l"(v.y) : "r"(at));
-    return v;
-}
 __device__ __forceinline__ uint32_t halves_add(uint32_t u, uint32_t v, bool bf16) {
     uint32_t r;
     if (bf16) asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(u), "r"(v));
@@ -85,6 +82,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const Atten
     __shared__ __align__(8) TileBarriers bar;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t base = (smem_u32(tiles_smem) + 1023u) & ~1023u;
+    unsigned char *const at_base = tiles_smem + (base - smem_u32(tiles_smem));
     const CacheView &c = a.c;
     const auto wait = [&](uint64_t *b, uint32_t parity, unsigned nap) {
         if (mbar_wait(b, parity, nap, a.wait_cycles)) return true;
@@ -94,19 +92,21 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const Atten
     if (threadIdx.x == 0) {
         for (int s = 0; s < TA_RUNS; ++s) {
             mbar_init(&bar.run_full[s], 1);
-            mbar_init(&bar.run_empty[s], 1 + 4 + 8);  // the issuing thread, the coders' and the rows' warps
+            mbar_init(&bar.run_empty[s], 1 + 4 + 4 + TA_ROW_WARPS);  // the issuing thread, both teams of coders, the rows' warps
         }
         for (int s = 0; s < 2; ++s) {
-            mbar_init(&bar.q_full[s], 4);
+            mbar_init(&bar.q_full[s], TA_ROW_WARPS / 2);
             mbar_init(&bar.k_full[s], 4);
             mbar_init(&bar.k_empty[s], 1);
             mbar_init(&bar.v_full[s], 4);
             mbar_init(&bar.v_empty[s], 1);
             mbar_init(&bar.s_full[s], 1);
-            mbar_init(&bar.p_full[s], 4);
+            mbar_init(&bar.p_full[s], TA_ROW_WARPS / 2);
             mbar_init(&bar.o_full[s], 1);
+            mbar_init(&bar.halves[s], TA_ROW_WARPS / 2);
         }
         for (int s = 0; s < TA_SCALES; ++s) mbar_init(&bar.scale_full[s], 4);
+        mbar_init(&bar.tops_full, 4);
         mbar_init(&bar.drained, 1);
         bar.failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const Atten
     const auto second = [&](const TileRun &r) { return (int64_t)r.s.count * a.group - (int64_t)r.pair * TA_ROWS > 128; };  // whether the item has a second tile
 
     if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");  // 28 warps of 72 registers in all: 4 x 40 + 8 x 72 + 16 x 80
         if (warp == 0) {
             // ---- the share's runs ----
             TileCursor cur;
@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const Atten
             const auto results = [&](int tile, int stage, bool more) {
 #pragma unroll
                 for (int ks = 0; ks < TA_KEYS / 16; ++ks)
-                    mma_from_tmem(tmem + 2 * TA_KEYS + tile * D, tmem + tile * TA_KEYS + ks * 8, v0 + (uint64_t)(stage * (M::V_STAGE >> 4) + (ks >> 2) * (D * 128 >> 4) + (ks & 3) * 2), O_DESC, more || ks > 0);
+                    mma_from_tmem(tmem + 2 * TA_KEYS + tile * D, tmem + tile * TA_KEYS + (ks >> 2) * 64 + (ks & 3) * 8, v0 + (uint64_t)(stage * (M::V_STAGE >> 4) + (ks >> 2) * (D * 128 >> 4) + (ks & 3) * 2), O_DESC, more || ks > 0);
             };
             const auto after = [] { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); };
             bool go = true;
@@ -227,22 +227,14 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const Atten
             }
         }
         __syncwarp();
-    } else if (warp < 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 120;");
-        // ---- operands ----
+    } else if (warp < 12) {
+        // ---- operands: four warps for the keys and all scales, four for the values ----
         constexpr int WORDS = D / 8, VW = D / 64;  // words of a key; of a thread's keys in V
         constexpr uint32_t MAGIC = BF16 ? 0x43004300u : 0x64006400u, LESS = BF16 ? 0xc308c308u : 0xe408e408u;
-        const int key = threadIdx.x - 128;                                             // of K and the scales
-        const int octet = (lane & 7) + 8 * ((warp - 4) & 1), word = ((lane >> 3) + 4 * ((warp - 4) >> 1)) * VW;  // of V: eight keys, VW words
-        int unit = 0;
-        uint32_t blocks_done = 0;
+        uint32_t blocks_done = 0, number = 0;
         bool go = true;
-        uint4 kr[WORDS / 4];
-        uint32_t vr[8][VW];
-        float ks = 0.f, vs = 0.f;
-        bool here = false;
         // the block that is on its way: number ahead_j of the run of number ahead
-        uint32_t ahead = 0, number = 0;
+        uint32_t ahead = 0;
         int ahead_n = 0, ahead_j = 0, ahead_keys = 0, ahead_first = 0, ahead_b = 0, ahead_head = 0;
         const auto open_ahead = [&] {
             const TileRun &r = run_of(ahead, go);
@@ -253,30 +245,9 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const Atten
             ahead_head = r.head;
             ahead_j = 0;
         };
-        const auto row_of = [&](int at) {  // row of the cache of a key of the block on its way, or -1
+        const auto row_of = [&](int at) -> int64_t {  // row of the cache of a key of the block on its way, or -1
             const int position = (ahead_first + ahead_j) * TA_KEYS + at;
-            return position < ahead_keys ? cache_row(c, ahead_b, position, ahead_head) : -1;
-        };
-        const auto fetch_k = [&] {
-            const int64_t row = ahead_n > 0 ? row_of(key) : -1;
-            here = row >= 0;
-#pragma unroll
-            for (int w = 0; w < WORDS / 4; ++w) kr[w] = here ? __ldg(reinterpret_cast<const uint4 *>(c.k_codes + row * (D / 2)) + w) : make_uint4(0u, 0u, 0u, 0u);
-            ks = here ? __half2float(c.k_scale[row]) : 0.f;
-            vs = here ? __half2float(c.v_scale[row]) : 0.f;
-        };
-        const auto fetch_v = [&] {
-            const int64_t row = ahead_n > 0 ? row_of(octet * 8) : -1;  // eight keys of one page: those past the last key lie in it, too, and count for nothing
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                if constexpr (VW == 2) {
-                    const uint2 v = row >= 0 ? __ldg(reinterpret_cast<const uint2 *>(c.v_codes + (row + k) * (D / 2) + word * 4)) : make_uint2(0u, 0u);
-                    vr[k][0] = v.x;
-                    vr[k][1] = v.y;
-                } else {
-                    vr[k][0] = row >= 0 ? __ldg(reinterpret_cast<const uint32_t *>(c.v_codes + (row + k) * (D / 2) + word * 4)) : 0u;
-                }
-            }
+            return ahead_n > 0 && position < ahead_keys ? cache_row(c, ahead_b, position, ahead_head) : -1;
         };
         const auto step_ahead = [&] {
             if (ahead_n == 0 || ++ahead_j < ahead_n) return;
@@ -284,94 +255,149 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const Atten
             open_ahead();
         };
         open_ahead();
-        fetch_k();
-        fetch_v();
-        for (;; ++number) {
-            const int n = run_of(number, go).n;
-            if (!__all_sync(0xffffffffu, go) || n == 0) break;
-            unit = 0;
-            for (int j = 0; j < n; ++j, ++blocks_done) {
-                const int stage = blocks_done & 1, slot = blocks_done % TA_SCALES;
-                // ---- K, and the scales of the block ----
-                if (blocks_done >= 2) go = wait(&bar.k_empty[stage], ((blocks_done >> 1) - 1) & 1, 20);
-                go = __all_sync(0xffffffffu, go && !bar.failed);
-                if (!go) break;
-                const uint32_t kt = base + M::K + stage * M::K_STAGE + key * 128;
+        if (warp < 8) {
+            const int key = threadIdx.x - 128;
+            int unit = 0;
+            uint4 kr[WORDS / 4];
+            float ks = 0.f, vs = 0.f;
+            bool here = false;
+            const auto fetch = [&] {
+                const int64_t row = row_of(key);
+                here = row >= 0;
 #pragma unroll
-                for (int w = 0; w < WORDS; ++w) {
-                    const uint4 &r = kr[w >> 2];
-                    const uint32_t x = (w & 3) == 0 ? r.x : (w & 3) == 1 ? r.y : (w & 3) == 2 ? r.z : r.w, x4 = x >> 4;
-                    store_16s(kt + (w >> 3) * TA_PANEL + (((w & 7) ^ (key & 7)) << 4), halves_add((__byte_perm(x, x4, 0x4400) & 0x000f000fu) | MAGIC, LESS, BF16),
-                              halves_add((__byte_perm(x, x4, 0x5511) & 0x000f000fu) | MAGIC, LESS, BF16), halves_add((__byte_perm(x, x4, 0x6622) & 0x000f000fu) | MAGIC, LESS, BF16),
-                              halves_add((__byte_perm(x, x4, 0x7733) & 0x000f000fu) | MAGIC, LESS, BF16));
-                }
-                // the largest scale so far (one that is not finite sets no unit), and the values' scales in its power of two
-                const unsigned size = __float_as_uint(vs) & 0x7fffffffu;
-                const unsigned top = __reduce_max_sync(0xffffffffu, size < 0x7f800000u ? size : 0u), got = __ballot_sync(0xffffffffu, here);
-                if (lane == 0) bar.tops[warp - 4] = (int)(top >> 23);
-                asm volatile("bar.sync 1, 128;" ::: "memory");
-                unit = max(max(unit, max(bar.tops[0], bar.tops[1])), max(bar.tops[2], bar.tops[3]));
-                const uint32_t sc = base + M::SCALES + slot * M::SCALE_STAGE + key * 4;
-                asm volatile("st.shared.f32 [%0], %1;" ::"r"(sc), "f"(ks * (MODS ? a.scale : a.scale * LOG2E)) : "memory");
-                asm volatile("st.shared.f32 [%0], %1;" ::"r"(sc + TA_KEYS * 4), "f"(vs * power_of_two(min(TA_UNIT - (unit - 127), 127))) : "memory");
-                if (lane == 0) bar.present[slot][warp - 4] = got;
-                if (threadIdx.x == 128) bar.unit[slot] = unit;
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                asm volatile("bar.sync 1, 128;" ::: "memory");  // the tops are read before the next block's are written
-                if (lane == 0) {
-                    mbar_arrive(&bar.scale_full[slot]);
-                    mbar_arrive(&bar.k_full[stage]);
-                }
-                step_ahead();
-                fetch_k();
-                // ---- V, transposed ----
-                if (blocks_done >= 2) go = wait(&bar.v_empty[stage], ((blocks_done >> 1) - 1) & 1, 20);
-                go = __all_sync(0xffffffffu, go && !bar.failed);
-                if (!go) break;
-                const uint32_t vt = base + M::V + stage * M::V_STAGE + (octet >> 3) * (D * 128);
+                for (int w = 0; w < WORDS / 4; ++w) kr[w] = here ? __ldg(reinterpret_cast<const uint4 *>(c.k_codes + row * (D / 2)) + w) : make_uint4(0u, 0u, 0u, 0u);
+                ks = here ? __half2float(c.k_scale[row]) : 0.f;
+                vs = here ? __half2float(c.v_scale[row]) : 0.f;
+            };
+            fetch();
+            for (;; ++number) {
+                const int n = run_of(number, go).n;
+                if (!__all_sync(0xffffffffu, go) || n == 0) break;
+                unit = 0;
+                for (int j = 0; j < n; ++j, ++blocks_done) {
+                    const int stage = blocks_done & 1, slot = blocks_done % TA_SCALES;
+                    if (blocks_done >= 2) go = wait(&bar.k_empty[stage], ((blocks_done >> 1) - 1) & 1, 20);
+                    // the products of values of that block as well: its rows have let the scales go then
+                    if (blocks_done >= 2) go = go && wait(&bar.v_empty[stage], ((blocks_done >> 1) - 1) & 1, 20);
+                    go = __all_sync(0xffffffffu, go && !bar.failed);
+                    if (!go) break;
+                    const uint32_t kt = base + M::K + stage * M::K_STAGE + key * 128;
 #pragma unroll
-                for (int w = 0; w < VW; ++w) {
-                    uint32_t lo[4], hi[4];  // of two keys each: the lower and the upper four codes
-#pragma unroll
-                    for (int p = 0; p < 4; ++p) {
-                        lo[p] = __byte_perm(vr[2 * p][w], vr[2 * p + 1][w], 0x5410);
-                        hi[p] = __byte_perm(vr[2 * p][w], vr[2 * p + 1][w], 0x7632);
+                    for (int w = 0; w < WORDS; ++w) {
+                        const uint4 &r = kr[w >> 2];
+                        const uint32_t x = (w & 3) == 0 ? r.x : (w & 3) == 1 ? r.y : (w & 3) == 2 ? r.z : r.w, x4 = x >> 4;
+                        store_16s(kt + (w >> 3) * TA_PANEL + (((w & 7) ^ (key & 7)) << 4), halves_add((__byte_perm(x, x4, 0x4400) & 0x000f000fu) | MAGIC, LESS, BF16),
+                                  halves_add((__byte_perm(x, x4, 0x5511) & 0x000f000fu) | MAGIC, LESS, BF16), halves_add((__byte_perm(x, x4, 0x6622) & 0x000f000fu) | MAGIC, LESS, BF16),
+                                  halves_add((__byte_perm(x, x4, 0x7733) & 0x000f000fu) | MAGIC, LESS, BF16));
                     }
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const int d = (word + w) * 8 + e;
-                        uint32_t v[4];
-#pragma unroll
-                        for (int p = 0; p < 4; ++p) v[p] = halves_add((((e < 4 ? lo[p] : hi[p]) >> (4 * (e & 3))) & 0x000f000fu) | 0x64006400u, 0xe408e408u, false);
-                        store_16s(vt + d * 128 + (((octet & 7) ^ (d & 7)) << 4), v[0], v[1], v[2], v[3]);
+                    // the largest scale so far (one that is not finite sets no unit), and the values' scales in its power of two
+                    const unsigned size = __float_as_uint(vs) & 0x7fffffffu;
+                    const unsigned top = __reduce_max_sync(0xffffffffu, size < 0x7f800000u ? size : 0u), got = __ballot_sync(0xffffffffu, here);
+                    if (lane == 0) {
+                        bar.tops[stage][warp - 4] = (int)(top >> 23);
+                        mbar_arrive(&bar.tops_full);
                     }
+                    go = __all_sync(0xffffffffu, wait(&bar.tops_full, blocks_done & 1, 20));  // of all four warps
+                    if (!go) break;
+                    unit = max(max(unit, max(bar.tops[stage][0], bar.tops[stage][1])), max(bar.tops[stage][2], bar.tops[stage][3]));
+                    float *const sc = reinterpret_cast<float *>(at_base + M::SCALES + slot * M::SCALE_STAGE) + key;
+                    sc[0] = ks * (MODS ? a.scale : a.scale * LOG2E);
+                    sc[TA_KEYS] = vs * power_of_two(min(TA_UNIT - (unit - 127), 127));
+                    if (lane == 0) bar.present[slot][warp - 4] = got;
+                    if (threadIdx.x == 128) bar.unit[slot] = unit;
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive(&bar.scale_full[slot]);
+                        mbar_arrive(&bar.k_full[stage]);
+                    }
+                    step_ahead();
+                    fetch();
                 }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                // the run's entry is needed no more: the block on its way belongs to the next one
+                if (!go) break;
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&bar.v_full[stage]);
-                fetch_v();
+                if (lane == 0) let_go(number);
             }
-            // the run's entry is needed no more: the block on its way belongs to the next one
-            if (!go) break;
-            __syncwarp();
-            if (lane == 0) let_go(number);
+        } else {
+            const int octet = (lane & 7) + 8 * (warp & 1), word = ((lane >> 3) + 4 * ((warp - 8) >> 1)) * VW;  // eight keys, VW words of each
+            uint32_t vr[8][VW];
+            const auto fetch = [&] {
+                const int64_t row = row_of(octet * 8);  // eight keys of one page: those past the last key lie in it, too, and count for nothing
+                const uint8_t *const from = c.v_codes + row * (D / 2) + word * 4;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    if constexpr (VW == 2) {
+                        const uint2 v = row >= 0 ? __ldg(reinterpret_cast<const uint2 *>(from + k * (D / 2))) : make_uint2(0u, 0u);
+                        vr[k][0] = v.x;
+                        vr[k][1] = v.y;
+                    } else {
+                        vr[k][0] = row >= 0 ? __ldg(reinterpret_cast<const uint32_t *>(from + k * (D / 2))) : 0u;
+                    }
+                }
+            };
+            fetch();
+            for (;; ++number) {
+                const int n = run_of(number, go).n;
+                if (!__all_sync(0xffffffffu, go) || n == 0) break;
+                for (int j = 0; j < n; ++j, ++blocks_done) {
+                    const int stage = blocks_done & 1;
+                    if (blocks_done >= 2) go = wait(&bar.v_empty[stage], ((blocks_done >> 1) - 1) & 1, 20);
+                    go = __all_sync(0xffffffffu, go && !bar.failed);
+                    if (!go) break;
+                    const uint32_t vt = base + M::V + stage * M::V_STAGE + (octet >> 3) * (D * 128);
+#pragma unroll
+                    for (int w = 0; w < VW; ++w) {
+                        uint32_t lo[4], hi[4];  // of two keys each: the lower and the upper four codes
+#pragma unroll
+                        for (int p = 0; p < 4; ++p) {
+                            lo[p] = __byte_perm(vr[2 * p][w], vr[2 * p + 1][w], 0x5410);
+                            hi[p] = __byte_perm(vr[2 * p][w], vr[2 * p + 1][w], 0x7632);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const int d = (word + w) * 8 + e;
+                            uint32_t v[4];
+#pragma unroll
+                            for (int p = 0; p < 4; ++p) v[p] = halves_add((((e < 4 ? lo[p] : hi[p]) >> (4 * (e & 3))) & 0x000f000fu) | 0x64006400u, 0xe408e408u, false);
+                            store_16s(vt + d * 128 + (((octet & 7) ^ (d & 7)) << 4), v[0], v[1], v[2], v[3]);
+                        }
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&bar.v_full[stage]);
+                    step_ahead();
+                    fetch();
+                }
+                if (!go) break;
+                __syncwarp();
+                if (lane == 0) let_go(number);
+            }
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
-        // ---- rows ----
-        const int tile = (warp - 8) >> 2, q = warp & 3, local = tile * 128 + q * 32 + lane;
-        const uint32_t s_at = tmem + ((uint32_t)(q * 32) << 16) + tile * TA_KEYS, o_at = tmem + ((uint32_t)(q * 32) << 16) + 2 * TA_KEYS + tile * D;
-        uint32_t sc = 0, tc = 0, oc = 0;  // blocks of the CTA, blocks and items of this tile
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 80;");
+        // ---- rows: two threads each, with 64 keys of every block and half of the channels ----
+        const int tile = (warp - 12) >> 3, half = ((warp - 12) >> 2) & 1, q = warp & 3, row = q * 32 + lane, local = tile * 128 + row;
+        const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16), s_at = lanes + tile * TA_KEYS + half * 64, o_at = lanes + 2 * TA_KEYS + tile * D + half * (D / 2);
+        uint32_t hc = 0;
         bool go = true;
+        const auto both = [&] {  // the warps of a tile meet (by a barrier whose wait has its limit)
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar.halves[tile]);
+            if (go && !wait(&bar.halves[tile], hc & 1, 20)) go = false;
+            ++hc;
+        };
+        uint32_t sc = 0, tc = 0, oc = 0;  // blocks of the CTA, blocks and items of this tile
         for (uint32_t number = 0;; ++number) {
             const TileRun &run = run_of(number, go);
             if (!__all_sync(0xffffffffu, go) || run.n == 0) break;
-            const AttendSequence seq = run.s;
             const int n = run.n, first = run.first;
             const bool mine = tile == 0 || second(run), whole = first == 0 && n == run.blocks;
-            const int64_t r = (int64_t)run.pair * TA_ROWS + local, rows = (int64_t)seq.count * a.group;
-            const bool real = r < rows;
-            const int token = real ? (int)(r / a.group) : 0, h = run.head * a.group + (real ? (int)(r % a.group) : 0);
+            const int r = run.pair * TA_ROWS + local;
+            const bool real = r < run.s.count * a.group;
+            const int token = real ? r / a.group : 0, h = run.head * a.group + (real ? r % a.group : 0), limit = real ? visible_keys(a, run.s, token) : 0x7fffffff;
+            const int place = run.s.length - run.s.count + token;
+            const int64_t at_token = run.s.first + token;
             __syncwarp();
             if (lane == 0) let_go(number);
             if (!mine) {  // blocks that the other tile has alone
@@ -379,70 +405,72 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const Atten
                 continue;
             }
             {
-                const uint4 *const from = reinterpret_cast<const uint4 *>((const uint16_t *)a.q + (int64_t)(seq.first + token) * a.q_token_stride + (int64_t)h * a.q_head_stride);
-                const uint32_t to = base + M::Q + tile * M::Q_TILE + (q * 32 + lane) * 128;
+                const uint4 *const from = reinterpret_cast<const uint4 *>((const uint16_t *)a.q + at_token * a.q_token_stride + (int64_t)h * a.q_head_stride) + half * (D / 16);
+                const uint32_t to = base + M::Q + tile * M::Q_TILE + row * 128;
 #pragma unroll
-                for (int w = 0; w < D / 8; ++w) {
+                for (int w = 0; w < D / 16; ++w) {
                     const uint4 v = real ? __ldg(from + w) : make_uint4(0u, 0u, 0u, 0u);
-                    store_16s(to + (w >> 3) * TA_PANEL + (((w & 7) ^ (lane & 7)) << 4), v.x, v.y, v.z, v.w);
+                    const int chunk = half * (D / 16) + w;
+                    store_16s(to + (chunk >> 3) * TA_PANEL + (((chunk & 7) ^ (lane & 7)) << 4), v.x, v.y, v.z, v.w);
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bar.q_full[tile]);
             }
-            const int limit = real ? visible_keys(a, seq, token) : 0x7fffffff;
             const int least = __reduce_min_sync(0xffffffffu, limit);
             const float slope = MODS && a.slopes ? a.slopes[h] : 0.f;
-            const int place = seq.length - seq.count + token;
-            float m = -INFINITY, l = 0.f;
+            float m = -INFINITY;
+            uint64_t l = 0ull;
             int unit = 0;
             for (int j = 0; j < n; ++j, ++sc, ++tc) {
-                const int slot = sc % TA_SCALES, key0 = (first + j) * TA_KEYS;
+                const int slot = sc % TA_SCALES, key0 = (first + j) * TA_KEYS + half * 64;
                 // The scores first: they come behind the scales, and a tile that left out blocks must not meet an earlier phase of the scales' barrier.
                 go = go && !bar.failed && wait(&bar.s_full[tile], tc & 1, 20) && wait(&bar.scale_full[slot], (sc / TA_SCALES) & 1, 20);
-                go = __all_sync(0xffffffffu, go);
-                if (!go) break;
+                if (!__all_sync(0xffffffffu, go)) go = false;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t scales = base + M::SCALES + slot * M::SCALE_STAGE;
-                const bool masked = key0 + TA_KEYS > least || (bar.present[slot][0] & bar.present[slot][1] & bar.present[slot][2] & bar.present[slot][3]) != 0xffffffffu;
+                const ulonglong2 *const scales = reinterpret_cast<const ulonglong2 *>(at_base + M::SCALES + slot * M::SCALE_STAGE) + half * 16;
+                const bool masked = key0 + 64 > least || (bar.present[slot][2 * half] & bar.present[slot][2 * half + 1]) != 0xffffffffu;
                 // Two passes over S in tensor memory, so that a thread need not hold a row: the maximum, then the exponentials.  Where scores are masked, capped or biased the
                 // first pass writes them back.
                 const bool stored = MODS || masked;
                 float top = -INFINITY;
 #pragma unroll 1
-                for (int cb = 0; cb < 4; ++cb) {
+                for (int cb = 0; cb < 2; ++cb) {
                     uint32_t v[32];
                     tmem_load_32(s_at + cb * 32, v);
-                    float u[32];
 #pragma unroll
                     for (int x = 0; x < 32; x += 4) {
-                        const ulonglong2 k4 = load_4p(scales + (cb * 32 + x) * 4);
-                        unpack2(mul2(pack2(v[x], v[x + 1]), k4.x), u[x], u[x + 1]);
-                        unpack2(mul2(pack2(v[x + 2], v[x + 3]), k4.y), u[x + 2], u[x + 3]);
+                        const ulonglong2 k4 = scales[cb * 8 + x / 4];
+                        float u[4];
+                        unpack2(mul2(pack2(v[x], v[x + 1]), k4.x), u[0], u[1]);
+                        unpack2(mul2(pack2(v[x + 2], v[x + 3]), k4.y), u[2], u[3]);
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) v[x + y] = __float_as_uint(u[y]);
                     }
                     if (MODS) {
 #pragma unroll
                         for (int x = 0; x < 32; ++x) {
-                            float w = u[x];
+                            float w = __uint_as_float(v[x]);
                             if (a.softcap > 0.f) w = capped(w, a.softcap, 2.f * LOG2E / a.softcap);
-                            u[x] = fmaf(slope, (float)(key0 + cb * 32 + x - place), w) * LOG2E;
+                            v[x] = __float_as_uint(fmaf(slope, (float)(key0 + cb * 32 + x - place), w) * LOG2E);
                         }
                     }
                     if (stored) {
                         if (masked) {
-                            const unsigned there = bar.present[slot][cb];
+                            const unsigned there = bar.present[slot][2 * half + cb];
 #pragma unroll
                             for (int x = 0; x < 32; ++x)
-                                if (key0 + cb * 32 + x >= limit || !((there >> x) & 1u)) u[x] = -INFINITY;
+                                if (key0 + cb * 32 + x >= limit || !((there >> x) & 1u)) v[x] = 0xff800000u;
                         }
-#pragma unroll
-                        for (int x = 0; x < 32; ++x) v[x] = __float_as_uint(u[x]);
                         tmem_store_32(s_at + cb * 32, v);
                     }
 #pragma unroll
-                    for (int x = 0; x < 32; x += 2) top = fmaxf(fmaxf(top, u[x]), u[x + 1]);
+                    for (int x = 0; x < 32; x += 2) top = fmaxf(fmaxf(top, __uint_as_float(v[x])), __uint_as_float(v[x + 1]));
                 }
                 if (stored) tmem_stored();
+                bar.tops2[tc & 1][tile][half][row] = top;
+                both();
+                top = fmaxf(top, bar.tops2[tc & 1][tile][half ^ 1][row]);
                 // the maximum that the exponentials refer to, and the unit of the scales
                 const int new_unit = bar.unit[slot];
                 const bool first_seen = m == -INFINITY, moves = top > m + TA_SLACK || (first_seen && top > -INFINITY) || new_unit != unit;
@@ -450,12 +478,12 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const Atten
                     const float now = moves && top > m ? top : m;
                     const float keep = first_seen ? 1.f : ex2(m - now);
                     const float f = unit == 0 ? keep : keep * power_of_two(max(unit - new_unit, -126));
-                    l *= keep;
+                    l = mul2(l, pack2(keep, keep));
                     m = now;
                     unit = new_unit;
                     if (j > 0) {
 #pragma unroll 1
-                        for (int cb = 0; cb < D / 32; ++cb) {
+                        for (int cb = 0; cb < D / 64; ++cb) {
                             uint32_t v[32];
                             tmem_load_32(o_at + cb * 32, v);
 #pragma unroll
@@ -465,24 +493,25 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const Atten
                     }
                 }
                 const float refer = m == -INFINITY ? 0.f : m;
-                const uint64_t less = pack2(__float_as_uint(-refer), __float_as_uint(-refer));
-                uint64_t sum = 0ull;
+                const uint64_t less = pack2(-refer, -refer);
+                const auto exponentials = [&](auto is_stored, auto is_masked) {
+                    constexpr bool STORED = decltype(is_stored)::value, MASKED = decltype(is_masked)::value;
 #pragma unroll 1
-                for (int cb = 0; cb < 4; ++cb) {
+                for (int cb = 0; cb < 2; ++cb) {
                     uint32_t v[32], p[16];
                     tmem_load_32(s_at + cb * 32, v);
 #pragma unroll
                     for (int x = 0; x < 32; x += 4) {
-                        const ulonglong2 k4 = load_4p(scales + (cb * 32 + x) * 4), v4 = load_4p(scales + (TA_KEYS + cb * 32 + x) * 4);
+                        const ulonglong2 k4 = scales[cb * 8 + x / 4], v4 = scales[TA_KEYS / 4 + cb * 8 + x / 4];
 #pragma unroll
                         for (int y = 0; y < 2; ++y) {
                             const uint64_t score = pack2(v[x + 2 * y], v[x + 2 * y + 1]);
                             float e0, e1, w0, w1;
-                            unpack2(stored ? add2(score, less) : fma2(score, y ? k4.y : k4.x, less), e0, e1);
-                            const uint64_t e = pack2(__float_as_uint(ex2(e0)), __float_as_uint(ex2(e1)));
-                            sum = add2(sum, e);
+                            unpack2(STORED ? add2(score, less) : fma2(score, y ? k4.y : k4.x, less), e0, e1);
+                            const uint64_t e = pack2(ex2(e0), ex2(e1));
+                            l = add2(l, e);
                             unpack2(mul2(e, y ? v4.y : v4.x), w0, w1);
-                            if (masked) {  // a masked key counts for nothing, whatever its scale
+                            if constexpr (MASKED) {  // a masked key counts for nothing, whatever its scale
                                 if (v[x + 2 * y] == 0xff800000u) w0 = 0.f;
                                 if (v[x + 2 * y + 1] == 0xff800000u) w1 = 0.f;
                             }
@@ -491,9 +520,9 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const Atten
                     }
                     tmem_store_16(s_at + cb * 16, p);  // over scores that this thread has read
                 }
-                float sum0, sum1;
-                unpack2(sum, sum0, sum1);
-                l += sum0 + sum1;
+                };
+                if (masked) exponentials(std::true_type(), std::true_type());
+                else exponentials(std::bool_constant<MODS>(), std::false_type());
                 tmem_stored();
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
@@ -502,41 +531,45 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const Atten
             // ---- this CTA's part of the item ----
             if (go) go = wait(&bar.o_full[tile], oc & 1, 20);
             ++oc;
-            go = __all_sync(0xffffffffu, go);
+            if (!__all_sync(0xffffffffu, go)) go = false;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            float l0, l1;
+            unpack2(l, l0, l1);
+            l0 += l1;
+            bar.tops2[tc & 1][tile][half][row] = l0;  // the block before used the other places
+            both();
+            l0 = half ? bar.tops2[tc & 1][tile][0][row] + l0 : l0 + bar.tops2[tc & 1][tile][1][row];
+            both();  // read before the next item's maxima come
             float f = power_of_two(max((unit - 127) - TA_UNIT, -126));
-            if (whole) f = l == 0.f ? 0.f : __fdividef(f, l);
+            if (whole) f = l0 == 0.f ? 0.f : __fdividef(f, l0);
             if (!go) f = NAN;
-            const bool none = whole && l == 0.f && go;
+            const bool none = whole && l0 == 0.f && go;
             float *const slot = tile_slot<D>(a, 2 * share + (first == 0 ? 1 : 0));
 #pragma unroll 1
-            for (int cb = 0; cb < D / 32; ++cb) {
+            for (int cb = 0; cb < D / 64; ++cb) {
                 uint32_t v[32];
-                if (go) {
-                    tmem_load_32(o_at + cb * 32, v);
-                } else {
-#pragma unroll
-                    for (int x = 0; x < 32; ++x) v[x] = 0u;
-                }
+                tmem_load_32(o_at + cb * 32, v);
                 if (!real) continue;
-                float o[32];
 #pragma unroll
-                for (int x = 0; x < 32; ++x) o[x] = none ? 0.f : __uint_as_float(v[x]) * f;
+                for (int x = 0; x < 32; ++x) v[x] = __float_as_uint(none ? 0.f : __uint_as_float(v[x]) * f);
                 if (whole) {
-                    uint4 *const to = reinterpret_cast<uint4 *>((uint16_t *)a.out + ((int64_t)(seq.first + token) * a.heads + h) * D + cb * 32);
+                    uint4 *const to = reinterpret_cast<uint4 *>((uint16_t *)a.out + (at_token * a.heads + h) * D + half * (D / 2) + cb * 32);
 #pragma unroll
-                    for (int x = 0; x < 4; ++x)
-                        to[x] = make_uint4(pack_halves(o[8 * x], o[8 * x + 1], BF16), pack_halves(o[8 * x + 2], o[8 * x + 3], BF16), pack_halves(o[8 * x + 4], o[8 * x + 5], BF16),
-                                           pack_halves(o[8 * x + 6], o[8 * x + 7], BF16));
+                    for (int x = 0; x < 4; ++x) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) w[y] = pack_halves(__uint_as_float(v[8 * x + 2 * y]), __uint_as_float(v[8 * x + 2 * y + 1]), BF16);
+                        to[x] = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
                 } else {
-                    float4 *const to = reinterpret_cast<float4 *>(slot + local * D + cb * 32);
+                    uint4 *const to = reinterpret_cast<uint4 *>(slot + local * D + half * (D / 2) + cb * 32);
 #pragma unroll
-                    for (int x = 0; x < 8; ++x) to[x] = make_float4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
+                    for (int x = 0; x < 8; ++x) to[x] = make_uint4(v[4 * x], v[4 * x + 1], v[4 * x + 2], v[4 * x + 3]);
                 }
             }
-            if (real && !whole) {
+            if (real && !whole && half == 0) {
                 slot[TA_ROWS * D + local] = m;
-                slot[TA_ROWS * D + TA_ROWS + local] = l;
+                slot[TA_ROWS * D + TA_ROWS + local] = l0;
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         }
