@@ -35,12 +35,13 @@ struct TileRun {
     int b, pair, head, first, n, blocks;  // n 0: there are no more
 };
 struct TileBarriers {
-    uint64_t run_full[TA_RUNS], run_empty[TA_RUNS], q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], scale_full[TA_SCALES], s_full[2], p_full[2], o_full[2], tops_full, halves[2], drained;
+    uint64_t run_full[TA_RUNS], run_empty[TA_RUNS], q_full, q_empty, o_empty[2], k_full[2], k_empty[2], v_full[2], v_empty[2], scale_full[TA_SCALES], s_full[2], p_full[2], o_full[2], tops_full, halves[2], drained;
     unsigned present[TA_SCALES][4];  // which keys of a block there are
     int unit[TA_SCALES];             // exponent bits of the largest scale so far
     int tops[2][4];                  // [block's parity][warp]
     TileRun runs[TA_RUNS];
-    float tops2[2][2][2][128];       // [block's parity][tile][half of the keys][row]: the halves' maxima, and at the end their sums
+    float tops2[2][2][2][128];       // [block's parity][tile][half of the keys][row]: the halves' maxima
+    float sums2[2][2][2][128];       // [item's parity][tile][half][row]: and the sums of their exponentials
     unsigned totals[TA_THREADS / 32];
     uint32_t tmem;
     int failed;
@@ -92,10 +93,10 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const Atten
     if (threadIdx.x == 0) {
         for (int s = 0; s < TA_RUNS; ++s) {
             mbar_init(&bar.run_full[s], 1);
-            mbar_init(&bar.run_empty[s], 1 + 4 + 4 + TA_ROW_WARPS);  // the issuing thread, both teams of coders, the rows' warps
+            mbar_init(&bar.run_empty[s], 1 + 2 + 4 + 4 + TA_ROW_WARPS);  // the issuing thread, the warps that bring queries, both teams of coders, the rows' warps
         }
         for (int s = 0; s < 2; ++s) {
-            mbar_init(&bar.q_full[s], TA_ROW_WARPS / 2);
+            mbar_init(&bar.o_empty[s], TA_ROW_WARPS / 2);
             mbar_init(&bar.k_full[s], 4);
             mbar_init(&bar.k_empty[s], 1);
             mbar_init(&bar.v_full[s], 4);
@@ -106,6 +107,8 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const Atten
             mbar_init(&bar.halves[s], TA_ROW_WARPS / 2);
         }
         for (int s = 0; s < TA_SCALES; ++s) mbar_init(&bar.scale_full[s], 4);
+        mbar_init(&bar.q_full, 2);
+        mbar_init(&bar.q_empty, 1);
         mbar_init(&bar.tops_full, 4);
         mbar_init(&bar.drained, 1);
         bar.failed = 0;
@@ -124,14 +127,14 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const Atten
     const unsigned share = blockIdx.x;
     // the run of that number, for every thread of a role; its entry stays until all roles have let it go
     const auto run_of = [&](uint32_t number, bool &go) -> const TileRun & {
-        if (go) go = wait(&bar.run_full[number % TA_RUNS], (number / TA_RUNS) & 1, 20);
+        if (go) go = wait(&bar.run_full[number % TA_RUNS], (number / TA_RUNS) & 1, 0);
         return bar.runs[number % TA_RUNS];
     };
     const auto let_go = [&](uint32_t number) { mbar_arrive(&bar.run_empty[number % TA_RUNS]); };
     const auto second = [&](const TileRun &r) { return (int64_t)r.s.count * a.group - (int64_t)r.pair * TA_ROWS > 128; };  // whether the item has a second tile
 
     if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");  // 28 warps of 72 registers in all: 4 x 40 + 8 x 72 + 16 x 80
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");  // 28 warps of 72 registers in all: 4 x 56 + 8 x 64 + 16 x 80
         if (warp == 0) {
             // ---- the share's runs ----
             TileCursor cur;
@@ -155,6 +158,44 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const Atten
                     if (cur.u >= cur.end) break;
                     cur.next(a);
                 }
+            }
+        } else if (warp >= 2) {
+            // ---- queries: the next item's while the last block of the one before is at its exponentials ----
+            constexpr int CHUNKS = D / 8, BATCH = 8;  // of 16 bytes; loads under way
+            const int id = threadIdx.x - 64;
+            bool go = true;
+            for (uint32_t number = 0;; ++number) {
+                const TileRun &run = run_of(number, go);
+                if (!__all_sync(0xffffffffu, go) || run.n == 0) break;
+                const int row0 = run.pair * TA_ROWS, rows = run.s.count * a.group, local = second(run) ? TA_ROWS : TA_ROWS / 2;
+                const int64_t first = run.s.first;
+                const int head0 = run.head * a.group;
+                __syncwarp();
+                if (lane == 0) let_go(number);
+                if (number > 0) go = wait(&bar.q_empty, (number - 1) & 1, 32);
+                if (!__all_sync(0xffffffffu, go)) break;
+                const int chunk = id % CHUNKS;
+#pragma unroll 1
+                for (int i0 = id / CHUNKS; i0 < local; i0 += BATCH * 64 / CHUNKS) {
+                    uint4 v[BATCH];
+#pragma unroll
+                    for (int k = 0; k < BATCH; ++k) {
+                        const int r = row0 + i0 + k * (64 / CHUNKS);
+                        v[k] = make_uint4(0u, 0u, 0u, 0u);
+                        if (r < rows) {
+                            const unsigned token = (unsigned)r / (unsigned)a.group, h = (unsigned)r - token * a.group;
+                            v[k] = __ldg(reinterpret_cast<const uint4 *>((const uint16_t *)a.q + (first + token) * a.q_token_stride + (int64_t)(head0 + h) * a.q_head_stride) + chunk);
+                        }
+                    }
+#pragma unroll
+                    for (int k = 0; k < BATCH; ++k) {
+                        const int i = i0 + k * (64 / CHUNKS);
+                        if (i < local) store_16s(base + M::Q + (i >> 7) * M::Q_TILE + (chunk >> 3) * TA_PANEL + (i & 127) * 128 + (((chunk & 7) ^ (i & 7)) << 4), v[k].x, v[k].y, v[k].z, v[k].w);
+                    }
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bar.q_full);
             }
         } else if (warp == 1 && elected()) {
             // ---- products ----
@@ -182,20 +223,22 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const Atten
                 const int n = run.n;
                 const bool two = second(run);
                 let_go(items);
-                go = wait(&bar.q_full[0], items & 1, 20) && (!two || wait(&bar.q_full[1], pairs++ & 1, 20)) && wait(&bar.k_full[kc & 1], (kc >> 1) & 1, 20);
+                go = wait(&bar.q_full, items & 1, 0) && wait(&bar.k_full[kc & 1], (kc >> 1) & 1, 0);
                 if (!go) break;
                 after();
                 scores(0, kc & 1);
                 if (two) scores(1, kc & 1);
+                if (n == 1) umma_commit(&bar.q_empty);
                 umma_commit(&bar.k_empty[kc++ & 1]);
                 for (int j = 0; j < n; ++j, ++vc) {
                     const int vs = vc & 1, ks = kc & 1;
-                    go = !bar.failed && wait(&bar.v_full[vs], (vc >> 1) & 1, 20) && wait(&bar.p_full[0], pc0++ & 1, 20);
+                    go = !bar.failed && wait(&bar.v_full[vs], (vc >> 1) & 1, 0) && wait(&bar.p_full[0], pc0++ & 1, 0);
+                    if (j == 0 && items > 0) go = go && wait(&bar.o_empty[0], (items - 1) & 1, 0);  // the item before has been read
                     if (!go) break;
                     after();
                     results(0, vs, j > 0);
                     if (j + 1 < n) {
-                        go = wait(&bar.k_full[ks], (kc >> 1) & 1, 20);
+                        go = wait(&bar.k_full[ks], (kc >> 1) & 1, 0);
                         if (!go) break;
                         after();
                         scores(0, ks);  // over the P that the products before have read: they are carried out in order
@@ -203,7 +246,8 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const Atten
                         umma_commit(&bar.o_full[0]);
                     }
                     if (two) {
-                        go = wait(&bar.p_full[1], pc1++ & 1, 20);
+                        go = wait(&bar.p_full[1], pc1++ & 1, 0);
+                        if (j == 0 && pairs > 0) go = go && wait(&bar.o_empty[1], (pairs - 1) & 1, 0);
                         if (!go) break;
                         after();
                         results(1, vs, j > 0);
@@ -211,12 +255,14 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const Atten
                     umma_commit(&bar.v_empty[vs]);
                     if (j + 1 < n) {
                         if (two) scores(1, ks);
+                        if (j + 2 == n) umma_commit(&bar.q_empty);
                         umma_commit(&bar.k_empty[ks]);
                         ++kc;
                     } else if (two) {
                         umma_commit(&bar.o_full[1]);
                     }
                 }
+                if (two) ++pairs;
             }
             if (bar.failed) {  // what was issued completes, or has its time to, before what it reads and writes is given back
                 umma_commit(&bar.drained);
@@ -224,10 +270,12 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const Atten
             } else if (vc > 0) {
                 mbar_wait(&bar.v_empty[(vc - 1) & 1], ((vc - 1) >> 1) & 1);
                 mbar_wait(&bar.k_empty[(kc - 1) & 1], ((kc - 1) >> 1) & 1);
+                mbar_wait(&bar.q_empty, (items - 1) & 1);
             }
         }
         __syncwarp();
     } else if (warp < 12) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
         // ---- operands: four warps for the keys and all scales, four for the values ----
         constexpr int WORDS = D / 8, VW = D / 64;  // words of a key; of a thread's keys in V
         constexpr uint32_t MAGIC = BF16 ? 0x43004300u : 0x64006400u, LESS = BF16 ? 0xc308c308u : 0xe408e408u;
@@ -276,9 +324,9 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const Atten
                 unit = 0;
                 for (int j = 0; j < n; ++j, ++blocks_done) {
                     const int stage = blocks_done & 1, slot = blocks_done % TA_SCALES;
-                    if (blocks_done >= 2) go = wait(&bar.k_empty[stage], ((blocks_done >> 1) - 1) & 1, 20);
+                    if (blocks_done >= 2) go = wait(&bar.k_empty[stage], ((blocks_done >> 1) - 1) & 1, 0);
                     // the products of values of that block as well: its rows have let the scales go then
-                    if (blocks_done >= 2) go = go && wait(&bar.v_empty[stage], ((blocks_done >> 1) - 1) & 1, 20);
+                    if (blocks_done >= 2) go = go && wait(&bar.v_empty[stage], ((blocks_done >> 1) - 1) & 1, 0);
                     go = __all_sync(0xffffffffu, go && !bar.failed);
                     if (!go) break;
                     const uint32_t kt = base + M::K + stage * M::K_STAGE + key * 128;
@@ -297,7 +345,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const Atten
                         bar.tops[stage][warp - 4] = (int)(top >> 23);
                         mbar_arrive(&bar.tops_full);
                     }
-                    go = __all_sync(0xffffffffu, wait(&bar.tops_full, blocks_done & 1, 20));  // of all four warps
+                    go = __all_sync(0xffffffffu, wait(&bar.tops_full, blocks_done & 1, 0));  // of all four warps
                     if (!go) break;
                     unit = max(max(unit, max(bar.tops[stage][0], bar.tops[stage][1])), max(bar.tops[stage][2], bar.tops[stage][3]));
                     float *const sc = reinterpret_cast<float *>(at_base + M::SCALES + slot * M::SCALE_STAGE) + key;
@@ -342,7 +390,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const Atten
                 if (!__all_sync(0xffffffffu, go) || n == 0) break;
                 for (int j = 0; j < n; ++j, ++blocks_done) {
                     const int stage = blocks_done & 1;
-                    if (blocks_done >= 2) go = wait(&bar.v_empty[stage], ((blocks_done >> 1) - 1) & 1, 20);
+                    if (blocks_done >= 2) go = wait(&bar.v_empty[stage], ((blocks_done >> 1) - 1) & 1, 0);
                     go = __all_sync(0xffffffffu, go && !bar.failed);
                     if (!go) break;
                     const uint32_t vt = base + M::V + stage * M::V_STAGE + (octet >> 3) * (D * 128);
@@ -384,7 +432,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const Atten
         const auto both = [&] {  // the warps of a tile meet (by a barrier whose wait has its limit)
             __syncwarp();
             if (lane == 0) mbar_arrive(&bar.halves[tile]);
-            if (go && !wait(&bar.halves[tile], hc & 1, 20)) go = false;
+            if (go && !wait(&bar.halves[tile], hc & 1, 0)) go = false;
             ++hc;
         };
         uint32_t sc = 0, tc = 0, oc = 0;  // blocks of the CTA, blocks and items of this tile
@@ -404,19 +452,6 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const Atten
                 sc += n;
                 continue;
             }
-            {
-                const uint4 *const from = reinterpret_cast<const uint4 *>((const uint16_t *)a.q + at_token * a.q_token_stride + (int64_t)h * a.q_head_stride) + half * (D / 16);
-                const uint32_t to = base + M::Q + tile * M::Q_TILE + row * 128;
-#pragma unroll
-                for (int w = 0; w < D / 16; ++w) {
-                    const uint4 v = real ? __ldg(from + w) : make_uint4(0u, 0u, 0u, 0u);
-                    const int chunk = half * (D / 16) + w;
-                    store_16s(to + (chunk >> 3) * TA_PANEL + (((chunk & 7) ^ (lane & 7)) << 4), v.x, v.y, v.z, v.w);
-                }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&bar.q_full[tile]);
-            }
             const int least = __reduce_min_sync(0xffffffffu, limit);
             const float slope = MODS && a.slopes ? a.slopes[h] : 0.f;
             float m = -INFINITY;
@@ -425,7 +460,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const Atten
             for (int j = 0; j < n; ++j, ++sc, ++tc) {
                 const int slot = sc % TA_SCALES, key0 = (first + j) * TA_KEYS + half * 64;
                 // The scores first: they come behind the scales, and a tile that left out blocks must not meet an earlier phase of the scales' barrier.
-                go = go && !bar.failed && wait(&bar.s_full[tile], tc & 1, 20) && wait(&bar.scale_full[slot], (sc / TA_SCALES) & 1, 20);
+                go = go && !bar.failed && wait(&bar.s_full[tile], tc & 1, 0) && wait(&bar.scale_full[slot], (sc / TA_SCALES) & 1, 0);
                 if (!__all_sync(0xffffffffu, go)) go = false;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const ulonglong2 *const scales = reinterpret_cast<const ulonglong2 *>(at_base + M::SCALES + slot * M::SCALE_STAGE) + half * 16;
@@ -529,17 +564,16 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const Atten
                 if (lane == 0) mbar_arrive(&bar.p_full[tile]);
             }
             // ---- this CTA's part of the item ----
-            if (go) go = wait(&bar.o_full[tile], oc & 1, 20);
-            ++oc;
-            if (!__all_sync(0xffffffffu, go)) go = false;
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             float l0, l1;
             unpack2(l, l0, l1);
             l0 += l1;
-            bar.tops2[tc & 1][tile][half][row] = l0;  // the block before used the other places
+            bar.sums2[oc & 1][tile][half][row] = l0;
             both();
-            l0 = half ? bar.tops2[tc & 1][tile][0][row] + l0 : l0 + bar.tops2[tc & 1][tile][1][row];
-            both();  // read before the next item's maxima come
+            l0 = half ? bar.sums2[oc & 1][tile][0][row] + l0 : l0 + bar.sums2[oc & 1][tile][1][row];
+            if (go) go = wait(&bar.o_full[tile], oc & 1, 0);
+            ++oc;
+            if (!__all_sync(0xffffffffu, go)) go = false;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             float f = power_of_two(max((unit - 127) - TA_UNIT, -126));
             if (whole) f = l0 == 0.f ? 0.f : __fdividef(f, l0);
             if (!go) f = NAN;
@@ -572,6 +606,8 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const Atten
                 slot[TA_ROWS * D + TA_ROWS + local] = l0;
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar.o_empty[tile]);
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");

@@ -241,13 +241,13 @@ __global__ void __launch_bounds__(LinearShape<NT, DUO>::THREADS, 1) linear_tc_ke
             int slot = 0, slice = 0;
             uint32_t parity = 0;
             const auto ready = [&] {
-                if (!wait(&bar.full[slot], parity, 20)) return false;
+                if (!wait(&bar.full[slot], parity, 0)) return false;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 return true;
             };
             const auto open = [&] {
                 if (slice < ACC) return true;
-                if (!wait(&bar.acc_empty[slice % ACC], (slice / ACC - 1) & 1, 20)) return false;
+                if (!wait(&bar.acc_empty[slice % ACC], (slice / ACC - 1) & 1, 0)) return false;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 return true;
             };
@@ -304,7 +304,7 @@ __global__ void __launch_bounds__(LinearShape<NT, DUO>::THREADS, 1) linear_tc_ke
         uint32_t turns = 0, coded = 0;
         bool go = true;
         const auto free_slot = [&] {
-            if (turns > 0) go = go && wait(&bar.empty[slot], (turns - 1) & 1, 20);
+            if (turns > 0) go = go && wait(&bar.empty[slot], (turns - 1) & 1, 0);
             go = __all_sync(0xffffffffu, go && !bar.failed);
             ++turns;
             return go;
@@ -340,7 +340,7 @@ __global__ void __launch_bounds__(LinearShape<NT, DUO>::THREADS, 1) linear_tc_ke
                     shift0 = float_to_bits(by0 + 8.f, BF16) * 0x10001u;
                     shift1 = float_to_bits(by1 + 8.f, BF16) * 0x10001u;
                 }
-                if (!wait(&bar.code_full[slot], coded++ & 1, 20)) go = false;
+                if (!wait(&bar.code_full[slot], coded++ & 1, 0)) go = false;
                 // rows of 32 bytes under the TMA's 32-byte swizzle: the two halves change places in every second group of four rows
                 const uint32_t flip = ((row >> 2) & 1) << 4;
                 if (!free_slot()) break;  // for the whole warp
@@ -391,7 +391,7 @@ __global__ void __launch_bounds__(LinearShape<NT, DUO>::THREADS, 1) linear_tc_ke
 #pragma unroll
             for (int x = 0; x < MINE; ++x) total[x] = 0.f;
             const auto arrived = [&] {
-                const bool ok = go && wait(&bar.acc_full[slice % ACC], (slice / ACC) & 1, 20);
+                const bool ok = go && wait(&bar.acc_full[slice % ACC], (slice / ACC) & 1, 0);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 go = __all_sync(0xffffffffu, ok && !bar.failed);
                 return go;

@@ -35,12 +35,12 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t *bar, uint32_t parity) {
     return ok != 0;
 }
 // false on time-out.  Between polls the warp sleeps for `nap` nanoseconds: several CTAs of an update kernel share an SM, and the
-// warps that work should not lose issue slots to those that wait.
+// warps that work should not lose issue slots to those that wait.  0 for waits in the middle of a chain: a sleep ends late.
 __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, unsigned nap = 32, long long limit = WAIT_CYCLES) {
     const long long start = clock64();
     while (!mbar_try_wait(bar, parity)) {
         if (clock64() - start > limit) return false;
-        __nanosleep(nap);
+        if (nap) __nanosleep(nap);
     }
     return true;
 }
