@@ -20,6 +20,7 @@ namespace g2d {
 constexpr int TA_THREADS = 896, TA_SCALES = 4, TA_ROW_WARPS = 16;
 constexpr int TA_PANEL = 128 * 128;  // bytes of 128 rows of 64 16-bit values
 constexpr float TA_SLACK = 8.f;      // how far scores may exceed the maximum that the exponentials refer to, as a power of two
+constexpr long long TA_APART = 2000;  // cycles
 constexpr int TA_UNIT = 6;           // the largest scale is brought to 2^6 .. 2^7: times 2^8, still a number of fp16
 
 template <int D>
@@ -76,8 +77,20 @@ __device__ __forceinline__ uint32_t halves_add(uint32_t u, uint32_t v, bool bf16
     return r;
 }
 
+struct TileJob {
+    CUtensorMap q;  // [tokens][heads][head_dim] in boxes of 64 channels x a group's heads x 128 / group tokens: 128 rows of a tile
+    int by_tma;     // 0 where a group does not divide 128
+    AttendArgs a;
+};
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map, int x, int y, int z, uint64_t *bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                 ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+                 : "memory");
+}
+
 template <int D, bool BF16, bool MODS>
-__global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const AttendArgs a) {
+__global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const __grid_constant__ TileJob job) {
+    const AttendArgs &a = job.a;
     using M = TileShared<D>;
     extern __shared__ unsigned char tiles_smem[];
     __shared__ __align__(8) TileBarriers bar;
@@ -164,6 +177,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const Atten
             constexpr int CHUNKS = D / 8, BATCH = 8;  // of 16 bytes; loads under way
             const int id = threadIdx.x - 64;
             bool go = true;
+            uint32_t landed = 0;  // loads issued so far: the last has landed before this CTA ends
             for (uint32_t number = 0;; ++number) {
                 const TileRun &run = run_of(number, go);
                 if (!__all_sync(0xffffffffu, go) || run.n == 0) break;
@@ -174,6 +188,18 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const Atten
                 if (lane == 0) let_go(number);
                 if (number > 0) go = wait(&bar.q_empty, (number - 1) & 1, 32);
                 if (!__all_sync(0xffffffffu, go)) break;
+                if (job.by_tma) {  // rows past the sequence's last are another's, or zeros: their results go nowhere
+                    if (lane == 0 && warp == 2) {
+                        mbar_expect_tx(&bar.q_full, (uint32_t)(local * D * 2));
+                        for (int t = 0; t < local / 128; ++t)
+                            for (int p = 0; p < D / 64; ++p)
+                                tma_load_3d(base + M::Q + t * M::Q_TILE + p * TA_PANEL, &job.q, p * 64, head0, (int)(first + (row0 + t * 128) / a.group), &bar.q_full);
+                    } else if (lane == 0) {
+                        mbar_arrive(&bar.q_full);
+                    }
+                    landed = number + 1;
+                    continue;
+                }
                 const int chunk = id % CHUNKS;
 #pragma unroll 1
                 for (int i0 = id / CHUNKS; i0 < local; i0 += BATCH * 64 / CHUNKS) {
@@ -197,6 +223,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const Atten
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bar.q_full);
             }
+            if (landed > 0) mbar_wait(&bar.q_full, (landed - 1) & 1);
         } else if (warp == 1 && elected()) {
             // ---- products ----
             constexpr uint32_t S_DESC = idesc_16(TA_KEYS, BF16 ? 1 : 0), O_DESC = idesc_16(D, 0);
@@ -227,7 +254,11 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const Atten
                 if (!go) break;
                 after();
                 scores(0, kc & 1);
-                if (two) scores(1, kc & 1);
+                if (two) {
+                    // The tiles start half a block apart: one's exponentials then run beside the other's maxima and products
+                    for (const long long start = clock64(); clock64() - start < TA_APART;) __nanosleep(100);
+                    scores(1, kc & 1);
+                }
                 if (n == 1) umma_commit(&bar.q_empty);
                 umma_commit(&bar.k_empty[kc++ & 1]);
                 for (int j = 0; j < n; ++j, ++vc) {
@@ -623,7 +654,20 @@ static int launch_tiles(const AttendArgs &a, cudaStream_t st) {
     static PerDeviceOnce configured;
     constexpr size_t smem = TileShared<D>::BYTES;
     if (configured.run([&] { return cudaFuncSetAttribute(attend_tiles_kernel<D, BF16, MODS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) == cudaSuccess; }) != G2D_OK) return G2D_ERR_CUDA;
-    attend_tiles_kernel<D, BF16, MODS><<<TA_GRID, TA_THREADS, smem, st>>>(a);
+    TileJob job;
+    job.a = a;
+    job.by_tma = 0;
+    EncodeTiledFn fn = encode_tiled_fn();
+    if (!fn) return G2D_ERR_CUDA;
+    const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)a.heads, (cuuint64_t)a.c.tokens};
+    const cuuint64_t strides[2] = {(cuuint64_t)a.q_head_stride * 2, (cuuint64_t)a.q_token_stride * 2};
+    const cuuint32_t elem[3] = {1, 1, 1};
+    if (128 % a.group == 0 && a.q_head_stride > 0 && a.q_token_stride > 0) {
+        const cuuint32_t box[3] = {64, (cuuint32_t)a.group, (cuuint32_t)(128 / a.group)};
+        job.by_tma = fn(&job.q, BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void *>(a.q), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    }
+    attend_tiles_kernel<D, BF16, MODS><<<TA_GRID, TA_THREADS, smem, st>>>(job);
     return check_launch();
 }
 
