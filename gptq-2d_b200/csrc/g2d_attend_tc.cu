@@ -28,6 +28,10 @@ struct TileShared {
     static constexpr int Q = 0, Q_TILE = 128 * D * 2, K = 2 * Q_TILE, K_STAGE = 128 * D * 2, V = K + 2 * K_STAGE, V_STAGE = 128 * D * 2, SCALES = V + 2 * V_STAGE;
     static constexpr int SCALE_STAGE = 2 * TA_KEYS * 4;  // ks, vs as floats
     static constexpr size_t BYTES = SCALES + TA_SCALES * SCALE_STAGE + 1024;
+    // Columns of tensor memory.  At 64 channels P has its own, and the scores of the next block are formed as soon as those of this one have been read; at 128 it lies over
+    // them, and they have to wait for the products with the values.
+    static constexpr bool OWN_P = D == 64;
+    static constexpr uint32_t O_AT = 2 * TA_KEYS, P_AT = OWN_P ? O_AT + 2 * D : 0, P_TILE = OWN_P ? TA_KEYS / 2 : TA_KEYS, P_HALF = OWN_P ? TA_KEYS / 4 : TA_KEYS / 2;
 };
 // Blocks of an item in a CTA's share: written by one warp, read by the others' roles
 constexpr int TA_RUNS = 4;
@@ -36,7 +40,7 @@ struct TileRun {
     int b, pair, head, first, n, blocks;  // n 0: there are no more
 };
 struct TileBarriers {
-    uint64_t run_full[TA_RUNS], run_empty[TA_RUNS], q_full, q_empty, o_empty[2], k_full[2], k_empty[2], v_full[2], v_empty[2], scale_full[TA_SCALES], s_full[2], p_full[2], o_full[2], tops_full, halves[2], drained;
+    uint64_t run_full[TA_RUNS], run_empty[TA_RUNS], q_full, q_empty, o_empty[2], k_full[2], k_empty[2], v_full[2], v_empty[2], scale_full[TA_SCALES], s_full[2], s_free[2], p_full[2], o_full[2], tops_full, halves[2], drained;
     unsigned present[TA_SCALES][4];  // which keys of a block there are
     int unit[TA_SCALES];             // exponent bits of the largest scale so far
     int tops[2][4];                  // [block's parity][warp]
@@ -115,6 +119,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const __gri
             mbar_init(&bar.v_full[s], 4);
             mbar_init(&bar.v_empty[s], 1);
             mbar_init(&bar.s_full[s], 1);
+            mbar_init(&bar.s_free[s], TA_ROW_WARPS / 2);
             mbar_init(&bar.p_full[s], TA_ROW_WARPS / 2);
             mbar_init(&bar.o_full[s], 1);
             mbar_init(&bar.halves[s], TA_ROW_WARPS / 2);
@@ -228,7 +233,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const __gri
             // ---- products ----
             constexpr uint32_t S_DESC = idesc_16(TA_KEYS, BF16 ? 1 : 0), O_DESC = idesc_16(D, 0);
             const uint64_t q0 = umma_desc(base + M::Q), k0 = umma_desc(base + M::K), v0 = umma_desc(base + M::V);
-            uint32_t items = 0, pairs = 0, kc = 0, vc = 0, pc0 = 0, pc1 = 0;
+            uint32_t items = 0, pairs = 0, kc = 0, vc = 0, pc0 = 0, pc1 = 0, sc0 = 0, sc1 = 0;
             const auto scores = [&](int tile, int stage) {
 #pragma unroll
                 for (int ks = 0; ks < D / 16; ++ks) {
@@ -240,7 +245,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const __gri
             const auto results = [&](int tile, int stage, bool more) {
 #pragma unroll
                 for (int ks = 0; ks < TA_KEYS / 16; ++ks)
-                    mma_from_tmem(tmem + 2 * TA_KEYS + tile * D, tmem + tile * TA_KEYS + (ks >> 2) * 64 + (ks & 3) * 8, v0 + (uint64_t)(stage * (M::V_STAGE >> 4) + (ks >> 2) * (D * 128 >> 4) + (ks & 3) * 2), O_DESC, more || ks > 0);
+                    mma_from_tmem(tmem + M::O_AT + tile * D, tmem + M::P_AT + tile * M::P_TILE + (ks >> 2) * M::P_HALF + (ks & 3) * 8, v0 + (uint64_t)(stage * (M::V_STAGE >> 4) + (ks >> 2) * (D * 128 >> 4) + (ks & 3) * 2), O_DESC, more || ks > 0);
             };
             const auto after = [] { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); };
             bool go = true;
@@ -261,6 +266,48 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const __gri
                 }
                 if (n == 1) umma_commit(&bar.q_empty);
                 umma_commit(&bar.k_empty[kc++ & 1]);
+                if constexpr (M::OWN_P) {
+                    for (int j = 0; j < n; ++j, ++vc) {
+                        const int vs = vc & 1, ks = kc & 1;
+                        const bool more = j + 1 < n;
+                        if (more) {
+                            go = !bar.failed && wait(&bar.s_free[0], sc0 & 1, 0) && wait(&bar.k_full[ks], (kc >> 1) & 1, 0);
+                            if (!go) break;
+                            after();
+                            scores(0, ks);
+                        }
+                        ++sc0;
+                        go = !bar.failed && wait(&bar.v_full[vs], (vc >> 1) & 1, 0) && wait(&bar.p_full[0], pc0++ & 1, 0);
+                        if (j == 0 && items > 0) go = go && wait(&bar.o_empty[0], (items - 1) & 1, 0);  // the item before has been read
+                        if (!go) break;
+                        after();
+                        results(0, vs, j > 0);
+                        if (!more) umma_commit(&bar.o_full[0]);
+                        if (two) {
+                            if (more) {
+                                go = wait(&bar.s_free[1], sc1 & 1, 0);
+                                if (!go) break;
+                                after();
+                                scores(1, ks);
+                            }
+                            ++sc1;
+                        }
+                        if (more) {
+                            if (j + 2 == n) umma_commit(&bar.q_empty);
+                            umma_commit(&bar.k_empty[ks]);
+                            ++kc;
+                        }
+                        if (two) {
+                            go = wait(&bar.p_full[1], pc1++ & 1, 0);
+                            if (j == 0 && pairs > 0) go = go && wait(&bar.o_empty[1], (pairs - 1) & 1, 0);
+                            if (!go) break;
+                            after();
+                            results(1, vs, j > 0);
+                            if (!more) umma_commit(&bar.o_full[1]);
+                        }
+                        umma_commit(&bar.v_empty[vs]);
+                    }
+                } else {
                 for (int j = 0; j < n; ++j, ++vc) {
                     const int vs = vc & 1, ks = kc & 1;
                     go = !bar.failed && wait(&bar.v_full[vs], (vc >> 1) & 1, 0) && wait(&bar.p_full[0], pc0++ & 1, 0);
@@ -292,6 +339,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const __gri
                     } else if (two) {
                         umma_commit(&bar.o_full[1]);
                     }
+                }
                 }
                 if (two) ++pairs;
             }
@@ -457,7 +505,8 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const __gri
         asm volatile("setmaxnreg.inc.sync.aligned.u32 80;");
         // ---- rows: two threads each, with 64 keys of every block and half of the channels ----
         const int tile = (warp - 12) >> 3, half = ((warp - 12) >> 2) & 1, q = warp & 3, row = q * 32 + lane, local = tile * 128 + row;
-        const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16), s_at = lanes + tile * TA_KEYS + half * 64, o_at = lanes + 2 * TA_KEYS + tile * D + half * (D / 2);
+        const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16), s_at = lanes + tile * TA_KEYS + half * 64, o_at = lanes + M::O_AT + tile * D + half * (D / 2),
+                       p_at = lanes + M::P_AT + tile * M::P_TILE + half * M::P_HALF;
         uint32_t hc = 0;
         bool go = true;
         const auto both = [&] {  // the warps of a tile meet (by a barrier whose wait has its limit)
@@ -566,6 +615,11 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const __gri
                 for (int cb = 0; cb < 2; ++cb) {
                     uint32_t v[32], p[16];
                     tmem_load_32(s_at + cb * 32, v);
+                    if (M::OWN_P && cb == 1) {  // the scores have been read
+                        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&bar.s_free[tile]);
+                    }
 #pragma unroll
                     for (int x = 0; x < 32; x += 4) {
                         const ulonglong2 k4 = scales[cb * 8 + x / 4], v4 = scales[TA_KEYS / 4 + cb * 8 + x / 4];
@@ -584,7 +638,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const __gri
                             p[x / 2 + y] = pack_halves(w0, w1, 0);
                         }
                     }
-                    tmem_store_16(s_at + cb * 16, p);  // over scores that this thread has read
+                    tmem_store_16(p_at + cb * 16, p);  // 128 channels: over scores that this thread has read
                 }
                 };
                 if (masked) exponentials(std::true_type(), std::true_type());
