@@ -40,7 +40,7 @@ struct TileRun {
     int b, pair, head, first, n, blocks;  // n 0: there are no more
 };
 struct TileBarriers {
-    uint64_t run_full[TA_RUNS], run_empty[TA_RUNS], q_full, q_empty, o_empty[2], k_full[2], k_empty[2], v_full[2], v_empty[2], scale_full[TA_SCALES], s_full[2], s_free[2], p_full[2], o_full[2], tops_full, halves[2], drained;
+    uint64_t run_full[TA_RUNS], run_empty[TA_RUNS], q_full, q_empty, o_empty[2], k_full[2], k_empty[2], v_full[2], v_empty[2], scale_full[TA_SCALES], scale_empty[TA_SCALES], s_full[2], s_free[2], p_full[2], o_full[2], tops_full, halves[2][4], drained;
     unsigned present[TA_SCALES][4];  // which keys of a block there are
     int unit[TA_SCALES];             // exponent bits of the largest scale so far
     int tops[2][4];                  // [block's parity][warp]
@@ -122,9 +122,12 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const __gri
             mbar_init(&bar.s_free[s], TA_ROW_WARPS / 2);
             mbar_init(&bar.p_full[s], TA_ROW_WARPS / 2);
             mbar_init(&bar.o_full[s], 1);
-            mbar_init(&bar.halves[s], TA_ROW_WARPS / 2);
+            for (int q = 0; q < 4; ++q) mbar_init(&bar.halves[s][q], 2);
         }
-        for (int s = 0; s < TA_SCALES; ++s) mbar_init(&bar.scale_full[s], 4);
+        for (int s = 0; s < TA_SCALES; ++s) {
+            mbar_init(&bar.scale_full[s], 4);
+            mbar_init(&bar.scale_empty[s], TA_ROW_WARPS);
+        }
         mbar_init(&bar.q_full, 2);
         mbar_init(&bar.q_empty, 1);
         mbar_init(&bar.tops_full, 4);
@@ -404,8 +407,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const __gri
                 for (int j = 0; j < n; ++j, ++blocks_done) {
                     const int stage = blocks_done & 1, slot = blocks_done % TA_SCALES;
                     if (blocks_done >= 2) go = wait(&bar.k_empty[stage], ((blocks_done >> 1) - 1) & 1, 0);
-                    // the products of values of that block as well: its rows have let the scales go then
-                    if (blocks_done >= 2) go = go && wait(&bar.v_empty[stage], ((blocks_done >> 1) - 1) & 1, 0);
+                    if (blocks_done >= TA_SCALES) go = go && wait(&bar.scale_empty[slot], (blocks_done / TA_SCALES - 1) & 1, 0);
                     go = __all_sync(0xffffffffu, go && !bar.failed);
                     if (!go) break;
                     const uint32_t kt = base + M::K + stage * M::K_STAGE + key * 128;
@@ -509,10 +511,10 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const __gri
                        p_at = lanes + M::P_AT + tile * M::P_TILE + half * M::P_HALF;
         uint32_t hc = 0;
         bool go = true;
-        const auto both = [&] {  // the warps of a tile meet (by a barrier whose wait has its limit)
+        const auto both = [&] {  // the two warps of 32 rows meet (by a barrier whose wait has its limit)
             __syncwarp();
-            if (lane == 0) mbar_arrive(&bar.halves[tile]);
-            if (go && !wait(&bar.halves[tile], hc & 1, 0)) go = false;
+            if (lane == 0) mbar_arrive(&bar.halves[tile][q]);
+            if (go && !wait(&bar.halves[tile][q], hc & 1, 0)) go = false;
             ++hc;
         };
         uint32_t sc = 0, tc = 0, oc = 0;  // blocks of the CTA, blocks and items of this tile
@@ -529,7 +531,11 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const __gri
             __syncwarp();
             if (lane == 0) let_go(number);
             if (!mine) {  // blocks that the other tile has alone
-                sc += n;
+                for (int j = 0; j < n; ++j, ++sc) {
+                    go = go && !bar.failed && wait(&bar.scale_full[sc % TA_SCALES], (sc / TA_SCALES) & 1, 32);
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&bar.scale_empty[sc % TA_SCALES]);
+                }
                 continue;
             }
             const int least = __reduce_min_sync(0xffffffffu, limit);
@@ -539,7 +545,6 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const __gri
             int unit = 0;
             for (int j = 0; j < n; ++j, ++sc, ++tc) {
                 const int slot = sc % TA_SCALES, key0 = (first + j) * TA_KEYS + half * 64;
-                // The scores first: they come behind the scales, and a tile that left out blocks must not meet an earlier phase of the scales' barrier.
                 go = go && !bar.failed && wait(&bar.s_full[tile], tc & 1, 0) && wait(&bar.scale_full[slot], (sc / TA_SCALES) & 1, 0);
                 if (!__all_sync(0xffffffffu, go)) go = false;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -646,7 +651,10 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const __gri
                 tmem_stored();
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&bar.p_full[tile]);
+                if (lane == 0) {
+                    mbar_arrive(&bar.p_full[tile]);
+                    mbar_arrive(&bar.scale_empty[slot]);
+                }
             }
             // ---- this CTA's part of the item ----
             float l0, l1;
