@@ -72,30 +72,40 @@ __global__ void __launch_bounds__(ROWS_THREADS, 2) linear_rows_kernel(const Line
     for (int s = 0; s < AHEAD; ++s) fetch(s, w0 + s);
 
     // ---- x: a thread takes eight columns of a token; the CHUNKS threads of a block and token stand together and add up its sum ----
-    for (int e0 = 0; e0 < mine * TOKENS * CHUNKS; e0 += ROWS_THREADS) {
-        const int e = e0 + threadIdx.x, chunk = e % CHUNKS, token = e / CHUNKS % TOKENS, block = e / (CHUNKS * TOKENS);
-        const int64_t k = (b_first + block) * KB + 8 * chunk;
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (block < mine && k < a.n && token0 + token < a.tokens) v = __ldg(reinterpret_cast<const uint4 *>((const uint16_t *)a.x + (int64_t)(token0 + token) * a.x_stride + k));
-        float sum = 0.f;
-        uint32_t u[4] = {v.x, v.y, v.z, v.w};
+    constexpr int TOGETHER = 4;  // loads of a thread on their way at once
+    for (int e0 = threadIdx.x; e0 - (int)threadIdx.x < mine * TOKENS * CHUNKS; e0 += TOGETHER * ROWS_THREADS) {
+        uint4 v[TOGETHER];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            sum += bits_to_float(u[i] & 0xffffu, BF16) + bits_to_float(u[i] >> 16, BF16);
-            if (BF16) {
-                __nv_bfloat162 p = *reinterpret_cast<__nv_bfloat162 *>(&u[i]);
-                p = __hmul2(p, __float2bfloat162_rn(72057594037927936.f));  // 2^56
-                u[i] = *reinterpret_cast<uint32_t *>(&p);
-            }
+        for (int q = 0; q < TOGETHER; ++q) {
+            const int e = e0 + q * ROWS_THREADS, chunk = e % CHUNKS, token = token0 + e / CHUNKS % TOKENS, block = e / (CHUNKS * TOKENS);
+            const int64_t k = (b_first + block) * KB + 8 * chunk;
+            v[q] = make_uint4(0u, 0u, 0u, 0u);
+            if (block < mine && k < a.n && token < a.tokens) v[q] = __ldg(reinterpret_cast<const uint4 *>((const uint16_t *)a.x + (int64_t)token * a.x_stride + k));
         }
 #pragma unroll
-        for (int o = 1; o < CHUNKS; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (block < mine) {
-            // columns (0, 4), (2, 6), (1, 5), (3, 7): two codes of a word that lie sixteen bits apart
-            const uint4 f = make_uint4(__byte_perm(u[0], u[2], 0x5410), __byte_perm(u[1], u[3], 0x5410), __byte_perm(u[0], u[2], 0x7632), __byte_perm(u[1], u[3], 0x7632));
-            const int w = chunk % WORDS, lane_of = (token & 7) * 4 + chunk / WORDS;
-            xs[((block * WORDS + w) * NT + (token >> 3)) * 32 + lane_of] = f;
-            if (chunk == 0) sums[block * TOKENS + token] = sum;
+        for (int q = 0; q < TOGETHER; ++q) {
+            const int e = e0 + q * ROWS_THREADS, chunk = e % CHUNKS, token = e / CHUNKS % TOKENS, block = e / (CHUNKS * TOKENS);
+            if (e - (int)threadIdx.x >= mine * TOKENS * CHUNKS) break;
+            float sum = 0.f;
+            uint32_t u[4] = {v[q].x, v[q].y, v[q].z, v[q].w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                sum += bits_to_float(u[i] & 0xffffu, BF16) + bits_to_float(u[i] >> 16, BF16);
+                if (BF16) {
+                    __nv_bfloat162 p = *reinterpret_cast<__nv_bfloat162 *>(&u[i]);
+                    p = __hmul2(p, __float2bfloat162_rn(72057594037927936.f));  // 2^56
+                    u[i] = *reinterpret_cast<uint32_t *>(&p);
+                }
+            }
+#pragma unroll
+            for (int o = 1; o < CHUNKS; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (block < mine) {
+                // columns (0, 4), (2, 6), (1, 5), (3, 7): two codes of a word that lie sixteen bits apart
+                const uint4 f = make_uint4(__byte_perm(u[0], u[2], 0x5410), __byte_perm(u[1], u[3], 0x5410), __byte_perm(u[0], u[2], 0x7632), __byte_perm(u[1], u[3], 0x7632));
+                const int w = chunk % WORDS, lane_of = (token & 7) * 4 + chunk / WORDS;
+                xs[((block * WORDS + w) * NT + (token >> 3)) * 32 + lane_of] = f;
+                if (chunk == 0) sums[block * TOKENS + token] = sum;
+            }
         }
     }
     __syncthreads();
@@ -260,14 +270,14 @@ static LinearSpace linear_space(const g2d_linear_desc *d) {
     LinearSpace s{};
     size_t at = 0;
     const bool many = d->tokens > ROWS_TOKENS;
-    const LinearTcPlan p = many ? linear_tc_plan(d->m, d->n, d->tokens) : LinearTcPlan{};
+    const LinearTcPlan p = many ? linear_tc_plan(d->m, d->n, d->tokens, d->adapters > 0 ? (int)d->rank : 0) : LinearTcPlan{};
     if (d->rank > 0) {
         s.factor = at += whole((size_t)d->tokens * INNER_LD * 2);
         s.plan = at += whole((size_t)d->tokens * sizeof(float));
         if (many) at += whole((size_t)p.token_tiles * (p.tile + 1) * sizeof(int));
     }
     s.partial = at;
-    if (many && p.splits > 1) at += whole((size_t)p.splits * d->tokens * d->m * sizeof(float));
+    if (many) at += whole(p.partial_bytes);
     s.all = at;
     return s;
 }
@@ -330,7 +340,7 @@ extern "C" int g2d_packed_linear(const g2d_linear_desc *d, void *stream) {
     a.wait_cycles = WAIT_CYCLES;
     cudaStream_t st = (cudaStream_t)stream;
     const bool many = a.tokens > ROWS_TOKENS;
-    const LinearTcPlan p = many ? linear_tc_plan(a.m, a.n, a.tokens) : LinearTcPlan{};
+    const LinearTcPlan p = many ? linear_tc_plan(a.m, a.n, a.tokens, a.rank) : LinearTcPlan{};
     int *const plan = many && a.rank > 0 ? (int *)((char *)d->workspace + space.plan) : nullptr;
     if (a.rank > 0) {
         const int launched = launch_inner(a, plan, p.tile, st);

@@ -39,11 +39,14 @@ __device__ __forceinline__ int adapter_of(const LinearArgs &a, int token) {
 __device__ __forceinline__ float bits_to_float(uint32_t bits, int bf16) { return bf16 ? __uint_as_float(bits << 16) : __half2float(__ushort_as_half((unsigned short)bits)); }
 __device__ __forceinline__ uint32_t float_to_bits(float v, int bf16) { return bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v)); }
 
-// Many tokens: tiles of 128 rows (duo: 256, by two CTAs) x `tile` tokens, the columns in `splits` parts.
+// Many tokens: tiles of 128 rows (duo: 256, by two CTAs) x `tile` tokens, in chunks of 64 columns.  Whole rounds of whole tiles, then `shared` tiles on one line
+// of chunks, cut into `ctas` pieces; a tile has at most `pieces` of them.
 struct LinearTcPlan {
-    int tile, duo, row_tiles, token_tiles, splits;
+    int tile, duo, row_tiles, token_tiles, chunks, whole;
+    int64_t shared, line, ctas, pieces;
+    size_t partial_bytes;
 };
-LinearTcPlan linear_tc_plan(int64_t m, int64_t n, int64_t tokens);
+LinearTcPlan linear_tc_plan(int64_t m, int64_t n, int64_t tokens, int rank);
 
 // Inner values and factors of all tokens; where `plan` is given, also the adapters of each tile of `tile` tokens: plan[i * (tile + 1)] of them, their numbers behind it
 int launch_inner(const LinearArgs &a, int *plan, int tile, cudaStream_t st);

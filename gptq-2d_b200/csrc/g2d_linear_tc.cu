@@ -14,6 +14,7 @@
 
 namespace g2d {
 
+constexpr int LT_OUTER_LATER = 64, LT_JOIN_TOKENS = 4;  // tiles of so many tokens have their adapters' outer halves added where the pieces are joined
 constexpr int LT_W_BYTES = 128 * 128, LT_CODE_BYTES = 128 * 32, LT_SLICE = 8;
 
 // DUO: a pair of CTAs on 256 rows x NT tokens (cta_group::2), each with its rows of W and half of the tokens' rows of x.
@@ -37,25 +38,53 @@ struct LinearShape {
 struct LinearTcJob {
     CUtensorMap x, inner, codes, up;
     LinearArgs a;
-    int row_tiles, token_tiles, splits, chunks, group_chunks;
+    LinearTcPlan p;
+    int group_chunks;
     const int *plan;  // per tile of tokens: how many adapters, and which
-    float *partial;   // [splits][tokens][m], where splits > 1
+    float *partial;   // [piece][shared tile][token][row]
 };
 
+// A CTA's (DUO: a pair's) work.  `p.whole` rounds of whole tiles first; what tiles are left lie on one line, chunk after chunk, and are cut into `p.ctas` pieces of the same length.
 struct LinearItem {
-    int row0, token0, token_tile, split, c0, c1;
+    int row0, token0, token_tile, c0, c1;
+    int piece;   // which of its tile
+    int shared;  // number of the tile among those that are cut, -1: a whole one
 };
+// the CTA's part of the line, of fewer than 2^31 chunks (8 TB of codes): worked out once
+struct LinePart {
+    int first, last, tile, begins, piece;  // the tile in which the part begins, where that tile begins, and which of its pieces this is
+};
+__host__ __device__ __forceinline__ int64_t line_owner(const LinearTcPlan &p, int64_t at) { return ((at + 1) * p.ctas - 1) / p.line; }  // which CTA has a chunk
+__device__ __forceinline__ LinePart line_part(const LinearTcPlan &p, int64_t cta) {
+    LinePart part{};
+    if (p.shared == 0 || cta >= p.ctas) return part;
+    part.first = (int)(cta * p.line / p.ctas);
+    part.last = (int)((cta + 1) * p.line / p.ctas);
+    part.tile = part.first / p.chunks;
+    part.begins = part.tile * p.chunks;
+    part.piece = (int)(cta - line_owner(p, part.begins));
+    return part;
+}
 template <int NT, bool DUO>
-__device__ __forceinline__ bool linear_item(const LinearTcJob &job, int rank, int number, LinearItem &it) {
-    const int64_t at = (blockIdx.x + (int64_t)number * gridDim.x) / (DUO ? 2 : 1);
-    if (at >= (int64_t)job.row_tiles * job.token_tiles * job.splits) return false;
-    it.split = (int)(at % job.splits);
-    const int64_t tile = at / job.splits;
-    it.token_tile = (int)(tile / job.row_tiles);
-    it.row0 = (int)(tile % job.row_tiles) * (DUO ? 256 : 128) + rank * 128;
+__device__ __forceinline__ bool linear_item(const LinearTcPlan &p, const LinePart &part, int rank, int number, LinearItem &it) {
+    const int cta = (int)blockIdx.x / (DUO ? 2 : 1), ctas = (int)gridDim.x / (DUO ? 2 : 1);
+    int tile = number * ctas + cta;
+    it.c0 = 0;
+    it.c1 = p.chunks;
+    it.piece = 0;
+    it.shared = -1;
+    if (number >= p.whole) {
+        const int along = number - p.whole, begins = part.begins + along * p.chunks;
+        if (max(begins, part.first) >= part.last) return false;
+        it.c0 = max(part.first - begins, 0);
+        it.c1 = min(p.chunks, part.last - begins);
+        it.piece = along == 0 ? part.piece : 0;
+        it.shared = part.tile + along;
+        tile = p.whole * ctas + it.shared;
+    }
+    it.token_tile = tile / p.row_tiles;
+    it.row0 = (tile - it.token_tile * p.row_tiles) * (DUO ? 256 : 128) + rank * 128;
     it.token0 = it.token_tile * NT;
-    it.c0 = (int)((int64_t)it.split * job.chunks / job.splits);
-    it.c1 = (int)((int64_t)(it.split + 1) * job.chunks / job.splits);
     return true;
 }
 // whether a slice ends with chunk ch
@@ -114,6 +143,7 @@ struct LinearBarriers {
     using S = LinearShape<NT, DUO>;
     // full: x has landed (or the rows of an adapter) and W is written, in both CTAs: the leader's; empty: the products have read the slot
     uint64_t full[S::SLOTS], empty[S::SLOTS], code_full[S::SLOTS], code_empty[S::SLOTS], acc_full[S::ACCUMULATORS], acc_empty[S::ACCUMULATORS], drained;
+    LinePart part;
     uint32_t tmem;
     int failed;
 };
@@ -144,6 +174,7 @@ __global__ void __launch_bounds__(LinearShape<NT, DUO>::THREADS, 1) linear_tc_ke
             mbar_init(&bar.acc_empty[s], CTAS * S::READERS);
         }
         mbar_init(&bar.drained, 1);
+        bar.part = line_part(job.p, blockIdx.x / CTAS);
         bar.failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -156,14 +187,15 @@ __global__ void __launch_bounds__(LinearShape<NT, DUO>::THREADS, 1) linear_tc_ke
     }
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = bar.tmem;
-    // how many adapters an item has to add: those of its tile, by the first split.  The launch before writes them.
+    let_the_next_launch_start();
+    // how many adapters an item has to add: those of its tile, by the first piece.  The launch before writes them.
     const auto adapters_in = [&](const LinearItem &it) {
-        if (a.rank == 0 || it.split != 0) return 0;
+        if (NT == LT_OUTER_LATER || a.rank == 0 || it.piece != 0) return 0;
         after_the_launch_before();
         return job.plan[(int64_t)it.token_tile * (NT + 1)];
     };
     const auto adapter_at = [&](const LinearItem &it, int j) { return job.plan[(int64_t)it.token_tile * (NT + 1) + 1 + j]; };
-    const auto item = [&](int number, LinearItem &it) { return linear_item<NT, DUO>(job, rank, number, it); };
+    const auto item = [&](int number, LinearItem &it) { return linear_item<NT, DUO>(job.p, bar.part, rank, number, it); };
     const int first_coder = 4, first_reader = 4 + S::CODERS;
 
     // Every role counts the turns of the slots over all items of the CTA: a chunk of columns is a turn, and an adapter two (its inner values' upper and lower parts).
@@ -323,12 +355,12 @@ __global__ void __launch_bounds__(LinearShape<NT, DUO>::THREADS, 1) linear_tc_ke
             bool exact = true;
             for (; ch < it.c1; ch += SLOTS) {
                 if (ch >= group_end) {  // another group
-                    const int group = min(ch, job.chunks - 1) / job.group_chunks;
+                    const int group = min(ch, job.p.chunks - 1) / job.group_chunks;
                     group_end = (group + 1) * job.group_chunks;
                     const float by0 = a.qmin - (group == next_group ? next0 : __ldg(zero0 + (int64_t)group * a.zero_group));
                     const float by1 = a.qmin - (group == next_group ? next1 : __ldg(zero1 + (int64_t)group * a.zero_group));
                     const int meets = (ch + (group_end - ch + SLOTS - 1) / SLOTS * SLOTS) / job.group_chunks;
-                    next_group = min(meets, (job.chunks - 1) / job.group_chunks);
+                    next_group = min(meets, (job.p.chunks - 1) / job.group_chunks);
                     next0 = __ldg(zero0 + (int64_t)next_group * a.zero_group);
                     next1 = __ldg(zero1 + (int64_t)next_group * a.zero_group);
                     // one addition where -1024 + qmin - zero is a number of the type (integers up to 2048; bf16: -128, 256), else two, the first exact
@@ -406,7 +438,7 @@ __global__ void __launch_bounds__(LinearShape<NT, DUO>::THREADS, 1) linear_tc_ke
                 ++slice;
             };
             const uint32_t from = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)t0;
-            const auto factor_of = [&](int ch) { return __ldg(scale + (int64_t)(min(ch, job.chunks - 1) / job.group_chunks) * a.scale_group); };
+            const auto factor_of = [&](int ch) { return __ldg(scale + (int64_t)(min(ch, job.p.chunks - 1) / job.group_chunks) * a.scale_group); };
             float factor = factor_of(it.c0);
             for (int ch = it.c0; go && ch < it.c1; ++ch) {
                 if (!slice_ends(job, ch, it.c1 - 1)) continue;
@@ -459,11 +491,12 @@ __global__ void __launch_bounds__(LinearShape<NT, DUO>::THREADS, 1) linear_tc_ke
             }
             if (row < a.m) {
                 const int count = min(MINE, a.tokens - it.token0 - t0);
-                if (job.splits > 1) {
-                    float *to = job.partial + ((int64_t)it.split * a.tokens + it.token0 + t0) * a.m + row;
+                if (it.shared >= 0) {
+                    constexpr int ROWS = DUO ? 256 : 128;
+                    float *to = job.partial + (((int64_t)it.piece * job.p.shared + it.shared) * NT + t0) * ROWS + rank * 128 + q * 32 + lane;
 #pragma unroll
                     for (int x = 0; x < MINE; ++x)
-                        if (x < count) to[x * a.m] = total[x];
+                        if (x < count) to[x * ROWS] = total[x];
                 } else {
                     uint16_t *to = (uint16_t *)a.out + (int64_t)(it.token0 + t0) * a.out_stride + row;
 #pragma unroll
@@ -486,13 +519,59 @@ __global__ void __launch_bounds__(LinearShape<NT, DUO>::THREADS, 1) linear_tc_ke
     if (threadIdx.x == 0 && bar.failed && a.status) atomicExch(a.status, -1);
 }
 
-// sums of the splits
-__global__ void __launch_bounds__(256) linear_join_kernel(const LinearArgs a, const float *__restrict__ partial, int splits) {
-    const int64_t count = (int64_t)a.tokens * a.m;
-    for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < count; e += (int64_t)gridDim.x * 256) {
-        float sum = partial[e];
-        for (int s = 1; s < splits; ++s) sum += partial[s * count + e];
-        ((uint16_t *)a.out)[e / a.m * a.out_stride + e % a.m] = (uint16_t)float_to_bits(sum, a.bf16);
+// The tiles that were cut: sums of their pieces, in their order, and (tiles of LT_OUTER_LATER tokens) the outer halves of the adapters.  A thread has a row and LT_JOIN_TOKENS tokens.
+__global__ void __launch_bounds__(128) linear_join_kernel(const LinearArgs a, const LinearTcPlan p, const float *__restrict__ partial, int grid_ctas) {
+    __shared__ float4 inner[LT_JOIN_TOKENS][RANK_MAX / 4];
+    const int rows = p.duo ? 256 : 128, parts = rows / 128;
+    const int64_t shared = blockIdx.x / parts, tile = (int64_t)p.whole * grid_ctas + shared;
+    const int in_tile = blockIdx.y * LT_JOIN_TOKENS;
+    const int64_t token0 = tile / p.row_tiles * p.tile + in_tile, row_in_tile = blockIdx.x % parts * 128 + threadIdx.x, row = tile % p.row_tiles * rows + row_in_tile;
+    const int pieces = (int)(line_owner(p, (shared + 1) * p.chunks - 1) - line_owner(p, shared * p.chunks)) + 1;
+    const bool outer = p.tile == LT_OUTER_LATER && a.rank > 0;
+    int id[LT_JOIN_TOKENS];
+#pragma unroll
+    for (int e = 0; e < LT_JOIN_TOKENS; ++e) id[e] = outer ? adapter_of(a, (int)token0 + e) : -1;
+    after_the_launch_before();
+    if (outer) {
+        for (int e = threadIdx.x; e < LT_JOIN_TOKENS * RANK_MAX; e += 128) {
+            const int64_t token = token0 + e / RANK_MAX;
+            const uint16_t *const h = a.inner + token * INNER_LD + e % RANK_MAX;
+            if (token < a.tokens) reinterpret_cast<float *>(inner)[e] = bits_to_float(h[0], a.bf16) + bits_to_float(h[RANK_MAX], a.bf16);
+        }
+        __syncthreads();
+    }
+    if (row >= a.m) return;
+    const int count = (int)min((int64_t)LT_JOIN_TOKENS, a.tokens - token0);
+    float sum[LT_JOIN_TOKENS];
+#pragma unroll
+    for (int e = 0; e < LT_JOIN_TOKENS; ++e) sum[e] = 0.f;
+    const float *from = partial + (shared * p.tile + in_tile) * rows + row_in_tile;
+#pragma unroll 2
+    for (int k = 0; k < pieces; ++k, from += p.shared * p.tile * rows) {
+#pragma unroll
+        for (int e = 0; e < LT_JOIN_TOKENS; ++e)
+            if (e < count) sum[e] += from[e * rows];
+    }
+#pragma unroll
+    for (int e = 0; e < LT_JOIN_TOKENS; ++e) {
+        if (e >= count) break;
+        if (id[e] >= 0) {
+            const uint4 *const up = reinterpret_cast<const uint4 *>((const uint16_t *)a.up + ((int64_t)id[e] * a.m + row) * a.rank);
+            float more = 0.f;
+            for (int r = 0; r < a.rank / 8; ++r) {
+                const uint4 v = __ldg(up + r);
+                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                const float4 h[2] = {inner[e][2 * r], inner[e][2 * r + 1]};
+                const float hh[8] = {h[0].x, h[0].y, h[0].z, h[0].w, h[1].x, h[1].y, h[1].z, h[1].w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    more = fmaf(bits_to_float(w[i] & 0xffffu, a.bf16), hh[2 * i], more);
+                    more = fmaf(bits_to_float(w[i] >> 16, a.bf16), hh[2 * i + 1], more);
+                }
+            }
+            sum[e] = fmaf(more, a.factor[token0 + e], sum[e]);
+        }
+        ((uint16_t *)a.out)[(token0 + e) * a.out_stride + row] = (uint16_t)float_to_bits(sum[e], a.bf16);
     }
 }
 
@@ -519,7 +598,7 @@ static bool make_map_up(CUtensorMap *map, const LinearArgs &a) {
               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-LinearTcPlan linear_tc_plan(int64_t m, int64_t n, int64_t tokens) {
+LinearTcPlan linear_tc_plan(int64_t m, int64_t n, int64_t tokens, int rank) {
     LinearTcPlan p;
     p.tile = tokens <= 64 ? 64 : 128;
     p.duo = 0;
@@ -534,10 +613,18 @@ LinearTcPlan linear_tc_plan(int64_t m, int64_t n, int64_t tokens) {
     }
     p.row_tiles = (int)rows;
     p.token_tiles = (int)columns;
-    const int64_t tiles = rows * columns, chunks = ceil_div(n, (int64_t)KH);
-    int64_t splits = (p.duo ? 74 : 148) / tiles;
-    if (splits > chunks / 8) splits = chunks / 8;
-    p.splits = splits < 1 ? 1 : (int)splits;
+    p.chunks = (int)ceil_div(n, (int64_t)KH);
+    const int64_t tiles = rows * columns, at_once = p.duo ? 74 : 148;
+    p.whole = p.tile == LT_OUTER_LATER && rank > 0 ? 0 : (int)(tiles / at_once);
+    p.shared = tiles - p.whole * at_once;
+    p.line = p.shared * p.chunks;
+    p.ctas = p.line / 8 < at_once ? (p.line / 8 > 0 ? p.line / 8 : 1) : at_once;  // pieces of eight chunks at least
+    p.pieces = 0;
+    if (p.shared > 0) {
+        p.pieces = ceil_div((int64_t)p.chunks - 1, p.line / p.ctas) + 1;
+        if (p.pieces > p.ctas) p.pieces = p.ctas;
+    }
+    p.partial_bytes = (size_t)p.pieces * p.shared * p.tile * (p.duo ? 256 : 128) * sizeof(float);
     return p;
 }
 
@@ -548,23 +635,17 @@ static int launch_tc(const LinearArgs &a, const LinearTcPlan &p, const int *plan
     if (configured.run([&] { return cudaFuncSetAttribute(linear_tc_kernel<BF16, NT, DUO>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM) == cudaSuccess; }) != G2D_OK) return G2D_ERR_CUDA;
     LinearTcJob job;
     job.a = a;
-    job.row_tiles = p.row_tiles;
-    job.token_tiles = p.token_tiles;
-    job.splits = p.splits;
-    job.chunks = (int)ceil_div(a.n, (int64_t)KH);
-    job.group_chunks = a.group >= a.n ? job.chunks : (int)(a.group / KH);
+    job.p = p;
+    job.group_chunks = a.group >= a.n ? p.chunks : (int)(a.group / KH);
     job.plan = plan;
     job.partial = partial;
     if (!make_map_16(&job.x, a.x, a.tokens, a.n, S::X_ROWS, BF16, a.x_stride) || !make_map_codes(&job.codes, a.codes, a.m, a.n / 2, a.row_bytes)) return G2D_ERR_CUDA;
     if (a.rank > 0 && (!make_map_16(&job.inner, a.inner, a.tokens, INNER_LD, S::X_ROWS, BF16) || !make_map_up(&job.up, a))) return G2D_ERR_CUDA;
     if (a.rank == 0) job.inner = job.up = job.x;
-    const int64_t items = (int64_t)p.row_tiles * p.token_tiles * p.splits;
-    const unsigned grid = DUO ? 2 * (unsigned)(items < 74 ? items : 74) : (unsigned)(items < 148 ? items : 148);
-    const int launched = launch_dependent(linear_tc_kernel<BF16, NT, DUO>, dim3(grid), S::THREADS, S::SMEM, DUO ? 2 : 1, a.rank > 0, st, job);
-    if (launched != G2D_OK || p.splits == 1) return launched;
-    const int64_t blocks = ceil_div((int64_t)a.tokens * a.m, (int64_t)256);
-    linear_join_kernel<<<(unsigned)(blocks < 148 * 8 ? blocks : 148 * 8), 256, 0, st>>>(a, partial, p.splits);
-    return check_launch();
+    const int64_t ctas = p.whole > 0 ? (DUO ? 74 : 148) : p.ctas;
+    const int launched = launch_dependent(linear_tc_kernel<BF16, NT, DUO>, dim3((unsigned)(DUO ? 2 * ctas : ctas)), S::THREADS, S::SMEM, DUO ? 2 : 1, a.rank > 0, st, job);
+    if (launched != G2D_OK || p.shared == 0) return launched;
+    return launch_dependent(linear_join_kernel, dim3((unsigned)p.shared * (DUO ? 2 : 1), NT / LT_JOIN_TOKENS), 128, 0, 1, true, st, a, p, partial, (int)ctas);
 }
 
 int launch_linear_tc(const LinearArgs &a, const LinearTcPlan &p, const int *plan, float *partial, cudaStream_t st) {
