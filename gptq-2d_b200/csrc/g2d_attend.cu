@@ -201,6 +201,7 @@ __global__ void __launch_bounds__(AttendShape<D, NT>::THREADS, 1) attend_rows_ke
         const int head = cur.item % c.kv_heads, row0 = cur.item / c.kv_heads * ROWS, rows = cur.s.count * a.group;
         const int first_block = cur.block, last_block = min(cur.blocks, cur.block + (cur.end - cur.u));
         const AttendSequence seq = cur.s;
+        const float cap = a.softcap * LOG2E;
         uint32_t qf[NT][KSTEPS][2];
         uint64_t factor[NT];
         float start[NT][2], slope[NT][2];
@@ -245,10 +246,10 @@ __global__ void __launch_bounds__(AttendShape<D, NT>::THREADS, 1) attend_rows_ke
             }
             sum += __shfl_xor_sync(0xffffffffu, sum, 1);
             sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            const float my_factor = fmaxf(16777216.f * fabsf(a.scale) * (MODS ? 1.f : LOG2E) * power_of_two(e2), 1e-38f),  // above zero: minus infinity stays what it is
+            const float my_factor = fmaxf(16777216.f * fabsf(a.scale) * score_unit<MODS>(a) * power_of_two(e2), 1e-38f),  // above zero: minus infinity stays what it is
                         my_start = -8.f / 16777216.f * sum;
             const int my_limit = real ? visible_keys(a, seq, token) : seq.keys;
-            const float my_slope = MODS && a.slopes ? a.slopes[h] : 0.f;
+            const float my_slope = MODS && a.slopes ? a.slopes[h] * LOG2E : 0.f;
             const int my_place = seq.length - seq.count + token;
             float two_factors[2];
 #pragma unroll
@@ -347,7 +348,15 @@ __global__ void __launch_bounds__(AttendShape<D, NT>::THREADS, 1) attend_rows_ke
             float top[NT][2];
 #pragma unroll
             for (int j = 0; j < NT; ++j) top[j][0] = top[j][1] = -INFINITY;
-            unsigned hidden[NT][2];
+            unsigned hidden[NT][2];  // MASKED: bit k: key 8 g + k is not for this row
+            float away[NT][2];       // MODS: the distance of key 8 g
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int x2 = 0; x2 < 2; ++x2) {
+                    if (MODS) away[j][x2] = (float)(key0 + 8 * g - place[j][x2]);
+                    if (MASKED) hidden[j][x2] = gone | (0xffu << min(max(limit[j][x2] - key0 - 8 * g, 0), 8));
+                }
 #pragma unroll
             for (int mt = 0; mt < 4; ++mt) {
                 const float2 ks = __half22float2(*reinterpret_cast<const __half2 *>(&kw[mt]));
@@ -358,22 +367,15 @@ __global__ void __launch_bounds__(AttendShape<D, NT>::THREADS, 1) attend_rows_ke
                     for (int j = 0; j < NT; ++j) {
                         float &u0 = s[mt][j][2 * half], &u1 = s[mt][j][2 * half + 1];
                         unpack2(mul2(pack2(u0, u1), k2), u0, u1);
-                        if constexpr (MODS) {
-                            float f0, f1;
-                            unpack2(factor[j], f0, f1);
-                            u0 *= f0;
-                            u1 *= f1;
-                            if (a.softcap > 0.f) u0 = capped(u0, a.softcap, 2.f * LOG2E / a.softcap), u1 = capped(u1, a.softcap, 2.f * LOG2E / a.softcap);
-                            const int key = key0 + 8 * g + 2 * mt + half;
-                            u0 = fmaf(slope[j][0], (float)(key - place[j][0]), u0) * LOG2E;
-                            u1 = fmaf(slope[j][1], (float)(key - place[j][1]), u1) * LOG2E;
+                        if constexpr (MODS) {  // in units of log2 from here on
+                            unpack2(mul2(pack2(u0, u1), factor[j]), u0, u1);
+                            if (a.softcap > 0.f) u0 = capped(u0, cap), u1 = capped(u1, cap);
+                            u0 = fmaf(slope[j][0], away[j][0] + (float)(2 * mt + half), u0);
+                            u1 = fmaf(slope[j][1], away[j][1] + (float)(2 * mt + half), u1);
                         }
                         if constexpr (MASKED) {
-                            const int key = key0 + 8 * g + 2 * mt + half;
-                            const bool not_there = (gone >> (2 * mt + half)) & 1u;
-                            if (mt == 0 && half == 0) hidden[j][0] = hidden[j][1] = 0u;
-                            if (not_there || key >= limit[j][0]) u0 = -INFINITY, hidden[j][0] |= 1u << (2 * mt + half);
-                            if (not_there || key >= limit[j][1]) u1 = -INFINITY, hidden[j][1] |= 1u << (2 * mt + half);
+                            if ((hidden[j][0] >> (2 * mt + half)) & 1u) u0 = -INFINITY;
+                            if ((hidden[j][1] >> (2 * mt + half)) & 1u) u1 = -INFINITY;
                         }
                         top[j][0] = fmaxf(top[j][0], u0);
                         top[j][1] = fmaxf(top[j][1], u1);
@@ -486,7 +488,7 @@ __global__ void __launch_bounds__(AttendShape<D, NT>::THREADS, 1) attend_rows_ke
             sound = __all_sync(0xffffffffu, sound);
             const int key0 = block * CACHE_BLOCK;
             const bool masked = key0 + CACHE_BLOCK > least || (here & 0x11111111u) != (0x11111111u >> (32 - 4 * pieces));
-            if (masked) take(std::true_type(), sh.stage[warp][stage], key0, here);
+            if (MODS || masked) take(std::true_type(), sh.stage[warp][stage], key0, here);
             else take(std::false_type(), sh.stage[warp][stage], key0, here);
             __syncwarp();  // all lanes have read the stage
             if (sound && ahead.u < ahead.end) {

@@ -43,13 +43,22 @@ __device__ __forceinline__ int visible_keys(const AttendArgs &a, const AttendSeq
 
 
 constexpr float LOG2E = 1.4426950408889634f;
+// What a score is taken times, so that its exponential is one to base 2: where it is capped, before that (a cap below 1e-20 is as good as none left)
+template <bool MODS>
+__device__ __forceinline__ float score_unit(const AttendArgs &a) {
+    return MODS && a.softcap > 0.f ? fminf(2.f * LOG2E / a.softcap, 1e20f) : LOG2E;
+}
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// cap tanh(u / cap) through one exponential: exact to 1e-7 of the cap, which is what a score's exponential sees
-__device__ __forceinline__ float capped(float u, float cap, float two_log2e_over_cap) { return cap - __fdividef(2.f * cap, 1.f + ex2(u * two_log2e_over_cap)); }
+// cap tanh(u / cap) through one exponential, from x = 2 log2(e) u / cap: exact to 1e-7 of the cap, which is what a score's exponential sees
+__device__ __forceinline__ float capped(float x, float cap) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + ex2(x)));
+    return fmaf(-2.f * cap, r, cap);
+}
 // pairs of floats: one instruction each
 __device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
     uint64_t r;

@@ -430,7 +430,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const __gri
                     if (!go) break;
                     unit = max(max(unit, max(bar.tops[stage][0], bar.tops[stage][1])), max(bar.tops[stage][2], bar.tops[stage][3]));
                     float *const sc = reinterpret_cast<float *>(at_base + M::SCALES + slot * M::SCALE_STAGE) + key;
-                    sc[0] = ks * (MODS ? a.scale : a.scale * LOG2E);
+                    sc[0] = ks * (a.scale * score_unit<MODS>(a));
                     sc[TA_KEYS] = vs * power_of_two(min(TA_UNIT - (unit - 127), 127));
                     if (lane == 0) bar.present[slot][warp - 4] = got;
                     if (threadIdx.x == 128) bar.unit[slot] = unit;
@@ -539,7 +539,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const __gri
                 continue;
             }
             const int least = __reduce_min_sync(0xffffffffu, limit);
-            const float slope = MODS && a.slopes ? a.slopes[h] : 0.f;
+            const float slope = MODS && a.slopes ? a.slopes[h] * LOG2E : 0.f, cap = a.softcap * LOG2E;
             float m = -INFINITY;
             uint64_t l = 0ull;
             int unit = 0;
@@ -568,19 +568,21 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const __gri
                         for (int y = 0; y < 4; ++y) v[x + y] = __float_as_uint(u[y]);
                     }
                     if (MODS) {
+                        const float away = (float)(key0 + cb * 32 - place);
+                        if (a.softcap > 0.f) {
 #pragma unroll
-                        for (int x = 0; x < 32; ++x) {
-                            float w = __uint_as_float(v[x]);
-                            if (a.softcap > 0.f) w = capped(w, a.softcap, 2.f * LOG2E / a.softcap);
-                            v[x] = __float_as_uint(fmaf(slope, (float)(key0 + cb * 32 + x - place), w) * LOG2E);
+                            for (int x = 0; x < 32; ++x) v[x] = __float_as_uint(capped(__uint_as_float(v[x]), cap));
                         }
+#pragma unroll
+                        for (int x = 0; x < 32; ++x) v[x] = __float_as_uint(fmaf(slope, away + (float)x, __uint_as_float(v[x])));
                     }
                     if (stored) {
                         if (masked) {
-                            const unsigned there = bar.present[slot][2 * half + cb];
+                            const int seen = min(max(limit - key0 - cb * 32, 0), 32);
+                            const unsigned there = bar.present[slot][2 * half + cb] & (uint32_t)((1ull << seen) - 1ull);
 #pragma unroll
                             for (int x = 0; x < 32; ++x)
-                                if (key0 + cb * 32 + x >= limit || !((there >> x) & 1u)) v[x] = 0xff800000u;
+                                if (!((there >> x) & 1u)) v[x] = 0xff800000u;
                         }
                         tmem_store_32(s_at + cb * 32, v);
                     }
