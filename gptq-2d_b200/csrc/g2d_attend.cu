@@ -167,32 +167,41 @@ __global__ void __launch_bounds__(AttendShape<D, NT>::THREADS, 1) attend_rows_ke
     const uint32_t key_bytes = what < 2 ? CODE_BYTES : 2;
     const uint8_t *const source = what == 0 ? c.k_codes : what == 1 ? c.v_codes : what == 2 ? (const uint8_t *)c.k_scale : (const uint8_t *)c.v_scale;
     const uint32_t target = (uint32_t)(what == 0 ? offsetof(AttendStage<D>, k) : what == 1 ? offsetof(AttendStage<D>, v) : what == 2 ? offsetof(AttendStage<D>, ks) : offsetof(AttendStage<D>, vs)) + to * key_bytes;
-    auto page_of = [&](const AttendCursor &at) {  // the page of this lane's piece, or -1
+    auto page_of = [&](const AttendCursor &at) {  // what the table says of this lane's piece, or -1
         const int key = at.block * CACHE_BLOCK + to;
         if (at.u >= at.end || lane >= 4 * pieces || key >= at.s.keys) return -1;
-        const int page = c.table[at.b * c.table_stride + (key >> c.page_shift)];
-        return page < c.pages ? page : -1;
+        return c.table[at.b * c.table_stride + (key >> c.page_shift)];
     };
     const uint64_t policy = read_once();
-    int next_page = page_of(ahead);
     unsigned present[ATTEND_STAGES];  // which pieces of a stage were loaded: four bits each
-#pragma unroll
-    for (int s = 0; s < ATTEND_STAGES; ++s) present[s] = 0u;
-    auto issue = [&](int stage, unsigned &here) {
+    auto issue = [&](int stage, unsigned &here, int page, int item, int block) {
         uint64_t *const bar = &sh.full[warp][stage];
-        here = __ballot_sync(0xffffffffu, next_page >= 0);
+        const bool there = page >= 0 && page < c.pages;
+        here = __ballot_sync(0xffffffffu, there);
         if (lane == 0) mbar_expect_tx(bar, (uint32_t)(__popc(here & 0x11111111u) * piece_keys * (2 * CODE_BYTES + 4)));
         __syncwarp();
-        if (next_page >= 0) {
-            const int64_t row = (((int64_t)next_page * c.kv_heads + ahead.item % c.kv_heads) << c.page_shift) + ((ahead.block * CACHE_BLOCK + to) & (c.page_size - 1));
+        if (there) {
+            const int64_t row = (((int64_t)page * c.kv_heads + item % c.kv_heads) << c.page_shift) + ((block * CACHE_BLOCK + to) & (c.page_size - 1));
             bulk_load(reinterpret_cast<unsigned char *>(&sh.stage[warp][stage]) + target, source + row * key_bytes, piece_keys * key_bytes, bar, policy);
         }
-        ahead.template step<ROWS>(a);
-        next_page = page_of(ahead);
     };
+    {
+        // the first blocks' pages are asked for together
+        int page[ATTEND_STAGES], item[ATTEND_STAGES], block[ATTEND_STAGES];
 #pragma unroll
-    for (int s = 0; s < ATTEND_STAGES; ++s)
-        if (ahead.u < ahead.end) issue(s, present[s]);
+        for (int s = 0; s < ATTEND_STAGES; ++s) {
+            page[s] = page_of(ahead);
+            item[s] = ahead.u < ahead.end ? ahead.item : -1;
+            block[s] = ahead.block;
+            if (item[s] >= 0) ahead.template step<ROWS>(a);
+        }
+#pragma unroll
+        for (int s = 0; s < ATTEND_STAGES; ++s) {
+            present[s] = 0u;
+            if (item[s] >= 0) issue(s, present[s], page[s], item[s], block[s]);
+        }
+    }
+    int next_page = page_of(ahead);
 
     int stage = 0, phase = 0;
     bool sound = true;
@@ -437,47 +446,52 @@ __global__ void __launch_bounds__(AttendShape<D, NT>::THREADS, 1) attend_rows_ke
 #pragma unroll
                 for (int x = 0; x < 4; ++x) base[j][0][x] = b[x & 1], base[j][1][x] = 16.f * b[x & 1];
             }
-            float acc[MTILES][NT][4];
+            // (sixteen rows: half of the channels after the other, as registers are short)
+            constexpr int PASSES = NT == 2 && D == 128 ? 2 : 1, HERE = MTILES / PASSES;
 #pragma unroll
-            for (int mt = 0; mt < 4; ++mt) {
-                const int k0 = 16 * t + 2 * mt;  // rows 2 t and 2 t + 1 of tile mt: the keys k0 and k0 + 8, and the ones behind them
-                uint32_t lo[2][2], hi[2][2];     // [pair of keys][word]: nibbles 0..3 and 4..7 of both keys
+            for (int pass = 0; pass < PASSES; ++pass) {
+                float acc[HERE][NT][4];
 #pragma unroll
-                for (int pair = 0; pair < 2; ++pair) {
-                    if constexpr (D == 128) {
-                        const uint2 x = *reinterpret_cast<const uint2 *>(st.v + (k0 + pair) * CODE_BYTES + g * 8), y = *reinterpret_cast<const uint2 *>(st.v + (k0 + pair + 8) * CODE_BYTES + g * 8);
-                        lo[pair][0] = __byte_perm(x.x, y.x, 0x5410);
-                        hi[pair][0] = __byte_perm(x.x, y.x, 0x7632);
-                        lo[pair][1] = __byte_perm(x.y, y.y, 0x5410);
-                        hi[pair][1] = __byte_perm(x.y, y.y, 0x7632);
-                    } else {
-                        const uint32_t x = *reinterpret_cast<const uint32_t *>(st.v + (k0 + pair) * CODE_BYTES + g * 4), y = *reinterpret_cast<const uint32_t *>(st.v + (k0 + pair + 8) * CODE_BYTES + g * 4);
-                        lo[pair][0] = __byte_perm(x, y, 0x5410);
-                        lo[pair][1] = __byte_perm(x, y, 0x7632);
+                for (int mt = 0; mt < 4; ++mt) {
+                    const int k0 = 16 * t + 2 * mt;  // rows 2 t and 2 t + 1 of tile mt: the keys k0 and k0 + 8, and the ones behind them
+                    uint32_t lo[2][2], hi[2][2];     // [pair of keys][word]: nibbles 0..3 and 4..7 of both keys
+#pragma unroll
+                    for (int pair = 0; pair < 2; ++pair) {
+                        if constexpr (D == 128) {
+                            const uint2 x = *reinterpret_cast<const uint2 *>(st.v + (k0 + pair) * CODE_BYTES + g * 8), y = *reinterpret_cast<const uint2 *>(st.v + (k0 + pair + 8) * CODE_BYTES + g * 8);
+                            lo[pair][0] = __byte_perm(x.x, y.x, 0x5410);
+                            hi[pair][0] = __byte_perm(x.x, y.x, 0x7632);
+                            lo[pair][1] = __byte_perm(x.y, y.y, 0x5410);
+                            hi[pair][1] = __byte_perm(x.y, y.y, 0x7632);
+                        } else {
+                            const uint32_t x = *reinterpret_cast<const uint32_t *>(st.v + (k0 + pair) * CODE_BYTES + g * 4), y = *reinterpret_cast<const uint32_t *>(st.v + (k0 + pair + 8) * CODE_BYTES + g * 4);
+                            lo[pair][0] = __byte_perm(x, y, 0x5410);
+                            lo[pair][1] = __byte_perm(x, y, 0x7632);
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < HERE; ++i) {
+                        const int e = pass * HERE + i, nibble = e & 3;
+                        uint32_t f[4];
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {  // a0, a1: word 0 and 1 of the first pair; a2, a3: of the second
+                            const uint32_t word = e < 4 ? lo[x >> 1][x & 1] : hi[x >> 1][x & 1];
+                            f[x] = (nibble & 2 ? word >> 8 : word) & (nibble & 1 ? 0x00f000f0u : 0x000f000fu);
+                        }
+#pragma unroll
+                        for (int j = 0; j < NT; ++j) {
+                            if (mt == 0) mma_f16(acc[i][j], f[0], f[1], f[2], f[3], pf[mt][j][0], pf[mt][j][1], base[j][e & 1]);
+                            else mma_f16(acc[i][j], f[0], f[1], f[2], f[3], pf[mt][j][0], pf[mt][j][1]);
+                        }
                     }
                 }
 #pragma unroll
-                for (int e = 0; e < MTILES; ++e) {
-                    const int nibble = e & 3;
-                    uint32_t f[4];
+                for (int i = 0; i < HERE; ++i)
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) {  // a0, a1: word 0 and 1 of the first pair; a2, a3: of the second
-                        const uint32_t word = e < 4 ? lo[x >> 1][x & 1] : hi[x >> 1][x & 1];
-                        f[x] = (nibble & 2 ? word >> 8 : word) & (nibble & 1 ? 0x00f000f0u : 0x000f000fu);
-                    }
+                    for (int j = 0; j < NT; ++j)
 #pragma unroll
-                    for (int j = 0; j < NT; ++j) {
-                        if (mt == 0) mma_f16(acc[e][j], f[0], f[1], f[2], f[3], pf[mt][j][0], pf[mt][j][1], base[j][e & 1]);
-                        else mma_f16(acc[e][j], f[0], f[1], f[2], f[3], pf[mt][j][0], pf[mt][j][1]);
-                    }
-                }
+                        for (int x = 0; x < 2; ++x) o[pass * HERE + i][j][x] = fma2(o[pass * HERE + i][j][x], keep[j], pack2(acc[i][j][2 * x], acc[i][j][2 * x + 1]));
             }
-#pragma unroll
-            for (int e = 0; e < MTILES; ++e)
-#pragma unroll
-                for (int j = 0; j < NT; ++j)
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) o[e][j][x] = fma2(o[e][j][x], keep[j], pack2(acc[e][j][2 * x], acc[e][j][2 * x + 1]));
         };
         for (int block = first_block; block < last_block; ++block) {
             unsigned here = 0u;
@@ -493,7 +507,9 @@ __global__ void __launch_bounds__(AttendShape<D, NT>::THREADS, 1) attend_rows_ke
             __syncwarp();  // all lanes have read the stage
             if (sound && ahead.u < ahead.end) {
                 unsigned loaded;
-                issue(stage, loaded);
+                issue(stage, loaded, next_page, ahead.item, ahead.block);
+                ahead.template step<ROWS>(a);
+                next_page = page_of(ahead);
 #pragma unroll
                 for (int s2 = 0; s2 < ATTEND_STAGES; ++s2)
                     if (s2 == stage) present[s2] = loaded;
@@ -562,18 +578,17 @@ __global__ void __launch_bounds__(AttendShape<D, NT>::THREADS, 1) attend_rows_ke
     }
     // ---- the warps' parts of an item, in the order of the keys: parts that stand together in the list ----
     __syncthreads();
-    const auto next_part = [&](int p) {
-        while (p < 2 * ATTEND_WARPS && sh.parts[p].last == 0) ++p;
-        return p;
-    };
-    for (int p0 = next_part(0); p0 < 2 * ATTEND_WARPS;) {
+    // a lane per part: which are there, and which begin an item
+    const AttendPart &at_lane = sh.parts[min(lane, 2 * ATTEND_WARPS - 1)];
+    const unsigned there = __ballot_sync(0xffffffffu, lane < 2 * ATTEND_WARPS && at_lane.last != 0);
+    const int before = max(31 - __clz((int)(there & ((1u << lane) - 1u))), 0), b_here = at_lane.b, item_here = at_lane.item;
+    const int b_before = __shfl_sync(0xffffffffu, b_here, before), item_before = __shfl_sync(0xffffffffu, item_here, before);
+    const bool begins = (there >> lane & 1u) && (!(there & ((1u << lane) - 1u)) || b_before != b_here || item_before != item_here);
+    for (unsigned left = __ballot_sync(0xffffffffu, begins); left; left &= left - 1) {
+        const int p0 = __ffs(left) - 1, end = left & (left - 1) ? __ffs(left & (left - 1)) - 1 : 32;
+        const unsigned group = there & ((end < 32 ? 1u << end : 0u) - (1u << p0));
+        const int count = __popc(group), p1 = 31 - __clz((int)group);
         const AttendPart &begin = sh.parts[p0];
-        int p1 = p0, count = 1, behind = next_part(p0 + 1);
-        while (behind < 2 * ATTEND_WARPS && sh.parts[behind].b == begin.b && sh.parts[behind].item == begin.item) {
-            p1 = behind;
-            ++count;
-            behind = next_part(behind + 1);
-        }
         const int first = begin.first, last = sh.parts[p1].last;
         const bool whole = first == 0 && last == begin.blocks;
         const int head = begin.item % c.kv_heads, row0 = begin.item / c.kv_heads * ROWS, rows = begin.s.count * a.group;
@@ -596,7 +611,6 @@ __global__ void __launch_bounds__(AttendShape<D, NT>::THREADS, 1) attend_rows_ke
                 }
             }
         }
-        p0 = behind;
     }
     after_the_launch_before();  // of the tiles' kernel: what follows waits for this one alone
 }

@@ -137,12 +137,20 @@ __device__ __forceinline__ int sequence_of_unit(int batch, Units units, unsigned
 // sums of the channels x, x + 32, ..
 template <int D, typename Row>
 __device__ __forceinline__ void merge_parts(int count, Row row, int reference, int total, float (&acc)[D / 32], float &m, float &l) {
+    constexpr int TOGETHER = 8;  // parts whose loads travel together, the first ones' with the references
     const int lane = threadIdx.x & 31;
-    float mine = -INFINITY, t = 0.f;
+    float mine = -INFINITY, t = 0.f, v[TOGETHER][D / 32];
+    const auto fetch = [&](int from) {
+#pragma unroll
+        for (int k = 0; k < TOGETHER; ++k)
+#pragma unroll
+            for (int x = 0; x < D / 32; ++x) v[k][x] = from + k < count ? __ldcg(row(from + k) + x * 32 + lane) : 0.f;
+    };
     if (lane < count) {
         mine = __ldcg(row(lane) + reference);
         t = __ldcg(row(lane) + total);
     }
+    fetch(0);
     m = mine;
     for (int i = lane + 32; i < count; i += 32) m = fmaxf(m, __ldcg(row(i) + reference));
 #pragma unroll
@@ -151,32 +159,28 @@ __device__ __forceinline__ void merge_parts(int count, Row row, int reference, i
     l = 0.f;
 #pragma unroll
     for (int x = 0; x < D / 32; ++x) acc[x] = 0.f;
-    for (int i0 = 0; i0 < count; i0 += 32) {
-        if (i0 > 0) {
-            mine = -INFINITY;
-            t = 0.f;
-            if (i0 + lane < count) {
-                mine = __ldcg(row(i0 + lane) + reference);
-                t = __ldcg(row(i0 + lane) + total);
-            }
-        }
-        const float w = ex2(mine - base);
-        const int here = min(32, count - i0);
+    float w = 0.f;
 #pragma unroll 1
-        for (int i = 0; i < here; i += 4) {  // four parts' loads travel together
-            float v[4][D / 32];
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-#pragma unroll
-                for (int x = 0; x < D / 32; ++x) v[k][x] = i + k < here ? __ldcg(row(i0 + i + k) + x * 32 + lane) : 0.f;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float f = __shfl_sync(0xffffffffu, w, (i + k) & 31), tk = __shfl_sync(0xffffffffu, t, (i + k) & 31);
-                if (i + k < here) {
-                    l = fmaf(tk, f, l);
-#pragma unroll
-                    for (int x = 0; x < D / 32; ++x) acc[x] = fmaf(v[k][x], f, acc[x]);
+    for (int i = 0; i < count; i += TOGETHER) {
+        if (i > 0) fetch(i);
+        if (i % 32 == 0) {
+            if (i > 0) {
+                mine = -INFINITY;
+                t = 0.f;
+                if (i + lane < count) {
+                    mine = __ldcg(row(i + lane) + reference);
+                    t = __ldcg(row(i + lane) + total);
                 }
+            }
+            w = ex2(mine - base);
+        }
+#pragma unroll
+        for (int k = 0; k < TOGETHER; ++k) {
+            const float f = __shfl_sync(0xffffffffu, w, (i + k) & 31), tk = __shfl_sync(0xffffffffu, t, (i + k) & 31);
+            if (i + k < count) {
+                l = fmaf(tk, f, l);
+#pragma unroll
+                for (int x = 0; x < D / 32; ++x) acc[x] = fmaf(v[k][x], f, acc[x]);
             }
         }
     }
