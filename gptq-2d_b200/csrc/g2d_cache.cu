@@ -37,11 +37,25 @@ __device__ __forceinline__ void tokens_of_warp(const CacheView &c, int &t0, int 
     t1 = (int)((w + 1) * c.tokens / warps);
 }
 
-// x / scale rounded to the nearest of -8 .. 7.  `rc` is 1 / scale, rounded; one correction leaves the quotient within its last bit.  That is enough: a quotient q of an x of 11 bits at most
-// and a scale of 11 bits is either a half-integer exactly, and then both steps are exact as well, or more than 2^-16 of itself away from one.
-__device__ __forceinline__ uint32_t code_of(float x, float scale, float rc) {
-    const float q0 = x * rc, q = fmaf(fmaf(-q0, scale, x), rc, q0);
-    return (uint32_t)(__float2int_rn(fminf(fmaxf(q, -8.f), 7.f)) + 8);
+// Quotients by one reciprocal (within two units of its last bit) and one correction, which leaves them within theirs.  That is enough: the quotient of an x of 11 bits at most by a scale of 11
+// bits (or by 7.5) is either a half-integer (or halfway between two halves) exactly, and then both steps are exact as well, or more than 2^-16 of itself away from one.
+__device__ __forceinline__ float reciprocal(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float scale_of(float absmax) {  // absmax / 7.5 as a half, 1 for zero
+    constexpr float RC = 1.f / 7.5f;
+    const float q0 = absmax * RC, q = __half2float(__float2half_rn(absmax < INFINITY ? fmaf(fmaf(-q0, 7.5f, absmax), RC, q0) : absmax));
+    return q == 0.f ? 1.f : q;
+}
+// two values over the scale, rounded to the nearest of -8 .. 7, plus 8: by the addition of 1.5 2^23 + 8, in the lowest bits of what is returned
+__device__ __forceinline__ void codes_of(uint64_t x, uint64_t minus_scale, uint64_t rc, uint32_t &lo, uint32_t &hi) {
+    const uint64_t q0 = mul2(x, rc);
+    float a, b;
+    unpack2(fma2(fma2(q0, minus_scale, x), rc, q0), a, b);
+    lo = __float_as_uint(fminf(fmaxf(a, -8.f), 7.f) + 12582920.f);
+    hi = __float_as_uint(fminf(fmaxf(b, -8.f), 7.f) + 12582920.f);
 }
 
 // rows of a token: (head, key or value), the latter fastest; LANES lanes each
@@ -67,21 +81,22 @@ __global__ void __launch_bounds__(CACHE_THREADS) cache_append_kernel(const Cache
             for (int n = 0; n < BATCH; ++n) {
                 const int r = r0 + n * ROWS + sub, head = r >> 1;
                 if (r0 + n * ROWS >= rows) break;  // for the whole warp
-                float x[8];
                 const uint32_t word[4] = {raw[n].x, raw[n].y, raw[n].z, raw[n].w};
-                unsigned largest = 0u;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    x[e] = half_bits_to_float((word[e >> 1] >> (16 * (e & 1))) & 0xffffu, c.bf16);
-                    largest = max(largest, __float_as_uint(x[e]) & 0x7fffffffu);
-                }
-                const float scale = absmax_scale_value(__uint_as_float(lanes_max<LANES>(largest)), 7.5f, G2D_FP16);
-                const float rc = __frcp_rn(scale);
+                // the largest as the bits of a half, whose order is that of the values (NaN above infinity)
+                const uint32_t pair = __vmaxu2(__vmaxu2(word[0] & 0x7fff7fffu, word[1] & 0x7fff7fffu), __vmaxu2(word[2] & 0x7fff7fffu, word[3] & 0x7fff7fffu));
+                const float scale = scale_of(half_bits_to_float(lanes_max<LANES>(max(pair & 0xffffu, pair >> 16)), c.bf16));
                 uint32_t codes = 0x88888888u;  // a row that is not finite: zeros under a scale that is not
                 if (scale <= 65504.f) {
+                    const uint64_t minus = pack2(-scale, -scale);
+                    const float r1 = reciprocal(scale);
+                    const uint64_t rc = pack2(r1, r1);
                     codes = 0u;
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) codes |= code_of(x[e], scale, rc) << (4 * e);
+                    for (int e = 0; e < 4; ++e) {
+                        uint32_t lo, hi;
+                        codes_of(pack2(half_bits_to_float(word[e] & 0xffffu, c.bf16), half_bits_to_float(word[e] >> 16, c.bf16)), minus, rc, lo, hi);
+                        codes |= (lo & 15u) << (8 * e) | (hi & 15u) << (8 * e + 4);
+                    }
                 }
                 if (r < rows) {
                     const int64_t row = at + ((int64_t)head << c.page_shift);
