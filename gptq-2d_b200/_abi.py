@@ -209,7 +209,7 @@ _NO_CONTEXT = contextlib.nullcontext()
 
 def on_device(index: int):
     """``torch.cuda.device(index)`` where another device is the current one."""
-    return _NO_CONTEXT if torch.cuda.current_device() == index else torch.cuda.device(index)
+    return _NO_CONTEXT if torch._C._cuda_getDevice() == index else torch.cuda.device(index)
 
 
 def raw_stream(index: int) -> int:

@@ -70,18 +70,19 @@ def _cache_fields(cache: PackedCache, dtype, tokens: int, page_table, lengths, o
     head_dim, page_size, kv_heads, pages = cache.layout
     k_codes, k_scale, v_codes, v_scale = cache
     device = k_codes.device
+    index = device.index
     half = _HALF.get(dtype)
     assert half is not None, "expected float16 or bfloat16 values"
-    assert page_table.dim() == 2 and page_table.dtype == torch.int32 and page_table.device == device, "expected an int32 page table [batch, pages per sequence] on the cache's device"
+    assert page_table.dim() == 2 and page_table.dtype == torch.int32 and page_table.get_device() == index, "expected an int32 page table [batch, pages per sequence] on the cache's device"
     batch, width = page_table.shape
     table_stride, last = page_table.stride()
     assert last == 1 or width <= 1, "the rows of the page table must be contiguous"
-    assert lengths.shape == (batch,) and lengths.dtype == torch.int32 and lengths.device == device and lengths.is_contiguous(), "expected contiguous int32 lengths [batch] on the cache's device"
+    assert lengths.shape == (batch,) and lengths.dtype == torch.int32 and lengths.get_device() == index and lengths.is_contiguous(), "expected contiguous int32 lengths [batch] on the cache's device"
     if offsets is None:
         assert tokens == 0 or (batch > 0 and tokens % batch == 0), "without offsets every sequence has the same number of tokens"
         offsets_at = 0
     else:
-        assert offsets.shape == (batch + 1,) and offsets.dtype == torch.int32 and offsets.device == device and offsets.is_contiguous(), "expected contiguous int32 offsets [batch + 1] on the cache's device"
+        assert offsets.shape == (batch + 1,) and offsets.dtype == torch.int32 and offsets.get_device() == index and offsets.is_contiguous(), "expected contiguous int32 offsets [batch + 1] on the cache's device"
         offsets_at = offsets.data_ptr()
     return device, (half, head_dim, page_size, kv_heads, pages, batch, width, table_stride, tokens, k_codes.data_ptr(), k_scale.data_ptr(), v_codes.data_ptr(), v_scale.data_ptr(),
                     page_table.data_ptr(), lengths.data_ptr(), offsets_at)
@@ -89,7 +90,7 @@ def _cache_fields(cache: PackedCache, dtype, tokens: int, page_table, lengths, o
 
 def _rows(x: torch.Tensor, device, heads: int, dim: int, what: str) -> torch.Tensor:
     """``x [tokens, heads, dim]`` as the kernels read it: any strides of tokens and heads that keep 16-byte vectors whole, else a copy."""
-    assert x.device == device, f"{what} must be on the cache's device"
+    assert x.get_device() == device.index, f"{what} must be on the cache's device"
     assert x.dim() == 3 and x.shape[1:] == (heads, dim), f"expected {what} [tokens, {heads}, {dim}]"
     token, head, last = x.stride()
     if last != 1 or token % 8 or head % 8 or x.data_ptr() % 16:
@@ -101,7 +102,7 @@ def append_packed(cache: PackedCache, k: torch.Tensor, v: torch.Tensor, page_tab
     """Round the step's keys and values ``[tokens, kv_heads, head_dim]`` (float16 or bfloat16; strided views, such as parts of a fused projection, are
     read in place) and write them into the cache, in place.  ``lengths`` counts the step's tokens already.  A row with an infinity or a NaN reads back as NaN."""
     assert k.dtype == v.dtype and k.dim() == 3 and k.shape == v.shape, "expected keys and values of one shape and type"
-    device, fields = _cache_fields(cache, k.dtype, k.size(0), page_table, lengths, offsets)
+    device, fields = _cache_fields(cache, k.dtype, k.shape[0], page_table, lengths, offsets)
     k, v = _rows(k, device, fields[3], fields[1], "keys"), _rows(v, device, fields[3], fields[1], "values")
     index = device.index
     with _abi.on_device(index):
@@ -115,8 +116,8 @@ def read_packed(cache: PackedCache, page_table: torch.Tensor, lengths: torch.Ten
     """The keys and values ``[tokens, kv_heads, head_dim]`` that the cache holds for the last tokens of every sequence, ``offsets`` saying how many (all of them, where
     they add up to ``lengths``).  Rows of no sequence, and positions that the cache does not hold, are zeros."""
     device, fields = _cache_fields(cache, dtype, tokens, page_table, lengths, offsets)
-    both = (torch.empty if offsets is None else torch.zeros)((2, tokens, fields[3], fields[1]), dtype=dtype, device=device)
-    k, v = both.unbind(0)
+    k = (torch.empty if offsets is None else torch.zeros)((tokens, fields[3], fields[1]), dtype=dtype, device=device)
+    v = (torch.empty_like if offsets is None else torch.zeros_like)(k)
     index = device.index
     with _abi.on_device(index):
         status = _abi.library().g2d_cache_read(_abi.CACHE_DESC.pack(*fields), k.data_ptr(), v.data_ptr(), _abi.raw_stream(index))
@@ -148,15 +149,15 @@ def attend_packed(q: torch.Tensor, cache: PackedCache, page_table: torch.Tensor,
     assert math.isfinite(scale), "scale must be finite"
     slopes_at = prefix_at = 0
     if slopes is not None:
-        assert slopes.shape == (heads,) and slopes.dtype == torch.float32 and slopes.device == device and slopes.is_contiguous(), "expected contiguous float32 slopes [heads] on the cache's device"
+        assert slopes.shape == (heads,) and slopes.dtype == torch.float32 and slopes.get_device() == device.index and slopes.is_contiguous(), "expected contiguous float32 slopes [heads] on the cache's device"
         slopes_at = slopes.data_ptr()
     if prefix is not None:
-        assert prefix.shape == lengths.shape and prefix.dtype == torch.int32 and prefix.device == device and prefix.is_contiguous(), "expected a contiguous int32 prefix [batch] on the cache's device"
+        assert prefix.shape == lengths.shape and prefix.dtype == torch.int32 and prefix.get_device() == device.index and prefix.is_contiguous(), "expected a contiguous int32 prefix [batch] on the cache's device"
         prefix_at = prefix.data_ptr()
     if out is None:
-        out = (torch.empty if offsets is None else torch.zeros)((tokens, heads, head_dim), dtype=dtype, device=device)
+        out = (torch.empty_like if offsets is None else torch.zeros_like)(q, memory_format=torch.contiguous_format)
     else:
-        assert out.shape == q.shape and out.dtype == dtype and out.device == device and out.is_contiguous() and out.data_ptr() % 16 == 0, "out must be a contiguous, 16-byte aligned tensor like q"
+        assert out.shape == q.shape and out.dtype == dtype and out.get_device() == device.index and out.is_contiguous() and out.data_ptr() % 16 == 0, "out must be a contiguous, 16-byte aligned tensor like q"
     if tokens == 0:
         return out
     lib, index = _abi.library(), device.index

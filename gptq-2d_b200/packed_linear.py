@@ -29,7 +29,7 @@ _WORKSPACE: dict[tuple, int] = {}  # bytes by sizes
 
 def _parameter(t, m: int, n: int, name: str, device):
     """A scale or zero point: one value, one per row, or one per row and group of columns; with its strides over rows and groups, and how many groups."""
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.device != device:
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.get_device() != device.index:
         t = torch.as_tensor(t, dtype=torch.float32, device=device)
     shape = t.shape
     assert len(shape) <= 2, f"{name} must be one value, one per row, or one per row and group of columns"
@@ -52,21 +52,20 @@ def packed_linear(x: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor, zer
     overlap the inputs.  bfloat16 activations of 2**72 and more may overflow."""
     assert bits == 4, "only codes of 4 bits can be multiplied with"
     device, dtype, shape = x.device, x.dtype, x.shape
-    assert device.type == "cuda", "the product with packed codes requires CUDA tensors (there is no CPU path)"
+    index = device.index
+    assert x.is_cuda, "the product with packed codes requires CUDA tensors (there is no CPU path)"
     half = _HALF.get(dtype)
     assert half is not None and len(shape) >= 1, "expected float16 or bfloat16 activations [..., n]"
-    assert codes.dim() == 2 and codes.dtype == torch.uint8 and codes.is_contiguous() and codes.device == device, "expected contiguous uint8 codes on the activations' device"
+    assert codes.dim() == 2 and codes.dtype == torch.uint8 and codes.is_contiguous() and codes.get_device() == index, "expected contiguous uint8 codes on the activations' device"
     n, (m, row_bytes), codes_at = shape[-1], codes.shape, codes.data_ptr()
     assert n > 0 and n % 32 == 0, "the number of columns must be a multiple of 32"
     assert row_bytes >= n // 2 and row_bytes % 16 == 0 and codes_at % 16 == 0, "rows of codes must hold n entries and be 16-byte aligned"
-    rows = x.detach()
-    if len(shape) != 2:
-        rows = rows.reshape(-1, n)
+    rows = x if len(shape) == 2 else x.detach().reshape(-1, n)
     row_stride, last = rows.stride()
     if last != 1 or row_stride % 8 or rows.data_ptr() % 16:
-        rows = rows.clone(memory_format=torch.contiguous_format)
+        rows = rows.detach().clone(memory_format=torch.contiguous_format)
         row_stride = n
-    tokens = rows.size(0)
+    tokens = rows.shape[0]
     scale, scale_row, scale_group, groups = _parameter(scale, m, n, "scale", device)
     zero, zero_row, zero_group, zero_groups = _parameter(zero_point, m, n, "zero_point", device)
     assert groups == zero_groups or groups == 1 or zero_groups == 1, "scale and zero_point must have the same groups"
@@ -78,13 +77,13 @@ def packed_linear(x: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor, zer
         count, rank, _ = down.shape
         assert down.shape == (count, rank, n) and up.shape == (count, m, rank), "expected down [adapters, rank, n] and up [adapters, m, rank]"
         assert rank % 8 == 0 and 0 < rank <= 64, "the rank must be a multiple of 8, at most 64"
-        assert down.dtype == dtype and up.dtype == dtype and down.device == device and up.device == device, "the adapters must have the activations' type and device"
+        assert down.dtype == dtype and up.dtype == dtype and down.get_device() == index and up.get_device() == index, "the adapters must have the activations' type and device"
         down_at, up_at = down.data_ptr(), up.data_ptr()
         assert down.is_contiguous() and up.is_contiguous() and not (down_at | up_at) & 15, "the adapters must be contiguous and 16-byte aligned"
-        assert adapter_index.dtype == torch.int32 and adapter_index.device == device and adapter_index.numel() == tokens and adapter_index.is_contiguous(), "expected a contiguous int32 adapter index per token"
+        assert adapter_index.dtype == torch.int32 and adapter_index.get_device() == index and adapter_index.numel() == tokens and adapter_index.is_contiguous(), "expected a contiguous int32 adapter index per token"
         index_at = adapter_index.data_ptr()
         if scaling is not None:
-            assert scaling.shape == (count,) and scaling.dtype == torch.float32 and scaling.device == device and scaling.is_contiguous(), "expected contiguous float32 scaling [adapters]"
+            assert scaling.shape == (count,) and scaling.dtype == torch.float32 and scaling.get_device() == index and scaling.is_contiguous(), "expected contiguous float32 scaling [adapters]"
             scaling_at = scaling.data_ptr()
         if count == 0:
             rank = 0
@@ -93,10 +92,10 @@ def packed_linear(x: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor, zer
     if out is None:
         out = torch.empty((*shape[:-1], m), dtype=dtype, device=device)
     else:
-        assert out.shape == (*shape[:-1], m) and out.dtype == dtype and out.device == device and out.is_contiguous(), "out must be a contiguous tensor of x's type [..., m]"
+        assert out.shape == (*shape[:-1], m) and out.dtype == dtype and out.get_device() == index and out.is_contiguous(), "out must be a contiguous tensor of x's type [..., m]"
     if tokens == 0 or m == 0:
         return out
-    lib, index = _abi.library(), device.index
+    lib = _abi.library()
     fields = (half, bits, m, n, tokens, rows.data_ptr(), row_stride, codes_at, row_bytes, max(groups, zero_groups), scale.data_ptr(), scale_row, scale_group,
               zero.data_ptr(), zero_row, zero_group, float(qmin), count, rank, 0, down_at, up_at, scaling_at, index_at, out.data_ptr(), m)
     sizes = (m, n, tokens, rank, count)
