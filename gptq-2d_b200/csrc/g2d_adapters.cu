@@ -65,10 +65,9 @@ __device__ void write_plan(const LinearArgs &a, int *plan, int tile, int token0)
     if (threadIdx.x == 0) plan[0] = all;
 }
 
-__global__ void __launch_bounds__(INNER_THREADS) inner_rows_kernel(const LinearArgs a, int *plan, int tile) {
+__global__ void __launch_bounds__(INNER_THREADS) inner_rows_kernel(const LinearArgs a) {
     __shared__ float part[RANK_MAX], tops[2];
     let_the_next_launch_start();
-    if (plan && blockIdx.x == INNER_SPLIT - 1) write_plan(a, plan, tile, 0);  // 64 tokens at most: one tile
     const int token = blockIdx.x / INNER_SPLIT, rank = (int)cluster_rank(), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int id = adapter_of(a, token);
     const int64_t chunks = a.n / 8, c0 = rank * chunks / INNER_SPLIT, c1 = (rank + 1) * chunks / INNER_SPLIT;  // eight columns each
@@ -211,8 +210,9 @@ __global__ void __launch_bounds__(INNER_THREADS, TILES == 8 ? 1 : 2) inner_block
 }
 
 int launch_inner(const LinearArgs &a, int *plan, int tile, cudaStream_t st) {
-    // Both sides of the line: see the figures above.
-    if (a.tokens <= 64) return launch_dependent(inner_rows_kernel, dim3((unsigned)a.tokens * INNER_SPLIT), INNER_THREADS, 0, INNER_SPLIT, false, st, a, plan, tile);
+    // Whole calls, 4096 x 4096, 64 tokens of 40 adapters of rank 64: 38.7 us by tokens, 63.1 by blocks; of 32 of rank 16: 25.2, 45.3; of one or four alike (23.6, 23.3; 34.8, 33.7).  Beyond, a
+    // prompt's tokens stand together: 2048 of 8 adapters of rank 32 over 28672 columns 53 us by blocks, and one adapter would be read 2048 times by tokens.
+    if (a.tokens <= LINEAR_FEW) return launch_dependent(inner_rows_kernel, dim3((unsigned)a.tokens * INNER_SPLIT), INNER_THREADS, 0, INNER_SPLIT, false, st, a);
     const unsigned blocks = (unsigned)ceil_div((int64_t)a.tokens, (int64_t)INNER_BLOCK);
     const dim3 grid(blocks * INNER_SPLIT, (unsigned)(a.adapters < 4 ? a.adapters + 1 : 4));
     const auto launch = [&](auto kernel) { return launch_dependent(kernel, grid, INNER_THREADS, 0, INNER_SPLIT, false, st, a, plan, tile); };

@@ -722,8 +722,10 @@ static int launch_attend(const AttendArgs &rows, const AttendArgs &tiles, bool f
     return launch_behind(attend_join_kernel<D, NT>, (unsigned)(j.tile_ctas + (few ? ATTEND_GRID : 0)), JOIN_THREADS, 0, j, st);
 }
 
-// From here on a sequence's rows go by tiles; both sides of the line: see the figures in g2d_attend_tc.cu.
-constexpr int TILE_ROWS_FROM = 33;
+// From how many rows of a kv head on a sequence goes by tiles.  Tiles cost more to begin with, so few items (sequences and kv heads) cross the line later.
+// 32 heads on 8, head_dim 128: 1 sequence of 4096 keys, 64 rows: 27.3 us by rows, 35.3 by tiles; 8 of 2000, 64 rows: 47.1, 54.5, 128 rows: 74.5, 59.3;
+// 32 of 1000, 32 rows: 62.0, 67.4, 48 rows: 86.8, 69.2
+static int tile_rows_from(const CacheView &c) { return (int64_t)c.batch * c.kv_heads <= 64 ? 65 : 33; }
 
 struct AttendSpace {
     size_t tiles, all;  // the warps' partial results first
@@ -778,13 +780,14 @@ extern "C" int g2d_cache_attend(const g2d_attend_desc *d, void *stream) {
     cudaStream_t st = (cudaStream_t)stream;
     // How many rows a sequence has is known here only where all have the same; else the kernels share the sequences out between them.
     const int64_t rows = a.c.offsets ? -1 : (int64_t)(a.c.tokens / a.c.batch) * a.group;
-    const bool many = rows < 0 ? (int64_t)a.c.tokens * a.group >= TILE_ROWS_FROM : rows >= TILE_ROWS_FROM, few = rows < TILE_ROWS_FROM;
+    const int line = tile_rows_from(a.c);
+    const bool many = rows < 0 ? (int64_t)a.c.tokens * a.group >= line : rows >= line, few = rows < line;
     AttendArgs t = a;
-    t.rows_from = TILE_ROWS_FROM;
+    t.rows_from = line;
     t.rows_to = 0x7fffffff;
     t.partial = (float *)((char *)d->workspace + attend_space(a.c.head_dim).tiles);
     a.rows_from = 1;
-    a.rows_to = TILE_ROWS_FROM;
+    a.rows_to = line;
     a.partial = (float *)d->workspace;
     const bool narrow = a.group <= 8 && (rows < 0 || rows <= 8);
     if (a.c.head_dim == 128) return narrow ? launch_attend<128, 1>(a, t, few, many, st) : launch_attend<128, 2>(a, t, few, many, st);

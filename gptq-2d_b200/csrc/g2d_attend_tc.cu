@@ -20,7 +20,6 @@ namespace g2d {
 constexpr int TA_THREADS = 896, TA_SCALES = 4, TA_ROW_WARPS = 16;
 constexpr int TA_PANEL = 128 * 128;  // bytes of 128 rows of 64 16-bit values
 constexpr float TA_SLACK = 8.f;      // how far scores may exceed the maximum that the exponentials refer to, as a power of two
-constexpr long long TA_APART = 2000;  // cycles
 constexpr int TA_UNIT = 6;           // the largest scale is brought to 2^6 .. 2^7: times 2^8, still a number of fp16
 
 template <int D>
@@ -262,11 +261,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const __gri
                 if (!go) break;
                 after();
                 scores(0, kc & 1);
-                if (two) {
-                    // The tiles start half a block apart: one's exponentials then run beside the other's maxima and products
-                    for (const long long start = clock64(); clock64() - start < TA_APART;) __nanosleep(100);
-                    scores(1, kc & 1);
-                }
+                if (two) scores(1, kc & 1);
                 if (n == 1) umma_commit(&bar.q_empty);
                 umma_commit(&bar.k_empty[kc++ & 1]);
                 if constexpr (M::OWN_P) {

@@ -7,8 +7,10 @@
 // A lane reads 16 bytes of codes (32 columns) of two rows, four times ahead; x lies in shared memory in the order in which such
 // words hold their columns, so a fragment of it is one 16-byte load.  With groups of an odd number of 64 columns a lane reads 8 bytes at a time.
 //
-// A CTA has 16 ROW_TILES rows; its eight warps split them and the columns; a cluster of CTAs splits the columns further, and sums meet through shared memory
-// in a fixed order.  Bound: HBM (half a byte per weight), for small matrices the latency of one chain of loads.
+// A CTA has 128 rows, each of its eight warps 16; a cluster of CTAs splits the columns, and sums meet through shared memory in a fixed order.  (64 rows and the
+// columns halved between warps: 1024 x 4096, 1 token 5.5 us, as it is 5.2; 8192 x 8192, 16 tokens 28.6, 20.2.)
+// Bound: HBM (half a byte per weight) and, from about 12 tokens on, the rate of these products (16 cycles each for a quarter of an SM); for small matrices the latency of one chain
+// of loads.  Without adapters 8192 x 8192 takes 16.0 us with 1 token (2.1 TB/s) and 20.2 with 16; 28672 x 4096 25.9 (2.3 TB/s); 1024 x 4096, 1 token, an adapter of rank 16 6.9.
 #include "g2d_linear.cuh"
 #include "g2d_tc.cuh"
 
@@ -29,9 +31,9 @@ __device__ __forceinline__ void mma_codes(float (&d)[4], uint32_t a0, uint32_t a
 }
 
 // KB: columns of a block, 128 or 64; NT: tiles of eight tokens
-template <bool BF16, int NT, int KB, int ROW_TILES>
+template <bool BF16, int NT, int KB>
 __global__ void __launch_bounds__(ROWS_THREADS, 2) linear_rows_kernel(const LinearArgs a) {
-    constexpr int WORDS = KB / 32, K_GROUPS = ROWS_WARPS / ROW_TILES, ROWS = 16 * ROW_TILES, TOKENS = 8 * NT, CHUNKS = KB / 8, AHEAD = 4;
+    constexpr int WORDS = KB / 32, ROWS = 16 * ROWS_WARPS, TOKENS = 8 * NT, CHUNKS = KB / 8, AHEAD = 4;
     extern __shared__ __align__(16) unsigned char linear_smem_raw[];
     const int splits = (int)gridDim.x, rank = (int)blockIdx.x;  // a cluster has all CTAs along x
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -41,16 +43,14 @@ __global__ void __launch_bounds__(ROWS_THREADS, 2) linear_rows_kernel(const Line
     const int mine = (int)(b_last - b_first), most = (int)ceil_div(blocks, (int64_t)splits);  // the same layout in every CTA of the cluster
     uint4 *const xs = reinterpret_cast<uint4 *>(linear_smem_raw);            // [block][word][tile of tokens][lane]
     float *const sums = reinterpret_cast<float *>(xs + (int64_t)most * WORDS * NT * 32);  // [block][token]
-    float *const part = sums + most * TOKENS;                                // [k group][token][row], then the results
-    const int tile = warp % ROW_TILES, kg = warp / ROW_TILES;
-    const int w0 = (int)((int64_t)kg * mine / K_GROUPS), w1 = (int)((int64_t)(kg + 1) * mine / K_GROUPS);
+    float *const part = sums + most * TOKENS;                                // [token][row]
 
     // the first codes are on their way while x is brought
     uint32_t code[AHEAD][2][WORDS];
-    const int64_t row_lo = row0 + tile * 16 + g, row_hi = row_lo + 8;
+    const int64_t row_lo = row0 + warp * 16 + g, row_hi = row_lo + 8;
     const auto fetch = [&](int slot, int block) {
         const int64_t k = (b_first + block) * KB + t * (KB / 4);
-        const bool inside = block < w1 && k < a.n;  // n is a multiple of 32: a lane's columns are all inside or, 64 of 128 (or 32 of 64), checked by word
+        const bool inside = block < mine && k < a.n;  // n is a multiple of 32: a lane's columns are all inside or, 64 of 128 (or 32 of 64), checked by word
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int64_t row = h ? row_hi : row_lo;
@@ -69,7 +69,7 @@ __global__ void __launch_bounds__(ROWS_THREADS, 2) linear_rows_kernel(const Line
         }
     };
 #pragma unroll
-    for (int s = 0; s < AHEAD; ++s) fetch(s, w0 + s);
+    for (int s = 0; s < AHEAD; ++s) fetch(s, s);
 
     // ---- x: a thread takes eight columns of a token; the CHUNKS threads of a block and token stand together and add up its sum ----
     constexpr int TOGETHER = 4;  // loads of a thread on their way at once
@@ -119,11 +119,11 @@ __global__ void __launch_bounds__(ROWS_THREADS, 2) linear_rows_kernel(const Line
     const bool single = a.group >= a.n;
     const float *const scale_lo = a.scale + min(row_lo, a.m - 1) * a.scale_row, *const scale_hi = a.scale + min(row_hi, a.m - 1) * a.scale_row;
     const float *const zero_lo = a.zero + min(row_lo, a.m - 1) * a.zero_row, *const zero_hi = a.zero + min(row_hi, a.m - 1) * a.zero_row;
-    int block = w0;
-    while (block < w1) {
+    int block = 0;
+    while (block < mine) {
         // a run of blocks under one scale
         const int64_t group = single ? 0 : (b_first + block) / per_group;
-        const int end = single ? w1 : (int)min((int64_t)w1, (group + 1) * per_group - b_first);
+        const int end = single ? mine : (int)min((int64_t)mine, (group + 1) * per_group - b_first);
         const float s_lo = __ldg(scale_lo + group * a.scale_group), s_hi = __ldg(scale_hi + group * a.scale_group);
         const float o_lo = a.qmin - __ldg(zero_lo + group * a.zero_group), o_hi = a.qmin - __ldg(zero_hi + group * a.zero_group);
         float low[NT][4], high[NT][4], xsum[NT][2];
@@ -135,7 +135,7 @@ __global__ void __launch_bounds__(ROWS_THREADS, 2) linear_rows_kernel(const Line
 #pragma unroll
             for (int s = 0; s < AHEAD; ++s) {
                 // the slots go round with the blocks of the whole share, not of the run
-                if (((block - w0) & (AHEAD - 1)) != s || block >= end) continue;
+                if ((block & (AHEAD - 1)) != s || block >= end) continue;
                 const uint4 *const xb = xs + (int64_t)block * WORDS * NT * 32 + lane;
                 uint32_t lo[WORDS], hi[WORDS];
 #pragma unroll
@@ -169,21 +169,12 @@ __global__ void __launch_bounds__(ROWS_THREADS, 2) linear_rows_kernel(const Line
             }
         }
     }
-    // ---- sums of the warps, then of the cluster ----
+    // ---- sums of the cluster ----
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
-        for (int x = 0; x < 4; ++x) part[(kg * TOKENS + 8 * j + 2 * t + (x & 1)) * ROWS + tile * 16 + 8 * (x >> 1) + g] = total[j][x];
+        for (int x = 0; x < 4; ++x) part[(8 * j + 2 * t + (x & 1)) * ROWS + warp * 16 + 8 * (x >> 1) + g] = total[j][x];
     __syncthreads();
-    if (K_GROUPS > 1) {
-        for (int e = threadIdx.x; e < TOKENS * ROWS; e += ROWS_THREADS) {
-            float sum = part[e];
-#pragma unroll
-            for (int k = 1; k < K_GROUPS; ++k) sum += part[k * TOKENS * ROWS + e];
-            part[e] = sum;
-        }
-        __syncthreads();
-    }
     if (splits > 1) cluster_sync();
     if (a.rank) after_the_launch_before();
     // results: the cluster's CTAs share them, each a part of the rows and tokens; consecutive threads have consecutive rows
@@ -222,32 +213,30 @@ __global__ void __launch_bounds__(ROWS_THREADS, 2) linear_rows_kernel(const Line
     }
 }
 
-template <bool BF16, int NT, int KB, int ROW_TILES>
+template <bool BF16, int NT, int KB>
 static int launch_rows_kernel(const LinearArgs &a, cudaStream_t st) {
     static PerDeviceOnce configured;
-    constexpr int K_GROUPS = ROWS_WARPS / ROW_TILES, ROWS = 16 * ROW_TILES, TOKENS = 8 * NT;
+    constexpr int ROWS = 16 * ROWS_WARPS, TOKENS = 8 * NT;
     constexpr size_t MOST = 200 * 1024;
     const int64_t blocks = ceil_div(a.n, (int64_t)KB), rows = ceil_div(a.m, (int64_t)ROWS), tiles = ceil_div((int64_t)a.tokens, (int64_t)TOKENS);
     const auto bytes = [&](int64_t splits) {
         const int64_t most = ceil_div(blocks, splits);
-        return (size_t)(most * (KB * TOKENS * 2 + TOKENS * 4) + K_GROUPS * TOKENS * ROWS * 4);
+        return (size_t)(most * (KB * TOKENS * 2 + TOKENS * 4) + TOKENS * ROWS * 4);
     };
     // as many parts of the columns as two CTAs per SM take at once, of four blocks per warp at least; more where x would not fit
     int splits = 1;
-    while (splits < 8 && ((rows * tiles * splits * 2 <= 2 * 148 && blocks >= 2 * splits * K_GROUPS * 4) || bytes(splits) > 96 * 1024)) splits *= 2;
+    while (splits < 8 && ((rows * tiles * splits * 2 <= 2 * 148 && blocks >= 2 * splits * 4) || bytes(splits) > 96 * 1024)) splits *= 2;
     if (bytes(splits) > MOST) return G2D_ERR_TOO_LARGE;
     if (rows > 65535 || tiles > 65535) return G2D_ERR_TOO_LARGE;
-    if (configured.run([&] { return cudaFuncSetAttribute(linear_rows_kernel<BF16, NT, KB, ROW_TILES>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)MOST) == cudaSuccess; }) != G2D_OK)
+    if (configured.run([&] { return cudaFuncSetAttribute(linear_rows_kernel<BF16, NT, KB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)MOST) == cudaSuccess; }) != G2D_OK)
         return G2D_ERR_CUDA;
-    return launch_dependent(linear_rows_kernel<BF16, NT, KB, ROW_TILES>, dim3((unsigned)splits, (unsigned)rows, (unsigned)tiles), ROWS_THREADS, bytes(splits), splits, a.rank > 0, st, a);
+    return launch_dependent(linear_rows_kernel<BF16, NT, KB>, dim3((unsigned)splits, (unsigned)rows, (unsigned)tiles), ROWS_THREADS, bytes(splits), splits, a.rank > 0, st, a);
 }
 
 template <bool BF16, int NT>
 static int launch_rows_tokens(const LinearArgs &a, cudaStream_t st) {
     const bool odd = a.group < a.n && a.group % 128 != 0;
-    const bool small = a.m * a.n < (int64_t)148 * 2 * 128 * 1024;
-    if (odd) return small ? launch_rows_kernel<BF16, NT, 64, 4>(a, st) : launch_rows_kernel<BF16, NT, 64, 8>(a, st);
-    return small ? launch_rows_kernel<BF16, NT, 128, 4>(a, st) : launch_rows_kernel<BF16, NT, 128, 8>(a, st);
+    return odd ? launch_rows_kernel<BF16, NT, 64>(a, st) : launch_rows_kernel<BF16, NT, 128>(a, st);
 }
 
 int launch_linear_rows(const LinearArgs &a, cudaStream_t st) {
@@ -259,7 +248,8 @@ int launch_linear_rows(const LinearArgs &a, cudaStream_t st) {
 
 using namespace g2d;
 
-// Up to here the tokens are columns of m16n8k16 products; both sides of the line: see the figures above.
+// Up to here the tokens are columns of m16n8k16 products.  28672 x 8192, no adapters: 16 tokens 68.3 us, by tiles 83.9; 24 tokens 117 (two tiles of 16), by tiles 83.8; 4096 x 4096: 16 tokens 8.7,
+// by tiles 16.5; 24 tokens 14.5, by tiles 16.8.
 constexpr int64_t ROWS_TOKENS = 16;
 
 struct LinearSpace {
@@ -274,7 +264,7 @@ static LinearSpace linear_space(const g2d_linear_desc *d) {
     if (d->rank > 0) {
         s.factor = at += whole((size_t)d->tokens * INNER_LD * 2);
         s.plan = at += whole((size_t)d->tokens * sizeof(float));
-        if (many) at += whole((size_t)p.token_tiles * (p.tile + 1) * sizeof(int));
+        if (d->tokens > LINEAR_FEW) at += whole((size_t)p.token_tiles * (p.tile + 1) * sizeof(int));
     }
     s.partial = at;
     if (many) at += whole(p.partial_bytes);
@@ -341,7 +331,7 @@ extern "C" int g2d_packed_linear(const g2d_linear_desc *d, void *stream) {
     cudaStream_t st = (cudaStream_t)stream;
     const bool many = a.tokens > ROWS_TOKENS;
     const LinearTcPlan p = many ? linear_tc_plan(a.m, a.n, a.tokens, a.rank) : LinearTcPlan{};
-    int *const plan = many && a.rank > 0 ? (int *)((char *)d->workspace + space.plan) : nullptr;
+    int *const plan = a.tokens > LINEAR_FEW && a.rank > 0 ? (int *)((char *)d->workspace + space.plan) : nullptr;
     if (a.rank > 0) {
         const int launched = launch_inner(a, plan, p.tile, st);
         if (launched != G2D_OK) return launched;

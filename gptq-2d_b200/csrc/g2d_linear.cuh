@@ -5,6 +5,7 @@
 namespace g2d {
 
 constexpr int RANK_MAX = 64;
+constexpr int LINEAR_FEW = 64;  // up to so many tokens each has its adapter for itself: no plan
 constexpr int INNER_LD = 2 * RANK_MAX;  // an inner row: 64 upper parts, 64 lower parts
 
 struct LinearArgs {
@@ -48,7 +49,7 @@ struct LinearTcPlan {
 };
 LinearTcPlan linear_tc_plan(int64_t m, int64_t n, int64_t tokens, int rank);
 
-// Inner values and factors of all tokens; where `plan` is given, also the adapters of each tile of `tile` tokens: plan[i * (tile + 1)] of them, their numbers behind it
+// Inner values and factors of all tokens; where they are more than LINEAR_FEW, also the adapters of each tile of `tile` tokens: plan[i * (tile + 1)] of them, their numbers behind it
 int launch_inner(const LinearArgs &a, int *plan, int tile, cudaStream_t st);
 int launch_linear_rows(const LinearArgs &a, cudaStream_t st);  // few tokens
 int launch_linear_tc(const LinearArgs &a, const LinearTcPlan &p, const int *plan, float *partial, cudaStream_t st);

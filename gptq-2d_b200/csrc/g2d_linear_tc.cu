@@ -14,7 +14,7 @@
 
 namespace g2d {
 
-constexpr int LT_OUTER_LATER = 64, LT_JOIN_TOKENS = 4;  // tiles of so many tokens have their adapters' outer halves added where the pieces are joined
+constexpr int LT_OUTER_LATER = LINEAR_FEW, LT_JOIN_TOKENS = 4;  // tiles of so many tokens have their adapters' outer halves added where the pieces are joined
 constexpr int LT_W_BYTES = 128 * 128, LT_CODE_BYTES = 128 * 32, LT_SLICE = 8;
 
 // DUO: a pair of CTAs on 256 rows x NT tokens (cta_group::2), each with its rows of W and half of the tokens' rows of x.
@@ -520,8 +520,10 @@ __global__ void __launch_bounds__(LinearShape<NT, DUO>::THREADS, 1) linear_tc_ke
 }
 
 // The tiles that were cut: sums of their pieces, in their order, and (tiles of LT_OUTER_LATER tokens) the outer halves of the adapters.  A thread has a row and LT_JOIN_TOKENS tokens.
+template <bool STAGED>
 __global__ void __launch_bounds__(128) linear_join_kernel(const LinearArgs a, const LinearTcPlan p, const float *__restrict__ partial, int grid_ctas) {
     __shared__ float4 inner[LT_JOIN_TOKENS][RANK_MAX / 4];
+    __shared__ uint4 up_rows[STAGED ? 128 * (RANK_MAX / 8 + 1) : 1];
     const int rows = p.duo ? 256 : 128, parts = rows / 128;
     const int64_t shared = blockIdx.x / parts, tile = (int64_t)p.whole * grid_ctas + shared;
     const int in_tile = blockIdx.y * LT_JOIN_TOKENS;
@@ -540,26 +542,52 @@ __global__ void __launch_bounds__(128) linear_join_kernel(const LinearArgs a, co
         }
         __syncthreads();
     }
-    if (row >= a.m) return;
     const int count = (int)min((int64_t)LT_JOIN_TOKENS, a.tokens - token0);
+    // The CTA's rows of a token's `up` are one piece of memory: they come as that, through shared memory, the next token's under way while one's are used.  (32 tokens, 40 adapters of rank 64,
+    // 4096 rows: 14 us; each thread its own row, 16 bytes after the others: 78, as the first-level cache is small beside the products' shared memory.)  Rows of 16 bytes are read
+    // as well as they lie (61 tokens, rank 8, 14333 rows, the whole call: 41.0 us, through shared memory 43.7).
+    const int words = a.rank / 8, pitch = words | 1, per_row = words > 0 ? (65535 + words) / words : 0;  // x / words = x per_row >> 16 for x up to 1024
+    uint4 next[RANK_MAX / 8];
+    const auto fetch = [&](int e) {
+        if (e >= count || id[e] < 0) return;
+        const int64_t first = row - threadIdx.x;
+        const uint4 *const up = reinterpret_cast<const uint4 *>((const uint16_t *)a.up + ((int64_t)id[e] * a.m + first) * a.rank);
+        const int there = (int)min((int64_t)128, a.m - first) * words;
+#pragma unroll
+        for (int i = 0; i < RANK_MAX / 8; ++i)
+            if (i < words && i * 128 + (int)threadIdx.x < there) next[i] = __ldg(up + i * 128 + threadIdx.x);
+    };
+    if (STAGED) fetch(0);
     float sum[LT_JOIN_TOKENS];
 #pragma unroll
     for (int e = 0; e < LT_JOIN_TOKENS; ++e) sum[e] = 0.f;
-    const float *from = partial + (shared * p.tile + in_tile) * rows + row_in_tile;
+    if (row < a.m) {
+        const float *from = partial + (shared * p.tile + in_tile) * rows + row_in_tile;
 #pragma unroll 2
-    for (int k = 0; k < pieces; ++k, from += p.shared * p.tile * rows) {
+        for (int k = 0; k < pieces; ++k, from += p.shared * p.tile * rows) {
 #pragma unroll
-        for (int e = 0; e < LT_JOIN_TOKENS; ++e)
-            if (e < count) sum[e] += from[e * rows];
+            for (int e = 0; e < LT_JOIN_TOKENS; ++e)
+                if (e < count) sum[e] += from[e * rows];
+        }
     }
 #pragma unroll
     for (int e = 0; e < LT_JOIN_TOKENS; ++e) {
         if (e >= count) break;
-        if (id[e] >= 0) {
+        if (STAGED && id[e] >= 0) {
+            __syncthreads();  // the rows before have been read
+#pragma unroll
+            for (int i = 0; i < RANK_MAX / 8; ++i) {
+                const int x = i * 128 + (int)threadIdx.x, r = x * per_row >> 16;
+                if (i < words) up_rows[r * pitch + x - r * words] = next[i];
+            }
+            __syncthreads();
+        }
+        if (STAGED && e + 1 < LT_JOIN_TOKENS) fetch(e + 1);
+        if (id[e] >= 0 && row < a.m) {
             const uint4 *const up = reinterpret_cast<const uint4 *>((const uint16_t *)a.up + ((int64_t)id[e] * a.m + row) * a.rank);
             float more = 0.f;
-            for (int r = 0; r < a.rank / 8; ++r) {
-                const uint4 v = __ldg(up + r);
+            for (int r = 0; r < words; ++r) {
+                const uint4 v = STAGED ? up_rows[threadIdx.x * pitch + r] : __ldg(up + r);
                 const uint32_t w[4] = {v.x, v.y, v.z, v.w};
                 const float4 h[2] = {inner[e][2 * r], inner[e][2 * r + 1]};
                 const float hh[8] = {h[0].x, h[0].y, h[0].z, h[0].w, h[1].x, h[1].y, h[1].z, h[1].w};
@@ -571,7 +599,7 @@ __global__ void __launch_bounds__(128) linear_join_kernel(const LinearArgs a, co
             }
             sum[e] = fmaf(more, a.factor[token0 + e], sum[e]);
         }
-        ((uint16_t *)a.out)[(token0 + e) * a.out_stride + row] = (uint16_t)float_to_bits(sum[e], a.bf16);
+        if (row < a.m) ((uint16_t *)a.out)[(token0 + e) * a.out_stride + row] = (uint16_t)float_to_bits(sum[e], a.bf16);
     }
 }
 
@@ -600,12 +628,13 @@ static bool make_map_up(CUtensorMap *map, const LinearArgs &a) {
 
 LinearTcPlan linear_tc_plan(int64_t m, int64_t n, int64_t tokens, int rank) {
     LinearTcPlan p;
-    p.tile = tokens <= 64 ? 64 : 128;
+    p.tile = tokens <= LINEAR_FEW ? LINEAR_FEW : 128;
     p.duo = 0;
     int64_t rows = ceil_div(m, (int64_t)128), columns = ceil_div(tokens, (int64_t)p.tile);
-    // 256 x 256 by pairs of CTAs where they fill the GPU as well: four times the work of a 128 x 128 tile in 1.6 times its time
+    // 256 x 256 by pairs of CTAs, four times the work of a 128 x 128 tile in 1.6 times its time, unless a pair's share is too short for what each tile costs besides.  4096 x 4096: 256 tokens
+    // (14 chunks a pair) 36.8 us by 128 x 128, 39.0 by pairs; 512 tokens (28) 53.5, 49.8; 8192 x 8192, 129 tokens (55) 73.3, 59.6; 28672 x 4096, 1024 tokens 402, 261
     const int64_t pairs = ceil_div(m, (int64_t)256) * ceil_div(tokens, (int64_t)256);
-    if (p.tile == 128 && 8 * ceil_div(pairs, (int64_t)74) <= 5 * ceil_div(rows * columns, (int64_t)148)) {
+    if (tokens > 128 && pairs * ceil_div(n, (int64_t)KH) >= 74 * 20) {
         p.tile = 256;
         p.duo = 1;
         rows = ceil_div(m, (int64_t)256);
@@ -645,7 +674,8 @@ static int launch_tc(const LinearArgs &a, const LinearTcPlan &p, const int *plan
     const int64_t ctas = p.whole > 0 ? (DUO ? 74 : 148) : p.ctas;
     const int launched = launch_dependent(linear_tc_kernel<BF16, NT, DUO>, dim3((unsigned)(DUO ? 2 * ctas : ctas)), S::THREADS, S::SMEM, DUO ? 2 : 1, a.rank > 0, st, job);
     if (launched != G2D_OK || p.shared == 0) return launched;
-    return launch_dependent(linear_join_kernel, dim3((unsigned)p.shared * (DUO ? 2 : 1), NT / LT_JOIN_TOKENS), 128, 0, 1, true, st, a, p, partial, (int)ctas);
+    const auto join = NT == LT_OUTER_LATER && a.rank > 8 ? linear_join_kernel<true> : linear_join_kernel<false>;
+    return launch_dependent(join, dim3((unsigned)p.shared * (DUO ? 2 : 1), NT / LT_JOIN_TOKENS), 128, 0, 1, true, st, a, p, partial, (int)ctas);
 }
 
 int launch_linear_tc(const LinearArgs &a, const LinearTcPlan &p, const int *plan, float *partial, cudaStream_t st) {
