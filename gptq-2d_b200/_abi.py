@@ -102,7 +102,7 @@ class AttendDesc(ctypes.Structure):
 # Descriptors of the calls of a serving step, which are as short as the host code around them: packed in one go instead of field by field (2 us less
 # for thirty fields).  Native alignment, so the formats follow the header's fields in order.
 CACHE_DESC = struct.Struct("@4i5q7P")  # g2d_cache_desc
-ATTEND_DESC = struct.Struct("@4i5q7P" "2i2fP2q3PPNP")  # g2d_attend_desc
+ATTEND_DESC = struct.Struct("@4i5q7P" "2i2f2iP2q3PPNP")  # g2d_attend_desc
 LINEAR_DESC = struct.Struct("@2i3qPqP2qP2qP2qdq2i4PPqPNP")  # g2d_linear_desc
 
 

@@ -139,6 +139,7 @@ __global__ void __launch_bounds__(AttendShape<D, NT>::THREADS, 1) attend_rows_ke
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     let_the_next_launch_start();
+    if (threadIdx.x == 0) a.joins[blockIdx.x] = AttendJoin{};
     if (lane < 2) sh.parts[2 * warp + lane].last = 0;
     const auto units_of = [&](int b) { return attend_units<ROWS>(a, b); };
     unsigned mine_units;
@@ -592,6 +593,10 @@ __global__ void __launch_bounds__(AttendShape<D, NT>::THREADS, 1) attend_rows_ke
         const int first = begin.first, last = sh.parts[p1].last;
         const bool whole = first == 0 && last == begin.blocks;
         const int head = begin.item % c.kv_heads, row0 = begin.item / c.kv_heads * ROWS, rows = begin.s.count * a.group;
+        if (threadIdx.x == 0 && first == 0 && !whole) {  // it goes on in the next share
+            const unsigned behind = shares.begin(share + 1) - last + begin.blocks;
+            a.joins[share] = AttendJoin{(int)(shares.of(behind - 1) - share) + 1, row0, rows, begin.s.first, head, {}};
+        }
         // the parts of an item but its first are the first ones of the warps that follow
         const float *const from = attend_slot<D, ROWS>(a, WARP_SLOTS + 2 * ATTEND_WARPS * (int64_t)share + p0), *const next = attend_slot<D, ROWS>(a, WARP_SLOTS + 2 * ATTEND_WARPS * (int64_t)share + (p0 & ~1));
         for (int i = warp; i < ROWS && row0 + i < rows; i += ATTEND_WARPS) {
@@ -612,11 +617,11 @@ __global__ void __launch_bounds__(AttendShape<D, NT>::THREADS, 1) attend_rows_ke
             }
         }
     }
-    after_the_launch_before();  // of the tiles' kernel: what follows waits for this one alone
+    after_the_launch_before();  // of the tiles' kernel, where that is the first: what follows waits for this one alone
 }
 
 // Adds up what items that lie in several CTAs' shares left, in the order of the keys.  A CTA per share and (tiles) 32 rows or (rows) all rows of an item: the one whose
-// share an item begins in and does not end in.
+// share an item begins in and does not end in, as that share's kernel has noted.
 constexpr int JOIN_THREADS = 256, TILE_JOINS = TA_ROWS / 32;
 struct JoinArgs {
     AttendArgs tiles, rows;
@@ -625,101 +630,54 @@ struct JoinArgs {
 template <int D, int NT>
 __global__ void __launch_bounds__(JOIN_THREADS) attend_join_kernel(const JoinArgs j) {
     constexpr int ROWS = 8 * NT, WARPS = JOIN_THREADS / 32;
-    __shared__ unsigned totals[WARPS];
     const int warp = threadIdx.x >> 5;
-    unsigned mine, u0 = 0, u1 = 0, end = 0;
-    if ((int)blockIdx.x < j.tile_ctas) {
-        const AttendArgs &a = j.tiles;
-        const AttendShares shares(count_tile_units<WARPS>(a, totals, mine), TA_GRID);
-        const unsigned share = blockIdx.x / TILE_JOINS;
-        TileCursor cur;
-        if (share + 1 < shares.count) {
-            end = shares.begin(share + 1);
-            cur.find(a, mine, end - 1);
-            u0 = end - 1 - cur.block;
-            u1 = u0 + cur.blocks;
-        }
-        after_the_launch_before();  // by every CTA: what follows on the stream must not start before the results are there
-        if (u1 <= end || u0 < shares.begin(share)) return;
-        const int count = (int)(shares.of(u1 - 1) - share) + 1;
-        constexpr int SLOT = TA_ROWS * (D + 2);
-        const float *const from = tile_slot<D>(a, 2 * share + 1), *const next = tile_slot<D>(a, 2 * share);
-        for (int i = blockIdx.x % TILE_JOINS * 32 + warp, n = 0; n < 32 / WARPS; ++n, i += WARPS) {
-            const int r = cur.pair * TA_ROWS + i;
-            if (r >= cur.s.count * a.group) break;
-            float acc[D / 32], m, l;
-            const auto row = [&](int k) { return (k == 0 ? from : next + (int64_t)k * (2 * SLOT)) + i * D; };
-            merge_parts<D>(count, row, TA_ROWS * D + i - i * D, TA_ROWS * D + TA_ROWS + i - i * D, acc, m, l);
-            write_row<D>((uint16_t *)a.out + ((int64_t)(cur.s.first + r / a.group) * a.heads + cur.head * a.group + r % a.group) * D, acc, l, a.c.bf16);
-        }
-    } else {
-        const AttendArgs &a = j.rows;
-        const auto units_of = [&](int b) { return attend_units<ROWS>(a, b); };
-        const AttendShares shares(count_units<WARPS>(a.c.batch, units_of, totals, mine), ATTEND_GRID);
-        const unsigned share = blockIdx.x - j.tile_ctas;
-        AttendCursor cur;
-        if (share + 1 < shares.count) {
-            unsigned before;
-            end = shares.begin(share + 1);
-            cur.u = 0;
-            cur.end = 1;
-            cur.b = sequence_of_unit(a.c.batch, units_of, mine, end - 1, before);
-            cur.template open<ROWS>(a);
-            cur.item = (int)((end - 1 - before) / cur.blocks);
-            u0 = before + (unsigned)cur.item * cur.blocks;
-            u1 = u0 + cur.blocks;
-        }
-        after_the_launch_before();
-        if (u1 <= end || u0 < shares.begin(share)) return;
-        const int count = (int)(shares.of(u1 - 1) - share) + 1;
-        constexpr int SLOT = ROWS * (D + 2);
-        const float *const from = attend_slot<D, ROWS>(a, 2 * share + 1), *const next = attend_slot<D, ROWS>(a, 2 * share);
-        for (int i = warp; i < ROWS; i += WARPS) {
-            const int r = cur.item / a.c.kv_heads * ROWS + i;
-            if (r >= cur.s.count * a.group) break;
-            float acc[D / 32], m, l;
-            const auto row = [&](int k) { return (k == 0 ? from : next + (int64_t)k * (2 * SLOT)) + i * D; };
-            merge_parts<D>(count, row, ROWS * D + i - i * D, ROWS * D + ROWS + i - i * D, acc, m, l);
-            write_row<D>((uint16_t *)a.out + ((int64_t)(cur.s.first + r / a.group) * a.heads + cur.item % a.c.kv_heads * a.group + r % a.group) * D, acc, l, a.c.bf16);
+    const bool of_tiles = (int)blockIdx.x < j.tile_ctas;
+    const AttendArgs &a = of_tiles ? j.tiles : j.rows;
+    if (a.clear) {
+        const int row = a.heads * D / 8;  // of 16 bytes
+        for (int64_t token = blockIdx.x * JOIN_THREADS + threadIdx.x; token < a.c.tokens; token += gridDim.x * JOIN_THREADS) {
+            int first, count;
+            if (sequence_of(a.c, (int)token, first, count) >= 0) continue;
+            for (int i = 0; i < row; ++i) reinterpret_cast<uint4 *>(a.out)[token * row + i] = make_uint4(0u, 0u, 0u, 0u);
         }
     }
-}
-
-// A launch on the stream behind the one before, as a programmatic dependent launch
-template <typename Args>
-static int launch_behind(void (*kernel)(Args), unsigned grid, int threads, size_t smem, const Args &args, cudaStream_t st) {
-    cudaLaunchConfig_t config{};
-    config.gridDim = dim3(grid);
-    config.blockDim = dim3((unsigned)threads);
-    config.dynamicSmemBytes = smem;
-    config.stream = st;
-    cudaLaunchAttribute attribute{};
-    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attribute.val.programmaticStreamSerializationAllowed = 1;
-    config.attrs = &attribute;
-    config.numAttrs = 1;
-    return cudaLaunchKernelEx(&config, kernel, args) == cudaSuccess ? check_launch() : G2D_ERR_CUDA;
+    after_the_launch_before();  // by every CTA: what follows on the stream must not start before the results are there
+    const int share = of_tiles ? blockIdx.x / TILE_JOINS : blockIdx.x - j.tile_ctas;
+    const AttendJoin join = a.joins[share];
+    if (join.count == 0) return;
+    const int rows = of_tiles ? TA_ROWS : ROWS, i0 = of_tiles ? blockIdx.x % TILE_JOINS * 32 : 0, i1 = min(of_tiles ? i0 + 32 : ROWS, join.rows - join.row0);
+    const int64_t slot = rows * (D + 2);
+    const float *const from = a.partial + (2 * share + 1) * slot, *const next = a.partial + 2 * share * slot;
+    for (int i = i0 + warp; i < i1; i += WARPS) {
+        float acc[D / 32], m, l;
+        const auto row = [&](int k) { return (k == 0 ? from : next + k * (2 * slot)) + i * D; };
+        merge_parts<D>(join.count, row, rows * D + i - i * D, rows * D + rows + i - i * D, acc, m, l);
+        const int r = join.row0 + i;
+        write_row<D>((uint16_t *)a.out + ((int64_t)(join.first + r / a.group) * a.heads + join.head * a.group + r % a.group) * D, acc, l, a.c.bf16);
+    }
 }
 
 // rows and tiles: either or both; both launches share the sequences out between them
 template <int D, int NT, bool MODS>
-static int launch_rows(const AttendArgs &a, bool behind_tiles, cudaStream_t st) {
+static int launch_rows(const AttendArgs &a, bool behind, cudaStream_t st) {
     static PerDeviceOnce configured;
     constexpr size_t smem = sizeof(AttendShared<D, NT>);
     if (configured.run([&] { return cudaFuncSetAttribute(attend_rows_kernel<D, NT, MODS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) == cudaSuccess; }) != G2D_OK)
         return G2D_ERR_CUDA;
-    if (behind_tiles) return launch_behind(attend_rows_kernel<D, NT, MODS>, ATTEND_GRID, AttendShape<D, NT>::THREADS, smem, a, st);
-    attend_rows_kernel<D, NT, MODS><<<ATTEND_GRID, AttendShape<D, NT>::THREADS, smem, st>>>(a);
-    return check_launch();
+    return launch_attention(attend_rows_kernel<D, NT, MODS>, ATTEND_GRID, AttendShape<D, NT>::THREADS, smem, behind, a, st);
 }
 template <int D, int NT>
-static int launch_attend(const AttendArgs &rows, const AttendArgs &tiles, bool few, bool many, cudaStream_t st) {
-    int launched = G2D_OK;
-    if (many) launched = launch_attend_tiles(tiles, st);
-    if (launched == G2D_OK && few) launched = rows.softcap > 0.f || rows.slopes ? launch_rows<D, NT, true>(rows, many, st) : launch_rows<D, NT, false>(rows, many, st);
+static int launch_attend(const AttendArgs &rows, const AttendArgs &tiles, bool few, bool many, bool rows_first, cudaStream_t st) {
+    const auto launch_few = [&](bool behind) -> int {
+        if (!few) return G2D_OK;
+        return rows.softcap > 0.f || rows.slopes ? launch_rows<D, NT, true>(rows, behind, st) : launch_rows<D, NT, false>(rows, behind, st);
+    };
+    int launched = rows_first ? launch_few(false) : G2D_OK;
+    if (launched == G2D_OK && many) launched = launch_attend_tiles(tiles, rows_first && few, st);
+    if (launched == G2D_OK && !rows_first) launched = launch_few(many);
     if (launched != G2D_OK) return launched;
     const JoinArgs j{tiles, rows, many ? TA_GRID * TILE_JOINS : 0};
-    return launch_behind(attend_join_kernel<D, NT>, (unsigned)(j.tile_ctas + (few ? ATTEND_GRID : 0)), JOIN_THREADS, 0, j, st);
+    return launch_attention(attend_join_kernel<D, NT>, (unsigned)(j.tile_ctas + (few ? ATTEND_GRID : 0)), JOIN_THREADS, 0, true, j, st);
 }
 
 // From how many rows of a kv head on a sequence goes by tiles.  Tiles cost more to begin with, so few items (sequences and kv heads) cross the line later.
@@ -728,12 +686,13 @@ static int launch_attend(const AttendArgs &rows, const AttendArgs &tiles, bool f
 static int tile_rows_from(const CacheView &c) { return (int64_t)c.batch * c.kv_heads <= 64 ? 65 : 33; }
 
 struct AttendSpace {
-    size_t tiles, all;  // the warps' partial results first
+    size_t tiles, joins, all;  // the warps' partial results first
 };
 static AttendSpace attend_space(int head_dim) {
     AttendSpace s;
     s.tiles = ((size_t)ATTEND_GRID * (ATTEND_MOST_WARPS + 1) * 2 * 16 * (head_dim + 2) * sizeof(float) + 255) & ~(size_t)255;
-    s.all = s.tiles + attend_tiles_bytes(head_dim);
+    s.joins = (s.tiles + attend_tiles_bytes(head_dim) + 255) & ~(size_t)255;
+    s.all = s.joins + (TA_GRID + ATTEND_GRID) * sizeof(AttendJoin);
     return s;
 }
 
@@ -755,7 +714,7 @@ extern "C" int g2d_cache_attend(const g2d_attend_desc *d, void *stream) {
     if (!d) return G2D_ERR_BAD_ARGUMENT;
     const int status = cache_view(&d->cache, &a.c);
     if (status != G2D_OK) return status;
-    if (d->heads < 1 || d->heads % a.c.kv_heads != 0 || !(d->softcap >= 0.f)) return G2D_ERR_BAD_ARGUMENT;
+    if (d->heads < 1 || d->heads % a.c.kv_heads != 0 || !(d->softcap >= 0.f) || d->reserved != 0) return G2D_ERR_BAD_ARGUMENT;
     if (a.c.tokens == 0 || a.c.batch == 0) return G2D_OK;
     if ((int64_t)a.c.tokens * d->heads > 0x7fffffff) return G2D_ERR_TOO_LARGE;
     {  // units of 64 keys and eight rows: counted in 32 bits
@@ -775,6 +734,7 @@ extern "C" int g2d_cache_attend(const g2d_attend_desc *d, void *stream) {
     a.softcap = d->softcap;
     a.slopes = d->slopes;
     a.prefix = d->prefix;
+    a.clear = d->clear != 0 && a.c.offsets;
     a.status = d->status;
     a.wait_cycles = WAIT_CYCLES;
     cudaStream_t st = (cudaStream_t)stream;
@@ -785,11 +745,16 @@ extern "C" int g2d_cache_attend(const g2d_attend_desc *d, void *stream) {
     AttendArgs t = a;
     t.rows_from = line;
     t.rows_to = 0x7fffffff;
-    t.partial = (float *)((char *)d->workspace + attend_space(a.c.head_dim).tiles);
+    const AttendSpace space = attend_space(a.c.head_dim);
+    t.partial = (float *)((char *)d->workspace + space.tiles);
+    t.joins = (AttendJoin *)((char *)d->workspace + space.joins);
+    a.joins = t.joins + TA_GRID;
     a.rows_from = 1;
     a.rows_to = line;
     a.partial = (float *)d->workspace;
     const bool narrow = a.group <= 8 && (rows < 0 || rows <= 8);
-    if (a.c.head_dim == 128) return narrow ? launch_attend<128, 1>(a, t, few, many, st) : launch_attend<128, 2>(a, t, few, many, st);
-    return narrow ? launch_attend<64, 1>(a, t, few, many, st) : launch_attend<64, 2>(a, t, few, many, st);
+    // Of two kernels one has most of the work, as a rule: the one for the sequences' mean.  The other finds its part, or that it has none, while that one's last CTAs work
+    const bool rows_first = (int64_t)a.c.tokens * a.group < (int64_t)line * a.c.batch;
+    if (a.c.head_dim == 128) return narrow ? launch_attend<128, 1>(a, t, few, many, rows_first, st) : launch_attend<128, 2>(a, t, few, many, rows_first, st);
+    return narrow ? launch_attend<64, 1>(a, t, few, many, rows_first, st) : launch_attend<64, 2>(a, t, few, many, rows_first, st);
 }

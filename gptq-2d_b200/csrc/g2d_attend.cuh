@@ -8,6 +8,11 @@ namespace g2d {
 int cache_view(const g2d_cache_desc *d, CacheView *c);
 
 // ---- attention: what its kernels share ----
+// An item that begins in a share and does not end in it: what is to be added up, and for which rows.  Each share's kernel writes one; count 0: none.
+struct AttendJoin {
+    int count, row0, rows, first, head;  // parts; the first row and how many the sequence has, its first token, kv head
+    int reserved[3];
+};
 struct AttendArgs {
     CacheView c;
     const void *q;
@@ -21,6 +26,8 @@ struct AttendArgs {
     const int32_t *prefix;   // per sequence, or null
     int rows_from, rows_to;  // the kernel's sequences: those with rows_from <= queries x group < rows_to
     float *partial;
+    AttendJoin *joins;  // one per share
+    int clear;          // rows of no sequence become zeros
     int *status;
     long long wait_cycles;
 };
@@ -264,6 +271,22 @@ __device__ __forceinline__ float *tile_slot(const AttendArgs &a, int64_t slot) {
     return a.partial + slot * (TA_ROWS * (D + 2));
 }
 size_t attend_tiles_bytes(int head_dim);
-int launch_attend_tiles(const AttendArgs &a, cudaStream_t st);
+int launch_attend_tiles(const AttendArgs &a, bool behind, cudaStream_t st);
+
+// A launch; `behind`: as a programmatic dependent launch behind the one before on the stream
+template <typename Args>
+inline int launch_attention(void (*kernel)(Args), unsigned grid, int threads, size_t smem, bool behind, const Args &args, cudaStream_t st) {
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(grid);
+    config.blockDim = dim3((unsigned)threads);
+    config.dynamicSmemBytes = smem;
+    config.stream = st;
+    cudaLaunchAttribute attribute{};
+    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &attribute;
+    config.numAttrs = behind ? 1 : 0;
+    return cudaLaunchKernelEx(&config, kernel, args) == cudaSuccess ? check_launch() : G2D_ERR_CUDA;
+}
 
 }  // namespace g2d

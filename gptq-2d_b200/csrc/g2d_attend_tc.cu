@@ -137,7 +137,11 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const __gri
     let_the_next_launch_start();
     unsigned mine_units;
     const unsigned units = count_tile_units<TA_THREADS / 32>(a, bar.totals, mine_units);
-    if (units == 0) return;                                                // sequences of few rows only
+    if (threadIdx.x == 0) a.joins[blockIdx.x] = AttendJoin{};
+    if (units == 0) {  // sequences of few rows only
+        after_the_launch_before();
+        return;
+    }
     if (warp == 1) tmem_alloc<false>(&bar.tmem, 512);
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
@@ -164,10 +168,19 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const __gri
                 cur.end = shares.begin(share + 1);
             }
             if (lane == 0) {
+                AttendJoin join{};
                 for (uint32_t number = 0;; ++number) {
                     if (number >= TA_RUNS && (bar.failed || !wait(&bar.run_empty[number % TA_RUNS], (number / TA_RUNS - 1) & 1, 32))) break;
                     TileRun &r = bar.runs[number % TA_RUNS];
                     r.n = cur.u < cur.end ? cur.run() : 0;
+                    if (r.n > 0 && cur.block == 0 && r.n < cur.blocks) {
+                        join.count = (int)(shares.of(cur.u + cur.blocks - 1) - share) + 1;
+                        join.row0 = cur.pair * TA_ROWS;
+                        join.rows = cur.s.count * a.group;
+                        join.first = cur.s.first;
+                        join.head = cur.head;
+                        a.joins[share] = join;
+                    }
                     r.s = cur.s;
                     r.b = cur.b;
                     r.pair = cur.pair;
@@ -702,6 +715,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const __gri
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    after_the_launch_before();  // of the rows' kernel, where that is the first: what follows waits for this one alone
     if (warp == 1) tmem_free<false>(tmem, 512);
     if (threadIdx.x == 0 && bar.failed && a.status) atomicExch(a.status, -1);
 }
@@ -709,7 +723,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const __gri
 size_t attend_tiles_bytes(int head_dim) { return (size_t)TA_GRID * 2 * TA_ROWS * (head_dim + 2) * sizeof(float); }
 
 template <int D, bool BF16, bool MODS>
-static int launch_tiles(const AttendArgs &a, cudaStream_t st) {
+static int launch_tiles(const AttendArgs &a, bool behind, cudaStream_t st) {
     static PerDeviceOnce configured;
     constexpr size_t smem = TileShared<D>::BYTES;
     if (configured.run([&] { return cudaFuncSetAttribute(attend_tiles_kernel<D, BF16, MODS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) == cudaSuccess; }) != G2D_OK) return G2D_ERR_CUDA;
@@ -726,18 +740,17 @@ static int launch_tiles(const AttendArgs &a, cudaStream_t st) {
         job.by_tma = fn(&job.q, BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void *>(a.q), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
     }
-    attend_tiles_kernel<D, BF16, MODS><<<TA_GRID, TA_THREADS, smem, st>>>(job);
-    return check_launch();
+    return launch_attention(attend_tiles_kernel<D, BF16, MODS>, TA_GRID, TA_THREADS, smem, behind, job, st);
 }
 
-int launch_attend_tiles(const AttendArgs &a, cudaStream_t st) {
+int launch_attend_tiles(const AttendArgs &a, bool behind, cudaStream_t st) {
     const bool mods = a.softcap > 0.f || a.slopes;
     if (a.c.head_dim == 128) {
-        if (a.c.bf16) return mods ? launch_tiles<128, true, true>(a, st) : launch_tiles<128, true, false>(a, st);
-        return mods ? launch_tiles<128, false, true>(a, st) : launch_tiles<128, false, false>(a, st);
+        if (a.c.bf16) return mods ? launch_tiles<128, true, true>(a, behind, st) : launch_tiles<128, true, false>(a, behind, st);
+        return mods ? launch_tiles<128, false, true>(a, behind, st) : launch_tiles<128, false, false>(a, behind, st);
     }
-    if (a.c.bf16) return mods ? launch_tiles<64, true, true>(a, st) : launch_tiles<64, true, false>(a, st);
-    return mods ? launch_tiles<64, false, true>(a, st) : launch_tiles<64, false, false>(a, st);
+    if (a.c.bf16) return mods ? launch_tiles<64, true, true>(a, behind, st) : launch_tiles<64, true, false>(a, behind, st);
+    return mods ? launch_tiles<64, false, true>(a, behind, st) : launch_tiles<64, false, false>(a, behind, st);
 }
 
 }  // namespace g2d

@@ -117,7 +117,6 @@ __global__ void __launch_bounds__(CACHE_THREADS) cache_read_kernel(const CacheVi
     CachePlace place;
     for (int token = t0; token < t1; ++token) {
         const int64_t at = place.of(c, token);
-        if (place.b < 0) continue;  // a row of no sequence stays as it is
         {
             uint32_t codes[BATCH];
             float scale[BATCH];
@@ -125,7 +124,7 @@ __global__ void __launch_bounds__(CACHE_THREADS) cache_read_kernel(const CacheVi
             for (int n = 0; n < BATCH; ++n) {
                 const int r = r0 + n * ROWS + sub;
                 const int64_t row = at + ((int64_t)(r >> 1) << c.page_shift);
-                codes[n] = 0x88888888u;  // a position that the cache does not hold reads as zeros
+                codes[n] = 0x88888888u;  // a row of no sequence and a position that the cache does not hold read as zeros
                 scale[n] = 0.f;
                 if (at >= 0 && r < rows) {
                     codes[n] = reinterpret_cast<const uint32_t *>((r & 1 ? c.v_codes : c.k_codes) + row * (LANES * 4))[part];

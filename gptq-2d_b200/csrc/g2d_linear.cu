@@ -273,7 +273,7 @@ static LinearSpace linear_space(const g2d_linear_desc *d) {
 }
 
 static int linear_check(const g2d_linear_desc *d) {
-    if (!d || (d->half != G2D_FP16 && d->half != G2D_BF16) || d->m < 0 || d->n < 0 || d->tokens < 0 || d->groups < 1 || d->rank < 0 || d->adapters < 0) return G2D_ERR_BAD_ARGUMENT;
+    if (!d || (d->half != G2D_FP16 && d->half != G2D_BF16) || d->m < 0 || d->n < 0 || d->tokens < 0 || d->groups < 1 || d->rank < 0 || d->adapters < 0 || d->reserved != 0) return G2D_ERR_BAD_ARGUMENT;
     if (d->bits != 4 || d->n % 32 != 0 || d->row_bytes % 16 != 0 || d->rank % 8 != 0 || d->rank > RANK_MAX) return G2D_ERR_UNSUPPORTED;
     if (d->row_bytes < d->n / 2) return G2D_ERR_BAD_ARGUMENT;
     if (d->groups > 1 && (d->n % d->groups != 0 || d->n / d->groups % 64 != 0)) return G2D_ERR_UNSUPPORTED;

@@ -116,8 +116,8 @@ def read_packed(cache: PackedCache, page_table: torch.Tensor, lengths: torch.Ten
     """The keys and values ``[tokens, kv_heads, head_dim]`` that the cache holds for the last tokens of every sequence, ``offsets`` saying how many (all of them, where
     they add up to ``lengths``).  Rows of no sequence, and positions that the cache does not hold, are zeros."""
     device, fields = _cache_fields(cache, dtype, tokens, page_table, lengths, offsets)
-    k = (torch.empty if offsets is None else torch.zeros)((tokens, fields[3], fields[1]), dtype=dtype, device=device)
-    v = (torch.empty_like if offsets is None else torch.zeros_like)(k)
+    k = (torch.empty if fields[5] else torch.zeros)((tokens, fields[3], fields[1]), dtype=dtype, device=device)
+    v = (torch.empty_like if fields[5] else torch.zeros_like)(k)
     index = device.index
     with _abi.on_device(index):
         status = _abi.library().g2d_cache_read(_abi.CACHE_DESC.pack(*fields), k.data_ptr(), v.data_ptr(), _abi.raw_stream(index))
@@ -154,14 +154,15 @@ def attend_packed(q: torch.Tensor, cache: PackedCache, page_table: torch.Tensor,
     if prefix is not None:
         assert prefix.shape == lengths.shape and prefix.dtype == torch.int32 and prefix.get_device() == device.index and prefix.is_contiguous(), "expected a contiguous int32 prefix [batch] on the cache's device"
         prefix_at = prefix.data_ptr()
-    if out is None:
-        out = (torch.empty_like if offsets is None else torch.zeros_like)(q, memory_format=torch.contiguous_format)
+    clear = out is None
+    if clear:
+        out = (torch.empty_like if fields[5] else torch.zeros_like)(q, memory_format=torch.contiguous_format)
     else:
         assert out.shape == q.shape and out.dtype == dtype and out.get_device() == device.index and out.is_contiguous() and out.data_ptr() % 16 == 0, "out must be a contiguous, 16-byte aligned tensor like q"
     if tokens == 0:
         return out
     lib, index = _abi.library(), device.index
-    fields = (*fields, heads, bool(causal), scale, float(softcap), q.data_ptr(), *q.stride()[:2], out.data_ptr(), slopes_at, prefix_at)
+    fields = (*fields, heads, bool(causal), scale, float(softcap), clear, 0, q.data_ptr(), *q.stride()[:2], out.data_ptr(), slopes_at, prefix_at)
     need = _WORKSPACE.get(head_dim)
     if need is None:
         size = ctypes.c_size_t()

@@ -341,7 +341,7 @@ typedef struct g2d_cache_desc {
  * table sends to the same place leave codes and scale of either there. */
 int g2d_cache_append(const g2d_cache_desc *desc, const void *k, int64_t k_token_stride, int64_t k_head_stride, const void *v,
                      int64_t v_token_stride, int64_t v_head_stride, void *stream);
-/* What the cache holds for the step's tokens, as values: k and v [tokens, kv_heads, head_dim]. */
+/* What the cache holds for the step's tokens, as values: k and v [tokens, kv_heads, head_dim]; zeros for tokens of no sequence and positions that the cache does not hold. */
 int g2d_cache_read(const g2d_cache_desc *desc, void *k, void *v, void *stream);
 
 /* Attention of the step's tokens over the cache.  Token i of a sequence with n tokens in the step stands at p = length - n + i; query head h reads kv
@@ -351,6 +351,7 @@ typedef struct g2d_attend_desc {
     g2d_cache_desc cache;
     int32_t heads, causal;
     float scale, softcap;
+    int32_t clear, reserved;     /* clear: rows of out that belong to no sequence become zeros, else they stay as they are; reserved must be 0 */
     const void *q;               /* element strides below, multiples of 8; 16-byte aligned */
     int64_t q_token_stride, q_head_stride;
     void *out;                   /* [tokens, heads, head_dim], 16-byte aligned */
