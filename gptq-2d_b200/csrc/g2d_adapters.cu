@@ -1,6 +1,6 @@
 // The inner halves of low-rank adapters: h_t = down[i_t] x_t for every token t and its adapter i_t.
 //
-// The outer halves, up[i_t] h_t, are added inside the product with the packed codes, while its sums are still in fp32; for the tensor cores h travels as a pair of
+// The outer halves, up[i_t] h_t, are added inside the product with the packed codes, or where its pieces are joined, while its sums are still in fp32; for the tensor cores h travels as a pair of
 // 16-bit values hi + lo in the type of the activations under a power of two per token (22 bits for fp16, 16 for bf16: nothing that a 16-bit result
 // shows), the power and the adapter's scaling as one factor per token.
 //

@@ -60,8 +60,14 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// cap tanh(u / cap) through one exponential, from x = 2 log2(e) u / cap: exact to 1e-7 of the cap, which is what a score's exponential sees
-__device__ __forceinline__ float capped(float x, float cap) {
+// cap tanh(u / cap) through one exponential, from x = 2 log2(e) u / cap: good to 1e-7 of the cap, which is what a score's exponential sees of a cap up to CAP_NEAR.  Larger caps: tanh's
+// series where |u / cap| < 1/4 (relative error 1e-8), so that a cap far above the scores leaves them what they are.
+constexpr float CAP_NEAR = 64.f;
+__device__ __forceinline__ float capped(float x, float cap, bool near) {
+    if (!near) {
+        const float y = x * 0.34657359f, z = y * y;  // ln(2) / 2
+        if (fabsf(y) < 0.25f) return cap * (y * fmaf(fmaf(fmaf(fmaf(62.f / 2835.f, z, -17.f / 315.f), z, 2.f / 15.f), z, -1.f / 3.f), z, 1.f));
+    }
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + ex2(x)));
     return fmaf(-2.f * cap, r, cap);

@@ -2,7 +2,7 @@
 //
 // An item is 256 rows (token, head of the group) of one kv head: two tiles of 128 rows that share every block of 128 keys.  A unit is one block of one item; the units
 // of all items, one after the other, are dealt out evenly to the CTAs, whatever the lengths; an item that lies in one CTA's share is written at once, the others
-// leave partial results (two per CTA at most) that attend_tiles_join_kernel adds up in the order of the keys.
+// leave partial results (two per CTA at most) that attend_join_kernel adds up in the order of the keys.
 //
 // A CTA: four warps turn codes of keys into an operand, code - 8 in the type of the queries, exactly, keys as rows; four others codes of values, code - 8 in fp16, channels as
 // rows (two keys' words interleaved by a byte permutation).  One thread issues the products S = Q K^T and O += P V, S in tensor memory (128 columns a tile), P as fp16 over
@@ -12,7 +12,10 @@
 //
 // The maximum that the exponentials refer to moves only when a row's scores exceed it by 2^8 (or the scales' power of two grows): then O is read and scaled in tensor memory.
 //
-// Bound: the exponentials (16 per cycle and SM: 2048 cycles for the 256 x 128 of a block, as long as its four products) and the instructions around them.
+// Bound: the exponentials (16 per cycle and SM: 2048 cycles for the 256 x 128 of a block, as long as its four products at 128 channels) and the instructions and exchanges around them: a
+// block takes about 3500 cycles at 128 channels, where P lies over S and the products wait for it, and 4100 at 64.  32 heads on 8: 4096 queries on 8192 keys, 128 channels, bf16, 602 us
+// (685 TFLOP/s, 0.41 of what the library's products reach); five prompts of up to 1500 on up to 2500 keys, 64 channels, under a prefix, 152 us.  A quarter of the exponentials by a
+// polynomial made both slower (665, 164 us: the instructions are the scarcer), the second tile half a block behind the first made no difference.
 #include "g2d_attend.cuh"
 
 namespace g2d {
@@ -577,9 +580,10 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const __gri
                     }
                     if (MODS) {
                         const float away = (float)(key0 + cb * 32 - place);
+                        const bool near = a.softcap <= CAP_NEAR;
                         if (a.softcap > 0.f) {
 #pragma unroll
-                            for (int x = 0; x < 32; ++x) v[x] = __float_as_uint(capped(__uint_as_float(v[x]), cap));
+                            for (int x = 0; x < 32; ++x) v[x] = __float_as_uint(capped(__uint_as_float(v[x]), cap, near));
                         }
 #pragma unroll
                         for (int x = 0; x < 32; ++x) v[x] = __float_as_uint(fmaf(slope, away + (float)x, __uint_as_float(v[x])));

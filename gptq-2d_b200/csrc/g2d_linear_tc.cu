@@ -8,7 +8,14 @@
 // An adapter is two more slices of k: for every adapter among a tile's tokens A is its rows of `up` (times nothing) and B the tokens' inner values, upper and lower
 // parts (see g2d_adapters.cu).  The product has a column for every token of the tile; the reading warps add it, times the token's factor, only where the token has this adapter.
 //
-// Few tiles: the columns are split over several CTAs, whose sums meet in a second kernel, in a fixed order.
+// Up to 64 tokens each may have an adapter of its own, and two turns for each would be more than the matrix takes (61 tokens of 32 adapters: 128 turns a tile instead of 64): their outer
+// halves are added where the pieces are joined (53 us so, 41 that way).
+//
+// Whole rounds of tiles are done tile by tile; what is left over is cut into pieces of the same length, chunk after chunk on one line, whose sums meet in a second kernel in the order of the
+// columns (8192 x 28672, 2048 tokens, 3.46 rounds: 845 us with a fourth round, 738 with the line).
+//
+// Bound: 256 x 256 tiles by the products and the power that they draw (8192 x 28672, 2048 tokens, adapters of rank 32: 780 us with all launches, 1240 TFLOP/s, 0.74 of what the library's 16-bit products
+// reach); 64 tokens by the chain of a slot (codes, operand, products, release: about 700 cycles a chunk, 14333 x 4096, 61 tokens 40 us, 0.16 of HBM's rate).
 #include "g2d_linear.cuh"
 #include "g2d_tc.cuh"
 

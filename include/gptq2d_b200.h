@@ -338,7 +338,7 @@ typedef struct g2d_cache_desc {
 } g2d_cache_desc;
 
 /* The step's keys and values (element strides of tokens and heads, multiples of 8; 16-byte aligned) into the cache.  Two tokens of a step that the
- * table sends to the same place leave codes and scale of either there. */
+ * table sends to the same place leave the row of either there, or a mixture. */
 int g2d_cache_append(const g2d_cache_desc *desc, const void *k, int64_t k_token_stride, int64_t k_head_stride, const void *v,
                      int64_t v_token_stride, int64_t v_head_stride, void *stream);
 /* What the cache holds for the step's tokens, as values: k and v [tokens, kv_heads, head_dim]; zeros for tokens of no sequence and positions that the cache does not hold. */

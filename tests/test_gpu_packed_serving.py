@@ -153,6 +153,17 @@ def test_decoding_and_prompts_in_one_batch(sequences, head_dim):
     gptq_2d.check_status()
 
 
+@pytest.mark.parametrize("softcap", [1e-25, 1e-3, 63.0, 65.0, 1000.0, 1e6, 1e12, 1e31])
+@pytest.mark.parametrize("queries", [1, 3, 100])
+def test_caps_of_any_size(queries, softcap):
+    """From caps that leave no score to caps far above all of them."""
+    import packed_cache as C
+
+    batch = Batch([(300, queries)] * 2, 1, 64, 32, torch.float16)
+    q = 4 * batch.randn(batch.tokens, 4, 64)
+    assert_near(C.attend_packed(q, batch.cache, batch.table, batch.lengths, softcap=softcap), *reference(batch, q, softcap=softcap))
+
+
 @pytest.mark.parametrize("rows", [31, 32, 33, 63, 64, 65, 66])
 @pytest.mark.parametrize("batch_size", [1, 70])
 def test_either_side_of_the_line_between_rows_and_tiles(rows, batch_size):
