@@ -296,7 +296,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const __gri
                         if (!go) break;
                         after();
                         results(0, vs, j > 0);
-                        if (!more) umma_commit(&bar.o_full[0]);
+                        umma_commit(&bar.o_full[0]);
                         if (two) {
                             if (more) {
                                 go = wait(&bar.s_free[1], sc1 & 1, 0);
@@ -317,7 +317,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const __gri
                             if (!go) break;
                             after();
                             results(1, vs, j > 0);
-                            if (!more) umma_commit(&bar.o_full[1]);
+                            umma_commit(&bar.o_full[1]);
                         }
                         umma_commit(&bar.v_empty[vs]);
                     }
@@ -605,6 +605,11 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const __gri
                 bar.tops2[tc & 1][tile][half][row] = top;
                 both();
                 top = fmaxf(top, bar.tops2[tc & 1][tile][half ^ 1][row]);
+                if (M::OWN_P && tc > 0) {  // these scores came before the products of the last block with its values, which read P and add to O
+                    go = go && wait(&bar.o_full[tile], (tc - 1) & 1, 0);
+                    if (!__all_sync(0xffffffffu, go)) go = false;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                }
                 // the maximum that the exponentials refer to, and the unit of the scales
                 const int new_unit = bar.unit[slot];
                 const bool first_seen = m == -INFINITY, moves = top > m + TA_SLACK || (first_seen && top > -INFINITY) || new_unit != unit;
@@ -677,7 +682,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const __gri
             bar.sums2[oc & 1][tile][half][row] = l0;
             both();
             l0 = half ? bar.sums2[oc & 1][tile][0][row] + l0 : l0 + bar.sums2[oc & 1][tile][1][row];
-            if (go) go = wait(&bar.o_full[tile], oc & 1, 0);
+            if (go) go = wait(&bar.o_full[tile], (M::OWN_P ? tc - 1 : oc) & 1, 0);
             ++oc;
             if (!__all_sync(0xffffffffu, go)) go = false;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");

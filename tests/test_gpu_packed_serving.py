@@ -230,3 +230,25 @@ def test_two_graphs_that_are_replayed_at_once():
     torch.cuda.synchronize()
     for got, want in zip(outs, alone):
         assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+@pytest.mark.parametrize("head_dim", [64, 128])
+@pytest.mark.parametrize("queries", ["prompts", "drafts"])
+def test_cold_caches_change_nothing(queries, head_dim):
+    """Keys, values and scales that come late in any order: what was pushed out of the caches in between gives the same results bit for bit."""
+    import gptq_2d
+    import packed_cache as C
+
+    sequences = [(2500, 1500), (1801, 700), (900, 900), (2000, 70)] if queries == "prompts" else [(3000, 4), (1, 1), (2222, 7)] * 8
+    batch = Batch(sequences, 4, head_dim, 64, torch.float16)
+    q = batch.randn(batch.tokens, 16, head_dim)
+    flush = torch.empty(256 << 20, dtype=torch.uint8, device="cuda")
+    first = None
+    for i in range(16):
+        flush.fill_(i)
+        got = C.attend_packed(q, batch.cache, batch.table, batch.lengths, batch.offsets, causal=i % 2 == 0)
+        if i < 2:
+            assert_near(got, *reference(batch, q, causal=i == 0))
+            first = (first or []) + [got]
+        assert torch.equal(got, first[i % 2])
+    gptq_2d.check_status()
