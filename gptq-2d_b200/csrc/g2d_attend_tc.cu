@@ -14,7 +14,7 @@
 //
 // Bound: the exponentials (16 per cycle and SM: 2048 cycles for the 256 x 128 of a block, as long as its four products at 128 channels) and the instructions and exchanges around them: a
 // block takes about 3500 cycles at 128 channels, where P lies over S and the products wait for it, and 4100 at 64.  32 heads on 8: 4096 queries on 8192 keys, 128 channels, bf16, 602 us
-// (685 TFLOP/s, 0.41 of what the library's products reach); five prompts of up to 1500 on up to 2500 keys, 64 channels, under a prefix, 152 us.  A quarter of the exponentials by a
+// (685 TFLOP/s, 0.41 of what the library's products reach); five prompts of up to 1500 on up to 2500 keys, 64 channels, under a prefix, 153 us.  A quarter of the exponentials by a
 // polynomial made both slower (665, 164 us: the instructions are the scarcer), the second tile half a block behind the first made no difference.
 #include "g2d_attend.cuh"
 
