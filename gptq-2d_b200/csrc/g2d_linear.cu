@@ -251,6 +251,8 @@ using namespace g2d;
 // Up to here the tokens are columns of m16n8k16 products.  28672 x 8192, no adapters: 16 tokens 68.3 us, by tiles 83.9; 24 tokens 117 (two tiles of 16), by tiles 83.8; 4096 x 4096: 16 tokens 8.7,
 // by tiles 16.5; 24 tokens 14.5, by tiles 16.8.
 constexpr int64_t ROWS_TOKENS = 16;
+// ... where x fits the shared memory of a cluster, and the rows a grid: else the tiles, which take x as it comes.
+static bool linear_many(const g2d_linear_desc *d) { return d->tokens > ROWS_TOKENS || d->n > 32768 || d->m > (int64_t)65535 * 128; }
 
 struct LinearSpace {
     size_t factor, plan, partial, all;  // inner values first
@@ -259,8 +261,8 @@ static LinearSpace linear_space(const g2d_linear_desc *d) {
     const auto whole = [](size_t bytes) { return (bytes + 255) & ~(size_t)255; };
     LinearSpace s{};
     size_t at = 0;
-    const bool many = d->tokens > ROWS_TOKENS;
-    const LinearTcPlan p = many ? linear_tc_plan(d->m, d->n, d->tokens, d->adapters > 0 ? (int)d->rank : 0) : LinearTcPlan{};
+    const bool many = linear_many(d);
+    const LinearTcPlan p = many ? linear_tc_plan(d->m, d->n, d->tokens, d->adapters > 0 ? (int)d->rank : 0, d->adapters) : LinearTcPlan{};
     if (d->rank > 0) {
         s.factor = at += whole((size_t)d->tokens * INNER_LD * 2);
         s.plan = at += whole((size_t)d->tokens * sizeof(float));
@@ -329,8 +331,8 @@ extern "C" int g2d_packed_linear(const g2d_linear_desc *d, void *stream) {
     a.status = d->status;
     a.wait_cycles = WAIT_CYCLES;
     cudaStream_t st = (cudaStream_t)stream;
-    const bool many = a.tokens > ROWS_TOKENS;
-    const LinearTcPlan p = many ? linear_tc_plan(a.m, a.n, a.tokens, a.rank) : LinearTcPlan{};
+    const bool many = linear_many(d);
+    const LinearTcPlan p = many ? linear_tc_plan(a.m, a.n, a.tokens, a.rank, a.adapters) : LinearTcPlan{};
     int *const plan = a.tokens > LINEAR_FEW && a.rank > 0 ? (int *)((char *)d->workspace + space.plan) : nullptr;
     if (a.rank > 0) {
         const int launched = launch_inner(a, plan, p.tile, st);

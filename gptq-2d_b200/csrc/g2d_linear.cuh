@@ -44,10 +44,11 @@ __device__ __forceinline__ uint32_t float_to_bits(float v, int bf16) { return bf
 // of chunks, cut into `ctas` pieces; a tile has at most `pieces` of them.
 struct LinearTcPlan {
     int tile, duo, row_tiles, token_tiles, chunks, whole;
+    int later;  // the adapters' outer halves are added where the pieces are joined, and every tile is cut
     int64_t shared, line, ctas, pieces;
     size_t partial_bytes;
 };
-LinearTcPlan linear_tc_plan(int64_t m, int64_t n, int64_t tokens, int rank);
+LinearTcPlan linear_tc_plan(int64_t m, int64_t n, int64_t tokens, int rank, int64_t adapters);
 
 // Inner values and factors of all tokens; where they are more than LINEAR_FEW, also the adapters of each tile of `tile` tokens: plan[i * (tile + 1)] of them, their numbers behind it
 int launch_inner(const LinearArgs &a, int *plan, int tile, cudaStream_t st);

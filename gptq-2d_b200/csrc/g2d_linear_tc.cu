@@ -8,7 +8,7 @@
 // An adapter is two more slices of k: for every adapter among a tile's tokens A is its rows of `up` (times nothing) and B the tokens' inner values, upper and lower
 // parts (see g2d_adapters.cu).  The product has a column for every token of the tile; the reading warps add it, times the token's factor, only where the token has this adapter.
 //
-// Up to 64 tokens each may have an adapter of its own, and two turns for each would be more than the matrix takes (61 tokens of 32 adapters: 128 turns a tile instead of 64): their outer
+// Few tokens may each have an adapter of their own, and two turns for each would be more than the matrix takes (61 tokens of 32 adapters: 128 turns a tile instead of 64): their outer
 // halves are added where the pieces are joined (53 us so, 41 that way).
 //
 // Whole rounds of tiles are done tile by tile; what is left over is cut into pieces of the same length, chunk after chunk on one line, whose sums meet in a second kernel in the order of the
@@ -21,7 +21,7 @@
 
 namespace g2d {
 
-constexpr int LT_OUTER_LATER = LINEAR_FEW, LT_JOIN_TOKENS = 4;  // tiles of so many tokens have their adapters' outer halves added where the pieces are joined
+constexpr int LT_JOIN_TOKENS = 4;
 constexpr int LT_W_BYTES = 128 * 128, LT_CODE_BYTES = 128 * 32, LT_SLICE = 8;
 
 // DUO: a pair of CTAs on 256 rows x NT tokens (cta_group::2), each with its rows of W and half of the tokens' rows of x.
@@ -197,7 +197,7 @@ __global__ void __launch_bounds__(LinearShape<NT, DUO>::THREADS, 1) linear_tc_ke
     let_the_next_launch_start();
     // how many adapters an item has to add: those of its tile, by the first piece.  The launch before writes them.
     const auto adapters_in = [&](const LinearItem &it) {
-        if (NT == LT_OUTER_LATER || a.rank == 0 || it.piece != 0) return 0;
+        if (job.p.later || a.rank == 0 || it.piece != 0) return 0;
         after_the_launch_before();
         return job.plan[(int64_t)it.token_tile * (NT + 1)];
     };
@@ -526,7 +526,7 @@ __global__ void __launch_bounds__(LinearShape<NT, DUO>::THREADS, 1) linear_tc_ke
     if (threadIdx.x == 0 && bar.failed && a.status) atomicExch(a.status, -1);
 }
 
-// The tiles that were cut: sums of their pieces, in their order, and (tiles of LT_OUTER_LATER tokens) the outer halves of the adapters.  A thread has a row and LT_JOIN_TOKENS tokens.
+// The tiles that were cut: sums of their pieces, in their order, and (`later`) the outer halves of the adapters.  A thread has a row and LT_JOIN_TOKENS tokens.
 template <bool STAGED>
 __global__ void __launch_bounds__(128) linear_join_kernel(const LinearArgs a, const LinearTcPlan p, const float *__restrict__ partial, int grid_ctas) {
     __shared__ float4 inner[LT_JOIN_TOKENS][RANK_MAX / 4];
@@ -536,7 +536,7 @@ __global__ void __launch_bounds__(128) linear_join_kernel(const LinearArgs a, co
     const int in_tile = blockIdx.y * LT_JOIN_TOKENS;
     const int64_t token0 = tile / p.row_tiles * p.tile + in_tile, row_in_tile = blockIdx.x % parts * 128 + threadIdx.x, row = tile % p.row_tiles * rows + row_in_tile;
     const int pieces = (int)(line_owner(p, (shared + 1) * p.chunks - 1) - line_owner(p, shared * p.chunks)) + 1;
-    const bool outer = p.tile == LT_OUTER_LATER && a.rank > 0;
+    const bool outer = p.later;
     int id[LT_JOIN_TOKENS];
 #pragma unroll
     for (int e = 0; e < LT_JOIN_TOKENS; ++e) id[e] = outer ? adapter_of(a, (int)token0 + e) : -1;
@@ -633,7 +633,12 @@ static bool make_map_up(CUtensorMap *map, const LinearArgs &a) {
               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-LinearTcPlan linear_tc_plan(int64_t m, int64_t n, int64_t tokens, int rank) {
+// Adapters' outer halves at the join: up to LINEAR_FEW tokens always; up to 256 where so many adapters may be among a tile's tokens that two turns for each are many, and a rank is short enough for
+// the join's fp32 sums.  14336 x 4096, 128 tokens: 32 adapters of rank 8 62.5 us at the join, 73.9 as turns, 100 of rank 16 76.4, 89.2; 8 of rank 64 86.9, 61.5, 4 of rank 16 60.0, 48.9; 512 tokens, 100
+// of rank 16 159.6, 158.3.  4096 x 4096, 256 tokens: 32 of rank 8 43.8, 51.8, 32 of rank 64 82.4, 75.8.
+constexpr int64_t LATER_TOKENS = 256, LATER_ADAPTERS = 24;
+constexpr int LATER_RANK = 16;
+LinearTcPlan linear_tc_plan(int64_t m, int64_t n, int64_t tokens, int rank, int64_t adapters) {
     LinearTcPlan p;
     p.tile = tokens <= LINEAR_FEW ? LINEAR_FEW : 128;
     p.duo = 0;
@@ -651,7 +656,8 @@ LinearTcPlan linear_tc_plan(int64_t m, int64_t n, int64_t tokens, int rank) {
     p.token_tiles = (int)columns;
     p.chunks = (int)ceil_div(n, (int64_t)KH);
     const int64_t tiles = rows * columns, at_once = p.duo ? 74 : 148;
-    p.whole = p.tile == LT_OUTER_LATER && rank > 0 ? 0 : (int)(tiles / at_once);
+    p.later = rank > 0 && (tokens <= LINEAR_FEW || (tokens <= LATER_TOKENS && adapters >= LATER_ADAPTERS && rank <= LATER_RANK));
+    p.whole = p.later ? 0 : (int)(tiles / at_once);
     p.shared = tiles - p.whole * at_once;
     p.line = p.shared * p.chunks;
     p.ctas = p.line / 8 < at_once ? (p.line / 8 > 0 ? p.line / 8 : 1) : at_once;  // pieces of eight chunks at least
@@ -681,7 +687,7 @@ static int launch_tc(const LinearArgs &a, const LinearTcPlan &p, const int *plan
     const int64_t ctas = p.whole > 0 ? (DUO ? 74 : 148) : p.ctas;
     const int launched = launch_dependent(linear_tc_kernel<BF16, NT, DUO>, dim3((unsigned)(DUO ? 2 * ctas : ctas)), S::THREADS, S::SMEM, DUO ? 2 : 1, a.rank > 0, st, job);
     if (launched != G2D_OK || p.shared == 0) return launched;
-    const auto join = NT == LT_OUTER_LATER && a.rank > 8 ? linear_join_kernel<true> : linear_join_kernel<false>;
+    const auto join = p.later && a.rank > 8 ? linear_join_kernel<true> : linear_join_kernel<false>;
     return launch_dependent(join, dim3((unsigned)p.shared * (DUO ? 2 : 1), NT / LT_JOIN_TOKENS), 128, 0, 1, true, st, a, p, partial, (int)ctas);
 }
 

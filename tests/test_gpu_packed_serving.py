@@ -175,12 +175,20 @@ def test_either_side_of_the_line_between_rows_and_tiles(rows, batch_size):
 
 
 @pytest.mark.parametrize("m, n, tokens, adapters, rank", [(19200, 256, 128, 3, 16), (20480, 2048, 200, 2, 8), (20000, 1984, 150, 0, 8), (19328, 192, 64, 40, 64), (300, 4096, 33, 5, 24), (9600, 64, 50, 2, 8),
-                                                          (5000, 4096, 700, 4, 32)])
+                                                          (5000, 4096, 700, 4, 32), (4000, 512, 100, 40, 16), (4096, 320, 250, 30, 8), (9000, 1024, 256, 24, 16)])
 def test_whole_rounds_of_tiles_and_tiles_that_are_cut(m, n, tokens, adapters, rank):
     litter()
     Problem(m, n, tokens, torch.float16, adapters=adapters, rank=rank).check()
     litter()
     Problem(m, n, tokens, torch.bfloat16, groups=1 if n % 128 else n // 64, adapters=adapters, rank=rank).check()
+
+
+@pytest.mark.parametrize("tokens", [1, 9, 16])
+@pytest.mark.parametrize("n", [32768, 32800, 65536])
+def test_rows_that_are_longer_than_shared_memory(n, tokens):
+    Problem(70, n, tokens, torch.bfloat16, adapters=3, rank=8).check()
+    if n % 128 == 0:
+        Problem(70, n, tokens, torch.float16, groups=n // 64).check()
 
 
 def test_two_streams_at_once():
