@@ -214,7 +214,9 @@ int launch_inner(const LinearArgs &a, int *plan, int tile, cudaStream_t st) {
     // prompt's tokens stand together: 2048 of 8 adapters of rank 32 over 28672 columns 53 us by blocks, and one adapter would be read 2048 times by tokens.
     if (a.tokens <= LINEAR_FEW) return launch_dependent(inner_rows_kernel, dim3((unsigned)a.tokens * INNER_SPLIT), INNER_THREADS, 0, INNER_SPLIT, false, st, a);
     const unsigned blocks = (unsigned)ceil_div((int64_t)a.tokens, (int64_t)INNER_BLOCK);
-    const dim3 grid(blocks * INNER_SPLIT, (unsigned)(a.adapters < 4 ? a.adapters + 1 : 4));
+    // several CTAs share a block's adapters only while blocks are few (256 x 28672, 4096 tokens of 32 adapters of rank 64: 270 us with four always, 252)
+    const int64_t room = 2 * 148 / ((int64_t)blocks * INNER_SPLIT), most = a.adapters < 4 ? a.adapters + 1 : 4;
+    const dim3 grid(blocks * INNER_SPLIT, (unsigned)(room < 1 ? 1 : room < most ? room : most));
     const auto launch = [&](auto kernel) { return launch_dependent(kernel, grid, INNER_THREADS, 0, INNER_SPLIT, false, st, a, plan, tile); };
     if (a.rank <= 16) return a.bf16 ? launch(inner_block_kernel<true, 2>) : launch(inner_block_kernel<false, 2>);
     if (a.rank <= 32) return a.bf16 ? launch(inner_block_kernel<true, 4>) : launch(inner_block_kernel<false, 4>);

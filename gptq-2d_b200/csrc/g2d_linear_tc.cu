@@ -14,7 +14,7 @@
 // Whole rounds of tiles are done tile by tile; what is left over is cut into pieces of the same length, chunk after chunk on one line, whose sums meet in a second kernel in the order of the
 // columns (8192 x 28672, 2048 tokens, 3.46 rounds: 845 us with a fourth round, 738 with the line).
 //
-// Bound: 256 x 256 tiles by the products and the power that they draw (8192 x 28672, 2048 tokens, adapters of rank 32: 780 us with all launches, 1240 TFLOP/s, 0.74 of what the library's 16-bit products
+// Bound: 256 x 256 tiles by the products and the power that they draw (8192 x 28672, 2048 tokens, adapters of rank 32: 751 us with all launches, 1287 TFLOP/s, 0.77 of what the library's 16-bit products
 // reach); 64 tokens by the chain of a slot (codes, operand, products, release: about 700 cycles a chunk, 14333 x 4096, 61 tokens 40 us, 0.16 of HBM's rate).
 #include "g2d_linear.cuh"
 #include "g2d_tc.cuh"
@@ -636,7 +636,8 @@ static bool make_map_up(CUtensorMap *map, const LinearArgs &a) {
 
 // Adapters' outer halves at the join: up to LINEAR_FEW tokens always; up to 256 where so many adapters may be among a tile's tokens that two turns for each are many, and a rank is short enough for
 // the join's fp32 sums.  14336 x 4096, 128 tokens: 32 adapters of rank 8 62.5 us at the join, 73.9 as turns, 100 of rank 16 76.4, 89.2; 8 of rank 64 86.9, 61.5, 4 of rank 16 60.0, 48.9; 512 tokens, 100
-// of rank 16 159.6, 158.3.  4096 x 4096, 256 tokens: 32 of rank 8 43.8, 51.8, 32 of rank 64 82.4, 75.8.
+// of rank 16 159.6, 158.3.  256 tokens: 32 of rank 8 70.0, 80.0, of rank 16 92.4, 82.2; 4096 x 4096 41.1, 56.3
+// and 47.4, 56.2.
 constexpr int64_t LATER_TOKENS = 256, LATER_ADAPTERS = 24;
 constexpr int LATER_RANK = 16;
 LinearTcPlan linear_tc_plan(int64_t m, int64_t n, int64_t tokens, int rank, int64_t adapters) {
@@ -644,10 +645,11 @@ LinearTcPlan linear_tc_plan(int64_t m, int64_t n, int64_t tokens, int rank, int6
     p.tile = tokens <= LINEAR_FEW ? LINEAR_FEW : 128;
     p.duo = 0;
     int64_t rows = ceil_div(m, (int64_t)128), columns = ceil_div(tokens, (int64_t)p.tile);
-    // 256 x 256 by pairs of CTAs, four times the work of a 128 x 128 tile in 1.6 times its time, unless a pair's share is too short for what each tile costs besides.  4096 x 4096: 256 tokens
-    // (14 chunks a pair) 36.8 us by 128 x 128, 39.0 by pairs; 512 tokens (28) 53.5, 49.8; 8192 x 8192, 129 tokens (55) 73.3, 59.6; 28672 x 4096, 1024 tokens 402, 261
+    // 256 x 256 by pairs of CTAs, four times the work of a 128 x 128 tile in little more than its time, unless a pair's share is too short for what each tile costs besides.  2048 x 2048, 256 tokens
+    // (3.5 chunks a pair) 14.6 us by 128 x 128, 16.1 by pairs; 512 tokens (7) 19.4, 17.9; 4096 x 4096, 256 tokens (14) 25.6, 23.5; 8192 x 8192, 512 tokens 110.6, 70.3.  Up to 128 tokens half of
+    // such a tile would be empty: 8192 x 8192, 100 tokens 36.3, 37.5, in groups of 128 45.7, 51.6.
     const int64_t pairs = ceil_div(m, (int64_t)256) * ceil_div(tokens, (int64_t)256);
-    if (tokens > 128 && pairs * ceil_div(n, (int64_t)KH) >= 74 * 20) {
+    if (tokens > 128 && pairs * ceil_div(n, (int64_t)KH) >= 74 * 6) {
         p.tile = 256;
         p.duo = 1;
         rows = ceil_div(m, (int64_t)256);
