@@ -1,7 +1,7 @@
 // y = x W^T for a matrix W held as packed 4-bit codes, many tokens, on tcgen05; low-rank adapters of the tokens' requests beside it.
 //
-// A tile is 128 rows of W times NT tokens: A is W, so a scale belongs to a lane of tensor memory.  Codes travel as they are: the TMA brings 128 rows x 256 columns
-// (16 KB) of them, four or eight warps turn 64 columns at a time into 16-bit values in the swizzled layout of an MMA operand (code - 8 exactly, plus 8 + qmin - zero rounded to the type), and
+// A tile is 128 rows of W times NT tokens: A is W, so a scale belongs to a lane of tensor memory.  Codes travel as they are: the TMA brings 128 rows x 64 columns
+// (4 KB) of them to a slot, whose two warps turn them into 16-bit values in the swizzled layout of an MMA operand (code - 8 exactly, plus 8 + qmin - zero rounded to the type), and
 // x comes by TMA beside them.  What is accumulated in tensor memory is a slice of the columns under one scale (512 columns at most: the tensor cores add with truncation);
 // warps of their own read each slice while the next is accumulated, and add scale times slice in registers, in fp32.
 //

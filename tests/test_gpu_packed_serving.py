@@ -260,3 +260,14 @@ def test_cold_caches_change_nothing(queries, head_dim):
             first = (first or []) + [got]
         assert torch.equal(got, first[i % 2])
     gptq_2d.check_status()
+
+
+@pytest.mark.parametrize("tokens", [3, 16, 50, 120, 400])
+@pytest.mark.parametrize("groups", [1, 32])
+def test_products_from_cold_caches_are_the_same(groups, tokens):
+    p = Problem(5000, 2048, tokens, torch.bfloat16, groups=groups, adapters=6, rank=16)
+    flush = torch.empty(256 << 20, dtype=torch.uint8, device="cuda")
+    first = p.check()
+    for i in range(8):
+        flush.fill_(i)
+        assert torch.equal(p.run(), first)
