@@ -83,7 +83,7 @@ __device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t b
 template <int ROWS>
 __device__ __forceinline__ unsigned attend_units(const AttendArgs &a, const AttendSequence &s, int &blocks, int &items) {
     const unsigned rows = (unsigned)(s.count * a.group);  // of no more than tokens x heads
-    blocks = max((int)(((unsigned)s.keys + CACHE_BLOCK - 1) / CACHE_BLOCK), 1);
+    blocks = a.even ? a.even : max((int)(((unsigned)s.keys + CACHE_BLOCK - 1) / CACHE_BLOCK), 1);
     items = rows >= (unsigned)a.rows_from && rows < (unsigned)a.rows_to ? a.c.kv_heads * (int)((rows + ROWS - 1) / ROWS) : 0;
     return (unsigned)items * blocks;
 }
@@ -145,13 +145,14 @@ __global__ void __launch_bounds__(AttendShape<D, NT>::THREADS, 1) attend_rows_ke
     if (lane < 2) sh.parts[2 * warp + lane].last = 0;
     const auto units_of = [&](int b) { return attend_units<ROWS>(a, b); };
     unsigned mine_units;
-    const AttendShares shares(count_units<ATTEND_WARPS>(c.batch, units_of, sh.totals, mine_units), gridDim.x);
+    const unsigned grain = max(a.even, 1);  // units that stay together
+    const AttendShares shares(count_units<ATTEND_WARPS>(c.batch, units_of, sh.totals, mine_units) / grain, gridDim.x);
     const unsigned share = blockIdx.x;
     AttendCursor cur;
     cur.u = cur.end = 0;
     if (share < shares.count) {
         // of n units the first warps have one each, where there are not enough for all: a warp between two others of an item has a part of it
-        const unsigned u0 = shares.begin(share), n = shares.begin(share + 1) - u0, active = min(n, (unsigned)ATTEND_WARPS);
+        const unsigned u0 = shares.begin(share) * grain, n = shares.begin(share + 1) * grain - u0, active = min(n, (unsigned)ATTEND_WARPS);
         if ((unsigned)warp < active) {
             const unsigned mine = u0 + warp * n / active;
             cur.end = (int)(u0 + (warp + 1) * n / active - mine);
@@ -680,6 +681,7 @@ static int launch_attend(const AttendArgs &rows, const AttendArgs &tiles, bool f
     if (launched == G2D_OK && many) launched = launch_attend_tiles(tiles, rows_first && few, st);
     if (launched == G2D_OK && !rows_first) launched = launch_few(many);
     if (launched != G2D_OK) return launched;
+    if (rows.even) return G2D_OK;  // no item lies in two shares
     const JoinArgs j{tiles, rows, many ? TA_GRID * TILE_JOINS : 0};
     return launch_attention(attend_join_kernel<D, NT>, (unsigned)(j.tile_ctas + (few ? ATTEND_GRID : 0)), JOIN_THREADS, 0, true, j, st);
 }
@@ -688,6 +690,8 @@ static int launch_attend(const AttendArgs &rows, const AttendArgs &tiles, bool f
 // 32 heads on 8, head_dim 128: 1 sequence of 4096 keys, 64 rows: 27.3 us by rows, 35.3 by tiles; 8 of 2000, 64 rows: 47.1, 54.5, 128 rows: 74.5, 59.3;
 // 32 of 1000, 32 rows: 62.0, 67.4, 48 rows: 86.8, 69.2
 static int tile_rows_from(const CacheView &c) { return (int64_t)c.batch * c.kv_heads <= 64 ? 65 : 33; }
+
+constexpr int64_t EVEN_KEYS = 512;
 
 struct AttendSpace {
     size_t tiles, joins, all;  // the warps' partial results first
@@ -753,9 +757,13 @@ extern "C" int g2d_cache_attend(const g2d_attend_desc *d, void *stream) {
     t.partial = (float *)((char *)d->workspace + space.tiles);
     t.joins = (AttendJoin *)((char *)d->workspace + space.joins);
     a.joins = t.joins + TA_GRID;
+    t.even = 0;
     a.rows_from = 1;
     a.rows_to = line;
     a.partial = (float *)d->workspace;
+    // Short tables (512 positions at most), the same number of queries everywhere: items whole in their shares, a CTA's warps a block or so each, and no join.
+    const int64_t most_keys = (int64_t)a.c.table_width << a.c.page_shift;
+    a.even = !many && !a.c.offsets && most_keys <= EVEN_KEYS ? (int)(most_keys > CACHE_BLOCK ? ceil_div(most_keys, (int64_t)CACHE_BLOCK) : 1) : 0;
     const bool narrow = a.group <= 8 && (rows < 0 ? ceil_div((int64_t)a.c.tokens * a.group, (int64_t)a.c.batch) : rows) <= 8;
     // Of two kernels one has most of the work, as a rule: the one for the sequences' mean.  The other finds its part, or that it has none, while that one's last CTAs work
     const bool rows_first = (int64_t)a.c.tokens * a.group < (int64_t)line * a.c.batch;

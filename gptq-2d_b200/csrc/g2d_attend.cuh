@@ -24,6 +24,7 @@ struct AttendArgs {
     float softcap;           // 0: none
     const float *slopes;     // per head, or null
     const int32_t *prefix;   // per sequence, or null
+    int even;                // rows: not 0: every item counts as so many units, and shares have whole items
     int rows_from, rows_to;  // the kernel's sequences: those with rows_from <= queries x group < rows_to
     float *partial;
     AttendJoin *joins;  // one per share
