@@ -5,7 +5,7 @@
 // with k_j = s_j (c_j - 8), v_j likewise, codes c in 0 .. 15, and zeros where no j is left.  The rows of one kv head are all (token, head of its group).
 //
 // Work.  A unit is a block of 64 keys of one item (sequence, kv head, eight or sixteen rows).  The units of all items, one after the other, are dealt
-// out evenly to the CTAs, and a CTA's to its warps, however long each sequence is: lengths are known on the device only.  A warp goes through its units with a
+// out evenly to the CTAs, and a CTA's to its warps, however long each sequence is: lengths are known on the device only (`even`: whole items to each CTA, where tables are short).  A warp goes through its units with a
 // running maximum and sum per row and keeps its results in registers; an item that lies within one warp's share is written at once, the others leave
 // partial results (at most two per warp), which the CTA adds up in the order of the keys; what of an item lies in several CTAs (at most two parts
 // per CTA) attend_join_kernel adds up.
@@ -21,7 +21,7 @@
 //
 // Bound: HBM (head_dim + 4 bytes per key and head), behind it the products (16 cycles each for a quarter of an SM: 68 for a block of 64 keys and eight rows) and the instructions per key, and
 // for short calls the start (counting units, the first pages and codes: about 6 us) and the joins.  64 heads on 8, 128 channels: 131072 keys of one sequence 41 us (3.4 TB/s), 48
-// sequences of up to 8191 61 us; 16 sequences of 2000 keys, four queries of 32 heads, capped and biased, 37 us; one of 137 keys 9 us.
+// sequences of up to 8191 61 us; 16 sequences of 2000 keys, four queries of 32 heads, capped and biased, 30 us; one of 137 keys 7.6 us.
 #include "g2d_attend.cuh"
 
 namespace g2d {
@@ -691,8 +691,6 @@ static int launch_attend(const AttendArgs &rows, const AttendArgs &tiles, bool f
 // 32 of 1000, 32 rows: 62.0, 67.4, 48 rows: 86.8, 69.2
 static int tile_rows_from(const CacheView &c) { return (int64_t)c.batch * c.kv_heads <= 64 ? 65 : 33; }
 
-constexpr int64_t EVEN_KEYS = 512;
-
 struct AttendSpace {
     size_t tiles, joins, all;  // the warps' partial results first
 };
@@ -761,10 +759,13 @@ extern "C" int g2d_cache_attend(const g2d_attend_desc *d, void *stream) {
     a.rows_from = 1;
     a.rows_to = line;
     a.partial = (float *)d->workspace;
-    // Short tables (512 positions at most), the same number of queries everywhere: items whole in their shares, a CTA's warps a block or so each, and no join.
-    const int64_t most_keys = (int64_t)a.c.table_width << a.c.page_shift;
-    a.even = !many && !a.c.offsets && most_keys <= EVEN_KEYS ? (int)(most_keys > CACHE_BLOCK ? ceil_div(most_keys, (int64_t)CACHE_BLOCK) : 1) : 0;
     const bool narrow = a.group <= 8 && (rows < 0 ? ceil_div((int64_t)a.c.tokens * a.group, (int64_t)a.c.batch) : rows) <= 8;
+    // Short tables, the same number of queries everywhere: items whole in their shares, a CTA's warps some blocks each, and no join; longer ones where there are about as many items as CTAs.
+    // 32 heads on 8, 128 channels, four queries, (16 x) 2000 keys, capped: 39.4 us cut evenly, 30.9 whole; sequences of 4 to 2000 keys 33.8, 28.8; 32 sequences of 500 30.9, 21.4; but 8 of 4 to
+    // 2000 23.2, 27.6, one of 2000 19.8, 28.4, and 64 of 4 to 2000 74.9, 83.9
+    const int64_t most_keys = (int64_t)a.c.table_width << a.c.page_shift, items = rows < 0 ? 0 : (int64_t)a.c.batch * a.c.kv_heads * ceil_div(rows, (int64_t)(narrow ? 8 : 16));
+    const bool whole = !many && !a.c.offsets && (most_keys <= 512 || (most_keys <= 2048 && items >= 96 && items <= 2 * ATTEND_GRID));
+    a.even = !whole ? 0 : most_keys > CACHE_BLOCK ? (int)ceil_div(most_keys, (int64_t)CACHE_BLOCK) : 1;
     // Of two kernels one has most of the work, as a rule: the one for the sequences' mean.  The other finds its part, or that it has none, while that one's last CTAs work
     const bool rows_first = (int64_t)a.c.tokens * a.group < (int64_t)line * a.c.batch;
     if (a.c.head_dim == 128) return narrow ? launch_attend<128, 1>(a, t, few, many, rows_first, st) : launch_attend<128, 2>(a, t, few, many, rows_first, st);

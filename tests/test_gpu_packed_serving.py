@@ -275,12 +275,12 @@ def test_products_from_cold_caches_are_the_same(groups, tokens):
 
 @pytest.mark.parametrize("head_dim", [64, 128])
 @pytest.mark.parametrize("queries, heads", [(1, 8), (3, 8), (16, 4), (2, 32)])
-@pytest.mark.parametrize("width", [1, 64, 65, 130, 511, 512, 513])
+@pytest.mark.parametrize("width", [1, 64, 65, 130, 511, 512, 513, 2048])
 def test_short_tables(width, queries, heads, head_dim):
     """Sequences of all lengths that a short table holds, more items than SMs and fewer; queries before the first position."""
     import packed_cache as C
 
-    for count in (1, 90):
+    for count in (1, 25, 90):
         lengths = [width if b == 0 else (37 * b) % (width + 1) for b in range(count)]
         batch = Batch([(max(n, 1), 1) for n in lengths], 4, head_dim, 16, torch.float16, seed=width)
         batch.sequences = [(n, queries) for n in lengths]
