@@ -298,6 +298,7 @@ extern "C" int g2d_packed_linear(const g2d_linear_desc *d, void *stream) {
     if (!d->out || ((uintptr_t)d->out & 1) != 0 || d->out_stride < d->m) return G2D_ERR_BAD_ARGUMENT;
     if (d->n == 0) return G2D_ERR_UNSUPPORTED;
     if (!d->x || !d->codes || !d->scale || !d->zero || (((uintptr_t)d->x | (uintptr_t)d->codes) & 15) != 0 || d->x_stride % 8 != 0) return G2D_ERR_BAD_ARGUMENT;
+    if (linear_many(d) && d->tokens > 1 && d->x_stride < d->n) return G2D_ERR_BAD_ARGUMENT;  // the tiles' copies take x as rows that stand apart
     if (d->rank > 0 && (!d->down || !d->up || !d->index || (((uintptr_t)d->down | (uintptr_t)d->up) & 15) != 0)) return G2D_ERR_BAD_ARGUMENT;
     const LinearSpace space = linear_space(d);
     if (space.all > 0 && (!d->workspace || d->workspace_bytes < space.all || ((uintptr_t)d->workspace & 255) != 0)) return G2D_ERR_WORKSPACE;
@@ -310,7 +311,7 @@ extern "C" int g2d_packed_linear(const g2d_linear_desc *d, void *stream) {
     a.m = d->m;
     a.n = d->n;
     a.row_bytes = d->row_bytes;
-    a.x_stride = d->x_stride;
+    a.x_stride = d->tokens > 1 ? d->x_stride : d->n;  // of one row it says nothing
     a.out_stride = d->out_stride;
     a.scale_row = d->scale_row_stride;
     a.scale_group = d->scale_group_stride;

@@ -62,10 +62,11 @@ def packed_linear(x: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor, zer
     assert row_bytes >= n // 2 and row_bytes % 16 == 0 and codes_at % 16 == 0, "rows of codes must hold n entries and be 16-byte aligned"
     rows = x if len(shape) == 2 else x.detach().reshape(-1, n)
     row_stride, last = rows.stride()
-    if last != 1 or row_stride % 8 or rows.data_ptr() % 16:
+    tokens = rows.shape[0]
+    # rows that lie over one another (one row for every token, windows of a longer one) are copied: the tiles' copies need rows that stand apart
+    if last != 1 or row_stride % 8 or rows.data_ptr() % 16 or (row_stride < n and tokens > 1):
         rows = rows.detach().clone(memory_format=torch.contiguous_format)
         row_stride = n
-    tokens = rows.shape[0]
     scale, scale_row, scale_group, groups = _parameter(scale, m, n, "scale", device)
     zero, zero_row, zero_group, zero_groups = _parameter(zero_point, m, n, "zero_point", device)
     assert groups == zero_groups or groups == 1 or zero_groups == 1, "scale and zero_point must have the same groups"

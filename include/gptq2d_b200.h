@@ -373,7 +373,7 @@ int g2d_cache_attend(const g2d_attend_desc *desc, void *stream);
 typedef struct g2d_linear_desc {
     int32_t half, bits;          /* g2d_half of x, down, up and out; 4 */
     int64_t m, n, tokens;
-    const void *x;               /* [tokens, n], rows x_stride apart (a multiple of 8), 16-byte aligned */
+    const void *x;               /* [tokens, n], rows x_stride apart (a multiple of 8; n at least where there are more than 16 tokens, or n > 32768), 16-byte aligned */
     int64_t x_stride;
     const uint8_t *codes;        /* [m, row_bytes], 16-byte aligned */
     int64_t row_bytes, groups;
