@@ -333,7 +333,10 @@ __global__ void __launch_bounds__(AttendShape<D, NT>::THREADS, 1) attend_rows_ke
             }
             // ---- scales: of the keys 8 g .. 8 g + 7, key 2 mt + half for the rows of tile mt ----
             const uint4 kraw = *reinterpret_cast<const uint4 *>(st.ks + 8 * g), vraw = *reinterpret_cast<const uint4 *>(st.vs + 8 * g);
-            const uint32_t kw[4] = {kraw.x, kraw.y, kraw.z, kraw.w};
+            // a scale that is not finite makes its key's scores NaN: for an infinite one, zeros in its codes leave what -8 sum(q) and the products lose to rounding, times infinity
+            uint32_t kw[4] = {kraw.x, kraw.y, kraw.z, kraw.w};
+#pragma unroll
+            for (int mt = 0; mt < 4; ++mt) kw[mt] = nan_unless_finite(kw[mt]);
             uint32_t vw[4] = {vraw.x, vraw.y, vraw.z, vraw.w};
             unsigned gone = 0u;  // MASKED: keys that are not there
             if constexpr (MASKED) {

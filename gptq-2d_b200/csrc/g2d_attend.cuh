@@ -61,6 +61,11 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// two halves, NaN in the place of one that is not finite
+__device__ __forceinline__ uint32_t nan_unless_finite(uint32_t halves) {
+    const __half2 h = *reinterpret_cast<const __half2 *>(&halves), r = __hfma2(h, __float2half2_rn(0.f), h);
+    return *reinterpret_cast<const uint32_t *>(&r);
+}
 // cap tanh(u / cap) through one exponential, from x = 2 log2(e) u / cap: good to 1e-7 of the cap, which is what a score's exponential sees of a cap up to CAP_NEAR.  Larger caps: tanh's
 // series where |u / cap| < 1/4 (relative error 1e-8), so that a cap far above the scores leaves them what they are.
 constexpr float CAP_NEAR = 64.f;

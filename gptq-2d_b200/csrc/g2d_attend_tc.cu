@@ -441,7 +441,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const __gri
                     if (!go) break;
                     unit = max(max(unit, max(bar.tops[stage][0], bar.tops[stage][1])), max(bar.tops[stage][2], bar.tops[stage][3]));
                     float *const sc = reinterpret_cast<float *>(at_base + M::SCALES + slot * M::SCALE_STAGE) + key;
-                    sc[0] = ks * (a.scale * score_unit<MODS>(a));
+                    sc[0] = fmaf(ks, 0.f, ks) * (a.scale * score_unit<MODS>(a));  // NaN for a scale that is not finite, whatever the codes
                     sc[TA_KEYS] = vs * power_of_two(min(TA_UNIT - (unit - 127), 127));
                     if (lane == 0) bar.present[slot][warp - 4] = got;
                     if (threadIdx.x == 128) bar.unit[slot] = unit;

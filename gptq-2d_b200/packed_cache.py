@@ -100,7 +100,8 @@ def _rows(x: torch.Tensor, device, heads: int, dim: int, what: str) -> torch.Ten
 
 def append_packed(cache: PackedCache, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, offsets: torch.Tensor | None = None) -> None:
     """Round the step's keys and values ``[tokens, kv_heads, head_dim]`` (float16 or bfloat16; strided views, such as parts of a fused projection, are
-    read in place) and write them into the cache, in place.  ``lengths`` counts the step's tokens already.  A row with an infinity or a NaN reads back as NaN."""
+    read in place) and write them into the cache, in place.  ``lengths`` counts the step's tokens already.  A row with an infinity, a NaN or a
+    magnitude whose scale a half cannot hold (491400 and more) reads back as NaN, and makes NaN every query that sees it."""
     assert k.dtype == v.dtype and k.dim() == 3 and k.shape == v.shape, "expected keys and values of one shape and type"
     device, fields = _cache_fields(cache, k.dtype, k.shape[0], page_table, lengths, offsets)
     k, v = _rows(k, device, fields[3], fields[1], "keys"), _rows(v, device, fields[3], fields[1], "values")
