@@ -141,12 +141,13 @@ __global__ void __launch_bounds__(AttendShape<D, NT>::THREADS, 1) attend_rows_ke
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     let_the_next_launch_start();
-    if (threadIdx.x == 0) a.joins[blockIdx.x] = AttendJoin{};
     if (lane < 2) sh.parts[2 * warp + lane].last = 0;
     const auto units_of = [&](int b) { return attend_units<ROWS>(a, b); };
     unsigned mine_units;
     const unsigned grain = max(a.even, 1);  // units that stay together
-    const AttendShares shares(count_units<ATTEND_WARPS>(c.batch, units_of, sh.totals, mine_units) / grain, gridDim.x);
+    const unsigned units = count_units<ATTEND_WARPS>(c.batch, units_of, sh.totals, mine_units);
+    if (threadIdx.x == 0) a.joins[blockIdx.x] = AttendJoin{units < UNITS_END ? 0 : -1};
+    const AttendShares shares((units < UNITS_END ? units : 0u) / grain, gridDim.x);
     const unsigned share = blockIdx.x;
     AttendCursor cur;
     cur.u = cur.end = 0;
@@ -653,6 +654,13 @@ __global__ void __launch_bounds__(JOIN_THREADS) attend_join_kernel(const JoinArg
     const int share = of_tiles ? blockIdx.x / TILE_JOINS : blockIdx.x - j.tile_ctas;
     const AttendJoin join = a.joins[share];
     if (join.count == 0) return;
+    if (join.count < 0) {  // of every share of the kernel, so that all of its CTAs are here: nothing has been computed
+        const int64_t pieces = (int64_t)a.c.tokens * a.heads * (D / 8), ctas = of_tiles ? j.tile_ctas : gridDim.x - j.tile_ctas;
+        const int cta = of_tiles ? blockIdx.x : blockIdx.x - j.tile_ctas;
+        for (int64_t i = cta * JOIN_THREADS + threadIdx.x; i < pieces; i += ctas * JOIN_THREADS) reinterpret_cast<uint4 *>(a.out)[i] = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);  // NaN in either type
+        if (cta == 0 && threadIdx.x == 0 && a.status) atomicExch(a.status, -1);
+        return;
+    }
     const int rows = of_tiles ? TA_ROWS : ROWS, i0 = of_tiles ? blockIdx.x % TILE_JOINS * 32 : 0, i1 = min(of_tiles ? i0 + 32 : ROWS, join.rows - join.row0);
     const int64_t slot = rows * (D + 2);
     const float *const from = a.partial + (2 * share + 1) * slot, *const next = a.partial + 2 * share * slot;

@@ -8,7 +8,7 @@ namespace g2d {
 int cache_view(const g2d_cache_desc *d, CacheView *c);
 
 // ---- attention: what its kernels share ----
-// An item that begins in a share and does not end in it: what is to be added up, and for which rows.  Each share's kernel writes one; count 0: none.
+// An item that begins in a share and does not end in it: what is to be added up, and for which rows.  Each share's kernel writes one; count 0: none, -1: the units could not be counted.
 struct AttendJoin {
     int count, row0, rows, first, head;  // parts; the first row and how many the sequence has, its first token, kv head
     int reserved[3];
@@ -87,21 +87,32 @@ struct AttendShares {
     __device__ __forceinline__ unsigned of(unsigned u) const { return u < more * (each + 1) ? u / (each + 1) : more + (u - more * (each + 1)) / each; }
 };
 __device__ __forceinline__ unsigned warp_add(unsigned v) { return __reduce_add_sync(0xffffffffu, v); }
+// A sequence has fewer than 2^31 units, and all have, as long as no token belongs to two.  Offsets that lie over one another may make more of them: sums stop at UNITS_END.
+constexpr unsigned UNITS_END = 0x80000000u;
+__device__ __forceinline__ unsigned units_add(unsigned a, unsigned b) { return min(a + b, UNITS_END); }  // of two up to UNITS_END, one of them below it
+__device__ __forceinline__ unsigned warp_units(unsigned v) {
+    if (warp_add(v >> 6) > UNITS_END >> 6) return UNITS_END;  // else the sum is below 2^31 + 2^11
+    return min(warp_add(v), UNITS_END);
+}
 // All threads of a CTA of WARPS warps: the units of all sequences, units(b) of one, and this lane's first one (of sequence `lane`).  Few sequences: every warp by itself.
 template <int WARPS, typename Units>
 __device__ __forceinline__ unsigned count_units(int batch, Units units, unsigned (&totals)[WARPS], unsigned &mine) {
     const int lane = threadIdx.x & 31;
     mine = units(lane);
-    if (batch <= 32) return warp_add(mine);
+    if (batch <= 32) return warp_units(mine);
     unsigned sum = 0u;
-    for (int b = threadIdx.x; b < batch; b += 32 * WARPS) sum += units(b);
-    sum = warp_add(sum);
+    for (int b = threadIdx.x; b < batch; b += 32 * WARPS) sum = units_add(sum, units(b));
+    sum = warp_units(sum);
     if (lane == 0) totals[threadIdx.x >> 5] = sum;
     __syncthreads();
+    bool past = false;
     unsigned all = 0u;
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) all += totals[w];
-    return all;
+    for (int w = 0; w < WARPS; ++w) {
+        past |= totals[w] == UNITS_END;
+        all = units_add(all, totals[w] & (UNITS_END - 1u));
+    }
+    return past ? UNITS_END : all;
 }
 // A warp: which of its lanes' counts the unit `at` falls into, the first of them beginning at `base` (32: none); `base` becomes where that count begins, or the end
 __device__ __forceinline__ int lane_of_unit(unsigned count, unsigned at, unsigned &base) {
@@ -223,7 +234,7 @@ template <int WARPS>
 __device__ __forceinline__ unsigned count_tile_units(const AttendArgs &a, unsigned (&totals)[WARPS], unsigned &mine) {
     if (a.c.batch <= 8) {
         mine = tile_units_of_few(a);
-        return warp_add(mine);
+        return warp_units(mine);
     }
     return count_units<WARPS>(a.c.batch, [&](int b) { return tile_units(a, b); }, totals, mine);
 }

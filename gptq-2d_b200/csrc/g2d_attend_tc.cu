@@ -140,8 +140,8 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const __gri
     let_the_next_launch_start();
     unsigned mine_units;
     const unsigned units = count_tile_units<TA_THREADS / 32>(a, bar.totals, mine_units);
-    if (threadIdx.x == 0) a.joins[blockIdx.x] = AttendJoin{};
-    if (units == 0) {  // sequences of few rows only
+    if (threadIdx.x == 0) a.joins[blockIdx.x] = AttendJoin{units < UNITS_END ? 0 : -1};
+    if (units == 0 || units >= UNITS_END) {  // sequences of few rows only, or more than can be counted
         after_the_launch_before();
         return;
     }

@@ -8,7 +8,9 @@ The cache is paged.  A step's tokens belong to sequences: sequence ``b`` has the
 ``offsets`` every sequence has the same number of them) and holds ``lengths[b]`` positions, this step's tokens being the last; position ``p`` lies in
 page ``page_table[b, p // page_size]``.  These three are read on the device, so a captured graph follows them.  What they say is never
 trusted with an address: positions beyond the table and page numbers outside the cache are absent (not written, read as zeros, seen by no query).
-Pages may be shared for reading; two tokens of a step that go to the same place leave the row of either, or a mixture.
+Offsets are meant to ascend: where they do
+not, a token may be that of two sequences, and its row is either's (or, where that makes more work than can be counted, all results are NaN and
+``check_status`` reports it).  Pages may be shared for reading; two tokens of a step that go to the same place leave the row of either, or a mixture.
 CUDA only, like the rest of the package; no gradients.
 """
 from __future__ import annotations

@@ -346,7 +346,8 @@ int g2d_cache_read(const g2d_cache_desc *desc, void *k, void *v, void *stream);
 
 /* Attention of the step's tokens over the cache.  Token i of a sequence with n tokens in the step stands at p = length - n + i; query head h reads kv
  * head h / (heads / kv_heads).  Scores u = scale q . k, then softcap tanh(u / softcap) if softcap > 0, then + slopes[h] (j - p) if slopes is given.
- * Seen are the keys j < length; causal: those with j <= p or j < prefix[b] among them.  A row that sees none becomes zeros. */
+ * Seen are the keys j < length; causal: those with j <= p or j < prefix[b] among them.  A row that sees none becomes zeros.  Offsets that do not ascend may
+ * make a token that of two sequences, whose row is either's then; if that makes 2^31 units of work and more, out is NaN and the status word set. */
 typedef struct g2d_attend_desc {
     g2d_cache_desc cache;
     int32_t heads, causal;

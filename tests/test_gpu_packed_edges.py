@@ -86,3 +86,77 @@ def test_a_key_that_is_not_finite_makes_nan_what_sees_it(dtype, head_dim, querie
     for value in (float("inf"), -float("inf"), float("nan")):
         batch.cache.k_scale[pages, :, bad % 32] = value
         seen_and_unseen()
+
+
+def guarded(shape, dtype, fill, room=4096):
+    """A tensor in the middle of a larger one, and what lies around it."""
+    n = torch.Size(shape).numel()
+    whole = torch.full((n + 2 * room,), fill, dtype=dtype, device="cuda")
+    return whole[room:room + n].view(shape), (whole[:room], whole[room + n:])
+
+
+@pytest.mark.parametrize("heads, tokens", [(2, 6), (8, 40), (2, 300)])
+@pytest.mark.parametrize("which", ["beyond both ends", "descending", "all behind", "empty", "overlapping"])
+def test_wild_offsets_touch_nothing_else(which, heads, tokens):
+    """Whatever the offsets say: rows and cache rows outside what they leave after they are brought into range stay as they were, with few rows and with tiles."""
+    import gptq_2d
+    import packed_cache as C
+
+    offsets = {"beyond both ends": [-7, 3, 900], "descending": [5, 2, 1], "all behind": [900, 901, 1 << 30], "empty": [3, 3, 3], "overlapping": [0, tokens, 0, tokens]}[which]
+    count = len(offsets) - 1
+    batch = Batch([(400, 1)] * count, 1, 64, 16, torch.float16)
+    q, k = batch.randn(tokens, heads, 64), batch.randn(tokens, 1, 64)
+    device = torch.tensor(offsets, dtype=torch.int32, device="cuda")
+    pieces = []  # (first, last) of each sequence's tokens as they are brought into range
+    for b in range(count):
+        lo = min(max(offsets[b], 0), tokens)
+        pieces.append((lo, min(max(offsets[b + 1], lo), tokens)))
+    out, around = guarded((tokens, heads, 64), torch.float16, 7.0)
+    C.attend_packed(q, batch.cache, batch.table, batch.lengths, device, out=out)
+    gptq_2d.check_status()
+    torch.cuda.synchronize()
+    assert all((side == 7).all() for side in around)
+    mine = torch.zeros(tokens, dtype=torch.bool, device="cuda")
+    for lo, hi in pieces:
+        mine[lo:hi] = True
+    assert (out[~mine] == 7).all() and not (out[mine] == 7).all(-1).any()
+    if which == "beyond both ends":
+        for b, (lo, hi) in enumerate(pieces):
+            alone = C.attend_packed(q[lo:hi], batch.cache, batch.table[b:b + 1], batch.lengths[b:b + 1])
+            assert (out[lo:hi].float() - alone.float()).abs().max() <= 2 * 8.4 * (2.0 ** -11 + 2.0 ** -12 + 2.0 ** -16)  # cut otherwise, so summed otherwise: both as near as they have to be, |v| <= 8 * 1.05
+    before = [t.clone() for t in batch.cache]
+    C.append_packed(batch.cache, k, k, batch.table, batch.lengths, device)
+    places = torch.zeros(batch.cache.k_scale.shape, dtype=torch.bool, device="cuda")
+    for b, (lo, hi) in enumerate(pieces):
+        for p in range(400 - (hi - lo), 400):
+            places[int(batch.table[b, p // 16]), :, p % 16] = True
+    for old, new in zip(before, batch.cache):
+        assert torch.equal(old[~places].view(torch.uint8), new[~places].view(torch.uint8))
+    got = C.read_packed(batch.cache, batch.table, batch.lengths, device, tokens=tokens, dtype=torch.float16)
+    torch.cuda.synchronize()
+    gptq_2d.check_status()
+    if which != "overlapping":
+        assert not got[0][~mine].any() and got[0][mine].any(-1).all()
+
+
+@pytest.mark.parametrize("heads, tokens, step, page_size, width", [(1, 65536, 65536, 4096, 2040), (8, 64, 8, 1 << 20, 680)])
+def test_offsets_that_make_more_work_than_can_be_counted(heads, tokens, step, page_size, width):
+    """Overlapping sequences whose units pass 32 bits, of tiles and of few rows: refused on the device, at once."""
+    import gptq_2d
+    import packed_cache as C
+
+    batch = 4096 if step == tokens else 64
+    table = torch.full((1, width), -1, dtype=torch.int32, device="cuda").expand(batch, width)  # no page is there
+    offsets = torch.tensor([step * (b % (tokens // step + 1)) for b in range(batch + 1)], dtype=torch.int32, device="cuda")
+    lengths = torch.full((batch,), 2 ** 31 - 1, dtype=torch.int32, device="cuda")
+    cache = C.PackedCache(*(torch.zeros(0, 1, page_size, *rest, dtype=dtype, device="cuda") for dtype, rest in ((torch.uint8, (32,)), (torch.float16, ())) * 2))
+    q = torch.ones(tokens, heads, 64, dtype=torch.float16, device="cuda")
+    gptq_2d.check_status()
+    out, around = guarded(q.shape, torch.float16, 7.0)
+    C.attend_packed(q, cache, table, lengths, offsets, out=out)
+    with pytest.raises(RuntimeError):
+        gptq_2d.check_status()
+    assert out.isnan().all() and all((side == 7).all() for side in around)
+    gptq_2d.check_status()
+    assert not C.attend_packed(q[:8], cache, table[:1], torch.full_like(lengths[:1], 100)).any()  # and the next call is sound
+    gptq_2d.check_status()
