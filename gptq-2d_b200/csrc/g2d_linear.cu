@@ -2,7 +2,9 @@
 //
 // The rows of W are the rows of A of m16n8k16 products, the tokens its columns.  A code goes to the tensor cores as it lies in its word: the bits of c in the lowest
 // (or next) four bits of a 16-bit float are c (or 16 c) times the smallest subnormal, exactly, so eight codes cost a shift and four ANDs; the products
-// with the 16 c go to sums of their own.  fp16 activations are taken as they are; bf16 ones times 2^56, for codes of c 2^-133 (activations from 2^72 up overflow).
+// with the 16 c go to sums of their own.  fp16 activations are taken as they are; bf16 ones times 2^56, for codes of c 2^-133, or, where
+// a token's largest lies outside 2^-12 .. 2^64, times a power of two of the token's own: x is brought once more
+// then (8192 x 8192, 16 tokens: 20.2 us, then 28.2; looking for such tokens costs 2 %).
 // What the codes' origin and zero point add is (qmin - z) sum x, from sums of x over each group that the CTA forms while it brings x to shared memory.
 // A lane reads 16 bytes of codes (32 columns) of two rows, four times ahead; x lies in shared memory in the order in which such
 // words hold their columns, so a fragment of it is one 16-byte load.  With groups of an odd number of 64 columns a lane reads 8 bytes at a time.
@@ -17,6 +19,15 @@
 namespace g2d {
 
 constexpr int ROWS_WARPS = 8, ROWS_THREADS = 32 * ROWS_WARPS;
+
+// bf16: the power of two that brings a token's largest activation (its bits) to 2^100 .. 2^101, so that 2^93 below it nothing is lost to the codes' 2^-133
+__device__ __forceinline__ int token_exponent(unsigned top) { return top == 0u || top >= 0x7f80u ? 56 : 227 - (int)(top >> 7); }  // -27 .. 227
+__device__ __forceinline__ bool token_is_far(unsigned top) { return top != 0u && (top < 0x3980u || (top >= 0x5f80u && top < 0x7f80u)); }  // outside 2^-12 .. 2^64, and finite
+__device__ __forceinline__ uint32_t bf16_pair_times(uint32_t pair, uint32_t factors) {
+    const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162 *>(&pair), *reinterpret_cast<const __nv_bfloat162 *>(&factors));
+    return *reinterpret_cast<const uint32_t *>(&r);
+}
+__device__ __forceinline__ uint32_t bf16_pair_of_powers(int e) { return (uint32_t)(e + 127) * 0x00800080u; }  // of 2^e twice
 
 template <bool BF16>
 __device__ __forceinline__ void mma_codes(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -35,6 +46,7 @@ template <bool BF16, int NT, int KB>
 __global__ void __launch_bounds__(ROWS_THREADS, 2) linear_rows_kernel(const LinearArgs a) {
     constexpr int WORDS = KB / 32, ROWS = 16 * ROWS_WARPS, TOKENS = 8 * NT, CHUNKS = KB / 8, AHEAD = 4;
     extern __shared__ __align__(16) unsigned char linear_smem_raw[];
+    __shared__ unsigned tops[TOKENS];  // bf16: the bits of each token's largest magnitude in this CTA's columns
     const int splits = (int)gridDim.x, rank = (int)blockIdx.x;  // a cluster has all CTAs along x
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int64_t row0 = (int64_t)blockIdx.y * ROWS;
@@ -73,42 +85,77 @@ __global__ void __launch_bounds__(ROWS_THREADS, 2) linear_rows_kernel(const Line
 
     // ---- x: a thread takes eight columns of a token; the CHUNKS threads of a block and token stand together and add up its sum ----
     constexpr int TOGETHER = 4;  // loads of a thread on their way at once
-    for (int e0 = threadIdx.x; e0 - (int)threadIdx.x < mine * TOKENS * CHUNKS; e0 += TOGETHER * ROWS_THREADS) {
-        uint4 v[TOGETHER];
+    const auto piece = [&](int e, int &chunk, int &token, int &block) -> uint4 {  // number e of the share's pieces of eight columns
+        chunk = e % CHUNKS;
+        token = e / CHUNKS % TOKENS;
+        block = e / (CHUNKS * TOKENS);
+        const int64_t k = (b_first + block) * KB + 8 * chunk;
+        return block < mine && k < a.n && token0 + token < a.tokens ? __ldg(reinterpret_cast<const uint4 *>((const uint16_t *)a.x + (int64_t)(token0 + token) * a.x_stride + k)) : make_uint4(0u, 0u, 0u, 0u);
+    };
+    const int all = mine * TOKENS * CHUNKS;
+    float largest = 0.f;  // bf16: what shows that a token may be outside the range of the common power; its exact largest is looked at only then
+    bool small = false;
+    const auto bring = [&](auto own_powers) {
+        constexpr bool OWN = decltype(own_powers)::value;
+        for (int e0 = threadIdx.x; e0 - (int)threadIdx.x < all; e0 += TOGETHER * ROWS_THREADS) {
+            uint4 v[TOGETHER];
+            int chunk, token, block;
 #pragma unroll
-        for (int q = 0; q < TOGETHER; ++q) {
-            const int e = e0 + q * ROWS_THREADS, chunk = e % CHUNKS, token = token0 + e / CHUNKS % TOKENS, block = e / (CHUNKS * TOKENS);
-            const int64_t k = (b_first + block) * KB + 8 * chunk;
-            v[q] = make_uint4(0u, 0u, 0u, 0u);
-            if (block < mine && k < a.n && token < a.tokens) v[q] = __ldg(reinterpret_cast<const uint4 *>((const uint16_t *)a.x + (int64_t)token * a.x_stride + k));
-        }
+            for (int q = 0; q < TOGETHER; ++q) v[q] = piece(e0 + q * ROWS_THREADS, chunk, token, block);
 #pragma unroll
-        for (int q = 0; q < TOGETHER; ++q) {
-            const int e = e0 + q * ROWS_THREADS, chunk = e % CHUNKS, token = e / CHUNKS % TOKENS, block = e / (CHUNKS * TOKENS);
-            if (e - (int)threadIdx.x >= mine * TOKENS * CHUNKS) break;
-            float sum = 0.f;
-            uint32_t u[4] = {v[q].x, v[q].y, v[q].z, v[q].w};
+            for (int q = 0; q < TOGETHER; ++q) {
+                const int e = e0 + q * ROWS_THREADS;
+                if (e - (int)threadIdx.x >= all) break;
+                chunk = e % CHUNKS;
+                token = e / CHUNKS % TOKENS;
+                block = e / (CHUNKS * TOKENS);
+                float sum = 0.f;
+                uint32_t u[4] = {v[q].x, v[q].y, v[q].z, v[q].w};
+                if (OWN) {
+                    const int power = token_exponent(tops[token]), half = power >> 1;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                sum += bits_to_float(u[i] & 0xffffu, BF16) + bits_to_float(u[i] >> 16, BF16);
-                if (BF16) {
-                    __nv_bfloat162 p = *reinterpret_cast<__nv_bfloat162 *>(&u[i]);
-                    p = __hmul2(p, __float2bfloat162_rn(72057594037927936.f));  // 2^56
-                    u[i] = *reinterpret_cast<uint32_t *>(&p);
+                    for (int i = 0; i < 4; ++i) u[i] = bf16_pair_times(bf16_pair_times(u[i], bf16_pair_of_powers(half)), bf16_pair_of_powers(power - half));
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float x0 = bits_to_float(u[i] & 0xffffu, BF16), x1 = bits_to_float(u[i] >> 16, BF16);
+                    sum += x0 + x1;
+                    if (BF16 && !OWN) {
+                        largest = fmaxf(fmaxf(largest, fabsf(x0)), fabsf(x1));
+                        u[i] = bf16_pair_times(u[i], bf16_pair_of_powers(56));
+                    }
+                }
+#pragma unroll
+                for (int o = 1; o < CHUNKS; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                if (block < mine) {
+                    // columns (0, 4), (2, 6), (1, 5), (3, 7): two codes of a word that lie sixteen bits apart
+                    const uint4 f = make_uint4(__byte_perm(u[0], u[2], 0x5410), __byte_perm(u[1], u[3], 0x5410), __byte_perm(u[0], u[2], 0x7632), __byte_perm(u[1], u[3], 0x7632));
+                    const int w = chunk % WORDS, lane_of = (token & 7) * 4 + chunk / WORDS;
+                    xs[((block * WORDS + w) * NT + (token >> 3)) * 32 + lane_of] = f;
+                    if (BF16 && !OWN) small |= fabsf(sum) < 9.3e-10f && (u[0] | u[1] | u[2] | u[3]) != 0u;  // 2^-30: where a block's sum is not below that, its largest is not below 2^-37; zeros are no matter
+                    if (chunk == 0) sums[block * TOKENS + token] = OWN ? sum * 1.3877787807814457e-17f : sum;  // 2^-56: in the units of the common power's products
                 }
             }
-#pragma unroll
-            for (int o = 1; o < CHUNKS; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            if (block < mine) {
-                // columns (0, 4), (2, 6), (1, 5), (3, 7): two codes of a word that lie sixteen bits apart
-                const uint4 f = make_uint4(__byte_perm(u[0], u[2], 0x5410), __byte_perm(u[1], u[3], 0x5410), __byte_perm(u[0], u[2], 0x7632), __byte_perm(u[1], u[3], 0x7632));
-                const int w = chunk % WORDS, lane_of = (token & 7) * 4 + chunk / WORDS;
-                xs[((block * WORDS + w) * NT + (token >> 3)) * 32 + lane_of] = f;
-                if (chunk == 0) sums[block * TOKENS + token] = sum;
-            }
         }
+    };
+    bring(std::false_type());
+    bool own = false;  // bf16: every token under a power of two of its own
+    if (!BF16) {
+        __syncthreads();
+    } else if (__syncthreads_or(small || largest >= 18446744073709551616.f)) {  // 2^64
+        if (threadIdx.x < TOKENS) tops[threadIdx.x] = 0u;
+        __syncthreads();
+        for (int e = threadIdx.x; e < all; e += ROWS_THREADS) {
+            int chunk, token, block;
+            const uint4 v = piece(e, chunk, token, block);
+            const uint32_t pair = __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
+            atomicMax(&tops[token], max(pair & 0xffffu, pair >> 16));
+        }
+        __syncthreads();
+        for (int i = 0; i < TOKENS; ++i) own |= token_is_far(tops[i]);
+        if (own) bring(std::true_type());
+        __syncthreads();
     }
-    __syncthreads();
 
     // ---- products ----
     constexpr float BACK = BF16 ? 151115727451828646838272.f : 16777216.f;  // 2^(133 - 56) = 2^77, or 2^24
@@ -168,6 +215,15 @@ __global__ void __launch_bounds__(ROWS_THREADS, 2) linear_rows_kernel(const Line
                 total[j][x] = fmaf(x < 2 ? s_lo : s_hi, fmaf(x < 2 ? o_lo : o_hi, xsum[j][x & 1], products), total[j][x]);
             }
         }
+    }
+    if (BF16 && own) {  // from units of the token's power over the common one
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const int power = token_exponent(tops[8 * j + 2 * t + (x & 1)]) - 56, half = power >> 1;
+                total[j][x] = total[j][x] * power_of_two(-half) * power_of_two(half - power);
+            }
     }
     // ---- sums of the cluster ----
 #pragma unroll

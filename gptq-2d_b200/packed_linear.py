@@ -49,7 +49,7 @@ def packed_linear(x: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor, zer
     the same number).  Zero points are meant to be integers: with many tokens ``code + qmin - zero_point`` is rounded to x's type, exact up to 256 (bfloat16) or 2048 (float16).
     With ``adapters``, ``adapter_index`` (int32, one per token, in the order of ``x``'s leading dimensions) says whose adapter is added to a token's result; an index outside
     the adapters' range means none.  Sums are float32, results are rounded once to x's type.  ``out`` may be given as a contiguous ``[..., m]`` tensor, which must not
-    overlap the inputs.  bfloat16 activations of 2**72 and more may overflow."""
+    overlap the inputs."""
     assert bits == 4, "only codes of 4 bits can be multiplied with"
     device, dtype, shape = x.device, x.dtype, x.shape
     index = device.index

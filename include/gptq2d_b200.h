@@ -369,8 +369,7 @@ int g2d_cache_attend(const g2d_attend_desc *desc, void *stream);
  * activations times the transpose of a matrix in packed 4-bit codes (g2d_pack_codes; n a multiple of 32, row_bytes a multiple of 16), and beside it the low-rank
  * adapter of each token's request.  Tokens whose index lies outside [0, adapters) have none.  `groups` equal groups of columns (1, or of a multiple of
  * 64 columns each) have scales and zero points of their own, float, addressed by row and group strides in elements (0 = broadcast).  code + qmin - zero is
- * rounded to x's type where there are many tokens: exact for integers up to 256 (bf16) or 2048 (fp16).  Sums are float32; out is rounded once.
- * Few tokens: bf16 activations of 2^72 and more overflow. */
+ * rounded to x's type where there are many tokens: exact for integers up to 256 (bf16) or 2048 (fp16).  Sums are float32; out is rounded once. */
 typedef struct g2d_linear_desc {
     int32_t half, bits;          /* g2d_half of x, down, up and out; 4 */
     int64_t m, n, tokens;

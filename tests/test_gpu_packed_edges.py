@@ -160,3 +160,34 @@ def test_offsets_that_make_more_work_than_can_be_counted(heads, tokens, step, pa
     gptq_2d.check_status()
     assert not C.attend_packed(q[:8], cache, table[:1], torch.full_like(lengths[:1], 100)).any()  # and the next call is sound
     gptq_2d.check_status()
+
+
+POWERS = [-118, -100, -80, -73, -62, -50, -30, -13, -12, -11, 0, 40, 63, 64, 65, 71, 72, 73, 90, 110]
+
+
+@pytest.mark.parametrize("adapters", [0, 2])
+@pytest.mark.parametrize("groups, n", [(1, 1280), (5, 320), (1, 4096)])
+@pytest.mark.parametrize("tokens", [1, 8, 16, 20])
+def test_bf16_activations_of_any_magnitude(tokens, groups, n, adapters):
+    """Tokens each of a size of their own, from near the smallest normal numbers to near the largest."""
+    p = Problem(130, n, tokens, torch.bfloat16, groups=groups, adapters=adapters, rank=8)
+    x = p.x.float()
+    for first in range(0, len(POWERS), tokens):
+        powers = torch.tensor([POWERS[(first + t) % len(POWERS)] for t in range(tokens)], device="cuda").float()
+        p.x = (x * torch.exp2(powers)[:, None]).bfloat16()
+        p.check()
+
+
+@pytest.mark.parametrize("tokens", [1, 5, 16])
+@pytest.mark.parametrize("low, high", [(-100, 0), (-70, 70), (-126, -90), (0, 100), (-133, 0)])
+def test_bf16_activations_of_mixed_magnitudes(low, high, tokens):
+    """Columns of very different sizes: in halves (other CTAs' columns), in turn, a single large one, and zeros."""
+    p = Problem(200, 2048, tokens, torch.bfloat16)
+    x = p.x.float()
+    small, large = (x * 2.0 ** low).bfloat16(), (x * 2.0 ** high).bfloat16()
+    k = torch.arange(2048, device="cuda")
+    for pick in (k < 1024, k >= 1024, k % 2 == 0, k == 77, k < 0):
+        p.x = torch.where(pick, large, small)
+        p.check()
+        p.x = torch.where(pick, large, torch.zeros_like(small))
+        p.check()
