@@ -191,3 +191,30 @@ def test_bf16_activations_of_mixed_magnitudes(low, high, tokens):
         p.check()
         p.x = torch.where(pick, large, torch.zeros_like(small))
         p.check()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("m, n, groups", [(130, 96, 1), (200, 320, 5), (70, 4096, 1), (257, 2048, 16)])
+@pytest.mark.parametrize("tokens", [1, 4, 9, 16, 17, 80])
+def test_infinite_activations(tokens, m, n, groups, dtype):
+    """Infinities, or NaN where a weight is zero or they have both signs: as a product with the unpacked matrix has them, however many tokens there are."""
+    inf = float("inf")
+    p = Problem(m, n, tokens, dtype, groups)
+    clean, x = p.check(), p.x.clone()
+    field = torch.stack((p.codes & 15, p.codes >> 4), -1).flatten(1).double()
+    wide = lambda t: t.double().repeat_interleave(n // groups, 1)  # noqa: E731
+    w = (field + p.qmin - wide(p.zero)) * wide(p.scale)
+    some = 7 % tokens
+    for spots in ([(0, 5, inf)], [(0, n - 1, -inf)], [(some, 3, inf), (some, n // 2, -inf), (some, n - 2, inf)], [(0, 31, inf), (0, 32, inf)], [(0, 8, inf), (0, 9, float("nan"))],
+                  [(t, (37 * t) % n, inf if t % 3 else -inf) for t in range(tokens)]):
+        p.x = x.clone()
+        want, touched = torch.zeros(tokens, m, dtype=torch.float64, device="cuda"), set()
+        for token, k, value in spots:
+            p.x[token, k] = value
+            want[token] += w[:, k] * value
+            touched.add(token)
+        got = p.run()
+        for token in range(tokens):
+            assert torch.equal(got[token], clean[token]) if token not in touched else torch.equal(got[token].double().nan_to_num(nan=1.0), want[token].nan_to_num(nan=1.0)), (spots, token)
+    p.x = x.fill_(float("nan"))
+    assert p.run().isnan().all()
