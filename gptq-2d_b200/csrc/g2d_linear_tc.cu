@@ -140,17 +140,26 @@ __device__ __forceinline__ uint4 load_16(uint32_t at) {
     return v;
 }
 
-// A warp that arrives at another CTA's barrier with .release waits until all it wrote has arrived everywhere (a thousand cycles, in the middle of the pipeline's chain:
-// 8192 x 28672, 2048 tokens, 940 and 885 us).  What the coders write stays in their CTA's shared memory and is read by that SM's tensor core alone; they have brought it
-// there by their proxy fence before they arrive, so that the message itself need order nothing.  Nor need that of the warps that have read an accumulator: their loads have
-// ended (4096 x 4096, 1024 tokens, groups of 64: 113 and 80 us, one scale a row 51 and 49; 8192 x 28672, 2048 tokens 789 and 752).
+// The W that a CTA's coders have written is read by products that the other CTA, the leader, issues.  Arriving at the leader's barrier with .release takes a thread two thousand cycles (one
+// that does nothing else: 8192 x 28672, 2048 tokens, adapters of rank 32 1787 us, two 1079).  So the coders arrive at a barrier of their own CTA, and one thread,
+// which acquires that, lets a bulk copy tell the leader: of 16 bytes of that W, to be counted at the leader's barrier.  The copy is carried out behind what its thread has
+// acquired, its end is a release for the cluster, and the thread need not wait for it (775 us; 759 with a relaxed arrival, which
+// orders nothing).
+__device__ __forceinline__ void tell_leader(uint4 *to, uint32_t from, uint64_t *bar) {
+    uint32_t there;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(there) : "r"(smem_u32(to)));
+    asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], 16, [%2];" ::"r"(there), "r"(from), "r"(leaders(bar)) : "memory");
+}
+// The warps that have read an accumulator have written nothing, and their loads have ended: their message to the leader need order nothing (4096 x 4096, 1024 tokens, groups of
+// 64: 113 us with .release, 80 us, one scale a row 51 and 49; 8192 x 28672, 2048 tokens 789 and 752).
 __device__ __forceinline__ void arrive_relaxed(uint32_t bar) { asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
 
 template <int NT, bool DUO>
 struct LinearBarriers {
     using S = LinearShape<NT, DUO>;
-    // full: x has landed (or the rows of an adapter) and W is written, in both CTAs: the leader's; empty: the products have read the slot
-    uint64_t full[S::SLOTS], empty[S::SLOTS], code_full[S::SLOTS], code_empty[S::SLOTS], acc_full[S::ACCUMULATORS], acc_empty[S::ACCUMULATORS], drained;
+    uint4 told[S::SLOTS];  // what the other CTA's copies leave
+    // full: x has landed (or the rows of an adapter) and W is written, in both CTAs: the leader's; coded: W is written, in the other CTA; empty: the products have read the slot
+    uint64_t full[S::SLOTS], coded[S::SLOTS], empty[S::SLOTS], code_full[S::SLOTS], code_empty[S::SLOTS], acc_full[S::ACCUMULATORS], acc_empty[S::ACCUMULATORS], drained;
     LinePart part;
     uint32_t tmem;
     int failed;
@@ -161,7 +170,7 @@ __global__ void __launch_bounds__(LinearShape<NT, DUO>::THREADS, 1) linear_tc_ke
     using S = LinearShape<NT, DUO>;
     constexpr int CTAS = DUO ? 2 : 1, ACC = S::ACCUMULATORS, SLOTS = S::SLOTS;
     extern __shared__ unsigned char linear_tc_smem[];
-    __shared__ __align__(8) LinearBarriers<NT, DUO> bar;
+    __shared__ __align__(16) LinearBarriers<NT, DUO> bar;
     const LinearArgs &a = job.a;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = DUO ? (int)cluster_rank() : 0;
     const uint32_t base = (smem_u32(linear_tc_smem) + 1023u) & ~1023u, codes_base = base + SLOTS * S::SLOT;
@@ -172,7 +181,8 @@ __global__ void __launch_bounds__(LinearShape<NT, DUO>::THREADS, 1) linear_tc_ke
     };
     if (threadIdx.x == 0) {
         for (int s = 0; s < SLOTS; ++s) {
-            mbar_init(&bar.full[s], 1 + CTAS * S::TEAM);
+            mbar_init(&bar.full[s], 1 + S::TEAM);
+            mbar_init(&bar.coded[s], S::TEAM);
             mbar_init(&bar.empty[s], 1);
             mbar_init(&bar.code_full[s], 1);
             mbar_init(&bar.code_empty[s], S::TEAM);
@@ -213,10 +223,10 @@ __global__ void __launch_bounds__(LinearShape<NT, DUO>::THREADS, 1) linear_tc_ke
             LinearItem it;
             int slot = 0;
             uint32_t parity = 1, turns = 0;
-            const auto begin = [&](uint32_t bytes) {  // the next slot is free and expects so many bytes in each CTA
+            const auto begin = [&](uint32_t bytes, uint32_t more) {  // the next slot is free and expects so many bytes in each CTA, and more of the other one's copy
                 if (bar.failed || (turns >= SLOTS && !wait(&bar.empty[slot], parity, 32))) return false;
                 // DUO: both CTAs' bytes count at the leader's barrier (they may do so before it expects them: the phase waits for its arrival)
-                if (rank == 0) mbar_expect_tx(&bar.full[slot], CTAS * bytes);
+                if (rank == 0) mbar_expect_tx(&bar.full[slot], CTAS * bytes + more);
                 return true;
             };
             const auto bring = [&](const CUtensorMap *map, int column, int row) {
@@ -231,14 +241,14 @@ __global__ void __launch_bounds__(LinearShape<NT, DUO>::THREADS, 1) linear_tc_ke
             for (int i = 0; go && item(i, it); ++i) {
                 const int token = it.token0 + rank * S::X_ROWS;
                 for (int ch = it.c0; go && ch < it.c1; ++ch) {
-                    go = begin(S::X_BYTES);
+                    go = begin(S::X_BYTES, DUO ? 16 : 0);
                     if (!go) break;
                     bring(&job.x, ch * KH, token);
                     next();
                 }
                 const int extra = go ? 2 * adapters_in(it) : 0;
                 for (int e = 0; go && e < extra; ++e) {
-                    go = begin(S::X_BYTES + LT_W_BYTES);
+                    go = begin(S::X_BYTES + LT_W_BYTES, 0);
                     if (!go) break;
                     bring(&job.inner, (e & 1) * RANK_MAX, token);
                     const uint32_t to = base + slot * S::SLOT + S::X_BYTES;
@@ -281,7 +291,10 @@ __global__ void __launch_bounds__(LinearShape<NT, DUO>::THREADS, 1) linear_tc_ke
             int slot = 0, slice = 0;
             uint32_t parity = 0;
             const auto ready = [&] {
-                if (!wait(&bar.full[slot], parity, 0)) return false;
+                if (!(DUO ? mbar_wait_cluster(&bar.full[slot], parity, 0, a.wait_cycles) : mbar_wait(&bar.full[slot], parity, 0, a.wait_cycles))) {
+                    bar.failed = 1;
+                    return false;
+                }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 return true;
             };
@@ -331,6 +344,21 @@ __global__ void __launch_bounds__(LinearShape<NT, DUO>::THREADS, 1) linear_tc_ke
             } else {
                 for (int k = max(slice - ACC, 0); k < slice; ++k) mbar_wait(&bar.acc_full[k % ACC], (k / ACC) & 1);
             }
+        } else if (DUO && warp == 1 && rank != 0 && elected()) {  // the other CTA's W, slot after slot (rows of `up` come by the TMA, which counts at the leader's barrier itself)
+            LinearItem it;
+            int slot = 0;
+            uint32_t parity = 0;  // each slot's
+            bool go = true;
+            for (int i = 0; go && item(i, it); ++i) {
+                for (int ch = it.c0; ch < it.c1; ++ch) {
+                    go = !bar.failed && wait(&bar.coded[slot], (parity >> slot) & 1, 0);
+                    if (!go) break;
+                    parity ^= 1u << slot;
+                    tell_leader(&bar.told[slot], base + slot * S::SLOT + S::X_BYTES, &bar.full[slot]);
+                    if (++slot == SLOTS) slot = 0;
+                }
+                if (go) slot = (slot + 2 * adapters_in(it)) % SLOTS;
+            }
         }
         __syncwarp();
     } else if (warp < first_reader) {
@@ -350,10 +378,7 @@ __global__ void __launch_bounds__(LinearShape<NT, DUO>::THREADS, 1) linear_tc_ke
             return go;
         };
         const auto written = [&] {
-            if (lane == 0) {
-                if (DUO) arrive_relaxed(leaders(&bar.full[slot]));
-                else mbar_arrive(&bar.full[slot]);
-            }
+            if (lane == 0) mbar_arrive(DUO && rank != 0 ? &bar.coded[slot] : &bar.full[slot]);
         };
         for (int i = 0; go && item(i, it); ++i) {
             const float *const zero0 = a.zero + min((int64_t)it.row0 + row, a.m - 1) * a.zero_row, *const zero1 = a.zero + min((int64_t)it.row0 + row + 64, a.m - 1) * a.zero_row;
@@ -412,7 +437,7 @@ __global__ void __launch_bounds__(LinearShape<NT, DUO>::THREADS, 1) linear_tc_ke
             first = (first + it.c1 - it.c0) % SLOTS;
             for (int e = (slot - first + SLOTS) % SLOTS; e < extra; e += SLOTS) {  // rows of `up`, which the TMA brings: the slot is free for them
                 if (!free_slot()) break;
-                written();
+                if (rank == 0) written();
             }
             first = (first + extra) % SLOTS;
         }

@@ -146,7 +146,7 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint64_t *bar, uint32_t parity
             : "memory");
         if (ok) return true;
         if (clock64() - start > limit) return false;
-        __nanosleep(nap);
+        if (nap) __nanosleep(nap);
     }
 }
 // into this CTA's shared memory, counted at a barrier of either CTA

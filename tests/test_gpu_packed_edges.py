@@ -218,3 +218,15 @@ def test_infinite_activations(tokens, m, n, groups, dtype):
             assert torch.equal(got[token], clean[token]) if token not in touched else torch.equal(got[token].double().nan_to_num(nan=1.0), want[token].nan_to_num(nan=1.0)), (spots, token)
     p.x = x.fill_(float("nan"))
     assert p.run().isnan().all()
+
+
+@pytest.mark.parametrize("m, n, tokens, adapters, rank", [(5100, 1056, 600, 3, 8), (4097, 1440, 513, 7, 40), (2300, 3104, 300, 0, 8), (20000, 480, 1025, 5, 64), (4096, 2048, 2300, 2, 16)])
+def test_pairs_of_ctas(m, n, tokens, adapters, rank):
+    """Tiles by two CTAs, whose slots chunks and adapters take in turn: any number of both, the last rows and tokens in either CTA, the same from cold caches."""
+    for dtype, groups in ((torch.float16, 1), (torch.bfloat16, n // 32 if n % 64 else n // 64)):
+        p = Problem(m, n, tokens, dtype, groups=groups if n // groups % 64 == 0 else 1, adapters=adapters, rank=rank)
+        first = p.check()
+        flush = torch.empty(256 << 20, dtype=torch.uint8, device="cuda")
+        for i in range(3):
+            flush.fill_(i)
+            assert torch.equal(p.run(), first)
