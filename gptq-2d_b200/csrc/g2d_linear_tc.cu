@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(LinearShape<NT, DUO>::THREADS, 1) linear_tc_ke
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = DUO ? (int)cluster_rank() : 0;
     const uint32_t base = (smem_u32(linear_tc_smem) + 1023u) & ~1023u, codes_base = base + SLOTS * S::SLOT;
     const auto wait = [&](uint64_t *b, uint32_t parity, unsigned nap) {
-        if (mbar_wait(b, parity, nap, a.wait_cycles)) return true;
+        if (DUO ? mbar_wait_cluster(b, parity, nap, a.wait_cycles) : mbar_wait(b, parity, nap, a.wait_cycles)) return true;
         bar.failed = 1;
         return false;
     };
@@ -291,10 +291,7 @@ __global__ void __launch_bounds__(LinearShape<NT, DUO>::THREADS, 1) linear_tc_ke
             int slot = 0, slice = 0;
             uint32_t parity = 0;
             const auto ready = [&] {
-                if (!(DUO ? mbar_wait_cluster(&bar.full[slot], parity, 0, a.wait_cycles) : mbar_wait(&bar.full[slot], parity, 0, a.wait_cycles))) {
-                    bar.failed = 1;
-                    return false;
-                }
+                if (!wait(&bar.full[slot], parity, 0)) return false;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 return true;
             };
