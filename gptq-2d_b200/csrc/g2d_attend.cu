@@ -771,11 +771,13 @@ extern "C" int g2d_cache_attend(const g2d_attend_desc *d, void *stream) {
     a.rows_to = line;
     a.partial = (float *)d->workspace;
     const bool narrow = a.group <= 8 && (rows < 0 ? ceil_div((int64_t)a.c.tokens * a.group, (int64_t)a.c.batch) : rows) <= 8;
-    // Short tables, the same number of queries everywhere: items whole in their shares, a CTA's warps some blocks each, and no join; longer ones where there are about as many items as CTAs.
-    // 32 heads on 8, 128 channels, four queries, (16 x) 2000 keys, capped: 39.4 us cut evenly, 30.9 whole; sequences of 4 to 2000 keys 33.8, 28.8; 32 sequences of 500 30.9, 21.4; but 8 of 4 to
-    // 2000 23.2, 27.6, one of 2000 19.8, 28.4, and 64 of 4 to 2000 74.9, 83.9
+    // Short tables, the same number of queries everywhere: items whole in their shares, a CTA's warps some blocks each, and no join; longer ones where there are about as many items as CTAs.  Time cut
+    // evenly over time whole, 32 heads on 8, 128 channels, one and four queries, capped or not, all lengths alike or random, by the number of items: up to 300 and 500 keys 0.98 .. 1.37
+    // (8 .. 144 items), 0.94 .. 1.43 (152 .. 296), 0.89 .. 1.37 (384, 512); 1000 keys 1.01 .. 1.50 (96 .. 144), 0.89 .. 1.24 (152 .. 176), 1.02 .. 1.53 (200 .. 296); 2000 keys 1.06 .. 1.38 (96 .. 144),
+    // 0.80 .. 1.04, 0.89 in the mean (152 .. 176: a second round that few CTAs have), 0.93 .. 1.35 (200 .. 296).  Fewer and more, 2000 keys: 64 items 0.84, one sequence 0.70, 512 0.89.
     const int64_t most_keys = (int64_t)a.c.table_width << a.c.page_shift, items = rows < 0 ? 0 : (int64_t)a.c.batch * a.c.kv_heads * ceil_div(rows, (int64_t)(narrow ? 8 : 16));
-    const bool whole = !many && !a.c.offsets && (most_keys <= 512 || (most_keys <= 2048 && items >= 96 && items <= 2 * ATTEND_GRID));
+    const bool rounds_filled = items >= 96 && items <= 2 * ATTEND_GRID && (items <= ATTEND_GRID || items >= 200 || most_keys <= 1024);
+    const bool whole = !many && !a.c.offsets && (most_keys <= 512 || (most_keys <= 2048 && rounds_filled));
     a.even = !whole ? 0 : most_keys > CACHE_BLOCK ? (int)ceil_div(most_keys, (int64_t)CACHE_BLOCK) : 1;
     // Of two kernels one has most of the work, as a rule: the one for the sequences' mean.  The other finds its part, or that it has none, while that one's last CTAs work
     const bool rows_first = (int64_t)a.c.tokens * a.group < (int64_t)line * a.c.batch;

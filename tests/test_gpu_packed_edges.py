@@ -2,7 +2,7 @@
 64 bits and tolerances are those of the files that test the operators one by one."""
 import pytest
 import torch
-from test_gpu_packed_cache import Batch
+from test_gpu_packed_cache import Batch, assert_near, reference
 from test_gpu_packed_linear import Problem
 
 pytestmark = pytest.mark.gpu
@@ -230,3 +230,21 @@ def test_pairs_of_ctas(m, n, tokens, adapters, rank):
         for i in range(3):
             flush.fill_(i)
             assert torch.equal(p.run(), first)
+
+
+@pytest.mark.parametrize("width", [512, 528, 1024, 1040, 2048, 2064])
+@pytest.mark.parametrize("queries, heads", [(1, 8), (4, 32)])
+@pytest.mark.parametrize("count", [23, 24, 37, 38, 49, 50, 74, 75])
+def test_either_side_of_whole_items(count, queries, heads, width):
+    """Items cut evenly and items whole to each CTA: 92 to 300 of them on tables of 512 to 2064 positions."""
+    import packed_cache as C
+
+    lengths = [width if b == 0 else max((53 * b) % width, queries) for b in range(count)]
+    batch = Batch([(n, queries) for n in lengths], 4, 64, 16, torch.bfloat16, seed=count)
+    q = batch.randn(count * queries, heads, 64)
+    got = C.attend_packed(q, batch.cache, batch.table, batch.lengths)
+    want = reference(batch, q)
+    assert_near(got, *want)
+    wide = torch.cat((batch.table, torch.full((count, 300), -1, dtype=torch.int32, device="cuda")), 1)  # the same sequences in a table for longer ones
+    assert_near(C.attend_packed(q, batch.cache, wide, batch.lengths), *want)
+    assert_near(C.attend_packed(q, batch.cache, wide[:, :batch.table.shape[1]], batch.lengths), *want)
