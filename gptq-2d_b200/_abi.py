@@ -77,28 +77,6 @@ class StageDesc(ctypes.Structure):
     ]
 
 
-class CacheDesc(ctypes.Structure):
-    """Mirror of ``g2d_cache_desc``."""
-    _fields_ = [
-        ("half", _i32), ("head_dim", _i32), ("page_size", _i32), ("kv_heads", _i32),
-        ("pages", _i64), ("batch", _i64), ("table_width", _i64), ("table_stride", _i64), ("tokens", _i64),
-        ("k_codes", _vp), ("k_scale", _vp), ("v_codes", _vp), ("v_scale", _vp),
-        ("table", _vp), ("lengths", _vp), ("offsets", _vp),
-    ]
-
-
-class AttendDesc(ctypes.Structure):
-    """Mirror of ``g2d_attend_desc``."""
-    _fields_ = [
-        ("cache", CacheDesc),
-        ("heads", _i32), ("causal", _i32), ("scale", ctypes.c_float), ("softcap", ctypes.c_float),
-        ("q", _vp), ("q_token_stride", _i64), ("q_head_stride", _i64), ("out", _vp),
-        ("slopes", _vp), ("prefix", _vp),
-        ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
-        ("status", _vp),
-    ]
-
-
 # Descriptors of the calls of a serving step, which are as short as the host code around them: packed in one go instead of field by field (2 us less
 # for thirty fields).  Native alignment, so the formats follow the header's fields in order.
 CACHE_DESC = struct.Struct("@4i5q7P")  # g2d_cache_desc

@@ -11,3 +11,10 @@ def test_rows_of_activations_that_overlap_are_refused_by_tiles(lib, x_stride, to
 
     fields = {**half_of(LINEAR), "tokens": tokens, "n": n, "row_bytes": -(-n // 32) * 16, "x_stride": x_stride, "workspace": 256, "bytes": 1 << 40}
     assert refused(lib.g2d_packed_linear(_abi.LINEAR_DESC.pack(*fields.values()), 0))
+
+
+def test_the_library_has_one_description_of_each_descriptor():
+    """A mirror of a descriptor beside the packed formats would have to be kept like them, and nothing uses one."""
+    import _abi
+
+    assert not any(hasattr(_abi, name) for name in ("CacheDesc", "AttendDesc", "LinearDesc"))
