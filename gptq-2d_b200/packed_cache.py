@@ -52,6 +52,10 @@ class PackedCache(_Tensors):
         self.layout = (2 * half_dim, page_size, kv_heads, pages)
         return self
 
+    @classmethod
+    def _make(cls, tensors):  # what _replace goes through: checked as well
+        return cls(*tensors)
+
 
 def _check_layout(page_size: int, head_dim: int) -> None:
     assert head_dim in (64, 128), "head_dim must be 64 or 128"

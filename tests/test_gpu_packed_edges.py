@@ -248,3 +248,16 @@ def test_either_side_of_whole_items(count, queries, heads, width):
     wide = torch.cat((batch.table, torch.full((count, 300), -1, dtype=torch.int32, device="cuda")), 1)  # the same sequences in a table for longer ones
     assert_near(C.attend_packed(q, batch.cache, wide, batch.lengths), *want)
     assert_near(C.attend_packed(q, batch.cache, wide[:, :batch.table.shape[1]], batch.lengths), *want)
+
+
+def test_caches_made_from_others():
+    """A cache with some of its tensors replaced works like one that was made of them."""
+    import packed_cache as C
+
+    batch = Batch([(100, 3), (40, 1)], 2, 64, 16, torch.float16)
+    q = batch.randn(4, 4, 64)
+    want = C.attend_packed(q, batch.cache, batch.table, batch.lengths, batch.offsets)
+    other = batch.cache._replace(k_codes=batch.cache.k_codes.clone(), v_scale=batch.cache.v_scale.clone())
+    assert isinstance(other, C.PackedCache) and torch.equal(C.attend_packed(q, other, batch.table, batch.lengths, batch.offsets), want)
+    with pytest.raises(AssertionError):
+        batch.cache._replace(k_scale=batch.cache.k_scale.float())
