@@ -261,3 +261,44 @@ def test_caches_made_from_others():
     assert isinstance(other, C.PackedCache) and torch.equal(C.attend_packed(q, other, batch.table, batch.lengths, batch.offsets), want)
     with pytest.raises(AssertionError):
         batch.cache._replace(k_scale=batch.cache.k_scale.float())
+
+
+@pytest.mark.parametrize("queries", [1, 6, 90])
+@pytest.mark.parametrize("head_dim", [64, 128])
+def test_queries_of_any_strides(head_dim, queries):
+    """Heads before tokens, one head or one token for all, parts of something wider, windows that overlap, rows off 16 bytes: as their copies, to the last bit."""
+    import packed_cache as C
+
+    batch = Batch([(200, queries)] * 3, 2, head_dim, 16, torch.bfloat16)
+    tokens, heads = batch.tokens, 8
+    base = batch.randn(tokens + 4, heads + 4, 2 * head_dim + 8)
+    flat = batch.randn(tokens * heads * head_dim + 64 * heads + head_dim)
+    forms = [base[:tokens, :heads, :head_dim].transpose(0, 1).contiguous().transpose(0, 1), base[:tokens, :1, :head_dim].expand(tokens, heads, head_dim), base[:1, :heads, :head_dim].expand(tokens, heads, head_dim),
+             base[2:2 + tokens, 3:3 + heads, 16:16 + head_dim], base[:tokens, :heads, 1:1 + head_dim], flat.as_strided((tokens, heads, head_dim), (8, 64, 1)),
+             base[:tokens, :heads, :head_dim].transpose(1, 2).contiguous().transpose(1, 2)]
+    for q in forms:
+        plain = q.clone(memory_format=torch.contiguous_format)
+        want = C.attend_packed(plain, batch.cache, batch.table, batch.lengths)
+        assert_near(want, *reference(batch, plain))
+        assert torch.equal(C.attend_packed(q, batch.cache, batch.table, batch.lengths), want)
+        assert torch.equal(C.attend_packed(q, batch.cache, batch.table, batch.lengths, batch.offsets), C.attend_packed(plain, batch.cache, batch.table, batch.lengths, batch.offsets))
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.2, 1e-30, 3.0])
+@pytest.mark.parametrize("queries", [1, 5, 70])
+def test_scales_of_any_sign(queries, scale):
+    batch = Batch([(150, queries), (queries, queries)], 1, 64, 16, torch.float16)
+    q = 0.3 * batch.randn(batch.tokens, 4, 64)
+    import packed_cache as C
+
+    for options in ({}, {"softcap": 3.0}, {"slopes": torch.linspace(-0.05, 0.05, 4, device="cuda")}):
+        assert_near(C.attend_packed(q, batch.cache, batch.table, batch.lengths, batch.offsets, scale=scale, **options), *reference(batch, q, scale=scale, **options))
+
+
+def test_a_single_row_of_activations():
+    """``x [n]``: ``[m]``."""
+    p = Problem(70, 96, 1, torch.bfloat16, adapters=1, rank=8)
+    p.index.fill_(0)
+    want = p.check()
+    p.x = p.x[0]
+    assert torch.equal(p.run(), want[0])
