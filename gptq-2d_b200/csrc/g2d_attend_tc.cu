@@ -28,7 +28,7 @@ constexpr int TA_UNIT = 6;           // the largest scale is brought to 2^6 .. 2
 template <int D>
 struct TileShared {
     static constexpr int Q = 0, Q_TILE = 128 * D * 2, K = 2 * Q_TILE, K_STAGE = 128 * D * 2, V = K + 2 * K_STAGE, V_STAGE = 128 * D * 2, SCALES = V + 2 * V_STAGE;
-    static constexpr int SCALE_STAGE = 2 * TA_KEYS * 4;  // ks, vs as floats
+    static constexpr int SCALE_STAGE = 3 * TA_KEYS * 4;  // ks, vs as floats; where the unit grows behind some rows' limits the exponent of the largest value's scale up to each key
     static constexpr size_t BYTES = SCALES + TA_SCALES * SCALE_STAGE + 1024;
     // Columns of tensor memory.  At 64 channels P has its own, and the scores of the next block are formed as soon as those of this one have been read; at 128 it lies over
     // them, and they have to wait for the products with the values.
@@ -81,6 +81,14 @@ __device__ __forceinline__ uint32_t halves_add(uint32_t u, uint32_t v, bool bf16
     if (bf16) asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(u), "r"(v));
     else asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(u), "r"(v));
     return r;
+}
+
+// A warp, the one of that number: the largest of its lanes' values up to each lane, and of the warps before
+__device__ __forceinline__ int largest_up_to(int v, const int *tops, int number) {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) v = max(v, __shfl_up_sync(0xffffffffu, v, o));  // of its own below lane o
+    for (int w = 0; w < number; ++w) v = max(v, tops[w]);
+    return v;
 }
 
 struct TileJob {
@@ -412,7 +420,8 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const __gri
             };
             fetch();
             for (;; ++number) {
-                const int n = run_of(number, go).n;
+                const TileRun &run = run_of(number, go);
+                const int n = run.n;
                 if (!__all_sync(0xffffffffu, go) || n == 0) break;
                 unit = 0;
                 for (int j = 0; j < n; ++j, ++blocks_done) {
@@ -431,18 +440,21 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const __gri
                                   halves_add((__byte_perm(x, x4, 0x7733) & 0x000f000fu) | MAGIC, LESS, BF16));
                     }
                     // the largest scale so far (one that is not finite sets no unit), and the values' scales in its power of two
-                    const unsigned size = __float_as_uint(vs) & 0x7fffffffu;
-                    const unsigned top = __reduce_max_sync(0xffffffffu, size < 0x7f800000u ? size : 0u), got = __ballot_sync(0xffffffffu, here);
+                    const unsigned bits = __float_as_uint(vs) & 0x7fffffffu, size = bits < 0x7f800000u ? bits : 0u;
+                    const unsigned top = __reduce_max_sync(0xffffffffu, size), got = __ballot_sync(0xffffffffu, here);
                     if (lane == 0) {
                         bar.tops[stage][warp - 4] = (int)(top >> 23);
                         mbar_arrive(&bar.tops_full);
                     }
                     go = __all_sync(0xffffffffu, wait(&bar.tops_full, blocks_done & 1, 0));  // of all four warps
                     if (!go) break;
+                    const int old_unit = unit;
                     unit = max(max(unit, max(bar.tops[stage][0], bar.tops[stage][1])), max(bar.tops[stage][2], bar.tops[stage][3]));
                     float *const sc = reinterpret_cast<float *>(at_base + M::SCALES + slot * M::SCALE_STAGE) + key;
                     sc[0] = fmaf(ks, 0.f, ks) * (a.scale * score_unit<MODS>(a));  // NaN for a scale that is not finite, whatever the codes
                     sc[TA_KEYS] = vs * power_of_two(min(TA_UNIT - (unit - 127), 127));
+                    if (unit != old_unit && (run.first + j + 1) * TA_KEYS > visible_keys(a, run.s, run.pair * TA_ROWS / a.group))  // the item's first row, which sees least, not the whole block
+                        sc[2 * TA_KEYS] = __int_as_float(largest_up_to((int)(size >> 23), bar.tops[stage], warp - 4));
                     if (lane == 0) bar.present[slot][warp - 4] = got;
                     if (threadIdx.x == 128) bar.unit[slot] = unit;
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -614,7 +626,14 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const __gri
                 const int new_unit = bar.unit[slot];
                 const bool first_seen = m == -INFINITY, moves = top > m + TA_SLACK || (first_seen && top > -INFINITY) || new_unit != unit;
                 if (__any_sync(0xffffffffu, moves)) {
-                    const float now = moves && top > m ? top : m;
+                    float now = moves && top > m ? top : m;
+                    // A row sees whole blocks up to its limit, and of the block with its limit the first keys: there its reference is lower by as much as the largest scale that it has seen
+                    // lies below the unit, so that scales which the mask hides leave its P as large as they would be.  It sees no block behind that.
+                    if (new_unit != unit && (first + j + 1) * TA_KEYS > least) {
+                        const int visible = min(limit - (first + j) * TA_KEYS, TA_KEYS);
+                        const int seen = visible > 0 ? max(unit, __float_as_int(reinterpret_cast<const float *>(at_base + M::SCALES + slot * M::SCALE_STAGE)[2 * TA_KEYS + visible - 1])) : 0;
+                        if (seen > 0) now -= (float)(new_unit - seen);
+                    }
                     const float keep = first_seen ? 1.f : ex2(m - now);
                     const float f = unit == 0 ? keep : keep * power_of_two(max(unit - new_unit, -126));
                     l = mul2(l, pack2(keep, keep));

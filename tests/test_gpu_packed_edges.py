@@ -302,3 +302,41 @@ def test_a_single_row_of_activations():
     want = p.check()
     p.x = p.x[0]
     assert torch.equal(p.run(), want[0])
+
+
+@pytest.mark.parametrize("options", [{}, {"softcap": 20.0}, {"prefix": True}])
+@pytest.mark.parametrize("queries", [4, 12, 33, 128, 300])
+@pytest.mark.parametrize("small, large", [(1e-4, 6e4), (0.01, 6e4), (1e-4, 60.0), (1.0, 1.0)])
+def test_hidden_values_of_any_size_leave_no_trace(small, large, queries, options):
+    """Values far larger than those that a row sees, among the keys that the mask hides from it: the row is as near as if they were not there, that is, by the largest value that it sees
+    (rounded products with the scales are at most 2^-12 of themselves off, and 2^-31 of the largest that is seen)."""
+    import packed_cache as C
+
+    group = 2 if queries > 12 else 4
+    if queries <= 12 and large > 2.0 ** 26 * small * 0.05:
+        small = large * 2.0 ** -26 / 0.05  # few rows: the documented distance (scales are 0.05 and more times `small`)
+    batch = Batch([(queries, queries), (queries + 37, queries)], 1, 64, 16, torch.float16, seed=queries)
+    scale = batch.cache.v_scale
+    there = ~scale.isnan()
+    scale[there] = (scale[there].float() * small).half()
+    spots = {}  # every fifth position or so, from the middle of the queries on
+    for b, (length, _) in enumerate(batch.sequences):
+        spots[b] = list(range(length - queries // 2, length, 5))
+        for p in spots[b]:
+            scale[int(batch.table[b, p // 16]), :, p % 16] = large
+    q = batch.randn(batch.tokens, group, 64)
+    if options.get("prefix"):
+        options = {"prefix": torch.tensor([2, queries], dtype=torch.int32, device="cuda")}
+    got = C.attend_packed(q, batch.cache, batch.table, batch.lengths, batch.offsets, **options)
+    want, _ = reference(batch, q, **options)
+    size = torch.zeros(q.shape[:2], dtype=torch.float64, device="cuda")
+    for b, (length, _) in enumerate(batch.sequences):
+        largest = batch.values(b)[1].abs().amax((0, 2))
+        for i in range(queries):
+            visible = max(length - queries + i + 1, int(options["prefix"][b]) if options else 0) if "prefix" in options else length - queries + i + 1
+            size[b * queries + i] = largest[:visible].max()
+    bound = 2.0 ** -11 * want.abs() + (2.0 ** -12 + 2.0 ** -16) * size[..., None] + 2.0 ** -25  # the last: half a step among the subnormal halves
+    # a value from 65520 on, half a step above the largest half, rounds to infinity: 8 * 6e4 is one
+    infinite = got.isinf() & (want.abs() + bound >= 65520) & (got.sign() == want.sign())
+    gap = (got.double() - want).abs().masked_fill(infinite, 0.0)
+    assert bool((gap <= bound).all()), float((gap / bound).max())
