@@ -2,7 +2,7 @@
 64 bits and tolerances are those of the files that test the operators one by one."""
 import pytest
 import torch
-from test_gpu_packed_cache import Batch, assert_near, reference
+from test_gpu_packed_cache import Batch, assert_near, reference, rounded
 from test_gpu_packed_linear import Problem
 
 pytestmark = pytest.mark.gpu
@@ -340,3 +340,56 @@ def test_hidden_values_of_any_size_leave_no_trace(small, large, queries, options
     infinite = got.isinf() & (want.abs() + bound >= 65520) & (got.sign() == want.sign())
     gap = (got.double() - want).abs().masked_fill(infinite, 0.0)
     assert bool((gap <= bound).all()), float((gap / bound).max())
+
+
+@pytest.mark.parametrize("heads, kv_heads", [(33, 1), (64, 1), (65, 1), (128, 1), (160, 1), (256, 2), (71, 71)])
+@pytest.mark.parametrize("queries", [1, 2])
+def test_groups_of_any_size(queries, heads, kv_heads):
+    """Single queries whose heads alone make a tile, groups that divide its rows and groups that do not."""
+    import packed_cache as C
+
+    batch = Batch([(300, queries), (31, queries), (129, queries)], kv_heads, 64, 32, torch.float16)
+    q = batch.randn(batch.tokens, heads, 64)
+    for offsets in (None, batch.offsets):
+        assert_near(C.attend_packed(q, batch.cache, batch.table, batch.lengths, offsets), *reference(batch, q))
+
+
+@pytest.mark.parametrize("queries", [1, 5, 80])
+def test_caches_beyond_4_gb(queries):
+    """Pages whose codes begin behind the first 2^32 bytes are written, read and attended to like the first ones."""
+    import packed_cache as C
+
+    pages, kv_heads, page_size = 66000, 8, 128
+    big = C.new_packed_cache(pages, page_size, kv_heads, 128, "cuda")
+    assert big.k_codes.numel() > 2 ** 32
+    small = C.new_packed_cache(8, page_size, kv_heads, 128, "cuda")
+    batch = Batch([(300, 300), (150, 150)], kv_heads, 128, page_size, torch.bfloat16, fill=False)
+    k, v, q = batch.randn(450, kv_heads, 128), batch.randn(450, kv_heads, 128), batch.randn(2 * queries, 16, 128)
+    table = torch.tensor([[7, 1, 3], [2, 0, 6]], dtype=torch.int32, device="cuda")
+    results = []
+    for cache, shift in ((small, 0), (big, pages - 8)):
+        where = table + shift
+        C.append_packed(cache, k, v, where, batch.lengths, batch.offsets)
+        results.append((C.attend_packed(q, cache, where, batch.lengths), *C.read_packed(cache, where, batch.lengths, batch.offsets, tokens=450, dtype=torch.bfloat16)))
+    assert all(torch.equal(x, y) for x, y in zip(*results))
+    assert torch.equal(results[0][1], rounded(k)[0].bfloat16())
+    assert not any(t[:pages - 8].any() for t in big)
+
+
+@pytest.mark.parametrize("tokens", [2, 20, 300])
+def test_matrices_beyond_4_gb(tokens):
+    """The last rows of a matrix of more than 2^32 bytes of codes."""
+    import packed_linear as L
+
+    m, n, tail = 264000, 32768, 700
+    p = Problem(tail, n, tokens, torch.float16)
+    codes = torch.zeros(m, n // 2, dtype=torch.uint8, device="cuda")
+    assert codes.numel() > 2 ** 32
+    codes[-tail:], scale, zero = p.codes, torch.ones(m, 1, device="cuda"), torch.full((m, 1), -8.0, device="cuda")  # of zeros above: code 0, zero point -8, so 0
+    scale[-tail:], zero[-tail:] = p.scale, p.zero
+    got = L.packed_linear(p.x, codes, scale, zero, qmin=p.qmin)
+    want, slack = p.reference()
+    bound = 2.0 ** -11 * want.abs() * (1 + 2.0 ** -8) + slack + 2.0 ** -14
+    assert bool(((got[:, -tail:].double() - want).abs() <= bound).all())
+    # x times zero weights: what two sums of n terms, each lost to 2^-23 of 16 |x| a step, may leave
+    assert bool((got[:, :-tail].double().abs() <= (n / 16 + 16) * 2.0 ** -23 * 16 * p.x.double().abs().sum(1, keepdim=True)).all())
