@@ -21,7 +21,7 @@
 //
 // Bound: HBM (head_dim + 4 bytes per key and head), behind it the products (16 cycles each for a quarter of an SM: 68 for a block of 64 keys and eight rows) and the instructions per key, and
 // for short calls the start (counting units, the first pages and codes: about 6 us) and the joins.  64 heads on 8, 128 channels: 131072 keys of one sequence 41 us (3.4 TB/s), 48
-// sequences of up to 8191 61 us; 16 sequences of 2000 keys, four queries of 32 heads, capped and biased, 30 us; one of 137 keys 7.6 us.
+// sequences of up to 8191 62 us; 16 sequences of 2000 keys, four queries of 32 heads, capped and biased, 31 us; one of 137 keys 7.2 us.
 #include "g2d_attend.cuh"
 
 namespace g2d {

@@ -13,8 +13,9 @@
 // The maximum that the exponentials refer to moves only when a row's scores exceed it by 2^8 (or the scales' power of two grows): then O is read and scaled in tensor memory.
 //
 // Bound: the exponentials (16 per cycle and SM: 2048 cycles for the 256 x 128 of a block, as long as its four products at 128 channels) and the instructions and exchanges around them: a
-// block takes about 3500 cycles at 128 channels, where P lies over S and the products wait for it, and 4100 at 64.  32 heads on 8: 4096 queries on 8192 keys, 128 channels, bf16, 602 us
-// (685 TFLOP/s, 0.41 of what the library's products reach); five prompts of up to 1500 on up to 2500 keys, 64 channels, under a prefix, 153 us.  A quarter of the exponentials by a
+// unit takes about 6700 cycles at 128 channels, where P lies over S and the products wait for it, and 7800 at 64 (168 and 32 units a CTA), so that the exponentials are a third of it at most: the issue slots are
+// 53 and 57 % used, the tensor cores 32 and 16 %; S is read twice, and two warps exchange their maxima before the first exponential.  32 heads on 8: 4096 queries on 8192 keys, 128 channels, bf16, 607 us
+// (679 TFLOP/s, 0.40 of what the library's products reach); five prompts of up to 1500 on up to 2500 keys, 64 channels, under a prefix, 158 us.  A quarter of the exponentials by a
 // polynomial made both slower (665, 164 us: the instructions are the scarcer), the second tile half a block behind the first made no difference.
 #include "g2d_attend.cuh"
 

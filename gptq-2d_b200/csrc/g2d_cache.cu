@@ -6,7 +6,7 @@
 // scale that is not finite, so that it reads back as NaN: absmax is taken over the bits of |v|, where both are larger than any number.
 //
 // Bound: HBM, 2 bytes read per value and half a byte written (the other way round for reading).  A lane takes eight values (16 bytes), so a row is that
-// of 16 or 8 neighbouring lanes and its absmax 3 or 4 shuffles.  8.6 k tokens of 8 heads, 128 channels, written and read back: 22.5 us (2.9 TB/s of what has to move); one token of 8 sequences 6.5.
+// of 16 or 8 neighbouring lanes and its absmax 3 or 4 shuffles.  6293 tokens of 8 heads, 128 channels, written and read back: 25.3 us (2.6 TB/s of what has to move); one token of 8 sequences 6.5.
 #include "g2d_cache.cuh"
 
 namespace g2d {
@@ -179,7 +179,7 @@ int cache_view(const g2d_cache_desc *d, CacheView *c) {
     return G2D_OK;
 }
 
-static dim3 cache_grid(const CacheView &c) {  // a token and four times a warp's rows per warp; more tokens where that is more than 32 CTAs per SM (8.6 k tokens of 8 heads, written and read: 29.8 us, with 8 CTAs 31.0, both with 8 for clearing the results first)
+static dim3 cache_grid(const CacheView &c) {  // a token and four times a warp's rows per warp; more tokens where that is more than 32 CTAs per SM (6293 tokens of 8 heads, written and read: 29.8 us, with 8 CTAs 31.0, both with 8 for clearing the results first)
     const int64_t blocks = ceil_div((int64_t)c.tokens, (int64_t)(CACHE_THREADS / 32)), groups = ceil_div((int64_t)2 * c.kv_heads * (c.head_dim / 8), (int64_t)(32 * 4));
     const int64_t most = groups < 148 * 32 ? 148 * 32 / groups : 1;
     return dim3((unsigned)(blocks < most ? blocks : most), (unsigned)groups);

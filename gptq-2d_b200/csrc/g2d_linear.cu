@@ -10,9 +10,9 @@
 // words hold their columns, so a fragment of it is one 16-byte load.  With groups of an odd number of 64 columns a lane reads 8 bytes at a time.
 //
 // A CTA has 128 rows, each of its eight warps 16; a cluster of CTAs splits the columns, and sums meet through shared memory in a fixed order.  (64 rows and the
-// columns halved between warps: 1024 x 4096, 1 token 5.5 us, as it is 5.2; 8192 x 8192, 16 tokens 28.6, 20.2.)
+// columns halved between warps: 1024 x 4096, 1 token 5.5 us where this takes 5.2; 8192 x 8192, 16 tokens 28.6, 20.2.)
 // Bound: HBM (half a byte per weight) and, from about 12 tokens on, the rate of these products (16 cycles each for a quarter of an SM); for small matrices the latency of one chain
-// of loads.  Without adapters 8192 x 8192 takes 16.0 us with 1 token (2.1 TB/s) and 20.2 with 16; 28672 x 4096 25.9 (2.3 TB/s); 1024 x 4096, 1 token, an adapter of rank 16 6.9.
+// of loads.  Without adapters 8192 x 8192 takes 16.0 us with 1 token (2.1 TB/s) and 20.2 with 16; 28672 x 4096 25.8 (2.3 TB/s); 1024 x 4096, 1 token, an adapter of rank 16 6.8.
 #include "g2d_linear.cuh"
 #include "g2d_tc.cuh"
 

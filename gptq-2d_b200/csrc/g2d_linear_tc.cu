@@ -8,14 +8,16 @@
 // An adapter is two more slices of k: for every adapter among a tile's tokens A is its rows of `up` (times nothing) and B the tokens' inner values, upper and lower
 // parts (see g2d_adapters.cu).  The product has a column for every token of the tile; the reading warps add it, times the token's factor, only where the token has this adapter.
 //
-// Few tokens may each have an adapter of their own, and two turns for each would be more than the matrix takes (61 tokens of 32 adapters: 128 turns a tile instead of 64): their outer
+// Few tokens may each have an adapter of their own, and two turns for each would be nearly as many as the matrix takes (61 tokens of 24 adapters: 112 turns a tile instead of 64): their outer
 // halves are added where the pieces are joined (53 us so, 41 that way).
 //
 // Whole rounds of tiles are done tile by tile; what is left over is cut into pieces of the same length, chunk after chunk on one line, whose sums meet in a second kernel in the order of the
 // columns (8192 x 28672, 2048 tokens, 3.46 rounds: 845 us with a fourth round, 738 with the line).
 //
-// Bound: 256 x 256 tiles by the products and the power that they draw (8192 x 28672, 2048 tokens, adapters of rank 32: 751 us with all launches, 1287 TFLOP/s, 0.77 of what the library's 16-bit products
-// reach); 64 tokens by the chain of a slot (codes, operand, products, release: about 700 cycles a chunk, 14333 x 4096, 61 tokens 40 us, 0.16 of HBM's rate).
+// Bound: 256 x 256 tiles by the products and the power that they draw (8192 x 28672, 2048 tokens, adapters of rank 32: 794 us with all launches, one call after the other, 1218 TFLOP/s, 0.72 of what
+// the library's 16-bit products reach at once and 0.86 of what they reach for seconds).  64 tokens: a CTA is through with a chunk every 820 cycles (28672 x 8192, 24 tokens: 83.8 us, 194 chunks an SM), while the
+// chunk's products take 128 and its decoding about as much, and eight slots are under way; what they all wait for has not been found (issue slots half used, tensor cores 12 %, HBM 12 %;
+// 14333 x 4096, 61 tokens 41 us).
 #include "g2d_linear.cuh"
 #include "g2d_tc.cuh"
 
@@ -143,8 +145,8 @@ __device__ __forceinline__ uint4 load_16(uint32_t at) {
 // The W that a CTA's coders have written is read by products that the other CTA, the leader, issues.  Arriving at the leader's barrier with .release takes a thread two thousand cycles (one
 // that does nothing else: 8192 x 28672, 2048 tokens, adapters of rank 32 1787 us, two 1079).  So the coders arrive at a barrier of their own CTA, and one thread,
 // which acquires that, lets a bulk copy tell the leader: of 16 bytes of that W, to be counted at the leader's barrier.  The copy is carried out behind what its thread has
-// acquired, its end is a release for the cluster, and the thread need not wait for it (775 us; 759 with a relaxed arrival, which
-// orders nothing).
+// acquired, its end is a release for the cluster, and the thread need not wait for it (794 us; 775 with a relaxed arrival, which
+// orders nothing; 14336 x 4096, 512 tokens 117, 116, and 125 where each coding warp sends a copy of its own).
 __device__ __forceinline__ void tell_leader(uint4 *to, uint32_t from, uint64_t *bar) {
     uint32_t there;
     asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(there) : "r"(smem_u32(to)));
