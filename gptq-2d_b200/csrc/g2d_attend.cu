@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(AttendShape<D, NT>::THREADS, 1) attend_rows_ke
                         my_start = -8.f / 16777216.f * sum;
             const int my_limit = real ? visible_keys(a, seq, token) : seq.keys;
             const float my_slope = MODS && a.slopes ? a.slopes[h] * LOG2E : 0.f;
-            const int my_place = seq.length - seq.count + token;
+            const int my_place = bias_origin(my_slope, my_limit);
             float two_factors[2];
 #pragma unroll
             for (int x2 = 0; x2 < 2; ++x2) {

@@ -50,6 +50,10 @@ __device__ __forceinline__ int visible_keys(const AttendArgs &a, const AttendSeq
 }
 
 
+// Where a row's biases are counted from.  A constant added to all of a row's scores changes no result, so that it need not be the query's position: from the key with the largest bias on, the keys
+// that count have small ones, whose rounding does not show (slopes of -0.5, 2e5 keys, from the query's position on: off by seven times the bound of a result).
+__device__ __forceinline__ int bias_origin(float slope, int limit) { return slope > 0.f ? limit - 1 : 0; }
+
 constexpr float LOG2E = 1.4426950408889634f;
 // What a score is taken times, so that its exponential is one to base 2: where it is capped, before that (a cap below 1e-20 is as good as none left)
 template <bool MODS>

@@ -550,7 +550,6 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const __gri
             const int r = run.pair * TA_ROWS + local;
             const bool real = r < run.s.count * a.group;
             const int token = real ? r / a.group : 0, h = run.head * a.group + (real ? r % a.group : 0), limit = real ? visible_keys(a, run.s, token) : 0x7fffffff;
-            const int place = run.s.length - run.s.count + token;
             const int64_t at_token = run.s.first + token;
             __syncwarp();
             if (lane == 0) let_go(number);
@@ -564,6 +563,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) attend_tiles_kernel(const __gri
             }
             const int least = __reduce_min_sync(0xffffffffu, limit);
             const float slope = MODS && a.slopes ? a.slopes[h] * LOG2E : 0.f, cap = a.softcap * LOG2E;
+            const int place = bias_origin(slope, limit);
             float m = -INFINITY;
             uint64_t l = 0ull;
             int unit = 0;

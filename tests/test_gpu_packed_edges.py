@@ -7,6 +7,10 @@ from test_gpu_packed_linear import Problem
 
 pytestmark = pytest.mark.gpu
 
+# What a result of the attention may be off beside its own rounding, of the largest |v| that its row sees: each product of an exponential and a value's scale is rounded to fp16, by half a step, which is
+# 2^-11 of a value just above a power of two (finfo(float16).eps / 2), and 2^-16 for exponentials, scores and sums in fp32.
+NEAR = 2.0 ** -11 + 2.0 ** -16
+
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("adapters", [0, 3])
@@ -123,7 +127,7 @@ def test_wild_offsets_touch_nothing_else(which, heads, tokens):
     if which == "beyond both ends":
         for b, (lo, hi) in enumerate(pieces):
             alone = C.attend_packed(q[lo:hi], batch.cache, batch.table[b:b + 1], batch.lengths[b:b + 1])
-            assert (out[lo:hi].float() - alone.float()).abs().max() <= 2 * 8.4 * (2.0 ** -11 + 2.0 ** -12 + 2.0 ** -16)  # cut otherwise, so summed otherwise: both as near as they have to be, |v| <= 8 * 1.05
+            assert (out[lo:hi].float() - alone.float()).abs().max() <= 2 * 8.4 * (2.0 ** -11 + 2.0 ** -11 + 2.0 ** -16)  # cut otherwise, so summed otherwise: both as near as they have to be (see `NEAR`), |v| <= 8 * 1.05
     before = [t.clone() for t in batch.cache]
     C.append_packed(batch.cache, k, k, batch.table, batch.lengths, device)
     places = torch.zeros(batch.cache.k_scale.shape, dtype=torch.bool, device="cuda")
@@ -309,7 +313,7 @@ def test_a_single_row_of_activations():
 @pytest.mark.parametrize("small, large", [(1e-4, 6e4), (0.01, 6e4), (1e-4, 60.0), (1.0, 1.0)])
 def test_hidden_values_of_any_size_leave_no_trace(small, large, queries, options):
     """Values far larger than those that a row sees, among the keys that the mask hides from it: the row is as near as if they were not there, that is, by the largest value that it sees
-    (rounded products with the scales are at most 2^-12 of themselves off, and 2^-31 of the largest that is seen)."""
+    (`NEAR`; and 2^-31 of the largest that is seen)."""
     import packed_cache as C
 
     group = 2 if queries > 12 else 4
@@ -335,7 +339,7 @@ def test_hidden_values_of_any_size_leave_no_trace(small, large, queries, options
         for i in range(queries):
             visible = max(length - queries + i + 1, int(options["prefix"][b]) if options else 0) if "prefix" in options else length - queries + i + 1
             size[b * queries + i] = largest[:visible].max()
-    bound = 2.0 ** -11 * want.abs() + (2.0 ** -12 + 2.0 ** -16) * size[..., None] + 2.0 ** -25  # the last: half a step among the subnormal halves
+    bound = 2.0 ** -11 * want.abs() + NEAR * size[..., None] + 2.0 ** -25  # the last: half a step among the subnormal halves
     # a value from 65520 on, half a step above the largest half, rounds to infinity: 8 * 6e4 is one
     infinite = got.isinf() & (want.abs() + bound >= 65520) & (got.sign() == want.sign())
     gap = (got.double() - want).abs().masked_fill(infinite, 0.0)
@@ -393,3 +397,19 @@ def test_matrices_beyond_4_gb(tokens):
     assert bool(((got[:, -tail:].double() - want).abs() <= bound).all())
     # x times zero weights: what two sums of n terms, each lost to 2^-23 of 16 |x| a step, may leave
     assert bool((got[:, :-tail].double().abs() <= (n / 16 + 16) * 2.0 ** -23 * 16 * p.x.double().abs().sum(1, keepdim=True)).all())
+
+
+@pytest.mark.parametrize("queries", [1, 5, 100])
+@pytest.mark.parametrize("length", [3000, 30000, 200000])
+def test_slopes_of_either_sign_over_long_distances(length, queries):
+    """Biases of tens of thousands where the keys that count are far from the query."""
+    import packed_cache as C
+
+    batch = Batch([(length, queries)], 1, 64, 128, torch.float16)
+    q = batch.randn(queries, 4, 64)
+    slopes = torch.tensor([-0.5, 0.5, -0.01, 0.0], device="cuda")
+    for options in ({}, {"softcap": 30.0}, {"prefix": torch.full((1,), length - 10, dtype=torch.int32, device="cuda")}):
+        got = C.attend_packed(q, batch.cache, batch.table, batch.lengths, slopes=slopes, **options)
+        want, size = reference(batch, q, slopes=slopes, **options)
+        gap = (got.double() - want).abs() / (2.0 ** -11 * want.abs() + NEAR * size[..., None])
+        assert bool((gap <= 1).all()), float(gap.max())
