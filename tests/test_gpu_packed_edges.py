@@ -413,3 +413,48 @@ def test_slopes_of_either_sign_over_long_distances(length, queries):
         want, size = reference(batch, q, slopes=slopes, **options)
         gap = (got.double() - want).abs() / (2.0 ** -11 * want.abs() + NEAR * size[..., None])
         assert bool((gap <= 1).all()), float(gap.max())
+
+
+def test_calls_from_several_threads():
+    """Host threads with streams of their own, each with calls of all kinds at once: bit for bit what one thread alone gets."""
+    import threading
+
+    import gptq_2d
+    import packed_cache as C
+
+    def work(seed):
+        problems = [Problem(700, 512, t, torch.float16, adapters=4, rank=8, seed=seed) for t in (1, 30, 90, 600)]
+        batch = Batch([(400, 1)] * 5 + [(300, 200)], 2, 64, 16, torch.float16, seed=seed)
+        q, k = batch.randn(batch.tokens, 8, 64), batch.randn(batch.tokens, 2, 64)
+        return problems, batch, q, k
+
+    def run(state):
+        problems, batch, q, k = state
+        out = [p.run() for p in problems]
+        C.append_packed(batch.cache, k, k, batch.table, batch.lengths, batch.offsets)
+        out.append(C.attend_packed(q, batch.cache, batch.table, batch.lengths, batch.offsets, softcap=20.0))
+        return out + list(C.read_packed(batch.cache, batch.table, batch.lengths, batch.offsets, tokens=batch.tokens, dtype=torch.float16))
+
+    states = [work(seed) for seed in range(4)]
+    want = [run(state) for state in states]
+    torch.cuda.synchronize()
+    got, errors = [None] * 4, []
+
+    def loop(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(10):
+                    got[i] = run(states[i])
+                torch.cuda.current_stream().synchronize()
+        except BaseException as error:  # a thread's failure is the test's
+            errors.append(error)
+
+    threads = [threading.Thread(target=loop, args=(i,)) for i in range(4)]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join()
+    assert not errors
+    gptq_2d.check_status()
+    for mine, alone in zip(got, want):
+        assert all(torch.equal(x, y) for x, y in zip(mine, alone))
